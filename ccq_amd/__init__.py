@@ -12,6 +12,8 @@ from .ccq_gla import chunk_ccq_gla, chunk_gla, fused_chunk_ccq_gla, fused_recurr
 from .clean import FusedCCQCleanRead, _ccq_compute_z_and_sum_kk, _CCQCleanQ, fused_ccq_clean_read
 from .l2norm import l2norm
 from .layers import CCQGDN, CCQGLA, LayerCache
+from .logprobs import TokenLogprobs, token_logprobs
+from .norm import layer_norm, rms_norm
 
 __all__ = [
     "chunk_ccq_gdn",
@@ -31,4 +33,8 @@ __all__ = [
     "CCQGDN",
     "CCQGLA",
     "LayerCache",
+    "layer_norm",
+    "rms_norm",
+    "token_logprobs",
+    "TokenLogprobs",
 ]

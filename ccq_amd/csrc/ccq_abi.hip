@@ -13,6 +13,7 @@
 
 #include "../../include/ccq_hip.h"
 #include "ccq_params.h"
+#include "ccq_block_args.h"
 #include "ccq_decode_args.h"
 #include "ccq_zclean_args.h"
 #include "ccq_walk_args.h"
@@ -28,6 +29,10 @@ hipError_t launch_gnorm(int stage, const GNormArgs& a, int blocks, hipStream_t s
 hipError_t launch_decode_prologue(const DecProArgs& a, hipStream_t st);
 hipError_t launch_narrow(int stage, const NarrowArgs& a, hipStream_t st);
 int narrow_blocks(long M);
+int norm_bwd_blocks(long rows, int D, int dtype);
+hipError_t launch_norm_fwd(const NormArgs& a, hipStream_t st);
+hipError_t launch_norm_bwd(const NormArgs& a, hipStream_t st);
+hipError_t launch_logprobs(bool bwd, const LogprobArgs& a, hipStream_t st);
 hipError_t launch_fill_zero(float* out, long n, hipStream_t st);
 hipError_t launch_gla_stage(int stage, const GlaArgs& a, hipStream_t st);
 hipError_t launch_decode(const DecodeArgs& a, hipStream_t st);
@@ -1479,6 +1484,128 @@ int ccq_clean_z_bwd(const void* q, const void* k, const void* z, const float* la
   a.dm0 = dm0;
   hipStream_t st = (hipStream_t)stream;
   return hip_status(timed("clean_z_bwd", st, [&] { return launch_zclean(1, a, st); }), "ccq_clean_z_bwd");
+}
+
+}  // extern "C"
+
+// ---- block norms and log probabilities of given tokens ----
+namespace {
+
+bool dtype_ok(int d) { return d == CCQ_DTYPE_BF16 || d == CCQ_DTYPE_F16 || d == CCQ_DTYPE_F32; }
+bool element_aligned(const void* p, int dtype) {
+  return (reinterpret_cast<uintptr_t>(p) & (dtype == CCQ_DTYPE_F32 ? 3 : 1)) == 0;
+}
+
+int norm_check(const char* who, int64_t rows, int D, int dtype, int wdtype, int layer, const void* b) {
+  if (rows < 0 || D < 1 || D > 8192) return fail(CCQ_ERR_SHAPE, "%s: rows=%lld D=%d (D in [1, 8192])", who, (long long)rows, D);
+  if (!dtype_ok(dtype) || (wdtype != dtype && wdtype != CCQ_DTYPE_F32))
+    return fail(CCQ_ERR_SHAPE, "%s: dtype=%d wdtype=%d (wdtype is dtype or fp32)", who, dtype, wdtype);
+  if (b && !layer) return fail(CCQ_ERR_SHAPE, "%s: an RMS norm has no bias", who);
+  return CCQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ccq_norm_bwd_workspace_bytes(int64_t rows, int D, int dtype) {
+  if (rows < 0 || D < 1 || !dtype_ok(dtype)) return 0;
+  Slicer sl{nullptr};
+  const size_t n = (size_t)norm_bwd_blocks(rows, D, dtype) * D;
+  sl.take<float>(n);
+  sl.take<float>(n);
+  return sl.off;
+}
+
+int ccq_norm_fwd(const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w, const void* b, void* y,
+                 void* s, float* mean, float* rstd, int64_t rows, int D, int dtype, int wdtype, int layer, float eps,
+                 void* stream) {
+  const char* who = "ccq_norm_fwd";
+  if (int e = norm_check(who, rows, D, dtype, wdtype, layer, b)) return e;
+  if (ldx < D || (r && ldr < D)) return fail(CCQ_ERR_SHAPE, "%s: row strides %lld, %lld below D=%d", who, (long long)ldx, (long long)ldr, D);
+  if (rows == 0) return CCQ_OK;
+  if (!x || !y || !r != !s || (layer && !mean != !rstd))
+    return fail(CCQ_ERR_NULL, "%s: x and y are required, r and s go together, so do mean and rstd", who);
+  for (const void* p : {x, r, (const void*)y, (const void*)s})
+    if (!element_aligned(p, dtype)) return fail(CCQ_ERR_ALIGN, "%s: rows must be aligned to their elements", who);
+  if (!element_aligned(w, wdtype) || !element_aligned(b, wdtype))
+    return fail(CCQ_ERR_ALIGN, "%s: w and b must be aligned to their elements", who);
+  if (int e = check_stream_device(stream, who)) return e;
+  NormArgs a{};
+  a.x = x; a.ldx = ldx; a.r = r; a.ldr = ldr; a.w = w; a.b = b; a.y = y; a.s = s; a.mean = mean; a.rstd = rstd;
+  a.rows = rows; a.D = D; a.dtype = dtype; a.wdtype = wdtype; a.layer = layer != 0; a.eps = eps;
+  hipStream_t st = (hipStream_t)stream;
+  return hip_status(timed("norm_fwd", st, [&] { return launch_norm_fwd(a, st); }), who);
+}
+
+int ccq_norm_bwd(const void* x, int64_t ldx, const void* w, const float* mean, const float* rstd, const void* dy,
+                 int64_t ldy, const void* ds, int64_t ldds, void* dx, void* dw, void* db, void* workspace,
+                 int64_t rows, int D, int dtype, int wdtype, int layer, void* stream) {
+  const char* who = "ccq_norm_bwd";
+  if (int e = norm_check(who, rows, D, dtype, wdtype, layer, db)) return e;
+  if (ldx < D || ldy < D || (ds && ldds < D))
+    return fail(CCQ_ERR_SHAPE, "%s: row strides %lld, %lld, %lld below D=%d", who, (long long)ldx, (long long)ldy, (long long)ldds, D);
+  if (!dx && !dw && !db) return CCQ_OK;
+  if (rows > 0 && (!x || !rstd || !dy || (layer && !mean) || ((dw || db) && !workspace)))
+    return fail(CCQ_ERR_NULL, "%s: x, mean, rstd, dy and (for dw, db) the workspace are required", who);
+  for (const void* p : {x, dy, ds, (const void*)dx})
+    if (!element_aligned(p, dtype)) return fail(CCQ_ERR_ALIGN, "%s: rows must be aligned to their elements", who);
+  if (!element_aligned(w, wdtype) || !element_aligned(dw, wdtype) || !element_aligned(db, wdtype))
+    return fail(CCQ_ERR_ALIGN, "%s: w, dw and db must be aligned to their elements", who);
+  if (!aligned16(workspace)) return fail(CCQ_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", who);
+  if (int e = check_stream_device(stream, who)) return e;
+  NormArgs a{};
+  a.x = x; a.ldx = ldx; a.w = w; a.mean = (float*)mean; a.rstd = (float*)rstd; a.dy = dy; a.ldy = ldy; a.ds = ds;
+  a.ldds = ldds; a.dx = dx; a.dw = dw; a.db = db; a.rows = rows; a.D = D; a.dtype = dtype; a.wdtype = wdtype;
+  a.layer = layer != 0;
+  Slicer sl{(char*)workspace};
+  const size_t n = (size_t)norm_bwd_blocks(rows, D, dtype) * D;
+  a.dw_part = sl.take<float>(n);
+  a.db_part = sl.take<float>(n);
+  hipStream_t st = (hipStream_t)stream;
+  return hip_status(timed("norm_bwd", st, [&] { return launch_norm_bwd(a, st); }), who);
+}
+
+static int logprobs_check(const char* who, int64_t ldx, int64_t rows, int V, int dtype) {
+  if (rows < 0 || rows > 0x7fffffff || V < 1 || V > (1 << 30) || ldx < V || !dtype_ok(dtype))
+    return fail(CCQ_ERR_SHAPE, "%s: rows=%lld V=%d ldx=%lld dtype=%d", who, (long long)rows, V, (long long)ldx, dtype);
+  return CCQ_OK;
+}
+
+int ccq_token_logprobs_fwd(const void* logits, int64_t ldx, const int64_t* ids, float* logp, float* entropy,
+                           float* stats, float* top, int64_t* top_ids, int64_t rows, int V, int k, int64_t ignore,
+                           int dtype, void* stream) {
+  const char* who = "ccq_token_logprobs_fwd";
+  if (int e = logprobs_check(who, ldx, rows, V, dtype)) return e;
+  if (k < 0 || k > 64 || k > V) return fail(CCQ_ERR_SHAPE, "%s: k=%d alternatives of V=%d (at most 64)", who, k, V);
+  if (rows == 0) return CCQ_OK;
+  if (!logits || !ids || !logp || !entropy || (k && (!top || !top_ids)))
+    return fail(CCQ_ERR_NULL, "%s: logits, ids, logp, entropy and (for k > 0) top, top_ids are required", who);
+  if (!element_aligned(logits, dtype)) return fail(CCQ_ERR_ALIGN, "%s: logits must be aligned to their elements", who);
+  if (int e = check_stream_device(stream, who)) return e;
+  LogprobArgs a{};
+  a.x = logits; a.ldx = ldx; a.ids = ids; a.logp = logp; a.ent = entropy; a.stats = stats; a.top = top;
+  a.top_ids = top_ids; a.rows = rows; a.V = V; a.k = k; a.ignore = ignore; a.dtype = dtype;
+  hipStream_t st = (hipStream_t)stream;
+  return hip_status(timed("logprobs_fwd", st, [&] { return launch_logprobs(false, a, st); }), who);
+}
+
+int ccq_token_logprobs_bwd(const void* logits, int64_t ldx, const int64_t* ids, const float* entropy,
+                           const float* stats, const float* dlogp, const float* dentropy, void* dlogits, int64_t rows,
+                           int V, int64_t ignore, int dtype, void* stream) {
+  const char* who = "ccq_token_logprobs_bwd";
+  if (int e = logprobs_check(who, ldx, rows, V, dtype)) return e;
+  if (rows == 0) return CCQ_OK;
+  if (!logits || !ids || !entropy || !stats || !dlogits)
+    return fail(CCQ_ERR_NULL, "%s: logits, ids, entropy, stats and dlogits are required", who);
+  if (!element_aligned(logits, dtype) || !element_aligned(dlogits, dtype))
+    return fail(CCQ_ERR_ALIGN, "%s: logits and dlogits must be aligned to their elements", who);
+  if (int e = check_stream_device(stream, who)) return e;
+  LogprobArgs a{};
+  a.x = logits; a.ldx = ldx; a.ids = ids; a.ent = (float*)entropy; a.stats = (float*)stats; a.dlogp = dlogp;
+  a.dent = dentropy; a.dx = dlogits; a.rows = rows; a.V = V; a.ignore = ignore; a.dtype = dtype;
+  hipStream_t st = (hipStream_t)stream;
+  return hip_status(timed("logprobs_bwd", st, [&] { return launch_logprobs(true, a, st); }), who);
 }
 
 }  // extern "C"

@@ -1,0 +1,128 @@
+"""Block norms: layer norm and RMS norm over the last dimension, with the residual stream's add in the same pass
+(``ccq_norm_fwd`` / ``ccq_norm_bwd`` of ``libccq_hip.so``).
+
+The reference's layers (``ccq/gdn/layer.py``, ``ccq/gla/layer.py``) sit in pre-norm blocks whose norms its HF
+model classes take from fla; ``prologue.gated_rmsnorm`` is the norm inside the layers.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import call, ptr, stream_of
+from ._rows import DTYPES, needs_grad, on_device, require_gpu, require_like, rows_of, stride_of
+
+__all__ = ["layer_norm", "rms_norm", "BlockNormFunction"]
+
+MAX_WIDTH = 8192
+
+
+def _forward(x, residual, weight, bias, layer, eps, keep):
+    """``(y, s or None, x as rows, mean or None, rstd or None)``; the statistics only with ``keep``."""
+    x2 = rows_of(x)
+    r2 = rows_of(residual) if residual is not None else None
+    rows, D = x2.shape
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    s = torch.empty(x.shape, device=x.device, dtype=x.dtype) if r2 is not None else None
+    mean = torch.empty(rows, device=x.device, dtype=torch.float32) if keep and layer else None
+    rstd = torch.empty(rows, device=x.device, dtype=torch.float32) if keep else None
+    wdtype = DTYPES[weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype]
+    with on_device(x):
+        call("ccq_norm_fwd", ptr(x2), stride_of(x2), ptr(r2), stride_of(r2) if r2 is not None else 0, ptr(weight),
+             ptr(bias), ptr(y), ptr(s), ptr(mean), ptr(rstd), rows, D, DTYPES[x.dtype], wdtype, int(layer), eps,
+             stream_of(x))
+    return y, s, x2, mean, rstd
+
+
+class BlockNormFunction(torch.autograd.Function):
+    """The norm of ``x`` (``+ residual``); returns ``y`` or ``(y, s)`` with ``s = x + residual``."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, layer, eps):
+        y, s, x2, mean, rstd = _forward(x, residual, weight, bias, layer, eps, True)
+        # the normalised rows: the stream where there is a residual (an output, saved as such), x otherwise
+        ctx.save_for_backward(x2 if s is None else s, weight, mean, rstd)
+        ctx.meta = (layer, x.shape, None if bias is None else bias.dtype)
+        ctx.set_materialize_grads(False)
+        return y if s is None else (y, s)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, ds=None):
+        rows_in, weight, mean, rstd = ctx.saved_tensors
+        layer, shape, bdtype = ctx.meta
+        need_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        need_w, need_b = ctx.needs_input_grad[2], ctx.needs_input_grad[3]
+        x2 = rows_of(rows_in)
+        rows, D = x2.shape
+        dev = x2.device
+        if dy is None:
+            if ds is None:
+                return (None,) * 6
+            dy = torch.zeros(shape, device=dev, dtype=x2.dtype)  # (only the stream was used)
+        d2 = rows_of(dy)
+        s2 = rows_of(ds) if ds is not None else None
+        wdt = weight.dtype if weight is not None else bdtype if bdtype is not None else x2.dtype
+        dx = torch.empty(shape, device=dev, dtype=x2.dtype) if need_x else None
+        dw = torch.empty(D, device=dev, dtype=wdt) if need_w else None
+        db = torch.empty(D, device=dev, dtype=wdt) if need_b else None
+        ws = None
+        with on_device(x2):
+            if need_w or need_b:
+                n = _lib.load().ccq_norm_bwd_workspace_bytes(rows, D, DTYPES[x2.dtype])
+                ws = torch.empty(n, device=dev, dtype=torch.uint8)
+            call("ccq_norm_bwd", ptr(x2), stride_of(x2), ptr(weight), ptr(mean), ptr(rstd), ptr(d2), stride_of(d2),
+                 ptr(s2), stride_of(s2) if s2 is not None else 0, ptr(dx), ptr(dw), ptr(db), ptr(ws), rows, D,
+                 DTYPES[x2.dtype], DTYPES[wdt], int(layer), stream_of(x2))
+        return dx if ctx.needs_input_grad[0] else None, dx if ctx.needs_input_grad[1] else None, dw, db, None, None
+
+
+def _norm(who, x, weight, bias, eps, residual, layer):
+    if x.dtype not in DTYPES:
+        raise TypeError(f"{who} takes bf16, fp16 or fp32 rows (got {x.dtype})")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
+        raise ValueError(f"{who}: x {tuple(x.shape)}: needs a last dimension in [1, {MAX_WIDTH}]")
+    if not eps >= 0:
+        raise ValueError(f"{who}: eps={eps} must not be negative")
+    require_like(who, x, weight=weight, bias=bias, residual=residual)
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.shape != (x.shape[-1],):
+            raise ValueError(f"{who}: {name} {tuple(t.shape)}: expected [{x.shape[-1]}]")
+        if t.dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"{who}: {name} {t.dtype}: expected x's type ({x.dtype}) or fp32")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"{who}: weight {weight.dtype} and bias {bias.dtype}: expected one type")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError(f"{who}: residual {tuple(residual.shape)} {residual.dtype}: expected x's {tuple(x.shape)} "
+                         f"{x.dtype}")
+    require_gpu(who, x)
+    weight = weight if weight is None else weight.contiguous()
+    bias = bias if bias is None else bias.contiguous()
+    eps = float(eps)
+    if needs_grad(x, residual, weight, bias):
+        return BlockNormFunction.apply(x, residual, weight, bias, layer, eps)
+    y, s, _, _, _ = _forward(x, residual, weight, bias, layer, eps, False)
+    return y if s is None else (y, s)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5, residual: Optional[torch.Tensor] = None
+               ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension (bf16, fp16 or fp32 on the GPU, 1 to
+    8192 wide, any row stride); ``weight`` and ``bias`` ``[D]`` in x's type or fp32, each optional.  With
+    ``residual`` (x's shape and type) the rows are ``s = x + residual``, rounded to their type as the residual
+    stream holds them, and it returns ``(y, s)``.  Statistics and sums in fp32, one rounding of y.  Gradients of x,
+    residual, weight and bias."""
+    return _norm("layer_norm", x, weight, bias, eps, residual, True)
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-5,
+             residual: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """``x / sqrt(mean(x^2) + eps) * weight`` over the last dimension; otherwise as ``layer_norm``."""
+    return _norm("rms_norm", x, weight, None, eps, residual, False)

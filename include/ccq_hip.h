@@ -37,6 +37,11 @@ extern "C" {
 #define CCQ_ERR_HIP (-4)       /* a HIP runtime error (see ccq_last_error) */
 #define CCQ_ERR_DEVICE (-5)    /* the stream belongs to a device other than the current one */
 
+/* element types of the entry points that take more than one (dtype, wdtype) */
+#define CCQ_DTYPE_BF16 0
+#define CCQ_DTYPE_F16 1
+#define CCQ_DTYPE_F32 2
+
 int ccq_abi_version(void);
 const char* ccq_last_error(void);
 
@@ -464,13 +469,56 @@ int ccq_l2norm_bwd(const void* x, const float* rstd, const float* dy_f32, const 
                    int D, void* stream);
 
 /*
+ * Block norms over rows of D in [1, 8192] (layer norm: layer != 0; RMS norm: layer == 0), with the
+ * residual stream's add in the same pass:
+ *   s = x + r (rounded to the rows' type), mu = mean s (RMS norm: 0), rstd = 1 / sqrt(mean (s - mu)^2 + eps),
+ *   y = (s - mu) rstd w + b.
+ * x, r, y, s rows of dtype (x and r with row strides ldx, ldr >= D; y and s contiguous); r and s both or
+ * neither (nullable); w, b [D] of wdtype, which is dtype or CCQ_DTYPE_F32 (each nullable: ones, none; b
+ * with layer norm only); mean (layer norm) and rstd fp32 [rows] for the backward (nullable: inference).
+ * Statistics and sums in fp32.  Any element-aligned address and any stride.
+ * Backward: x the normalised rows (s where the forward had a residual), dy [rows, D] (stride ldy), ds
+ * the gradient that reached s itself (nullable, stride ldds) -> dx [rows, D] contiguous (the gradient
+ * of x and of r; nullable), dw, db [D] of wdtype (nullable; db with layer norm only).  dw and db need the
+ * workspace of ccq_norm_bwd_workspace_bytes(rows, D, dtype) bytes; their sums run in a fixed order.  The
+ * norms around the reference's layers are fla's (its HF model classes); no counterpart in its operators.
+ */
+size_t ccq_norm_bwd_workspace_bytes(int64_t rows, int D, int dtype);
+int ccq_norm_fwd(const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w, const void* b, void* y,
+                 void* s, float* mean, float* rstd, int64_t rows, int D, int dtype, int wdtype, int layer, float eps,
+                 void* stream);
+int ccq_norm_bwd(const void* x, int64_t ldx, const void* w, const float* mean, const float* rstd, const void* dy,
+                 int64_t ldy, const void* ds, int64_t ldds, void* dx, void* dw, void* db, void* workspace,
+                 int64_t rows, int D, int dtype, int wdtype, int layer, void* stream);
+
+/*
+ * Log probabilities of given tokens: of logits [rows, V] of dtype (row stride ldx >= V) and tokens
+ * ids [rows], fp32 log softmax(logits)[id] into logp [rows], the entropy of each row's distribution into
+ * entropy [rows], each row's maximum and log sum exp(logits - maximum) into stats [rows, 2] (for the
+ * backward; nullable), and the k likeliest tokens of each row (0 <= k <= min(V, 64); ties to the lowest index, a NaN logit before any number) into top
+ * (fp32 log probabilities) and top_ids, [rows, k].  A row with ids == ignore is not read: logp, entropy and
+ * top 0, top_ids -1.  A token outside [0, V) has logp NaN; a row that holds a NaN or +inf, or nothing but
+ * -inf, is NaN throughout (as log softmax); an -inf logit has probability 0 and no share of the entropy.
+ * Backward: dlogp, dentropy fp32 [rows] (each nullable) and the forward's entropy and stats -> dlogits
+ * [rows, V] of dtype, contiguous; zeros for skipped rows, NaN for rows whose logp is NaN.  Follows the
+ * reference models' loss (HF cross entropy over the LM head's logits; none in its operators).
+ */
+int ccq_token_logprobs_fwd(const void* logits, int64_t ldx, const int64_t* ids, float* logp, float* entropy,
+                           float* stats, float* top, int64_t* top_ids, int64_t rows, int V, int k, int64_t ignore,
+                           int dtype, void* stream);
+int ccq_token_logprobs_bwd(const void* logits, int64_t ldx, const int64_t* ids, const float* entropy,
+                           const float* stats, const float* dlogp, const float* dentropy, void* dlogits, int64_t rows,
+                           int V, int64_t ignore, int dtype, void* stream);
+
+/*
  * Kernel timing (measurement facility; no counterpart in the reference).  While enabled, each
  * entry point records a HIP event pair around every launch of its kernels on the caller's
  * stream.  ccq_timing_read waits for the recorded events of `kernel` (names: conv_fwd, conv_bwd,
  * gnorm_fwd, gnorm_bwd, clean_fwd_sum, clean_fwd, clean_bwd_rows, clean_bwd_dq, clean_bwd_gsum,
  * clean_bwd_dk, clean_bwd_gate, gdn_prep, gdn_fwd_state, gdn_fwd_o, gdn_bwd_state, gdn_bwd_dqkw,
  * gdn_bwd_wy, gla_intra, gla_fwd_state, gla_fwd_o, gla_bwd_state, gla_bwd_dv, gla_bwd_dqk,
- * clean_z_fwd, clean_z_bwd, narrow_fwd, narrow_bwd) and returns the summed
+ * clean_z_fwd, clean_z_bwd, narrow_fwd, narrow_bwd, norm_fwd, norm_bwd, logprobs_fwd, logprobs_bwd) and
+ * returns the summed
  * milliseconds and the number of launches since the last ccq_timing_reset.  ccq_timing_select
  * restricts the events to the kernel of that name (NULL: every kernel), so that a timed loop carries
  * one event pair per step instead of one per kernel.

@@ -1,0 +1,110 @@
+"""Refusals of the operators around the mixers that need no GPU: arguments are checked before anything is launched,
+in the Python entry points and at the C ABI."""
+
+import ctypes
+
+import pytest
+import torch
+
+from ccq_amd import _lib, layer_norm, rms_norm, token_logprobs
+
+SHAPE, NULL, ALIGN = -1, -2, -3
+P = ctypes.c_void_p(0x1000)     # never dereferenced: the checks fail first
+ODD = ctypes.c_void_p(0x1001)
+
+
+@pytest.mark.parametrize("norm", [layer_norm, rms_norm])
+def test_norm_refusals(norm):
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    w = torch.ones(64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="GPU"):
+        norm(x, w)
+    with pytest.raises(TypeError, match="bf16, fp16 or fp32"):
+        norm(x.double(), w)
+    with pytest.raises(ValueError, match="last dimension"):
+        norm(torch.zeros(2, 8193, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="last dimension"):
+        norm(torch.zeros(2, 0, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="last dimension"):
+        norm(torch.zeros((), dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="weight"):
+        norm(x, w[:32])
+    with pytest.raises(TypeError, match="weight"):
+        norm(x, w.half())
+    with pytest.raises(ValueError, match="residual"):
+        norm(x, w, residual=x[:1])
+    with pytest.raises(ValueError, match="residual"):
+        norm(x, w, residual=x.float())
+    with pytest.raises(ValueError, match="eps"):
+        norm(x, w, eps=-1.0)
+    with pytest.raises(ValueError, match="eps"):
+        norm(x, w, eps=float("nan"))
+
+
+def test_layer_norm_bias_type():
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    with pytest.raises(TypeError, match="one type"):
+        layer_norm(x, torch.ones(64), torch.zeros(64, dtype=torch.bfloat16))
+
+
+def test_norm_abi_refusals():
+    lib = _lib.load()
+
+    def fwd(x=P, ldx=64, r=None, ldr=0, w=P, b=None, y=P, s=None, mean=None, rstd=None, D=64, dtype=0, wdtype=0,
+            layer=1):
+        return lib.ccq_norm_fwd(x, ldx, r, ldr, w, b, y, s, mean, rstd, 4, D, dtype, wdtype, layer, 1e-5, None)
+
+    assert fwd(D=0) == SHAPE and fwd(D=8193, ldx=9000) == SHAPE and fwd(ldx=63) == SHAPE
+    assert fwd(dtype=3) == SHAPE and fwd(wdtype=1) == SHAPE and fwd(b=P, layer=0) == SHAPE
+    assert fwd(r=P, s=P, ldr=63) == SHAPE
+    assert fwd(x=None) == NULL and fwd(y=None) == NULL and fwd(r=P, ldr=64) == NULL and fwd(rstd=P) == NULL
+    assert fwd(x=ODD) == ALIGN and fwd(w=ODD) == ALIGN
+
+    def bwd(x=P, ldy=64, mean=P, rstd=P, dy=P, dx=P, dw=P, db=P, ws=P, layer=1):
+        return lib.ccq_norm_bwd(x, 64, P, mean, rstd, dy, ldy, None, 0, dx, dw, db, ws, 4, 64, 0, 0, layer, None)
+
+    assert bwd(ldy=10) == SHAPE and bwd(layer=0) == SHAPE
+    assert bwd(x=None) == NULL and bwd(mean=None) == NULL and bwd(rstd=None) == NULL and bwd(ws=None) == NULL
+    assert bwd(ws=ctypes.c_void_p(0x1008)) == ALIGN and bwd(dx=ODD) == ALIGN
+    # partial rows of dw and db: one for each workgroup, at most 512
+    assert lib.ccq_norm_bwd_workspace_bytes(100000, 1024, 0) == 2 * 512 * 1024 * 4
+    assert lib.ccq_norm_bwd_workspace_bytes(8, 1024, 0) == 2 * 2 * 1024 * 4
+
+
+def test_token_logprobs_refusals():
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    ids = torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="GPU"):
+        token_logprobs(x, ids)
+    with pytest.raises(TypeError, match="logits"):
+        token_logprobs(x.double(), ids)
+    with pytest.raises(TypeError, match="ids"):
+        token_logprobs(x, ids.float())
+    with pytest.raises(ValueError, match="ids"):
+        token_logprobs(x, ids[:3])
+    with pytest.raises(ValueError, match="ids"):
+        token_logprobs(torch.zeros(4, 0, dtype=torch.bfloat16), ids)
+    with pytest.raises(ValueError, match="top_k"):
+        token_logprobs(x, ids, top_k=65)
+    with pytest.raises(ValueError, match="top_k"):
+        token_logprobs(x[:, :8], ids, top_k=9)
+    with pytest.raises(ValueError, match="top_k"):
+        token_logprobs(x, ids, top_k=-1)
+
+
+def test_token_logprobs_abi_refusals():
+    lib = _lib.load()
+
+    def fwd(x=P, ldx=64, ids=P, logp=P, ent=P, top=P, top_ids=P, V=64, k=4, dtype=0):
+        return lib.ccq_token_logprobs_fwd(x, ldx, ids, logp, ent, None, top, top_ids, 4, V, k, -100, dtype, None)
+
+    assert fwd(V=0) == SHAPE and fwd(ldx=63) == SHAPE and fwd(dtype=7) == SHAPE
+    assert fwd(k=65, V=100, ldx=100) == SHAPE and fwd(k=5, V=4) == SHAPE and fwd(k=-1) == SHAPE
+    assert fwd(x=None) == NULL and fwd(ids=None) == NULL and fwd(logp=None) == NULL and fwd(top=None) == NULL
+    assert fwd(x=ODD) == ALIGN
+
+    def bwd(x=P, ids=P, ent=P, stats=P, dx=P, V=64):
+        return lib.ccq_token_logprobs_bwd(x, 64, ids, ent, stats, P, P, dx, 4, V, -100, 0, None)
+
+    assert bwd(V=65) == SHAPE and bwd(ent=None) == NULL and bwd(stats=None) == NULL and bwd(dx=None) == NULL
+    assert bwd(dx=ODD) == ALIGN
