@@ -12,6 +12,7 @@ from .ccq_gla import chunk_ccq_gla, chunk_gla, fused_chunk_ccq_gla, fused_recurr
 from .clean import FusedCCQCleanRead, _ccq_compute_z_and_sum_kk, _CCQCleanQ, fused_ccq_clean_read
 from .l2norm import l2norm
 from .layers import CCQGDN, CCQGLA, LayerCache
+from .linear import fused_linear
 from .logprobs import TokenLogprobs, token_logprobs
 from .norm import layer_norm, rms_norm
 
@@ -35,6 +36,7 @@ __all__ = [
     "LayerCache",
     "layer_norm",
     "rms_norm",
+    "fused_linear",
     "token_logprobs",
     "TokenLogprobs",
 ]

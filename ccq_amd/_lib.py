@@ -74,6 +74,11 @@ SIGNATURES = {
     "ccq_norm_bwd": (_I, [_P, _I64] + [_P] * 4 + [_I64, _P, _I64] + [_P] * 4 + [_I64] + [_I] * 4 + [_P]),
     "ccq_token_logprobs_fwd": (_I, [_P, _I64] + [_P] * 6 + [_I64, _I, _I, _I64, _I, _P]),
     "ccq_token_logprobs_bwd": (_I, [_P, _I64] + [_P] * 6 + [_I64, _I, _I64, _I, _P]),
+    "ccq_linear_workspace_bytes": (_SZ, [_I64] * 3 + [_I]),
+    "ccq_linear_fwd": (_I, [_P, _I64] * 2 + [_P, _I, _P, _I64] + [_P] * 3 + [_I64] * 3 + [_I, _I, _P]),
+    "ccq_linear_bwd_workspace_bytes": (_SZ, [_I64] * 3 + [_I]),
+    "ccq_linear_bwd": (_I, [_P, _I64] * 2 + [_P, _P, _I64] + [_P] * 3 + [_I, _P] + [_I64] * 3 + [_I, _I, _P]),
+    "ccq_pad_rows": (_I, [_P, _I64, _P] + [_I64] * 3 + [_P]),
     "ccq_timing_enable": (_I, [_I]),
     "ccq_timing_reset": (_I, []),
     "ccq_timing_select": (_I, [ctypes.c_char_p]),
@@ -125,7 +130,7 @@ KERNELS = ("conv_fwd", "conv_bwd", "gnorm_fwd", "gnorm_bwd",
            "gdn_prep", "gdn_fwd_state", "gdn_fwd_o", "gdn_bwd_state", "gdn_bwd_dqkw", "gdn_bwd_wy",
            "gla_intra", "gla_fwd_state", "gla_fwd_o", "gla_bwd_state", "gla_bwd_dv", "gla_bwd_dqk",
            "clean_z_fwd", "clean_z_bwd", "narrow_fwd", "narrow_bwd", "norm_fwd", "norm_bwd",
-           "logprobs_fwd", "logprobs_bwd")
+           "logprobs_fwd", "logprobs_bwd", "linear_fwd", "linear_dz", "linear_dx", "linear_dw")
 
 
 def timing_enable(on: bool) -> None:

@@ -33,6 +33,11 @@ int norm_bwd_blocks(long rows, int D, int dtype);
 hipError_t launch_norm_fwd(const NormArgs& a, hipStream_t st);
 hipError_t launch_norm_bwd(const NormArgs& a, hipStream_t st);
 hipError_t launch_logprobs(bool bwd, const LogprobArgs& a, hipStream_t st);
+void product_plan(long M, long N, long K, bool* large, int* splits);
+hipError_t launch_product(int kind, const ProductArgs& p, hipStream_t st);
+int act_bwd_row_blocks(long M, long N);
+hipError_t launch_act_bwd(const ActBwdArgs& a, hipStream_t st);
+hipError_t launch_pad_rows(const PadRowsArgs& a, hipStream_t st);
 hipError_t launch_fill_zero(float* out, long n, hipStream_t st);
 hipError_t launch_gla_stage(int stage, const GlaArgs& a, hipStream_t st);
 hipError_t launch_decode(const DecodeArgs& a, hipStream_t st);
@@ -1606,6 +1611,142 @@ int ccq_token_logprobs_bwd(const void* logits, int64_t ldx, const int64_t* ids, 
   a.dent = dentropy; a.dx = dlogits; a.rows = rows; a.V = V; a.ignore = ignore; a.dtype = dtype;
   hipStream_t st = (hipStream_t)stream;
   return hip_status(timed("logprobs_bwd", st, [&] { return launch_logprobs(true, a, st); }), who);
+}
+
+}  // extern "C"
+
+// ---- linear map with an epilogue ----
+namespace {
+
+constexpr long kMaxStride = 1L << 22;  // a tile's rows stay inside 31 bits of bytes
+constexpr long kMaxSide = 1L << 30;
+
+long round8(long n) { return (n + 7) & ~7L; }
+long linear_outs(int64_t N, int act) { return act == CCQ_ACT_SWIGLU ? 2 * N : N; }
+size_t partial_bytes(long M, long N, long K) {
+  bool large;
+  int splits;
+  product_plan(M, N, K, &large, &splits);
+  return splits > 1 ? (size_t)splits * M * N * sizeof(float) : 0;
+}
+bool rows16(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
+
+int linear_check(const char* who, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int act, int dtype,
+                 int bdtype) {
+  if (M < 0 || N < 1 || K < 1 || M > kMaxSide || N > kMaxSide || linear_outs(N, act) > kMaxStride || K > kMaxStride ||
+      ((M + 127) / 128) * ((linear_outs(N, act) + 127) / 128) > 0x7fffffffL)
+    return fail(CCQ_ERR_SHAPE, "%s: M=%lld N=%lld K=%lld", who, (long long)M, (long long)N, (long long)K);
+  if (ldx < round8(K) || ldw < round8(K) || ldx % 8 || ldw % 8 || ldx > kMaxStride || ldw > kMaxStride)
+    return fail(CCQ_ERR_SHAPE, "%s: row strides %lld, %lld of K=%lld (multiples of 8, at most 4 Mi)", who, (long long)ldx,
+                (long long)ldw, (long long)K);
+  if (act < CCQ_ACT_NONE || act > CCQ_ACT_SWIGLU || (dtype != CCQ_DTYPE_BF16 && dtype != CCQ_DTYPE_F16) ||
+      (bdtype != dtype && bdtype != CCQ_DTYPE_F32))
+    return fail(CCQ_ERR_SHAPE, "%s: act=%d dtype=%d bdtype=%d", who, act, dtype, bdtype);
+  return CCQ_OK;
+}
+
+// Sub-buffers of the backward's workspace: dz, the partial sums of db and of a product.
+struct LinearBwd {
+  char* dz;
+  float* db_part;
+  float* part;
+};
+size_t carve_linear_bwd(char* base, int64_t M, int64_t N, int64_t K, int act, LinearBwd* out) {
+  Slicer sl{base};
+  const long Nz = linear_outs(N, act);
+  LinearBwd t;
+  t.dz = sl.take<char>((size_t)M * round8(Nz) * 2);
+  t.db_part = sl.take<float>((size_t)(M > 0 ? act_bwd_row_blocks(M, N) : 0) * Nz);
+  t.part = (float*)sl.take<char>(std::max(partial_bytes(M, K, Nz), partial_bytes(Nz, K, M)));
+  if (out) *out = t;
+  return sl.off;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ccq_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int act) {
+  return M > 0 && N > 0 && K > 0 ? partial_bytes(M, linear_outs(N, act), K) : 0;
+}
+
+int ccq_linear_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, int bdtype,
+                   const void* r, int64_t ldr, void* y, void* z, void* workspace, int64_t M, int64_t N, int64_t K,
+                   int act, int dtype, void* stream) {
+  const char* who = "ccq_linear_fwd";
+  if (int e = linear_check(who, M, N, K, ldx, ldw, act, dtype, bdtype)) return e;
+  if (r && ldr < N) return fail(CCQ_ERR_SHAPE, "%s: the residual's row stride %lld is below N=%lld", who, (long long)ldr, (long long)N);
+  if (M == 0) return CCQ_OK;
+  if (!x || !weight || !y || (!workspace && ccq_linear_workspace_bytes(M, N, K, act)))
+    return fail(CCQ_ERR_NULL, "%s: x, weight, y and the workspace are required", who);
+  if (!aligned16(x) || !aligned16(weight) || !aligned16(z) || !aligned16(workspace))
+    return fail(CCQ_ERR_ALIGN, "%s: x, weight, z and the workspace must be 16-byte aligned", who);
+  if (!element_aligned(y, dtype) || !element_aligned(r, dtype) || !element_aligned(bias, bdtype))
+    return fail(CCQ_ERR_ALIGN, "%s: y, r and bias must be aligned to their elements", who);
+  if (int e = check_stream_device(stream, who)) return e;
+  ProductArgs p{};
+  p.a = x; p.lda = ldx; p.b = weight; p.ldb = ldw; p.M = M; p.N = N; p.K = K; p.out = y; p.ldo = N;
+  p.bias = bias; p.bdtype = bdtype; p.res = r; p.ldr = ldr; p.z = z; p.ldz = round8(linear_outs(N, act));
+  p.part = (float*)workspace; p.act = act; p.dtype = dtype;
+  hipStream_t st = (hipStream_t)stream;
+  return hip_status(timed("linear_fwd", st, [&] { return launch_product(0, p, st); }), who);
+}
+
+size_t ccq_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int act) {
+  return M >= 0 && N > 0 && K > 0 ? carve_linear_bwd(nullptr, M, N, K, act, nullptr) : 0;
+}
+
+int ccq_linear_bwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* z, const void* dy,
+                   int64_t ldy, void* dx, void* dw, void* db, int bdtype, void* workspace, int64_t M, int64_t N,
+                   int64_t K, int act, int dtype, void* stream) {
+  const char* who = "ccq_linear_bwd";
+  if (int e = linear_check(who, M, N, K, ldx, ldw, act, dtype, bdtype)) return e;
+  if (ldy < N) return fail(CCQ_ERR_SHAPE, "%s: dy's row stride %lld is below N=%lld", who, (long long)ldy, (long long)N);
+  if (!dx && !dw && !db) return CCQ_OK;
+  if ((!workspace && ccq_linear_bwd_workspace_bytes(M, N, K, act)) || (M > 0 && (!dy || (dw && !x) || (dx && !weight) || (act != CCQ_ACT_NONE && !z))))
+    return fail(CCQ_ERR_NULL, "%s: dy, x (for dw), weight (for dx), z (with an activation) and the workspace are required", who);
+  if (!aligned16(x) || !aligned16(weight) || !aligned16(z) || !aligned16(workspace))
+    return fail(CCQ_ERR_ALIGN, "%s: x, weight, z and the workspace must be 16-byte aligned", who);
+  if (!element_aligned(dy, dtype) || !element_aligned(dx, dtype) || !element_aligned(dw, dtype) || !element_aligned(db, bdtype))
+    return fail(CCQ_ERR_ALIGN, "%s: dy, dx, dw and db must be aligned to their elements", who);
+  if (int e = check_stream_device(stream, who)) return e;
+  LinearBwd ws;
+  carve_linear_bwd((char*)workspace, M, N, K, act, &ws);
+  const long Nz = linear_outs(N, act), ldz = round8(Nz);
+  hipStream_t st = (hipStream_t)stream;
+  // without an activation dz is dy itself, where its rows can be read as an operand's
+  const bool direct = act == CCQ_ACT_NONE && N % 8 == 0 && rows16(dy, ldy) && ldy <= kMaxStride;
+  if (!direct || db) {
+    ActBwdArgs a{};
+    a.z = act == CCQ_ACT_NONE ? nullptr : z; a.dy = dy; a.dz = direct ? nullptr : ws.dz; a.db_part = db ? ws.db_part : nullptr;
+    a.db = db; a.M = M; a.N = N; a.ldz = ldz; a.ldy = ldy; a.act = act; a.bdtype = bdtype; a.dtype = dtype;
+    if (int e = hip_status(timed("linear_dz", st, [&] { return launch_act_bwd(a, st); }), who)) return e;
+  }
+  ProductArgs p{};
+  p.a = direct ? dy : ws.dz; p.lda = direct ? ldy : ldz; p.part = ws.part; p.act = CCQ_ACT_NONE; p.dtype = dtype;
+  p.bdtype = dtype; p.N = K; p.ldo = K;
+  if (dx) {
+    p.b = weight; p.ldb = ldw; p.M = M; p.K = Nz; p.out = dx;
+    if (int e = hip_status(timed("linear_dx", st, [&] { return launch_product(1, p, st); }), who)) return e;
+  }
+  if (dw) {
+    p.b = x; p.ldb = ldx; p.M = Nz; p.K = M; p.out = dw;
+    if (int e = hip_status(timed("linear_dw", st, [&] { return launch_product(2, p, st); }), who)) return e;
+  }
+  return CCQ_OK;
+}
+
+int ccq_pad_rows(const void* src, int64_t ld, void* dst, int64_t ldd, int64_t rows, int64_t K, void* stream) {
+  const char* who = "ccq_pad_rows";
+  if (rows < 0 || K < 1 || ld < K || ldd < K || ldd % 8)
+    return fail(CCQ_ERR_SHAPE, "%s: rows=%lld K=%lld ld=%lld ldd=%lld", who, (long long)rows, (long long)K, (long long)ld, (long long)ldd);
+  if (rows == 0) return CCQ_OK;
+  if (!src || !dst) return fail(CCQ_ERR_NULL, "%s: src and dst are required", who);
+  if (!aligned16(dst) || !element_aligned(src, CCQ_DTYPE_BF16))
+    return fail(CCQ_ERR_ALIGN, "%s: dst must be 16-byte aligned, src aligned to its elements", who);
+  if (int e = check_stream_device(stream, who)) return e;
+  PadRowsArgs a{src, dst, (long)rows, (long)K, (long)ld, (long)ldd};
+  return hip_status(launch_pad_rows(a, (hipStream_t)stream), who);
 }
 
 }  // extern "C"

@@ -45,4 +45,41 @@ struct LogprobArgs {
   int V, k, dtype;
 };
 
+// Activations of the linear map as the C ABI numbers them (CCQ_ACT_*).
+enum : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4, kActSwiglu = 5 };
+
+// One product out[M, N] = A B^T over K, its operands stored with the contraction running along the rows
+// (A [M, K], B [N, K]) or down them (A [K, M], B [K, N]), and what is done with the result.
+struct ProductArgs {
+  const void* a;       // row stride lda elements, rows 16-byte aligned
+  const void* b;       // row stride ldb
+  long lda, ldb;
+  long M, N, K;        // (swiglu: N outputs of 2 N rows of B)
+  void* out;           // [M, ldo]
+  long ldo;
+  const void* bias;    // [N] (swiglu: [2 N]) of bdtype (nullable)
+  const void* res;     // [M, N] row stride ldr (nullable)
+  void* z;             // [M, ldz] the values before the activation (nullable)
+  long ldr, ldz;
+  float* part;         // [splits, M, N (swiglu: 2 N)] partial sums (splits > 1)
+  int splits;          // parts of the contraction, whole steps each
+  int act, bdtype, dtype;
+};
+
+struct ActBwdArgs {
+  const void* z;       // [M, ldz] (nullable: no activation)
+  const void* dy;      // [M, N] row stride ldy
+  void* dz;            // [M, ldz], zeros behind the Nz columns (nullable: only db is wanted)
+  float* db_part;      // [row blocks, Nz] (nullable)
+  void* db;            // [Nz] of bdtype
+  long M, N, ldz, ldy;
+  int act, bdtype, dtype, row_blocks;
+};
+
+struct PadRowsArgs {
+  const void* src;     // [rows, K] row stride ld
+  void* dst;           // [rows, ldd], zeros behind the K columns
+  long rows, K, ld, ldd;
+};
+
 }  // namespace ccq

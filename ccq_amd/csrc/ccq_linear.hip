@@ -1,0 +1,568 @@
+// Linear map with an epilogue, y = act(x W^T + b) + r, for any number of rows, and its backward:
+//
+//   z = x W^T + b,  y = act(z) + r    act: none, relu, silu, gelu (erf), gelu (tanh), swiglu (z = [gate | up],
+//                                     silu(gate) up)
+//   dz = act'(z) dy,  dx = dz W,  dW = dz^T x,  db = sum over rows of dz
+//
+// All three products run on one tiled kernel: bf16 or fp16 operands, fp32 accumulation on the matrix cores
+// (16x16x32), tiles staged in LDS by direct loads.  Its operands are stored with the contraction along the rows
+// (x and W forward; dz in dx) or down them (W in dx; dz and x in dW); the second kind is read out of LDS by
+// transposing reads, so nothing is transposed in memory.
+#include <algorithm>
+
+#include "ccq_block_args.h"
+#include "ccq_oper.h"
+#include "ccq_rows.h"
+
+namespace ccq {
+
+namespace {
+
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+__device__ __forceinline__ f32x4 product16(const s16x8& a, const s16x8& b, const f32x4& c) {
+  if constexpr (__is_same(T, bf16))
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------------------
+// activations, in fp32
+// ---------------------------------------------------------------------------
+constexpr float kTanhA = 0.7978845608028654f, kTanhB = 0.044715f;  // gelu_tanh: tanh(a (z + b z^3))
+
+__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + __expf(-z)); }
+
+__device__ __forceinline__ float act_value(int act, float z) {
+  switch (act) {
+    case kActRelu: return fmaxf(z, 0.f);
+    case kActSilu: return z * sigmoid(z);
+    case kActGelu: return 0.5f * z * erfcf(z * -0.7071067811865476f);
+    case kActGeluTanh: return z * sigmoid(2.f * kTanhA * (z + kTanhB * z * z * z));
+    default: return z;
+  }
+}
+__device__ __forceinline__ float act_slope(int act, float z) {
+  switch (act) {
+    case kActRelu: return z > 0.f ? 1.f : 0.f;
+    case kActSilu: {
+      const float g = sigmoid(z);
+      return g * (1.f + z * (1.f - g));
+    }
+    case kActGelu: return 0.5f * erfcf(z * -0.7071067811865476f) + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+    case kActGeluTanh: {
+      z = fminf(fmaxf(z, -16.f), 16.f);  // (the slope is 0 or 1 long before; the square of a far z would overflow)
+      const float g = sigmoid(2.f * kTanhA * (z + kTanhB * z * z * z));
+      return g + z * 2.f * g * (1.f - g) * kTanhA * (1.f + 3.f * kTanhB * z * z);
+    }
+    default: return 1.f;
+  }
+}
+
+__device__ __forceinline__ float bias_at(const void* b, int bdtype, long i) {
+  if (bdtype == kF32) return *gmem((const float*)b + i);
+  if (bdtype == kBf16) return (float)*gmem((const bf16*)b + i);
+  return (float)*gmem((const f16*)b + i);
+}
+
+// C consecutive values of a row of N from column n on, at any element's address
+template <typename T, int C>
+__device__ __forceinline__ void store_row(T* row, long n, long N, const float (&v)[C]) {
+  typedef T vec __attribute__((ext_vector_type(C)));
+  typedef vec any __attribute__((aligned(sizeof(T))));
+  vec o;
+#pragma unroll
+  for (int i = 0; i < C; ++i) o[i] = (T)v[i];
+  if (n + C <= N) {
+    *gmem((any*)(row + n)) = o;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+    if (n + i < N) *gmem(row + n + i) = o[i];
+}
+template <typename T, int C>
+__device__ __forceinline__ void add_row(const T* row, long n, long N, float (&v)[C]) {
+  typedef T vec __attribute__((ext_vector_type(C)));
+  typedef vec any __attribute__((aligned(sizeof(T))));
+  if (n + C <= N) {
+    const vec r = *gmem((const any*)(row + n));
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] += (float)r[i];
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+    if (n + i < N) v[i] += (float)*gmem(row + n + i);
+}
+
+// The epilogue of C consecutive columns n .. of row m (swiglu: v the gates, up the other half).
+template <typename T, int C>
+__device__ __forceinline__ void finish(const ProductArgs& p, long m, long n, float (&v)[C], float (&up)[C]) {
+  const bool glu = p.act == kActSwiglu;
+  if (p.bias) {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (n + i < p.N) {
+        v[i] += bias_at(p.bias, p.bdtype, n + i);
+        if (glu) up[i] += bias_at(p.bias, p.bdtype, p.N + n + i);
+      }
+  }
+  if (p.z) {
+    T* z = (T*)p.z + m * p.ldz;
+    store_row<T, C>(z, n, p.N, v);
+    if (glu) store_row<T, C>(z + p.N, n, p.N, up);
+  }
+  if (glu) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = v[i] * sigmoid(v[i]) * up[i];
+  } else if (p.act != kActNone) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = act_value(p.act, v[i]);
+  }
+  if (p.res) add_row<T, C>((const T*)p.res + m * p.ldr, n, p.N, v);
+  store_row<T, C>((T*)p.out + m * p.ldo, n, p.N, v);
+}
+
+// ---------------------------------------------------------------------------
+// the tiled product
+// ---------------------------------------------------------------------------
+constexpr int kStep = 64;  // contraction elements a step
+
+// One operand's tile of a step in LDS: R rows of the product by 64 contraction elements.
+//   along the rows (DOWN = false): R rows of 128 bytes, 16-byte piece s of row r at piece s ^ swz(r)
+//   down the rows  (DOWN = true):  64 rows of 2 R bytes, piece s of row k at piece s ^ (swz(k) << 1)
+// so that the sixteen pieces that a fragment read takes at once lie in different banks.  Direct loads write 1 KiB
+// (64 pieces) each, in LDS order: the swizzle is in the address that a lane reads.
+// A buffer resource bounds every load by the operand's end; what lies behind it comes as zeros.
+struct Operand {
+  const char* base;  // first element of the tile in the step
+  long left;         // bytes from there to the operand's end
+};
+__device__ __forceinline__ u32x4 resource(const Operand& o) {
+  const unsigned n = o.left <= 0 ? 0u : o.left > 0x7fffffffL ? 0x7fffffffu : (unsigned)o.left;
+  return u32x4{(unsigned)(size_t)o.base, (unsigned)((size_t)o.base >> 32) & 0xffffu, n, 0x00020000u};
+}
+__device__ __forceinline__ void load_piece_lds(const u32x4& r, unsigned off, unsigned m0) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(off), "s"(r) : "memory", "m0");
+}
+constexpr unsigned kNowhere = 0x80000000u;  // behind every resource's end
+
+// swizzle of product row r of an operand read in consecutive rows (A), or in the order of column pairs (B)
+__device__ __forceinline__ int swz_a(int r) { return (r >> 1) & 7; }
+__device__ __forceinline__ int swz_b(int n) { return ((n >> 1) & 1) | (((n >> 3) & 3) << 1); }
+__device__ __forceinline__ int swz_k(int k) { return (k & 3) | (((k >> 3) & 1) << 2); }
+
+// Loads of a tile: wave w of NW takes instructions w * PER .. (consecutive pieces of LDS).
+template <int R, bool DOWN, bool B, int NW>
+struct TileLoad {
+  static constexpr int PER = R * kStep * 2 / 1024 / NW;
+  static_assert(PER >= 1 && R * kStep * 2 % (1024 * NW) == 0, "whole instructions a wave");
+  unsigned off[PER];  // byte offset of this lane's piece from the tile's base
+  unsigned lds;       // LDS byte address of this wave's first piece, in stage 0
+  __device__ void init(unsigned lds_base, int wave, int l, long ld) {
+    lds = lds_base + wave * PER * 1024;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int q = (wave * PER + i) * 64 + l;  // piece of the tile in LDS order
+      if (DOWN) {
+        const int k = q / (R / 8), s = q % (R / 8);
+        off[i] = (unsigned)(k * ld * 2) + ((s ^ (swz_k(k) << 1)) << 4);
+      } else {
+        const int r = q >> 3, s = q & 7;
+        off[i] = (unsigned)(r * ld * 2) + ((s ^ (B ? swz_b(r) : swz_a(r))) << 4);
+      }
+    }
+  }
+  // contraction elements at and behind `limit` of this step (limit < 64: the last one) as zeros
+  __device__ void issue(const Operand& o, unsigned stage, int limit, int wave, int l) const {
+    const u32x4 r = resource(o);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      unsigned f = off[i];
+      if (!DOWN && limit < kStep) {
+        const int q = (wave * PER + i) * 64 + l, row = q >> 3;
+        if ((((q & 7) ^ (B ? swz_b(row) : swz_a(row))) << 3) >= limit) f = kNowhere;
+      }
+      load_piece_lds(r, f, lds + stage + i * 1024);
+    }
+  }
+};
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) const s16x8 lds_s8;
+__device__ __forceinline__ s16x8 read16(unsigned at) { return *(lds_s8*)(size_t)at; }
+__device__ __forceinline__ s16x4_t read_tr4(unsigned at) {
+  typedef __attribute__((address_space(3))) s16x4_t lds_s4;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(size_t)at);
+}
+
+enum : int { kPlain = 0, kEpilogue = 1, kPartial = 2 };
+
+// BM x BN tile of the product by WM x WN waves, two stages of LDS.  Lane l of a wave holds, of each 16x16 tile
+// (it, j) of the wave, row m = 16 it + (l & 15) and four consecutive columns.  Along-the-row B operands (the forward)
+// are read so that the column tiles j = 2 q and 2 q + 1 of a lane are eight consecutive columns, one 16-byte store.
+// swiglu: the wave's columns are 32 gates and the 32 ups beside them, so a lane holds both.
+template <typename T, int BM, int BN, int WM, int WN, bool DA, bool DB, int MODE, bool GLU>
+__global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs p) {
+  constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
+  constexpr unsigned kA = BM * kStep * 2, kStage = kA + BN * kStep * 2;
+  static_assert(!GLU || (BN / WN == 64 && !DB && MODE == kEpilogue), "gates and ups of one wave");
+  __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
+  const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  constexpr int NT = GLU ? BN / 2 : BN;  // output columns of a tile
+  // tile of this workgroup: each XCD (workgroups are handed out round-robin over the 8) takes consecutive tiles, in
+  // column order within bands of 8 tile rows, so that its L2 holds what its workgroups share
+  const int tm = (int)((p.M + BM - 1) / BM), tn = (int)((p.N + NT - 1) / NT), tiles = tm * tn;
+  const int xcd = blockIdx.x & 7, q8 = tiles >> 3, r8 = tiles & 7;
+  const int t = xcd * q8 + min(xcd, r8) + (blockIdx.x >> 3);
+  const int band = t / (8 * tn), in = t - band * 8 * tn, rows = min(8, tm - band * 8);
+  const long m0 = (long)(band * 8 + in % rows) * BM, n0 = (long)(in / rows) * NT;
+  // steps of this workgroup
+  const int all = (int)((p.K + kStep - 1) / kStep), per = (all + p.splits - 1) / p.splits;
+  const int s0 = blockIdx.y * per, s1 = min(all, s0 + per);
+
+  const unsigned lds0 = lds_addr(smem);
+  TileLoad<BM, DA, false, NW> la;
+  TileLoad<BN, DB, !DB, NW> lb;
+  la.init(lds0, wave, l, p.lda);
+  lb.init(lds0 + kA, wave, l, p.ldb);
+  // elements of the operands: to the end of the last row's last whole piece
+  const long nb = GLU ? 2 * p.N : p.N;
+  const long ea = ((DA ? p.K : p.M) - 1) * p.lda + (((DA ? p.M : p.K) + 7) & ~7L);
+  const long eb = ((DB ? p.K : nb) - 1) * p.ldb + (((DB ? nb : p.K) + 7) & ~7L);
+  Operand oa, ob, ou;
+  {
+    const long fa = DA ? (long)s0 * kStep * p.lda + m0 : m0 * p.lda + (long)s0 * kStep;
+    oa = {(const char*)p.a + fa * 2, (ea - fa) * 2};
+    const long fb = DB ? (long)s0 * kStep * p.ldb + n0 : n0 * p.ldb + (long)s0 * kStep;
+    ob = {(const char*)p.b + fb * 2, (eb - fb) * 2};
+    const long fu = fb + p.N * p.ldb;
+    ou = {(const char*)p.b + fu * 2, (eb - fu) * 2};
+  }
+  if constexpr (GLU) {
+    // tile row 64 w + c of B: gate n0 + 32 w + c for c < 32, up n0 + 32 w + c - 32 behind
+#pragma unroll
+    for (int i = 0; i < lb.PER; ++i) {
+      const int r = ((wave * lb.PER + i) * 64 + l) >> 3, s = l & 7;
+      lb.off[i] = (unsigned)(((r >> 6) * 32 + (r & 31)) * p.ldb * 2) + ((s ^ swz_b(r)) << 4);
+    }
+  }
+  const long stepA = (DA ? kStep * p.lda : kStep) * 2, stepB = (DB ? kStep * p.ldb : kStep) * 2;
+  auto issue = [&](int s, unsigned stage) {
+    const int limit = (int)min((long)kStep, p.K - (long)s * kStep);
+    la.issue(oa, stage, limit, wave, l);
+    if constexpr (GLU) {
+      const u32x4 rg = resource(ob), ru = resource(ou);
+#pragma unroll
+      for (int i = 0; i < lb.PER; ++i) {
+        const int row = (wave * lb.PER + i) * 8;  // (uniform; 8 rows never straddle the halves)
+        unsigned f = lb.off[i];
+        const int r = row + (l >> 3);
+        if (limit < kStep && (((l & 7) ^ swz_b(r)) << 3) >= limit) f = kNowhere;
+        load_piece_lds((row & 32) ? ru : rg, f, lb.lds + stage + i * 1024);
+      }
+      ou.base += stepB;
+      ou.left -= stepB;
+    } else {
+      lb.issue(ob, stage, limit, wave, l);
+    }
+    oa.base += stepA;
+    oa.left -= stepA;
+    ob.base += stepB;
+    ob.left -= stepB;
+  };
+
+  // fragment addresses of this lane in stage 0
+  const int r = l & 15, g = l >> 4;
+  unsigned fa[DA ? TM : 2], fb[DB ? TN : 2];
+  if constexpr (DA) {
+    const int k = 8 * g + (r >> 2), s = wm * TM * 2 + ((r >> 1) & 1);
+#pragma unroll
+    for (int it = 0; it < TM; ++it)
+      fa[it] = lds0 + k * (BM * 2) + (((s + 2 * it) ^ (swz_k(k) << 1)) << 4) + 8 * (r & 1);
+  } else {
+    const int row = wm * TM * 16 + r;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) fa[kk] = lds0 + row * 128 + (((4 * kk + g) ^ swz_a(row)) << 4);
+  }
+  if constexpr (DB) {
+    const int k = 8 * g + (r >> 2), s = wn * TN * 2 + ((r >> 1) & 1);
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+      fb[j] = lds0 + kA + k * (BN * 2) + (((s + 2 * j) ^ (swz_k(k) << 1)) << 4) + 8 * (r & 1);
+  } else {
+    const int row = wn * TN * 16 + 8 * (r >> 2) + (r & 3);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) fb[kk] = lds0 + kA + row * 128 + (((4 * kk + g) ^ swz_b(row)) << 4);
+  }
+
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int it = 0; it < TM; ++it)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[it][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (s0 < s1) issue(s0, 0);
+  unsigned stage = 0;
+  for (int s = s0; s < s1; ++s) {
+    wait_loads<0>();
+    lds_barrier();  // this step's tiles are in LDS, and every wave has read the last step's
+    if (s + 1 < s1) issue(s + 1, stage ^ kStage);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      s16x8 a[TM], b[TN];
+#pragma unroll
+      for (int it = 0; it < TM; ++it) {
+        if constexpr (DA) {
+          const unsigned at = fa[it] + stage + kk * 32 * BM * 2;
+          const s16x4_t x = read_tr4(at), y = read_tr4(at + 4 * BM * 2);
+          a[it] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+          a[it] = read16(fa[kk] + stage + it * 16 * 128);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        if constexpr (DB) {
+          const unsigned at = fb[j] + stage + kk * 32 * BN * 2;
+          const s16x4_t x = read_tr4(at), y = read_tr4(at + 4 * BN * 2);
+          b[j] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+          b[j] = read16(fb[kk] + stage + (32 * (j >> 1) + 4 * (j & 1)) * 128);
+        }
+      }
+#pragma unroll
+      for (int it = 0; it < TM; ++it)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[it][j] = product16<T>(b[j], a[it], acc[it][j]);
+    }
+    stage ^= kStage;
+    asm volatile("" ::: "memory");
+  }
+
+#pragma unroll
+  for (int it = 0; it < TM; ++it) {
+    const long m = m0 + wm * TM * 16 + it * 16 + r;
+    if (m >= p.M) continue;
+    if constexpr (GLU) {
+      const long n = n0 + wn * 32 + 8 * g;
+      float v[8], up[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = acc[it][i >> 2][i & 3];
+        up[i] = acc[it][2 + (i >> 2)][i & 3];
+      }
+      if (n < p.N) finish<T, 8>(p, m, n, v, up);
+    } else {
+      constexpr int C = DB ? 4 : 8;  // consecutive columns a lane
+#pragma unroll
+      for (int c = 0; c < TN * 4 / C; ++c) {
+        const long n = n0 + wn * TN * 16 + (DB ? 16 * c + 4 * g : 32 * c + 8 * g);
+        if (n >= p.N) continue;
+        float v[C];
+#pragma unroll
+        for (int i = 0; i < C; ++i) v[i] = acc[it][(c * C + i) / 4][i & 3];
+        if constexpr (MODE == kEpilogue) finish<T, C>(p, m, n, v, v);
+        else if constexpr (MODE == kPlain) store_row<T, C>((T*)p.out + m * p.ldo, n, p.N, v);
+        else store_row<float, C>(p.part + ((long)blockIdx.y * p.M + m) * p.N, n, p.N, v);
+      }
+    }
+  }
+}
+
+// the parts of the contraction added in their order, then the epilogue
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_kernel(const ProductArgs p) {
+  constexpr int C = 4;
+  const bool glu = p.act == kActSwiglu;
+  const long cols = glu ? 2 * p.N : p.N, groups = (p.N + C - 1) / C;
+  const long at = (long)blockIdx.x * kThreads + threadIdx.x;
+  if (at >= p.M * groups) return;
+  const long m = at / groups, n = at % groups * C;
+  float v[C], up[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) v[i] = up[i] = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float* row = p.part + ((long)s * p.M + m) * cols;
+    add_row<float, C>(row, n, p.N, v);
+    if (glu) add_row<float, C>(row + p.N, n, p.N, up);
+  }
+  finish<T, C>(p, m, n, v, up);
+}
+
+// ---------------------------------------------------------------------------
+// dz = act'(z) dy, with the bias's gradient: a thread takes 8 columns of the rows of its block
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(kThreads) void act_bwd_kernel(const ActBwdArgs a) {
+  constexpr int C = 8;
+  const bool glu = a.act == kActSwiglu;
+  const long n = ((long)blockIdx.x * kThreads + threadIdx.x) * C, width = glu ? a.ldz - a.N : a.ldz;  // (with the columns behind)
+  if (n >= width) return;
+  const long per = (a.M + a.row_blocks - 1) / a.row_blocks, r0 = blockIdx.y * per, r1 = min(a.M, r0 + per);
+  float sum[2][C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) sum[0][i] = sum[1][i] = 0.f;
+  for (long m = r0; m < r1; ++m) {
+    float d[C], z[C], u[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) d[i] = z[i] = u[i] = 0.f;
+    add_row<T, C>((const T*)a.dy + m * a.ldy, n, a.N, d);
+    if (a.z) add_row<T, C>((const T*)a.z + m * a.ldz, n, a.N, z);
+    if (glu) {
+      add_row<T, C>((const T*)a.z + m * a.ldz + a.N, n, a.N, u);
+      float dg[C], du[C];
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const float g = sigmoid(z[i]);
+        dg[i] = d[i] * u[i] * (g * (1.f + z[i] * (1.f - g)));
+        du[i] = d[i] * z[i] * g;
+        sum[0][i] += dg[i];
+        sum[1][i] += du[i];
+      }
+      if (a.dz) {
+        store_row<T, C>((T*)a.dz + m * a.ldz, n, a.N, dg);
+        store_row<T, C>((T*)a.dz + m * a.ldz + a.N, n, a.ldz - a.N, du);  // (du is 0 behind the columns)
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        if (a.z) d[i] *= act_slope(a.act, z[i]);
+        sum[0][i] += d[i];
+      }
+      if (a.dz) store_row<T, C>((T*)a.dz + m * a.ldz, n, a.ldz, d);
+    }
+  }
+  if (a.db_part) {
+    float* row = a.db_part + (long)blockIdx.y * (glu ? 2 * a.N : a.N);
+    store_row<float, C>(row, n, a.N, sum[0]);
+    if (glu) store_row<float, C>(row + a.N, n, a.N, sum[1]);
+  }
+}
+
+// db[n] = sum of the partial rows, in their order inside 16 interleaved groups
+__global__ __launch_bounds__(1024) void bias_sum_kernel(const ActBwdArgs a) {
+  __shared__ float part[16][64];
+  const long n = a.act == kActSwiglu ? 2 * a.N : a.N, c = (long)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int g = threadIdx.x >> 6;
+  float s = 0.f;
+  if (c < n)
+#pragma unroll 4
+    for (int i = g; i < a.row_blocks; i += 16) s += *gmem(a.db_part + i * n + c);
+  part[g][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (g || c >= n) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += part[i][threadIdx.x];
+  if (a.bdtype == kF32) ((float*)a.db)[c] = s;
+  else if (a.bdtype == kBf16) ((bf16*)a.db)[c] = (bf16)s;
+  else ((f16*)a.db)[c] = (f16)s;
+}
+
+__global__ __launch_bounds__(kThreads) void pad_rows_kernel(const PadRowsArgs a) {
+  const long pieces = a.ldd / 8, at = (long)blockIdx.x * kThreads + threadIdx.x;
+  if (at >= a.rows * pieces) return;
+  const long m = at / pieces, n = at % pieces * 8;
+  const short* row = (const short*)a.src + m * a.ld;
+  s16x8 v;
+  typedef s16x8 any __attribute__((aligned(2)));
+  if (n + 8 <= a.K) {
+    v = *gmem((const any*)(row + n));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = n + i < a.K ? *gmem(row + n + i) : (short)0;
+  }
+  *gmem((s16x8*)((short*)a.dst + m * a.ldd + n)) = v;
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool DA, bool DB, int MODE, bool GLU>
+hipError_t launch_tiles(const ProductArgs& p, hipStream_t st) {
+  const long tiles = ((p.M + BM - 1) / BM) * ((p.N + (GLU ? BN / 2 : BN) - 1) / (GLU ? BN / 2 : BN));
+  hipLaunchKernelGGL((product_kernel<T, BM, BN, WM, WN, DA, DB, MODE, GLU>), dim3((unsigned)tiles, (unsigned)p.splits),
+                     dim3(WM * WN * 64), 0, st, p);
+  return hipGetLastError();
+}
+
+template <typename T, bool DA, bool DB, int MODE, bool GLU>
+hipError_t launch_size(const ProductArgs& p, bool large, hipStream_t st) {
+  if (large) return launch_tiles<T, 256, 256, 2, 4, DA, DB, MODE, GLU>(p, st);
+  return launch_tiles<T, 128, 128, 2, 2, DA, DB, MODE, GLU>(p, st);
+}
+
+template <typename T>
+hipError_t launch_typed(int kind, const ProductArgs& p, bool large, hipStream_t st) {
+  if (p.splits > 1) {
+    ProductArgs q = p;  // partial products of all rows of B
+    if (p.act == kActSwiglu) q.N = 2 * p.N;
+    q.act = kActNone;
+    const hipError_t e = kind == 0 ? launch_size<T, false, false, kPartial, false>(q, large, st)
+                         : kind == 1 ? launch_size<T, false, true, kPartial, false>(q, large, st)
+                                     : launch_size<T, true, true, kPartial, false>(q, large, st);
+    if (e != hipSuccess) return e;
+    const long threads = p.M * ((p.N + 3) / 4);
+    hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0, st, p);
+    return hipGetLastError();
+  }
+  if (kind == 0)
+    return p.act == kActSwiglu ? launch_size<T, false, false, kEpilogue, true>(p, large, st)
+                               : launch_size<T, false, false, kEpilogue, false>(p, large, st);
+  if (kind == 1) return launch_size<T, false, true, kPlain, false>(p, large, st);
+  return launch_size<T, true, true, kPlain, false>(p, large, st);
+}
+
+constexpr int kCus = 256;
+
+}  // namespace
+
+// Tile and parts of the contraction of a product of M x N outputs (swiglu: N = all rows of B) over K.
+void product_plan(long M, long N, long K, bool* large, int* splits) {
+  const long t256 = ((M + 255) / 256) * ((N + 255) / 256), t128 = ((M + 127) / 128) * ((N + 127) / 128);
+  const long steps = (K + kStep - 1) / kStep;
+  *large = t256 >= kCus / 2;
+  *splits = 1;
+  if (!*large && t128 > 0 && t128 < kCus) *splits = (int)std::max(1L, std::min({kCus / t128, steps / 4, 16L}));
+}
+
+// kind 0: y = act(x W^T + b) + r; 1: dx = dz W; 2: dW = dz^T x
+hipError_t launch_product(int kind, const ProductArgs& p, hipStream_t st) {
+  if (p.M <= 0 || p.N <= 0) return hipSuccess;
+  bool large;
+  int splits;
+  product_plan(p.M, p.act == kActSwiglu ? 2 * p.N : p.N, p.K, &large, &splits);
+  ProductArgs q = p;
+  q.splits = splits;
+  return p.dtype == kBf16 ? launch_typed<bf16>(kind, q, large, st) : launch_typed<f16>(kind, q, large, st);
+}
+
+int act_bwd_row_blocks(long M, long N) {
+  const long cols = (N + 8 * kThreads - 1) / (8 * kThreads);
+  return (int)std::max(1L, std::min((M + 15) / 16, std::max(1L, 2048 / cols)));
+}
+
+hipError_t launch_act_bwd(const ActBwdArgs& args, hipStream_t st) {
+  ActBwdArgs a = args;
+  const bool glu = a.act == kActSwiglu;
+  a.row_blocks = a.M > 0 ? act_bwd_row_blocks(a.M, a.N) : 0;
+  if (a.row_blocks) {
+    const long width = glu ? a.ldz - a.N : a.ldz;
+    const dim3 grid((unsigned)((width + 8 * kThreads - 1) / (8 * kThreads)), (unsigned)a.row_blocks);
+    if (a.dtype == kBf16) hipLaunchKernelGGL(act_bwd_kernel<bf16>, grid, dim3(kThreads), 0, st, a);
+    else hipLaunchKernelGGL(act_bwd_kernel<f16>, grid, dim3(kThreads), 0, st, a);
+  }
+  if (a.db)
+    hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)(((glu ? 2 * a.N : a.N) + 63) / 64)), dim3(1024), 0, st, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_pad_rows(const PadRowsArgs& a, hipStream_t st) {
+  const long n = a.rows * (a.ldd / 8);
+  if (n <= 0) return hipSuccess;
+  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, st, a);
+  return hipGetLastError();
+}
+
+}  // namespace ccq

@@ -511,14 +511,49 @@ int ccq_token_logprobs_bwd(const void* logits, int64_t ldx, const int64_t* ids, 
                            int V, int64_t ignore, int dtype, void* stream);
 
 /*
+ * Linear map with an epilogue for any number of rows, y = act(x W^T + b) + r, and its backward (the
+ * nn.Linear projections of a block and its MLP over a prompt or a training batch; ccq_decode_linear is
+ * the form for a decode step's few rows, without gradients).  x [M, K] (row stride ldx), weight [N, K]
+ * (ldw; swiglu: [2 N, K], the gate rows, then the up rows), of dtype BF16 or F16, their rows 16-byte
+ * aligned with strides a multiple of 8 (at most 4 Mi) and readable up to the next multiple of 8 columns,
+ * with zeros behind column K (ccq_pad_rows makes such a copy of any rows); bias [N] (swiglu: [2 N]) of
+ * bdtype, dtype or F32 (nullable); r [M, N] (row stride ldr, nullable); y [M, N] contiguous.
+ * z (nullable) [M, ldz], ldz = N (swiglu: 2 N) rounded up to a multiple of 8: x W^T + b, for the backward
+ * of an activation.  fp32 accumulation, bias, activation and residual; y and z round once.  act: CCQ_ACT_*:
+ * none, relu, silu, gelu (erf), gelu with tanh, swiglu (silu(gate) up).  workspace:
+ * ccq_linear_workspace_bytes bytes (partial sums where few tiles split the contraction).
+ * Backward: dz = act'(z) dy (rounded to dtype once, as it enters two products), dx = dz W [M, K],
+ * dw = dz^T x (weight's shape), both contiguous, db = the sum of dz's rows in fp32, rounded to bdtype
+ * (each nullable); dy [M, N] (row stride ldy); z as the forward left it (not for act none).  The residual's
+ * gradient is dy.  workspace: ccq_linear_bwd_workspace_bytes bytes.  All sums run in a fixed order.
+ */
+#define CCQ_ACT_NONE 0
+#define CCQ_ACT_RELU 1
+#define CCQ_ACT_SILU 2
+#define CCQ_ACT_GELU 3
+#define CCQ_ACT_GELU_TANH 4
+#define CCQ_ACT_SWIGLU 5
+size_t ccq_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int act);
+int ccq_linear_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, int bdtype,
+                   const void* r, int64_t ldr, void* y, void* z, void* workspace, int64_t M, int64_t N, int64_t K,
+                   int act, int dtype, void* stream);
+size_t ccq_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int act);
+int ccq_linear_bwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* z, const void* dy,
+                   int64_t ldy, void* dx, void* dw, void* db, int bdtype, void* workspace, int64_t M, int64_t N,
+                   int64_t K, int act, int dtype, void* stream);
+/* dst [rows, ldd] = src [rows, K] (16-bit elements, row stride ld, any address), zeros behind column K; ldd >= K a
+ * multiple of 8, dst 16-byte aligned. */
+int ccq_pad_rows(const void* src, int64_t ld, void* dst, int64_t ldd, int64_t rows, int64_t K, void* stream);
+
+/*
  * Kernel timing (measurement facility; no counterpart in the reference).  While enabled, each
  * entry point records a HIP event pair around every launch of its kernels on the caller's
  * stream.  ccq_timing_read waits for the recorded events of `kernel` (names: conv_fwd, conv_bwd,
  * gnorm_fwd, gnorm_bwd, clean_fwd_sum, clean_fwd, clean_bwd_rows, clean_bwd_dq, clean_bwd_gsum,
  * clean_bwd_dk, clean_bwd_gate, gdn_prep, gdn_fwd_state, gdn_fwd_o, gdn_bwd_state, gdn_bwd_dqkw,
  * gdn_bwd_wy, gla_intra, gla_fwd_state, gla_fwd_o, gla_bwd_state, gla_bwd_dv, gla_bwd_dqk,
- * clean_z_fwd, clean_z_bwd, narrow_fwd, narrow_bwd, norm_fwd, norm_bwd, logprobs_fwd, logprobs_bwd) and
- * returns the summed
+ * clean_z_fwd, clean_z_bwd, narrow_fwd, narrow_bwd, norm_fwd, norm_bwd, logprobs_fwd, logprobs_bwd,
+ * linear_fwd, linear_dz, linear_dx, linear_dw) and returns the summed
  * milliseconds and the number of launches since the last ccq_timing_reset.  ccq_timing_select
  * restricts the events to the kernel of that name (NULL: every kernel), so that a timed loop carries
  * one event pair per step instead of one per kernel.

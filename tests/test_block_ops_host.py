@@ -108,3 +108,63 @@ def test_token_logprobs_abi_refusals():
 
     assert bwd(V=65) == SHAPE and bwd(ent=None) == NULL and bwd(stats=None) == NULL and bwd(dx=None) == NULL
     assert bwd(dx=ODD) == ALIGN
+
+
+def test_fused_linear_refusals():
+    from ccq_amd import fused_linear
+    bf = torch.bfloat16
+    x, w = torch.zeros(4, 64, dtype=bf), torch.zeros(32, 64, dtype=bf)
+    with pytest.raises(RuntimeError, match="GPU"):
+        fused_linear(x, w)
+    with pytest.raises(TypeError, match="one type"):
+        fused_linear(x.float(), w.float())
+    with pytest.raises(TypeError, match="one type"):
+        fused_linear(x, w.half())
+    with pytest.raises(ValueError, match="activation"):
+        fused_linear(x, w, activation="tanh")
+    with pytest.raises(ValueError, match="weight"):
+        fused_linear(x, w[:, :32])
+    with pytest.raises(ValueError, match="weight"):
+        fused_linear(x, w[0])
+    with pytest.raises(ValueError, match="at least 1"):
+        fused_linear(x, w[:0])
+    with pytest.raises(ValueError, match="at least 1"):
+        fused_linear(x[:, :0], w[:, :0])
+    with pytest.raises(ValueError, match="up rows"):
+        fused_linear(x, w[:31], activation="swiglu")
+    with pytest.raises(ValueError, match="bias"):
+        fused_linear(x, w, torch.zeros(31, dtype=bf))
+    with pytest.raises(TypeError, match="bias"):
+        fused_linear(x, w, torch.zeros(32, dtype=torch.float16))
+    with pytest.raises(ValueError, match="residual"):
+        fused_linear(x, w, residual=torch.zeros(4, 16, dtype=bf))
+    with pytest.raises(ValueError, match="residual"):
+        fused_linear(x, w, residual=torch.zeros(1, 32, dtype=bf))
+    with pytest.raises(ValueError, match="residual"):
+        fused_linear(x, w, residual=torch.zeros(4, 32))
+
+
+def test_linear_abi_refusals():
+    lib = _lib.load()
+
+    def fwd(x=P, ldx=64, w=P, ldw=64, b=None, bd=0, r=None, ldr=32, y=P, z=None, ws=P, M=4, N=32, K=64, act=0, dt=0):
+        return lib.ccq_linear_fwd(x, ldx, w, ldw, b, bd, r, ldr, y, z, ws, M, N, K, act, dt, None)
+
+    assert fwd(N=0) == SHAPE and fwd(K=0) == SHAPE and fwd(M=-1) == SHAPE and fwd(ldx=60) == SHAPE
+    assert fwd(ldw=63) == SHAPE and fwd(ldx=68) == SHAPE and fwd(act=6) == SHAPE and fwd(dt=2) == SHAPE
+    assert fwd(bd=1) == SHAPE and fwd(r=P, ldr=31) == SHAPE and fwd(K=65) == SHAPE   # (rows of 65 need 72)
+    assert fwd(ldx=(1 << 22) + 8) == SHAPE
+    assert fwd(x=None) == NULL and fwd(w=None) == NULL and fwd(y=None) == NULL
+    assert fwd(x=ctypes.c_void_p(0x1008)) == ALIGN and fwd(y=ODD) == ALIGN and fwd(z=ODD) == ALIGN
+
+    def bwd(x=P, w=P, z=P, dy=P, ldy=32, dx=P, dw=P, db=None, ws=P, act=2):
+        return lib.ccq_linear_bwd(x, 64, w, 64, z, dy, ldy, dx, dw, db, 0, ws, 4, 32, 64, act, 0, None)
+
+    assert bwd(ldy=31) == SHAPE and bwd(ws=None) == NULL and bwd(z=None) == NULL and bwd(dy=None) == NULL
+    assert bwd(x=None) == NULL and bwd(w=None) == NULL and bwd(dx=ODD) == ALIGN and bwd(dy=ODD) == ALIGN
+    assert bwd(ws=ctypes.c_void_p(0x1008)) == ALIGN
+    assert lib.ccq_pad_rows(P, 5, P, 7, 3, 5, None) == SHAPE and lib.ccq_pad_rows(P, 5, P, 8, 3, 6, None) == SHAPE
+    assert lib.ccq_pad_rows(P, 5, ODD, 8, 3, 5, None) == ALIGN and lib.ccq_pad_rows(None, 5, P, 8, 3, 5, None) == NULL
+    # sizes of nothing: no rows, one output
+    assert lib.ccq_linear_workspace_bytes(0, 32, 64, 0) == 0
+    assert lib.ccq_linear_bwd_workspace_bytes(0, 32, 64, 0) >= 0 and lib.ccq_linear_bwd_workspace_bytes(1, 1, 1, 5) > 0
