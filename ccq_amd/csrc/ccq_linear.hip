@@ -18,15 +18,15 @@ namespace ccq {
 
 namespace {
 
-typedef f16 f16x8 __attribute__((ext_vector_type(8)));
-
+// c += a b on the matrix cores, the accumulator kept where it is: left to itself the register allocator moves the 256
+// accumulator registers of a wave about between the products.  What the compiler does not know of an instruction
+// written like this -- that its result may be read by others only after its passes -- is waited for by acc_settled.
 template <typename T>
-__device__ __forceinline__ f32x4 product16(const s16x8& a, const s16x8& b, const f32x4& c) {
-  if constexpr (__is_same(T, bf16))
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+__device__ __forceinline__ void product16(const s16x8& a, const s16x8& b, f32x4& c) {
+  if constexpr (__is_same(T, bf16)) asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  else asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
+__device__ __forceinline__ void acc_settled() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
 // activations, in fp32
@@ -99,9 +99,8 @@ __device__ __forceinline__ void add_row(const T* row, long n, long N, float (&v)
 }
 
 // The epilogue of C consecutive columns n .. of row m (swiglu: v the gates, up the other half).
-template <typename T, int C>
+template <typename T, int C, bool glu>
 __device__ __forceinline__ void finish(const ProductArgs& p, long m, long n, float (&v)[C], float (&up)[C]) {
-  const bool glu = p.act == kActSwiglu;
   if (p.bias) {
 #pragma unroll
     for (int i = 0; i < C; ++i)
@@ -142,11 +141,14 @@ struct Operand {
   long left;         // bytes from there to the operand's end
 };
 __device__ __forceinline__ u32x4 resource(const Operand& o) {
-  const unsigned n = o.left <= 0 ? 0u : o.left > 0x7fffffffL ? 0x7fffffffu : (unsigned)o.left;
+  // (by words: a 64-bit comparison would leave the scalar unit, and a resource has to come from there)
+  const int hi = (int)(o.left >> 32);
+  const unsigned lo = (unsigned)o.left;
+  const unsigned n = hi < 0 ? 0u : hi > 0 ? 0x7fffffffu : lo > 0x7fffffffu ? 0x7fffffffu : lo;
   return u32x4{(unsigned)(size_t)o.base, (unsigned)((size_t)o.base >> 32) & 0xffffu, n, 0x00020000u};
 }
 __device__ __forceinline__ void load_piece_lds(const u32x4& r, unsigned off, unsigned m0) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(off), "s"(r) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(off), "s"(r) : "memory", "m0");
 }
 constexpr unsigned kNowhere = 0x80000000u;  // behind every resource's end
 
@@ -176,18 +178,14 @@ struct TileLoad {
       }
     }
   }
-  // contraction elements at and behind `limit` of this step (limit < 64: the last one) as zeros
-  __device__ void issue(const Operand& o, unsigned stage, int limit, int wave, int l) const {
-    const u32x4 r = resource(o);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      unsigned f = off[i];
-      if (!DOWN && limit < kStep) {
-        const int q = (wave * PER + i) * 64 + l, row = q >> 3;
-        if ((((q & 7) ^ (B ? swz_b(row) : swz_a(row))) << 3) >= limit) f = kNowhere;
-      }
-      load_piece_lds(r, f, lds + stage + i * 1024);
+  // instruction i of the step at `stage` (bytes); `limit` < 64: contraction elements from there on as zeros
+  __device__ void issue(const u32x4& r, int i, unsigned stage, int limit, int wave, int l) const {
+    unsigned f = off[i];
+    if (!DOWN && limit < kStep) {
+      const int q = (wave * PER + i) * 64 + l, row = q >> 3;
+      if ((((q & 7) ^ (B ? swz_b(row) : swz_a(row))) << 3) >= limit) f = kNowhere;
     }
+    load_piece_lds(r, f, lds + stage + i * 1024);
   }
 };
 
@@ -204,13 +202,22 @@ enum : int { kPlain = 0, kEpilogue = 1, kPartial = 2 };
 // BM x BN tile of the product by WM x WN waves, two stages of LDS.  Lane l of a wave holds, of each 16x16 tile
 // (it, j) of the wave, row m = 16 it + (l & 15) and four consecutive columns.  Along-the-row B operands (the forward)
 // are read so that the column tiles j = 2 q and 2 q + 1 of a lane are eight consecutive columns, one 16-byte store.
-// swiglu: the wave's columns are 32 gates and the 32 ups beside them, so a lane holds both.
+// swiglu: half of a wave's columns are gates, the other half the ups beside them, so a lane holds both.
+//
+// A step of 64 contraction elements is two halves of 32.  While the matrix cores work on one half's fragments the
+// other half's are read from LDS into registers, a fragment of each operand and one direct load of the step after
+// next between two rows of products; the one barrier of a step lies between the halves, where every wave has read
+// the current stage (the loads may overwrite it) and the next stage has landed.
 template <typename T, int BM, int BN, int WM, int WN, bool DA, bool DB, int MODE, bool GLU>
 __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs p) {
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr unsigned kA = BM * kStep * 2, kStage = kA + BN * kStep * 2;
-  static_assert(!GLU || (BN / WN == 64 && !DB && MODE == kEpilogue), "gates and ups of one wave");
-  __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
+  constexpr int HALF = BN / WN / 2;  // swiglu: gates of a wave
+  static_assert(!GLU || (!DB && MODE == kEpilogue), "gates and ups of one wave");
+  static_assert(TM == TN, "one fragment of each operand between two rows of products");
+  constexpr int kPass = 64, kRow = TN * 16 + 4;  // rows of a wave in the epilogue at a time, floats a row
+  constexpr unsigned kOut = NW * kPass * kRow * 4;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * kStage > kOut ? 2 * kStage : kOut];
   const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
   constexpr int NT = GLU ? BN / 2 : BN;  // output columns of a tile
@@ -221,59 +228,54 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
   const int t = xcd * q8 + min(xcd, r8) + (blockIdx.x >> 3);
   const int band = t / (8 * tn), in = t - band * 8 * tn, rows = min(8, tm - band * 8);
   const long m0 = (long)(band * 8 + in % rows) * BM, n0 = (long)(in / rows) * NT;
-  // steps of this workgroup
+  // steps of this workgroup: whole ones, and the contraction's end
   const int all = (int)((p.K + kStep - 1) / kStep), per = (all + p.splits - 1) / p.splits;
   const int s0 = blockIdx.y * per, s1 = min(all, s0 + per);
+  const int tail = (!DA || !DB) && s1 == all && s0 < s1 ? (int)(p.K & (kStep - 1)) : 0;  // (down both: zeros by the end)
+  const int whole = max(0, s1 - s0 - (tail ? 1 : 0));
 
   const unsigned lds0 = lds_addr(smem);
-  TileLoad<BM, DA, false, NW> la;
-  TileLoad<BN, DB, !DB, NW> lb;
+  typedef TileLoad<BM, DA, false, NW> LoadA;
+  typedef TileLoad<BN, DB, !DB, NW> LoadB;
+  static_assert(LoadA::PER == TM && LoadB::PER == TN, "one load of each operand between two rows of products");
+  LoadA la;
+  LoadB lb;
   la.init(lds0, wave, l, p.lda);
   lb.init(lds0 + kA, wave, l, p.ldb);
-  // elements of the operands: to the end of the last row's last whole piece
-  const long nb = GLU ? 2 * p.N : p.N;
-  const long ea = ((DA ? p.K : p.M) - 1) * p.lda + (((DA ? p.M : p.K) + 7) & ~7L);
-  const long eb = ((DB ? p.K : nb) - 1) * p.ldb + (((DB ? nb : p.K) + 7) & ~7L);
-  Operand oa, ob, ou;
+  Operand oa, ob;
   {
+    // elements of the operands: to the end of the last row's last whole piece
+    const long nb = GLU ? 2 * p.N : p.N;
+    const long ea = ((DA ? p.K : p.M) - 1) * p.lda + (((DA ? p.M : p.K) + 7) & ~7L);
+    const long eb = ((DB ? p.K : nb) - 1) * p.ldb + (((DB ? nb : p.K) + 7) & ~7L);
     const long fa = DA ? (long)s0 * kStep * p.lda + m0 : m0 * p.lda + (long)s0 * kStep;
     oa = {(const char*)p.a + fa * 2, (ea - fa) * 2};
-    const long fb = DB ? (long)s0 * kStep * p.ldb + n0 : n0 * p.ldb + (long)s0 * kStep;
-    ob = {(const char*)p.b + fb * 2, (eb - fb) * 2};
-    const long fu = fb + p.N * p.ldb;
-    ou = {(const char*)p.b + fu * 2, (eb - fu) * 2};
-  }
-  if constexpr (GLU) {
-    // tile row 64 w + c of B: gate n0 + 32 w + c for c < 32, up n0 + 32 w + c - 32 behind
+    long fb = DB ? (long)s0 * kStep * p.ldb + n0 : n0 * p.ldb + (long)s0 * kStep;
+    if constexpr (GLU) {
+      // tile row 2 HALF w + c of B: gate n0 + HALF w + c for c < HALF, up n0 + HALF w + c - HALF behind
+      static_assert(LoadB::PER * 8 == HALF, "a wave loads gates or ups");
+      if (wave & 1) fb += p.N * p.ldb;
 #pragma unroll
-    for (int i = 0; i < lb.PER; ++i) {
-      const int r = ((wave * lb.PER + i) * 64 + l) >> 3, s = l & 7;
-      lb.off[i] = (unsigned)(((r >> 6) * 32 + (r & 31)) * p.ldb * 2) + ((s ^ swz_b(r)) << 4);
+      for (int i = 0; i < LoadB::PER; ++i) {
+        const int r = ((wave * LoadB::PER + i) * 64 + l) >> 3;
+        lb.off[i] = (unsigned)((r / (2 * HALF) * HALF + r % HALF) * p.ldb * 2) + (((l & 7) ^ swz_b(r)) << 4);
+      }
     }
+    ob = {(const char*)p.b + fb * 2, (eb - fb) * 2};
   }
   const long stepA = (DA ? kStep * p.lda : kStep) * 2, stepB = (DB ? kStep * p.ldb : kStep) * 2;
-  auto issue = [&](int s, unsigned stage) {
-    const int limit = (int)min((long)kStep, p.K - (long)s * kStep);
-    la.issue(oa, stage, limit, wave, l);
-    if constexpr (GLU) {
-      const u32x4 rg = resource(ob), ru = resource(ou);
-#pragma unroll
-      for (int i = 0; i < lb.PER; ++i) {
-        const int row = (wave * lb.PER + i) * 8;  // (uniform; 8 rows never straddle the halves)
-        unsigned f = lb.off[i];
-        const int r = row + (l >> 3);
-        if (limit < kStep && (((l & 7) ^ swz_b(r)) << 3) >= limit) f = kNowhere;
-        load_piece_lds((row & 32) ? ru : rg, f, lb.lds + stage + i * 1024);
-      }
-      ou.base += stepB;
-      ou.left -= stepB;
-    } else {
-      lb.issue(ob, stage, limit, wave, l);
+  int ahead = whole;  // whole steps not yet asked for; behind them the loads bring zeros, which nothing reads
+  u32x4 ra, rb;
+  auto next = [&] {
+    ra = resource(ahead > 0 ? oa : Operand{oa.base, 0});
+    rb = resource(ahead > 0 ? ob : Operand{ob.base, 0});
+    if (ahead > 0) {
+      oa.base += stepA;
+      oa.left -= stepA;
+      ob.base += stepB;
+      ob.left -= stepB;
     }
-    oa.base += stepA;
-    oa.left -= stepA;
-    ob.base += stepB;
-    ob.left -= stepB;
+    --ahead;
   };
 
   // fragment addresses of this lane in stage 0
@@ -299,86 +301,153 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) fb[kk] = lds0 + kA + row * 128 + (((4 * kk + g) ^ swz_b(row)) << 4);
   }
+  auto read_a = [&](int it, unsigned stage, int kk) -> s16x8 {
+    if constexpr (DA) {
+      const unsigned at = fa[it] + stage + kk * 32 * BM * 2;
+      return __builtin_shufflevector(read_tr4(at), read_tr4(at + 4 * BM * 2), 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      return read16(fa[kk] + stage + it * 16 * 128);
+    }
+  };
+  auto read_b = [&](int j, unsigned stage, int kk) -> s16x8 {
+    if constexpr (DB) {
+      const unsigned at = fb[j] + stage + kk * 32 * BN * 2;
+      return __builtin_shufflevector(read_tr4(at), read_tr4(at + 4 * BN * 2), 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      return read16(fb[kk] + stage + (32 * (j >> 1) + 4 * (j & 1)) * 128);
+    }
+  };
 
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int it = 0; it < TM; ++it)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[it][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < TN; ++j) {
+      acc[it][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      asm volatile("" : "+a"(acc[it][j]));
+    }
+  acc_settled();
+  s16x8 a0[TM], b0[TN], a1[TM], b1[TN];  // fragments of the two halves
 
-  if (s0 < s1) issue(s0, 0);
-  unsigned stage = 0;
-  for (int s = s0; s < s1; ++s) {
-    wait_loads<0>();
-    lds_barrier();  // this step's tiles are in LDS, and every wave has read the last step's
-    if (s + 1 < s1) issue(s + 1, stage ^ kStage);
+  if (whole > 0) {
+    next();
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      s16x8 a[TM], b[TN];
+    for (int i = 0; i < TM; ++i) {
+      la.issue(ra, i, 0, kStep, wave, l);
+      lb.issue(rb, i, 0, kStep, wave, l);
+    }
+    next();
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      la.issue(ra, i, kStage, kStep, wave, l);
+      lb.issue(rb, i, kStage, kStep, wave, l);
+    }
+    wait_loads<TM + TN>();
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      b0[i] = read_b(i, 0, 0);
+      a0[i] = read_a(i, 0, 0);
+    }
+    unsigned stage = 0;
+    for (int s = 0; s < whole; ++s) {
 #pragma unroll
       for (int it = 0; it < TM; ++it) {
-        if constexpr (DA) {
-          const unsigned at = fa[it] + stage + kk * 32 * BM * 2;
-          const s16x4_t x = read_tr4(at), y = read_tr4(at + 4 * BM * 2);
-          a[it] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-        } else {
-          a[it] = read16(fa[kk] + stage + it * 16 * 128);
+        if (it < TM / 2) {
+          b1[2 * it] = read_b(2 * it, stage, 1);
+          b1[2 * it + 1] = read_b(2 * it + 1, stage, 1);
+          a1[2 * it] = read_a(2 * it, stage, 1);
+          a1[2 * it + 1] = read_a(2 * it + 1, stage, 1);
         }
-      }
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        if constexpr (DB) {
-          const unsigned at = fb[j] + stage + kk * 32 * BN * 2;
-          const s16x4_t x = read_tr4(at), y = read_tr4(at + 4 * BN * 2);
-          b[j] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-        } else {
-          b[j] = read16(fb[kk] + stage + (32 * (j >> 1) + 4 * (j & 1)) * 128);
+        for (int j = 0; j < TN; ++j) product16<T>(b0[j], a0[it], acc[it][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      wait_loads<0>();
+      lds_barrier();  // this stage is read, the next one has landed
+      next();
+#pragma unroll
+      for (int it = 0; it < TM; ++it) {
+        la.issue(ra, it, stage, kStep, wave, l);
+        lb.issue(rb, it, stage, kStep, wave, l);
+        if (it < TM / 2) {
+          b0[2 * it] = read_b(2 * it, stage ^ kStage, 0);
+          b0[2 * it + 1] = read_b(2 * it + 1, stage ^ kStage, 0);
+          a0[2 * it] = read_a(2 * it, stage ^ kStage, 0);
+          a0[2 * it + 1] = read_a(2 * it + 1, stage ^ kStage, 0);
         }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) product16<T>(b1[j], a1[it], acc[it][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      stage ^= kStage;
+    }
+    wait_loads<0>();  // (the last steps' zeros)
+    lds_barrier();
+  }
+  if (tail) {
+    ahead = 1;
+    next();
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      la.issue(ra, i, 0, tail, wave, l);
+      lb.issue(rb, i, 0, tail, wave, l);
+    }
+    wait_loads<0>();
+    lds_barrier();
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        a0[i] = read_a(i, 0, kk);
+        b0[i] = read_b(i, 0, kk);
       }
 #pragma unroll
       for (int it = 0; it < TM; ++it)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[it][j] = product16<T>(b[j], a[it], acc[it][j]);
+        for (int j = 0; j < TN; ++j) product16<T>(b0[j], a0[it], acc[it][j]);
     }
-    stage ^= kStage;
-    asm volatile("" ::: "memory");
   }
 
+  // The epilogue, 64 rows of a wave at a time: through LDS (its own part, rows 16 bytes apart in the banks), so that a
+  // lane takes eight consecutive columns of a row whatever the fragments' order was, and its code exists once or twice
+  // rather than once for every tile of the wave.
+  acc_settled();
+  lds_barrier();
+  float* mine = (float*)(smem + wave * kPass * kRow * 4);
 #pragma unroll
-  for (int it = 0; it < TM; ++it) {
-    const long m = m0 + wm * TM * 16 + it * 16 + r;
-    if (m >= p.M) continue;
-    if constexpr (GLU) {
-      const long n = n0 + wn * 32 + 8 * g;
+  for (int h = 0; h < TM / 4; ++h) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        *(f32x4*)(mine + (16 * i + r) * kRow + (DB ? 16 * j + 4 * g : 32 * (j >> 1) + 4 * (j & 1) + 8 * g)) = acc[4 * h + i][j];
+    __builtin_amdgcn_wave_barrier();  // (LDS operations of a wave are in order)
+    constexpr int WC = GLU ? HALF : TN * 16, PR = WC / 8;  // output columns of the wave, pieces of a row
+    const int c = l % PR * 8;
+    const long n = n0 + wn * WC + c;
+    for (int i = l / PR; i < kPass; i += 64 / PR) {
+      const long m = m0 + wm * TM * 16 + h * kPass + i;
+      if (m >= p.M || n >= p.N) continue;
       float v[8], up[8];
+      const float* row = mine + i * kRow + c;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = acc[it][i >> 2][i & 3];
-        up[i] = acc[it][2 + (i >> 2)][i & 3];
+      for (int e = 0; e < 8; e += 4) {
+        *(f32x4*)(v + e) = *(const f32x4*)(row + e);
+        if (GLU) *(f32x4*)(up + e) = *(const f32x4*)(row + HALF + e);
       }
-      if (n < p.N) finish<T, 8>(p, m, n, v, up);
-    } else {
-      constexpr int C = DB ? 4 : 8;  // consecutive columns a lane
-#pragma unroll
-      for (int c = 0; c < TN * 4 / C; ++c) {
-        const long n = n0 + wn * TN * 16 + (DB ? 16 * c + 4 * g : 32 * c + 8 * g);
-        if (n >= p.N) continue;
-        float v[C];
-#pragma unroll
-        for (int i = 0; i < C; ++i) v[i] = acc[it][(c * C + i) / 4][i & 3];
-        if constexpr (MODE == kEpilogue) finish<T, C>(p, m, n, v, v);
-        else if constexpr (MODE == kPlain) store_row<T, C>((T*)p.out + m * p.ldo, n, p.N, v);
-        else store_row<float, C>(p.part + ((long)blockIdx.y * p.M + m) * p.N, n, p.N, v);
-      }
+      if constexpr (MODE == kEpilogue) finish<T, 8, GLU>(p, m, n, v, up);
+      else if constexpr (MODE == kPlain) store_row<T, 8>((T*)p.out + m * p.ldo, n, p.N, v);
+      else store_row<float, 8>(p.part + ((long)blockIdx.y * p.M + m) * p.N, n, p.N, v);
     }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
 // the parts of the contraction added in their order, then the epilogue
-template <typename T>
+template <typename T, bool glu>
 __global__ __launch_bounds__(kThreads) void join_kernel(const ProductArgs p) {
   constexpr int C = 4;
-  const bool glu = p.act == kActSwiglu;
   const long cols = glu ? 2 * p.N : p.N, groups = (p.N + C - 1) / C;
   const long at = (long)blockIdx.x * kThreads + threadIdx.x;
   if (at >= p.M * groups) return;
@@ -391,7 +460,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const ProductArgs p) {
     add_row<float, C>(row, n, p.N, v);
     if (glu) add_row<float, C>(row + p.N, n, p.N, up);
   }
-  finish<T, C>(p, m, n, v, up);
+  finish<T, C, glu>(p, m, n, v, up);
 }
 
 // ---------------------------------------------------------------------------
@@ -489,7 +558,7 @@ hipError_t launch_tiles(const ProductArgs& p, hipStream_t st) {
 
 template <typename T, bool DA, bool DB, int MODE, bool GLU>
 hipError_t launch_size(const ProductArgs& p, bool large, hipStream_t st) {
-  if (large) return launch_tiles<T, 256, 256, 2, 4, DA, DB, MODE, GLU>(p, st);
+  if (large) return launch_tiles<T, 256, 256, 2, 2, DA, DB, MODE, GLU>(p, st);
   return launch_tiles<T, 128, 128, 2, 2, DA, DB, MODE, GLU>(p, st);
 }
 
@@ -504,7 +573,9 @@ hipError_t launch_typed(int kind, const ProductArgs& p, bool large, hipStream_t 
                                      : launch_size<T, true, true, kPartial, false>(q, large, st);
     if (e != hipSuccess) return e;
     const long threads = p.M * ((p.N + 3) / 4);
-    hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0, st, p);
+    const dim3 grid((unsigned)((threads + kThreads - 1) / kThreads));
+    if (p.act == kActSwiglu) hipLaunchKernelGGL((join_kernel<T, true>), grid, dim3(kThreads), 0, st, p);
+    else hipLaunchKernelGGL((join_kernel<T, false>), grid, dim3(kThreads), 0, st, p);
     return hipGetLastError();
   }
   if (kind == 0)
