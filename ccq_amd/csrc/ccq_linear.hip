@@ -205,8 +205,8 @@ enum : int { kPlain = 0, kEpilogue = 1, kPartial = 2 };
 // swiglu: half of a wave's columns are gates, the other half the ups beside them, so a lane holds both.
 //
 // A step of 64 contraction elements is two halves of 32.  While the matrix cores work on one half's fragments the
-// other half's are read from LDS into registers, a fragment of each operand and one direct load of the step after
-// next between two rows of products; the one barrier of a step lies between the halves, where every wave has read
+// other half's are read from LDS into registers and the direct loads of the step after next are issued, each
+// between two products (in clumps they keep the one wave of a SIMD from issuing products); the one barrier of a step lies between the halves, where every wave has read
 // the current stage (the loads may overwrite it) and the next stage has landed.
 template <typename T, int BM, int BN, int WM, int WN, bool DA, bool DB, int MODE, bool GLU>
 __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs p) {
@@ -264,18 +264,26 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     ob = {(const char*)p.b + fb * 2, (eb - fb) * 2};
   }
   const long stepA = (DA ? kStep * p.lda : kStep) * 2, stepB = (DB ? kStep * p.ldb : kStep) * 2;
-  int ahead = whole;  // whole steps not yet asked for; behind them the loads bring zeros, which nothing reads
+  // Rows of an operand that lie a multiple of 4 KiB apart meet in one channel of the L2 at any one step.  So the tile
+  // rows of a band begin their contraction at different steps, 256 bytes apart, and come round to them at its end;
+  // those of one tile row keep together and find its operand in the L2.  (8192^3 forward: 849 -> 788 us; contractions
+  // of few steps gain nothing and lose the operands' meeting in the L2: 16384 x 5632 over 1024, 187 -> 193 us.)
+  const int turn = BM == 256 && whole >= 32 ? 2 * (int)(in % rows) : 0;
+  int ahead = whole, until = whole - turn;  // steps not yet asked for, steps to the end of the whole ones
+  const long wrapA = whole * stepA, wrapB = whole * stepB;
+  const Operand ta = {oa.base + wrapA, oa.left - wrapA}, tb = {ob.base + wrapB, ob.left - wrapB};  // the end's
+  oa = {oa.base + turn * stepA, oa.left - turn * stepA};
+  ob = {ob.base + turn * stepB, ob.left - turn * stepB};
   u32x4 ra, rb;
-  auto next = [&] {
-    ra = resource(ahead > 0 ? oa : Operand{oa.base, 0});
-    rb = resource(ahead > 0 ? ob : Operand{ob.base, 0});
-    if (ahead > 0) {
-      oa.base += stepA;
-      oa.left -= stepA;
-      ob.base += stepB;
-      ob.left -= stepB;
-    }
+  auto next = [&] {  // (selects, no branch: it runs between two products; behind the last step loads bring zeros)
+    const bool on = ahead > 0;
+    ra = resource({oa.base, on ? oa.left : 0});
+    rb = resource({ob.base, on ? ob.left : 0});
     --ahead;
+    --until;
+    const long da = stepA - (until == 0 ? wrapA : 0), db = stepB - (until == 0 ? wrapB : 0);
+    oa = {oa.base + da, oa.left - da};
+    ob = {ob.base + db, ob.left - db};
   };
 
   // fragment addresses of this lane in stage 0
@@ -318,15 +326,27 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     }
   };
 
+  // fragment k of a half in the order that its products need them: a[0], b[0..], a[1..]
+  auto read = [&](s16x8(&a)[TM], s16x8(&b)[TN], int k, unsigned stage, int kk) {
+    if (k == 0) a[0] = read_a(0, stage, kk);
+    else if (k <= TN) b[k - 1] = read_b(k - 1, stage, kk);
+    else a[k - TN] = read_a(k - TN, stage, kk);
+  };
+  // products between two loads, and between two fragment reads: the reads end at three quarters of the half, so that
+  // the last ones have arrived by its end
+  constexpr int kLoadGap = TM * TN / (TM + TN), kReadGap = TM * TN * 3 / 4 / (TM + TN);
+
   f32x4 acc[TM][TN];
+  auto clear = [&] {
 #pragma unroll
-  for (int it = 0; it < TM; ++it)
+    for (int it = 0; it < TM; ++it)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      acc[it][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      asm volatile("" : "+a"(acc[it][j]));
-    }
-  acc_settled();
+      for (int j = 0; j < TN; ++j) {
+        acc[it][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        asm volatile("" : "+a"(acc[it][j]));
+      }
+    acc_settled();
+  };
   s16x8 a0[TM], b0[TN], a1[TM], b1[TN];  // fragments of the two halves
 
   if (whole > 0) {
@@ -342,6 +362,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
       la.issue(ra, i, kStage, kStep, wave, l);
       lb.issue(rb, i, kStage, kStep, wave, l);
     }
+    clear();  // (while the first loads are on their way)
     wait_loads<TM + TN>();
     lds_barrier();
 #pragma unroll
@@ -352,42 +373,34 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     unsigned stage = 0;
     for (int s = 0; s < whole; ++s) {
 #pragma unroll
-      for (int it = 0; it < TM; ++it) {
-        if (it < TM / 2) {
-          b1[2 * it] = read_b(2 * it, stage, 1);
-          b1[2 * it + 1] = read_b(2 * it + 1, stage, 1);
-          a1[2 * it] = read_a(2 * it, stage, 1);
-          a1[2 * it + 1] = read_a(2 * it + 1, stage, 1);
-        }
-#pragma unroll
-        for (int j = 0; j < TN; ++j) product16<T>(b0[j], a0[it], acc[it][j]);
+      for (int q = 0; q < TM * TN; ++q) {
+        product16<T>(b0[q % TN], a0[q / TN], acc[q / TN][q % TN]);
+        if (q == 0) next();
+        if (q % kReadGap == kReadGap - 1 && q / kReadGap < TM + TN) read(a1, b1, q / kReadGap, stage, 1);
         __builtin_amdgcn_sched_barrier(0);
       }
       wait_loads<0>();
       lds_barrier();  // this stage is read, the next one has landed
-      next();
 #pragma unroll
-      for (int it = 0; it < TM; ++it) {
-        la.issue(ra, it, stage, kStep, wave, l);
-        lb.issue(rb, it, stage, kStep, wave, l);
-        if (it < TM / 2) {
-          b0[2 * it] = read_b(2 * it, stage ^ kStage, 0);
-          b0[2 * it + 1] = read_b(2 * it + 1, stage ^ kStage, 0);
-          a0[2 * it] = read_a(2 * it, stage ^ kStage, 0);
-          a0[2 * it + 1] = read_a(2 * it + 1, stage ^ kStage, 0);
+      for (int q = 0; q < TM * TN; ++q) {
+        product16<T>(b1[q % TN], a1[q / TN], acc[q / TN][q % TN]);
+        if (q % kLoadGap == 0) {
+          if (q / kLoadGap % 2) lb.issue(rb, q / kLoadGap / 2, stage, kStep, wave, l);
+          else la.issue(ra, q / kLoadGap / 2, stage, kStep, wave, l);
         }
-#pragma unroll
-        for (int j = 0; j < TN; ++j) product16<T>(b1[j], a1[it], acc[it][j]);
+        if (q % kReadGap == kReadGap - 1 && q / kReadGap < TM + TN) read(a0, b0, q / kReadGap, stage ^ kStage, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
       stage ^= kStage;
     }
     wait_loads<0>();  // (the last steps' zeros)
     lds_barrier();
+  } else {
+    clear();
   }
   if (tail) {
-    ahead = 1;
-    next();
+    ra = resource(ta);
+    rb = resource(tb);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       la.issue(ra, i, 0, tail, wave, l);
