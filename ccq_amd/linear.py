@@ -13,9 +13,8 @@ from typing import Optional
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib
-from ._lib import call, ptr, stream_of
-from ._rows import DTYPES, needs_grad, on_device, require_gpu, require_like, rows_of, stride_of
+from ._rows import (DTYPES, address, call, current, entry, needs_grad, require_gpu, require_on, rows_of, stream_on,
+                    stride_of)
 
 __all__ = ["fused_linear", "FusedLinearFunction", "ACTIVATIONS"]
 
@@ -26,14 +25,14 @@ MAX_STRIDE = 1 << 22
 
 def _operand(x2: torch.Tensor) -> torch.Tensor:
     """Rows as the products read them: 16-byte pieces, zeros up to a multiple of 8 columns.  A copy where x2's width,
-    stride or address does not allow that (on the current device)."""
+    stride or address does not allow that."""
     rows, K = x2.shape
     ld = stride_of(x2)
     if K % 8 == 0 and ld % 8 == 0 and ld <= MAX_STRIDE and x2.data_ptr() % 16 == 0:
         return x2
     ldd = -(-K // 8) * 8
     out = torch.empty(rows, ldd, device=x2.device, dtype=x2.dtype)
-    call("ccq_pad_rows", ptr(x2), ld, ptr(out), ldd, rows, K, stream_of(x2))
+    call("ccq_pad_rows", x2.data_ptr(), ld, out.data_ptr(), ldd, rows, K, stream_on(x2))
     return out
 
 
@@ -45,13 +44,12 @@ def _forward(x, weight, bias, residual, act, keep_z):
     dev = x.device
     y = torch.empty(*x.shape[:-1], N, device=dev, dtype=x.dtype)
     z = torch.empty(M, -(-outs // 8) * 8, device=dev, dtype=x.dtype) if keep_z and act else None
-    with on_device(x):
-        xp, wp = _operand(x2), _operand(w2)
-        n = _lib.load().ccq_linear_workspace_bytes(M, N, K, act)
-        ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
-        call("ccq_linear_fwd", ptr(xp), stride_of(xp), ptr(wp), stride_of(wp), ptr(bias),
-             DTYPES[bias.dtype if bias is not None else x.dtype], ptr(r2), stride_of(r2) if r2 is not None else 0,
-             ptr(y), ptr(z), ptr(ws), M, N, K, act, DTYPES[x.dtype], stream_of(x))
+    xp, wp = _operand(x2), _operand(w2)
+    n = entry("ccq_linear_workspace_bytes")(M, N, K, act)
+    ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
+    call("ccq_linear_fwd", xp.data_ptr(), stride_of(xp), wp.data_ptr(), stride_of(wp), address(bias),
+         DTYPES[bias.dtype if bias is not None else x.dtype], address(r2), stride_of(r2) if r2 is not None else 0,
+         y.data_ptr(), address(z), address(ws), M, N, K, act, DTYPES[x.dtype], stream_on(x))
     return y, z, x2, w2
 
 
@@ -60,34 +58,38 @@ class FusedLinearFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act):
         y, z, x2, w2 = _forward(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x2, w2, z)
-        ctx.meta = (x.shape, y.shape, act, None if bias is None else bias.dtype)
+        ctx.meta = (x.shape, y.shape[-1], act, None if bias is None else bias.dtype)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x2, w2, z = ctx.saved_tensors
-        shape, yshape, act, bdtype = ctx.meta
+        saved = ctx.saved_tensors
+        if not current(saved[0]):
+            with torch.cuda.device(saved[0].device):
+                return FusedLinearFunction._backward(ctx, *saved, dy)
+        return FusedLinearFunction._backward(ctx, *saved, dy)
+
+    @staticmethod
+    def _backward(ctx, x2, w2, z, dy):
+        shape, N, act, bdtype = ctx.meta
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dx = dw = db = None
         if need_x or need_w or need_b:
             (M, K), outs = x2.shape, w2.shape[0]
-            N = yshape[-1]
             dev, dtype = x2.device, x2.dtype
             d2 = rows_of(dy)
             dx = torch.empty(shape, device=dev, dtype=dtype) if need_x else None
             dw = torch.empty(outs, K, device=dev, dtype=dtype) if need_w else None
             db = torch.empty(outs, device=dev, dtype=bdtype) if need_b else None
-            with on_device(x2):
-                xp = _operand(x2) if need_w else None
-                wp = _operand(w2) if need_x else None
-                ld = -(-K // 8) * 8
-                ws = torch.empty(_lib.load().ccq_linear_bwd_workspace_bytes(M, N, K, act), device=dev,
-                                 dtype=torch.uint8)
-                call("ccq_linear_bwd", ptr(xp), stride_of(xp) if need_w else ld, ptr(wp),
-                     stride_of(wp) if need_x else ld, ptr(z), ptr(d2), stride_of(d2), ptr(dx), ptr(dw), ptr(db),
-                     DTYPES[bdtype if bdtype is not None else dtype], ptr(ws), M, N, K, act, DTYPES[dtype],
-                     stream_of(x2))
+            xp = _operand(x2) if need_w else None
+            wp = _operand(w2) if need_x else None
+            ld = -(-K // 8) * 8
+            ws = torch.empty(entry("ccq_linear_bwd_workspace_bytes")(M, N, K, act), device=dev, dtype=torch.uint8)
+            call("ccq_linear_bwd", address(xp), stride_of(xp) if need_w else ld, address(wp),
+                 stride_of(wp) if need_x else ld, address(z), d2.data_ptr(), stride_of(d2), address(dx), address(dw),
+                 address(db), DTYPES[bdtype if bdtype is not None else dtype], ws.data_ptr(), M, N, K, act,
+                 DTYPES[dtype], stream_on(x2))
         return dx, dw, db, dy if need_r else None, None
 
 
@@ -113,7 +115,9 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     outs = weight.shape[0]
     if act == SWIGLU and outs % 2:
         raise ValueError(f"fused_linear: swiglu needs as many gate as up rows (weight has {outs})")
-    require_like("fused_linear", x, weight=weight, bias=bias, residual=residual)
+    require_on("fused_linear", "weight", weight, x)
+    require_on("fused_linear", "bias", bias, x)
+    require_on("fused_linear", "residual", residual, x)
     if bias is not None:
         if bias.shape != (outs,):
             raise ValueError(f"fused_linear: bias {tuple(bias.shape)}: expected [{outs}]")
@@ -124,6 +128,9 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         raise ValueError(f"fused_linear: residual {tuple(residual.shape)} {residual.dtype}: expected "
                          f"{(*x.shape[:-1], N)} {x.dtype}")
     require_gpu("fused_linear", x)
+    if not current(x):
+        with torch.cuda.device(x.device):
+            return fused_linear(x, weight, bias, activation, residual)
     bias = bias if bias is None else bias.contiguous()
     if needs_grad(x, weight, bias, residual):
         return FusedLinearFunction.apply(x, weight, bias, residual, act)

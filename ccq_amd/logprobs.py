@@ -12,8 +12,8 @@ from typing import NamedTuple, Optional
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import call, ptr, stream_of
-from ._rows import DTYPES, needs_grad, on_device, require_gpu, require_like, rows_of, stride_of
+from ._rows import (DTYPES, address, call, current, needs_grad, require_gpu, require_on, rows_of, stream_on,
+                    stride_of)
 
 __all__ = ["token_logprobs", "TokenLogprobs", "TokenLogprobsFunction"]
 
@@ -39,9 +39,8 @@ def _forward(logits, ids, k, ignore, keep):
     stats = torch.empty(rows, 2, device=dev, dtype=torch.float32) if keep else None
     top = torch.empty(*ids.shape, k, device=dev, dtype=torch.float32) if k else None
     top_ids = torch.empty(*ids.shape, k, device=dev, dtype=torch.int64) if k else None
-    with on_device(logits):
-        call("ccq_token_logprobs_fwd", ptr(x2), stride_of(x2), ptr(i2), ptr(logp), ptr(ent), ptr(stats), ptr(top),
-             ptr(top_ids), rows, V, k, ignore, DTYPES[logits.dtype], stream_of(logits))
+    call("ccq_token_logprobs_fwd", x2.data_ptr(), stride_of(x2), i2.data_ptr(), logp.data_ptr(), ent.data_ptr(),
+         address(stats), address(top), address(top_ids), rows, V, k, ignore, DTYPES[logits.dtype], stream_on(logits))
     return logp, ent, top, top_ids, x2, i2, stats
 
 
@@ -61,14 +60,21 @@ class TokenLogprobsFunction(torch.autograd.Function):
     def backward(ctx, dlogp, dent, _top=None, _top_ids=None):
         if dlogp is None and dent is None:
             return None, None, None, None
-        x2, i2, ent, stats = ctx.saved_tensors
+        saved = ctx.saved_tensors
+        if not current(saved[0]):
+            with torch.cuda.device(saved[0].device):
+                return TokenLogprobsFunction._backward(ctx, *saved, dlogp, dent)
+        return TokenLogprobsFunction._backward(ctx, *saved, dlogp, dent)
+
+    @staticmethod
+    def _backward(ctx, x2, i2, ent, stats, dlogp, dent):
         shape, ignore = ctx.meta
         dx = torch.empty(shape, device=x2.device, dtype=x2.dtype)
         dlogp = dlogp.contiguous() if dlogp is not None else None
         dent = dent.contiguous() if dent is not None else None
-        with on_device(x2):
-            call("ccq_token_logprobs_bwd", ptr(x2), stride_of(x2), ptr(i2), ptr(ent), ptr(stats), ptr(dlogp), ptr(dent),
-                 ptr(dx), x2.shape[0], x2.shape[1], ignore, DTYPES[x2.dtype], stream_of(x2))
+        call("ccq_token_logprobs_bwd", x2.data_ptr(), stride_of(x2), i2.data_ptr(), ent.data_ptr(), stats.data_ptr(),
+             address(dlogp), address(dent), dx.data_ptr(), x2.shape[0], x2.shape[1], ignore, DTYPES[x2.dtype],
+             stream_on(x2))
         return dx, None, None, None
 
 
@@ -86,11 +92,14 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, igno
     if logits.dim() < 1 or logits.shape[-1] < 1 or ids.shape != logits.shape[:-1]:
         raise ValueError(f"token_logprobs: ids {tuple(ids.shape)}: expected the positions of logits "
                          f"{tuple(logits.shape)}")
-    require_like("token_logprobs", logits, ids=ids)
+    require_on("token_logprobs", "ids", ids, logits)
     top_k = int(top_k)
     if not 0 <= top_k <= min(MAX_TOP, logits.shape[-1]):
         raise ValueError(f"token_logprobs: top_k={top_k} must lie in [0, {min(MAX_TOP, logits.shape[-1])}]")
     require_gpu("token_logprobs", logits)
+    if not current(logits):
+        with torch.cuda.device(logits.device):
+            return token_logprobs(logits, ids, top_k, ignore_index)
     ids = ids.long()
     if needs_grad(logits):
         return TokenLogprobs(*TokenLogprobsFunction.apply(logits, ids, top_k, int(ignore_index)))

@@ -12,9 +12,8 @@ from typing import Optional, Tuple, Union
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib
-from ._lib import call, ptr, stream_of
-from ._rows import DTYPES, needs_grad, on_device, require_gpu, require_like, rows_of, stride_of
+from ._rows import (DTYPES, address, call, current, entry, needs_grad, require_gpu, require_on, rows_of, stream_on,
+                    stride_of)
 
 __all__ = ["layer_norm", "rms_norm", "BlockNormFunction"]
 
@@ -22,20 +21,20 @@ MAX_WIDTH = 8192
 
 
 def _forward(x, residual, weight, bias, layer, eps, keep):
-    """``(y, s or None, x as rows, mean or None, rstd or None)``; the statistics only with ``keep``."""
+    """``(y, s or None, x as rows, statistics or None)``; the statistics (mean, then 1 / deviation, of every row) only
+    with ``keep``."""
     x2 = rows_of(x)
     r2 = rows_of(residual) if residual is not None else None
     rows, D = x2.shape
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     s = torch.empty(x.shape, device=x.device, dtype=x.dtype) if r2 is not None else None
-    mean = torch.empty(rows, device=x.device, dtype=torch.float32) if keep and layer else None
-    rstd = torch.empty(rows, device=x.device, dtype=torch.float32) if keep else None
+    stats = torch.empty(2 * rows, device=x.device, dtype=torch.float32) if keep else None
+    mean = address(stats)
     wdtype = DTYPES[weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype]
-    with on_device(x):
-        call("ccq_norm_fwd", ptr(x2), stride_of(x2), ptr(r2), stride_of(r2) if r2 is not None else 0, ptr(weight),
-             ptr(bias), ptr(y), ptr(s), ptr(mean), ptr(rstd), rows, D, DTYPES[x.dtype], wdtype, int(layer), eps,
-             stream_of(x))
-    return y, s, x2, mean, rstd
+    call("ccq_norm_fwd", x2.data_ptr(), stride_of(x2), address(r2), stride_of(r2) if r2 is not None else 0,
+         address(weight), address(bias), y.data_ptr(), address(s), mean if layer else 0,
+         mean + 4 * rows if keep else 0, rows, D, DTYPES[x.dtype], wdtype, layer, eps, stream_on(x))
+    return y, s, x2, stats
 
 
 class BlockNormFunction(torch.autograd.Function):
@@ -43,9 +42,9 @@ class BlockNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, residual, weight, bias, layer, eps):
-        y, s, x2, mean, rstd = _forward(x, residual, weight, bias, layer, eps, True)
+        y, s, x2, stats = _forward(x, residual, weight, bias, layer, eps, True)
         # the normalised rows: the stream where there is a residual (an output, saved as such), x otherwise
-        ctx.save_for_backward(x2 if s is None else s, weight, mean, rstd)
+        ctx.save_for_backward(x2 if s is None else s, weight, stats)
         ctx.meta = (layer, x.shape, None if bias is None else bias.dtype)
         ctx.set_materialize_grads(False)
         return y if s is None else (y, s)
@@ -53,32 +52,38 @@ class BlockNormFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, ds=None):
-        rows_in, weight, mean, rstd = ctx.saved_tensors
+        if dy is None and ds is None:
+            return None, None, None, None, None, None
+        rows_in, weight, stats = ctx.saved_tensors
+        if not current(rows_in):
+            with torch.cuda.device(rows_in.device):
+                return BlockNormFunction._backward(ctx, rows_in, weight, stats, dy, ds)
+        return BlockNormFunction._backward(ctx, rows_in, weight, stats, dy, ds)
+
+    @staticmethod
+    def _backward(ctx, rows_in, weight, stats, dy, ds):
         layer, shape, bdtype = ctx.meta
-        need_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
-        need_w, need_b = ctx.needs_input_grad[2], ctx.needs_input_grad[3]
+        need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
         x2 = rows_of(rows_in)
         rows, D = x2.shape
-        dev = x2.device
+        dev, dtype = x2.device, x2.dtype
         if dy is None:
-            if ds is None:
-                return (None,) * 6
-            dy = torch.zeros(shape, device=dev, dtype=x2.dtype)  # (only the stream was used)
+            dy = torch.zeros(shape, device=dev, dtype=dtype)  # (only the stream was used)
         d2 = rows_of(dy)
         s2 = rows_of(ds) if ds is not None else None
-        wdt = weight.dtype if weight is not None else bdtype if bdtype is not None else x2.dtype
-        dx = torch.empty(shape, device=dev, dtype=x2.dtype) if need_x else None
+        wdt = weight.dtype if weight is not None else bdtype if bdtype is not None else dtype
+        dx = torch.empty(shape, device=dev, dtype=dtype) if need_x or need_r else None
         dw = torch.empty(D, device=dev, dtype=wdt) if need_w else None
         db = torch.empty(D, device=dev, dtype=wdt) if need_b else None
         ws = None
-        with on_device(x2):
-            if need_w or need_b:
-                n = _lib.load().ccq_norm_bwd_workspace_bytes(rows, D, DTYPES[x2.dtype])
-                ws = torch.empty(n, device=dev, dtype=torch.uint8)
-            call("ccq_norm_bwd", ptr(x2), stride_of(x2), ptr(weight), ptr(mean), ptr(rstd), ptr(d2), stride_of(d2),
-                 ptr(s2), stride_of(s2) if s2 is not None else 0, ptr(dx), ptr(dw), ptr(db), ptr(ws), rows, D,
-                 DTYPES[x2.dtype], DTYPES[wdt], int(layer), stream_of(x2))
-        return dx if ctx.needs_input_grad[0] else None, dx if ctx.needs_input_grad[1] else None, dw, db, None, None
+        if need_w or need_b:
+            ws = torch.empty(entry("ccq_norm_bwd_workspace_bytes")(rows, D, DTYPES[dtype]), device=dev,
+                             dtype=torch.uint8)
+        mean = stats.data_ptr()
+        call("ccq_norm_bwd", x2.data_ptr(), stride_of(x2), address(weight), mean if layer else 0, mean + 4 * rows,
+             d2.data_ptr(), stride_of(d2), address(s2), stride_of(s2) if s2 is not None else 0, address(dx),
+             address(dw), address(db), address(ws), rows, D, DTYPES[dtype], DTYPES[wdt], layer, stream_on(x2))
+        return dx if need_x else None, dx if need_r else None, dw, db, None, None
 
 
 def _norm(who, x, weight, bias, eps, residual, layer):
@@ -88,7 +93,9 @@ def _norm(who, x, weight, bias, eps, residual, layer):
         raise ValueError(f"{who}: x {tuple(x.shape)}: needs a last dimension in [1, {MAX_WIDTH}]")
     if not eps >= 0:
         raise ValueError(f"{who}: eps={eps} must not be negative")
-    require_like(who, x, weight=weight, bias=bias, residual=residual)
+    require_on(who, "weight", weight, x)
+    require_on(who, "bias", bias, x)
+    require_on(who, "residual", residual, x)
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
@@ -102,12 +109,15 @@ def _norm(who, x, weight, bias, eps, residual, layer):
         raise ValueError(f"{who}: residual {tuple(residual.shape)} {residual.dtype}: expected x's {tuple(x.shape)} "
                          f"{x.dtype}")
     require_gpu(who, x)
+    if not current(x):
+        with torch.cuda.device(x.device):
+            return _norm(who, x, weight, bias, eps, residual, layer)
     weight = weight if weight is None else weight.contiguous()
     bias = bias if bias is None else bias.contiguous()
     eps = float(eps)
     if needs_grad(x, residual, weight, bias):
         return BlockNormFunction.apply(x, residual, weight, bias, layer, eps)
-    y, s, _, _, _ = _forward(x, residual, weight, bias, layer, eps, False)
+    y, s, _, _ = _forward(x, residual, weight, bias, layer, eps, False)
     return y if s is None else (y, s)
 
 
@@ -119,10 +129,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     ``residual`` (x's shape and type) the rows are ``s = x + residual``, rounded to their type as the residual
     stream holds them, and it returns ``(y, s)``.  Statistics and sums in fp32, one rounding of y.  Gradients of x,
     residual, weight and bias."""
-    return _norm("layer_norm", x, weight, bias, eps, residual, True)
+    return _norm("layer_norm", x, weight, bias, eps, residual, 1)
 
 
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-5,
              residual: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """``x / sqrt(mean(x^2) + eps) * weight`` over the last dimension; otherwise as ``layer_norm``."""
-    return _norm("rms_norm", x, weight, None, eps, residual, False)
+    return _norm("rms_norm", x, weight, None, eps, residual, 0)
