@@ -10,10 +10,13 @@
 // one sign, so nothing cancels; m and log Z are kept apart, since their sum would lose log Z beside a large m (a row
 // masked to the type's lowest value is uniform).  A row belongs to one workgroup.
 //
-// The alternatives: pass one also leaves the maximum of each of 64 parts of the row; the k-th largest of those
-// (k <= 64) is a lower bound of the k-th largest logit, and few logits reach it (about 24 for k = 20).  Pass two
-// reads the row again (it lies in the L2) and lists those, and every listed logit counts those before it.  A
-// row with more than kTopList of them (equal logits) is ranked by k passes over it.
+// The alternatives come out of the same pass.  The 64 lanes stand for 64 parts of the row; after a thread's first few
+// pieces, which it holds in registers, the k-th largest of the 64 maxima (k <= 64) is a lower bound of the row's k-th
+// largest logit, and the logits that reach it are listed, those of the pieces behind as they are read: about 24 for
+// k = 20 where the first pieces are the whole row, 24 / f where they are a fraction f.  Every listed logit then counts
+// those before it.  A row that lists more than kTopList is read again with the bound of the whole row's maxima, and one
+// that still does (equal logits) is ranked by k passes over it.  (A second pass for all rows, as first built: 53.8 us
+// against 43.8 with pieces loaded ahead, and this, on 1531 x 32007 fp32 with half the rows skipped, k = 5.)
 #include <algorithm>
 
 #include "ccq_block_args.h"
@@ -28,26 +31,32 @@ constexpr int kTopList = 1024;   // listed candidates
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFar = -1e4f;    // e^(x - m) is 0 long before: stands for -inf in the products with it
 
+// 2^x, one instruction: results below 2^-126 are 0 (beside a sum of at least 1 they are nothing)
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
 // Running maximum m of a part of a row, s = sum e^(x - m), t = sum e^(x - m) (x - m).
 struct Part {
   float m, s, t;
 };
 // NaN enters s alone (comparisons and maxima pass it over), and makes every result of the row NaN.
+// Rounded the same whichever comes first, so that the lanes that merge with each other hold the same bits.
 __device__ __forceinline__ Part merge(const Part& a, const Part& b) {
+#pragma clang fp contract(off)
   const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;
   const float da = fmaxf(a.m - ref, kFar), db = fmaxf(b.m - ref, kFar);
-  const float ca = exp2f(da * kLog2e), cb = exp2f(db * kLog2e);
+  const float ca = exp2_(da * kLog2e), cb = exp2_(db * kLog2e);
   return {m, ca * a.s + cb * b.s, ca * (a.t + a.s * da) + cb * (b.t + b.s * db)};
 }
 
+// the values of a piece into p; returns their maximum
 template <int N>
-__device__ __forceinline__ void add_values(Part& p, const float (&v)[N]) {
+__device__ __forceinline__ float add_values(Part& p, const float (&v)[N]) {
   float m = v[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
   if (m > p.m) {
     if (p.m != -INFINITY) {
-      const float d = fmaxf(p.m - m, kFar), c = exp2f(d * kLog2e);
+      const float d = fmaxf(p.m - m, kFar), c = exp2_(d * kLog2e);
       p.t = c * (p.t + p.s * d);
       p.s *= c;
     }
@@ -56,10 +65,11 @@ __device__ __forceinline__ void add_values(Part& p, const float (&v)[N]) {
   const float ref = p.m == -INFINITY ? 0.f : p.m;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const float d = v[i] - ref, e = exp2f(d * kLog2e);
+    const float d = v[i] - ref, e = exp2_(d * kLog2e);
     p.s += e;
     p.t += e * fmaxf(d, kFar);
   }
+  return m;
 }
 
 // Order of the alternatives: NaN before any number, the larger logit first, the lower index first.
@@ -71,63 +81,96 @@ __device__ __forceinline__ unsigned long long rank_key(float x, int i) {
 }
 __device__ __forceinline__ int key_index(unsigned long long k) { return (int)~(unsigned)k; }
 
+// f(column, piece) over the thread's pieces of a row, kAhead of them loaded together
+constexpr int kAhead = 4;
 template <typename T, typename F>
 __device__ __forceinline__ void over_row(const T* row, int V, int tid, int threads, F&& f) {
   constexpr int N = Piece<T>::N;
-  for (int c = tid * N; c < V; c += threads * N) f(c, load_piece(row, c, V));
+  const int step = threads * N;
+  for (int c = tid * N; c < V; c += kAhead * step) {
+    typename Piece<T>::vec v[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (c + j * step < V) v[j] = load_piece(row, c + j * step, V);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (c + j * step < V) f(c + j * step, v[j]);
+  }
 }
 
-// The k first of the row in rank order, into out / ids.  part: the maximum of this thread's logits; m, logz: the row's.
-template <typename T, int THREADS>
-__device__ void top_of_row(const T* row, int V, int k, float part, float m, float logz, float* out, int64_t* ids) {
-  constexpr int N = Piece<T>::N, W = THREADS / 64;
-  __shared__ unsigned long long list[kTopList];
-  __shared__ float pm[kTopParts];
-  __shared__ int count;
-  const int tid = threadIdx.x;
-  constexpr int G = THREADS / kTopParts;  // threads of a part
-#pragma unroll
-  for (int o = 1; o < G; o <<= 1) part = fmaxf(part, __shfl_xor(part, o));
-  if (tid % G == 0) pm[tid / G] = part;
-  if (tid == 0) count = 0;
+// The candidates of a row: an index's logit in rank order.
+template <int THREADS>
+struct TopList {
+  unsigned long long list[kTopList];
+  float pm[THREADS / 64][kTopParts];
+  float bound;
+  int count;
+};
+
+// the k-th largest of the lanes' maxima over the workgroup's waves
+template <int THREADS>
+__device__ float top_bound(TopList<THREADS>& s, int k, float mine) {
+  const int l = threadIdx.x & 63;
+  __syncthreads();  // (the last use of pm and count)
+  s.pm[threadIdx.x >> 6][l] = mine;
+  if (threadIdx.x == 0) s.count = 0;
   __syncthreads();
-  float bound = -INFINITY;
-  {
-    const int l = tid & 63;
-    const float v = pm[l];
+  if (threadIdx.x < 64) {  // (one wave: sixteen at once would share the SIMDs for the same answer)
+    float v = s.pm[0][l];
+#pragma unroll
+    for (int w = 1; w < THREADS / 64; ++w) v = fmaxf(v, s.pm[w][l]);
     int before = 0;
+#pragma unroll
     for (int i = 0; i < kTopParts; ++i) {
-      const float u = pm[i];
+      const float u = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i));
       before += u > v || (u == v && i < l);
     }
-    const unsigned long long hit = __ballot(before == k - 1);  // one lane: the ranks are distinct
-    bound = __shfl(v, __ffsll(hit) - 1);
+    if (before == k - 1) s.bound = v;  // one lane: the ranks are distinct
   }
-  over_row(row, V, tid, THREADS, [&](int c, const typename Piece<T>::vec& v) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (c + i < V && !((float)v[i] < bound)) {
-        const int at = atomicAdd(&count, 1);
-        if (at < kTopList) list[at] = rank_key((float)v[i], c + i);
-      }
-  });
   __syncthreads();
-  const int n = count;
-  if (n <= kTopList) {
+  return s.bound;
+}
+
+template <typename T, int THREADS>
+__device__ __forceinline__ void list_piece(TopList<THREADS>& s, const typename Piece<T>::vec& v, int c, int V, float bound) {
+#pragma unroll
+  for (int i = 0; i < Piece<T>::N; ++i)
+    if (c + i < V && (float)v[i] >= bound) {
+      const int at = atomicAdd(&s.count, 1);
+      if (at < kTopList) s.list[at] = rank_key((float)v[i], c + i);
+    }
+}
+
+// The k first of the row in rank order, into out / ids.  The list holds every logit that reaches some bound below the
+// k-th largest, unless it overflowed; most: the maximum of this thread's logits; m, logz: the row's.
+template <typename T, int THREADS>
+__device__ void top_of_row(TopList<THREADS>& s, const T* row, int V, int k, float most, float m, float logz, float* out,
+                           int64_t* ids) {
+  constexpr int N = Piece<T>::N, W = THREADS / 64;
+  const int tid = threadIdx.x;
+  const bool bad = logz != logz;  // (a NaN is listed by no comparison)
+  __syncthreads();
+  int n = s.count;
+  if (n > kTopList && !bad) {
+    const float bound = top_bound<THREADS>(s, k, most);
+    over_row(row, V, tid, THREADS, [&](int c, const typename Piece<T>::vec& v) { list_piece<T, THREADS>(s, v, c, V, bound); });
+    __syncthreads();
+    n = s.count;
+  }
+  if (n <= kTopList && !bad) {
     for (int a = tid; a < n; a += THREADS) {
-      const unsigned long long mine = list[a];
+      const unsigned long long mine = s.list[a];
       int before = 0;
-      for (int i = 0; i < n; ++i) before += list[i] > mine;
+      for (int i = 0; i < n; ++i) before += s.list[i] > mine;
       if (before < k) {
         const int id = key_index(mine);
         out[before] = ((float)row[id] - m) - logz;
         ids[before] = id;
       }
     }
-    __syncthreads();
     return;
   }
-  // more candidates than the list holds: the first of the row behind the last one found, k times
+  // the first of the row behind the last one found, k times
   unsigned long long last = ~0ull;
   for (int j = 0; j < k; ++j) {
     __syncthreads();
@@ -143,9 +186,9 @@ __device__ void top_of_row(const T* row, int V, int k, float part, float m, floa
       const unsigned long long other = __shfl_xor(best, o);
       best = other > best ? other : best;
     }
-    if ((tid & 63) == 0) list[tid >> 6] = best;
+    if ((tid & 63) == 0) s.list[tid >> 6] = best;
     __syncthreads();
-    for (int i = 0; i < W; ++i) best = list[i] > best ? list[i] : best;
+    for (int i = 0; i < W; ++i) best = s.list[i] > best ? s.list[i] : best;
     last = best;
     if (tid == 0) {
       const int id = key_index(best);
@@ -155,18 +198,17 @@ __device__ void top_of_row(const T* row, int V, int k, float part, float m, floa
   }
 }
 
-template <typename T, int THREADS>
+template <typename T, int THREADS, bool TOP>
 __global__ __launch_bounds__(THREADS) void logprob_fwd_kernel(const LogprobArgs a) {
   constexpr int N = Piece<T>::N, W = THREADS / 64;
   __shared__ Part parts[W];
+  __shared__ TopList<TOP ? THREADS : 64> top;
   const int tid = threadIdx.x, V = a.V;
   const long r = blockIdx.x;
   const int64_t id = a.ids[r];
   if (id == a.ignore) {
-    if (tid == 0) {
-      a.logp[r] = a.ent[r] = 0.f;
-    }
-    if (tid < a.k) {
+    if (tid == 0) a.logp[r] = a.ent[r] = 0.f;
+    if (TOP && tid < a.k) {
       a.top[r * a.k + tid] = 0.f;
       a.top_ids[r * a.k + tid] = -1;
     }
@@ -174,20 +216,56 @@ __global__ __launch_bounds__(THREADS) void logprob_fwd_kernel(const LogprobArgs 
   }
   const T* row = (const T*)a.x + r * a.ldx;
   Part p{-INFINITY, 0.f, 0.f};
-  over_row(row, V, tid, THREADS, [&](int c, const typename Piece<T>::vec& x) {
-    float v[N];
+  float bound = INFINITY;
+  constexpr int step = THREADS * N;
+  constexpr bool kNext = THREADS < 1024;  // the next pieces on their way too (sixteen waves have the registers for one set)
+  typename Piece<T>::vec x[kAhead], y[kAhead];
+  auto fetch = [&](typename Piece<T>::vec(&v)[kAhead], int c) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = c + i < V ? (float)x[i] : -INFINITY;
-    add_values<N>(p, v);
-  });
+    for (int j = 0; j < kAhead; ++j)
+      if (c + j * step < V) v[j] = load_piece(row, c + j * step, V);
+  };
+  fetch(x, tid * N);
+  for (int c0 = 0; c0 < V; c0 += kAhead * step) {  // (the same rounds for every thread)
+    const int c = c0 + tid * N;
+    if (kNext) fetch(y, c + kAhead * step);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int at = c + j * step;
+      if (at >= V) break;
+      float v[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = (float)x[j][i];
+      if (at + N > V)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = at + i < V ? v[i] : -INFINITY;
+      const float most = add_values<N>(p, v);
+      if constexpr (TOP) {
+        if (most >= bound) list_piece<T, THREADS>(top, x[j], at, V, bound);
+      }
+    }
+    if constexpr (TOP) {
+      if (c0 == 0) {
+        bound = top_bound<THREADS>(top, a.k, p.m);
+        if (p.m >= bound)
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j)
+            if (c + j * step < V) list_piece<T, THREADS>(top, x[j], c + j * step, V, bound);
+      }
+    }
+    if (!kNext) fetch(x, c + kAhead * step);
+    else
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) x[j] = y[j];
+  }
   const float mine = p.m;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) p = merge(p, Part{__shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o)});
   if ((tid & 63) == 0) parts[tid >> 6] = p;
   __syncthreads();
-  p = parts[0];
+  p = parts[tid & (W - 1)];
 #pragma unroll
-  for (int i = 1; i < W; ++i) p = merge(p, parts[i]);
+  for (int o = 1; o < W; o <<= 1) p = merge(p, Part{__shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o)});
   const float logz = logf(p.s);
   if (tid == 0) {
     // a token outside the vocabulary has no log probability
@@ -198,7 +276,8 @@ __global__ __launch_bounds__(THREADS) void logprob_fwd_kernel(const LogprobArgs 
       a.stats[2 * r + 1] = logz;
     }
   }
-  if (a.k) top_of_row<T, THREADS>(row, V, a.k, mine, p.m, logz, a.top + r * a.k, a.top_ids + r * a.k);
+  if constexpr (TOP)
+    top_of_row<T, THREADS>(top, row, V, a.k, mine, p.m, logz, a.top + r * a.k, a.top_ids + r * a.k);
 }
 
 // grid: (parts of a row, rows)
@@ -236,7 +315,7 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(const LogprobArgs
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float v = fmaxf(((float)x[j][i] - m) - logz, kFar);
-      g[i] = exp2f(v * kLog2e) * (c - dent * v);
+      g[i] = exp2_(v * kLog2e) * (c - dent * v);
     }
     if (id >= at && id < at + N)
 #pragma unroll
@@ -248,6 +327,8 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(const LogprobArgs
   }
 }
 
+// Fewer rows than fill the chip's 8192 waves with four to a row: sixteen to a row.
+constexpr long kFewRows = 1024;
 template <typename T>
 void launch_typed(bool bwd, const LogprobArgs& a, hipStream_t st) {
   if (bwd) {
@@ -255,10 +336,12 @@ void launch_typed(bool bwd, const LogprobArgs& a, hipStream_t st) {
     const dim3 grid((unsigned)((a.V + per - 1) / per), (unsigned)std::min<long>(a.rows, 32768),
                     (unsigned)((a.rows + 32767) / 32768));
     hipLaunchKernelGGL(logprob_bwd_kernel<T>, grid, dim3(kThreads), 0, st, a);
-  } else if (a.rows < 512) {
-    hipLaunchKernelGGL((logprob_fwd_kernel<T, 1024>), dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+  } else if (a.rows < kFewRows) {
+    if (a.k) hipLaunchKernelGGL((logprob_fwd_kernel<T, 1024, true>), dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((logprob_fwd_kernel<T, 1024, false>), dim3((unsigned)a.rows), dim3(1024), 0, st, a);
   } else {
-    hipLaunchKernelGGL((logprob_fwd_kernel<T, 256>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
+    if (a.k) hipLaunchKernelGGL((logprob_fwd_kernel<T, 256, true>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((logprob_fwd_kernel<T, 256, false>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
   }
 }
 
