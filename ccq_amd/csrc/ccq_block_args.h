@@ -59,7 +59,7 @@ struct ProductArgs {
   long ldo;
   const void* bias;    // [N] (swiglu: [2 N]) of bdtype (nullable)
   const void* res;     // [M, N] row stride ldr (nullable)
-  void* z;             // [M, ldz] the values before the activation (nullable)
+  void* z;             // [M, ldz] the values before the activation, 16 bits, then 8 (nullable)
   long ldr, ldz;
   float* part;         // [splits, M, N (swiglu: 2 N)] partial sums (splits > 1)
   int splits;          // parts of the contraction, whole steps each
@@ -67,7 +67,7 @@ struct ProductArgs {
 };
 
 struct ActBwdArgs {
-  const void* z;       // [M, ldz] (nullable: no activation)
+  const void* z;       // [M, ldz] 16 bits, then 8 (nullable: no activation)
   const void* dy;      // [M, N] row stride ldy
   void* dz;            // [M, ldz], zeros behind the Nz columns (nullable: only db is wanted)
   float* db_part;      // [row blocks, Nz] (nullable)

@@ -9,6 +9,7 @@
 // (x and W forward; dz in dx) or down them (W in dx; dz and x in dW); the second kind is read out of LDS by
 // transposing reads, so nothing is transposed in memory.
 #include <algorithm>
+#include <type_traits>
 
 #include "ccq_block_args.h"
 #include "ccq_oper.h"
@@ -31,33 +32,84 @@ __device__ __forceinline__ void acc_settled() { asm volatile("s_nop 15\n\ts_nop 
 // ---------------------------------------------------------------------------
 // activations, in fp32
 // ---------------------------------------------------------------------------
+constexpr int kActOther = -1;  // (of a kernel: any but none and swiglu)
 constexpr float kTanhA = 0.7978845608028654f, kTanhB = 0.044715f;  // gelu_tanh: tanh(a (z + b z^3))
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + __expf(-z)); }
+__device__ __forceinline__ float exp_(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp_(-z)); }
 
-__device__ __forceinline__ float act_value(int act, float z) {
+// erfc(x) = t e^(P(t) - x^2), t = 1 / (1 + x / 2), for x >= 0, and 2 - erfc(-x): P the polynomial of degree 9 nearest
+// to log(erfc(x) e^(x^2) / t) over t in (0, 1] in the largest error (1.0e-7; fitted at 400 Chebyshev nodes with
+// weights that even the errors out).  In fp32 within 4e-7.
+__device__ __forceinline__ float erfc_(float x) {
+  const float a = fabsf(x), t = __builtin_amdgcn_rcpf(1.f + 0.5f * a);
+  float p = 0.168761006f;
+  p = p * t - 0.813325556f;
+  p = p * t + 1.47325527f;
+  p = p * t - 1.12109976f;
+  p = p * t + 0.271351518f;
+  p = p * t - 0.183966161f;
+  p = p * t + 0.0963881326f;
+  p = p * t + 0.374125038f;
+  p = p * t + 1.00002265f;
+  p = p * t - 1.26551222f;
+  const float e = t * exp_(p - a * a);
+  return x < 0.f ? 2.f - e : e;
+}
+
+// the activation of C values (one switch for all: the functions are small, their selection is not)
+template <int C>
+__device__ __forceinline__ void act_values(int act, float (&v)[C]) {
   switch (act) {
-    case kActRelu: return fmaxf(z, 0.f);
-    case kActSilu: return z * sigmoid(z);
-    case kActGelu: return 0.5f * z * erfcf(z * -0.7071067811865476f);
-    case kActGeluTanh: return z * sigmoid(2.f * kTanhA * (z + kTanhB * z * z * z));
-    default: return z;
+    case kActRelu:
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // (NaN stays)
+      break;
+    case kActSilu:
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[i] *= sigmoid(v[i]);
+      break;
+    case kActGelu:
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[i] *= 0.5f * erfc_(v[i] * -0.7071067811865476f);
+      break;
+    case kActGeluTanh:
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[i] *= sigmoid(2.f * kTanhA * (v[i] + kTanhB * v[i] * v[i] * v[i]));
+      break;
+    default: break;
   }
 }
-__device__ __forceinline__ float act_slope(int act, float z) {
+// d = d act'(z)
+template <int C, typename Z>
+__device__ __forceinline__ void act_slopes(int act, const Z& z, float (&d)[C]) {
   switch (act) {
-    case kActRelu: return z > 0.f ? 1.f : 0.f;
-    case kActSilu: {
-      const float g = sigmoid(z);
-      return g * (1.f + z * (1.f - g));
-    }
-    case kActGelu: return 0.5f * erfcf(z * -0.7071067811865476f) + z * 0.3989422804014327f * __expf(-0.5f * z * z);
-    case kActGeluTanh: {
-      z = fminf(fmaxf(z, -16.f), 16.f);  // (the slope is 0 or 1 long before; the square of a far z would overflow)
-      const float g = sigmoid(2.f * kTanhA * (z + kTanhB * z * z * z));
-      return g + z * 2.f * g * (1.f - g) * kTanhA * (1.f + 3.f * kTanhB * z * z);
-    }
-    default: return 1.f;
+    case kActRelu:
+#pragma unroll
+      for (int i = 0; i < C; ++i) d[i] *= z[i] > 0.f ? 1.f : z[i] <= 0.f ? 0.f : z[i];
+      break;
+    case kActSilu:
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const float g = sigmoid(z[i]);
+        d[i] *= g * (1.f + z[i] * (1.f - g));
+      }
+      break;
+    case kActGelu:
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+        d[i] *= 0.5f * erfc_(z[i] * -0.7071067811865476f) + z[i] * 0.3989422804014327f * exp_(-0.5f * z[i] * z[i]);
+      break;
+    case kActGeluTanh:
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        // (the slope is 0 or 1 long before 16; the square of a far z would overflow)
+        const float x = z[i] != z[i] ? z[i] : fminf(fmaxf(z[i], -16.f), 16.f);
+        const float g = sigmoid(2.f * kTanhA * (x + kTanhB * x * x * x));
+        d[i] *= g + x * 2.f * g * (1.f - g) * kTanhA * (1.f + 3.f * kTanhB * x * x);
+      }
+      break;
+    default: break;
   }
 }
 
@@ -98,30 +150,116 @@ __device__ __forceinline__ void add_row(const T* row, long n, long N, float (&v)
     if (n + i < N) v[i] += (float)*gmem(row + n + i);
 }
 
-// The epilogue of C consecutive columns n .. of row m (swiglu: v the gates, up the other half).
-template <typename T, int C, bool glu>
-__device__ __forceinline__ void finish(const ProductArgs& p, long m, long n, float (&v)[C], float (&up)[C]) {
-  if (p.bias) {
+// The values before the activation are kept for the backward in 24 bits, the upper three bytes of fp32: 16 bits of
+// them would be the largest error of dx and dW (swiglu, bf16: 1.76 times the one rounding of the result; so 1.42, the
+// other being that of dz), and 32 cost 8 bytes of traffic an element for 6.  A plane of 16 bits, then one of 8, both
+// [M, ldz].
+template <int C>
+__device__ __forceinline__ void keep_z(void* z, long rows, long ld, long m, long n, long end, const float (&v)[C]) {
+  unsigned short* hi = (unsigned short*)z + m * ld;
+  unsigned char* lo = (unsigned char*)z + rows * ld * 2 + m * ld;
+  typedef unsigned short hvec __attribute__((ext_vector_type(C)));
+  typedef unsigned char lvec __attribute__((ext_vector_type(C)));
+  typedef hvec hany __attribute__((aligned(2)));
+  typedef lvec lany __attribute__((aligned(1)));
+  hvec h;
+  lvec b;
 #pragma unroll
-    for (int i = 0; i < C; ++i)
-      if (n + i < p.N) {
-        v[i] += bias_at(p.bias, p.bdtype, n + i);
-        if (glu) up[i] += bias_at(p.bias, p.bdtype, p.N + n + i);
-      }
+  for (int i = 0; i < C; ++i) {
+    const unsigned u = __float_as_uint(v[i]);
+    // (a NaN whose payload lies in the lowest byte alone would come back as an infinity)
+    h[i] = (unsigned short)(u >> 16);
+    b[i] = (unsigned char)(v[i] != v[i] ? 0xff : u >> 8);
+  }
+  if (n + C <= end) {
+    *gmem((hany*)(hi + n)) = h;
+    *gmem((lany*)(lo + n)) = b;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+    if (n + i < end) {
+      *gmem(hi + n + i) = h[i];
+      *gmem(lo + n + i) = b[i];
+    }
+}
+template <int C>
+struct KeptZ {
+  typedef unsigned short hvec __attribute__((ext_vector_type(C)));
+  typedef unsigned char lvec __attribute__((ext_vector_type(C)));
+  typedef hvec hany __attribute__((aligned(2)));
+  typedef lvec lany __attribute__((aligned(1)));
+  hvec h;
+  lvec b;
+  __device__ void load(const void* z, long rows, long ld, long m, long n, long end) {
+    const unsigned short* hi = (const unsigned short*)z + m * ld;
+    const unsigned char* lo = (const unsigned char*)z + rows * ld * 2 + m * ld;
+    if (n + C <= end) {
+      h = *gmem((const hany*)(hi + n));
+      b = *gmem((const lany*)(lo + n));
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      h[i] = n + i < end ? *gmem(hi + n + i) : (unsigned short)0;
+      b[i] = n + i < end ? *gmem(lo + n + i) : (unsigned char)0;
+    }
+  }
+  __device__ float operator[](int i) const { return __uint_as_float((unsigned)h[i] << 16 | (unsigned)b[i] << 8); }
+};
+
+// C consecutive values of a row of T, at any element's address; zeros behind N
+template <typename T, int C>
+struct RowPiece {
+  typedef T vec __attribute__((ext_vector_type(C)));
+  typedef vec any __attribute__((aligned(sizeof(T))));
+  vec v;
+  __device__ void load(const T* row, long n, long N) {
+    if (n + C <= N) {
+      v = *gmem((const any*)(row + n));
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = n + i < N ? *gmem(row + n + i) : (T)0.f;
+  }
+};
+
+// What the epilogue of C columns from n on needs of them whatever the row: the bias (swiglu: of both halves).
+template <int C, bool glu>
+struct ColumnBias {
+  float v[C], up[glu ? C : 1];
+  __device__ void load(const ProductArgs& p, long n) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      v[i] = p.bias && n + i < p.N ? bias_at(p.bias, p.bdtype, n + i) : 0.f;
+      if (glu) up[glu ? i : 0] = p.bias && n + i < p.N ? bias_at(p.bias, p.bdtype, p.N + n + i) : 0.f;
+    }
+  }
+};
+
+// The epilogue of C consecutive columns n .. of row m (swiglu: v the gates, up the other half).  ACT: none, swiglu, or
+// any other (p.act), kept apart since the code of all of them takes up the instruction cache of those that need none.
+template <typename T, int C, int ACT, bool with_res, bool glu = ACT == kActSwiglu>
+__device__ __forceinline__ void finish(const ProductArgs& p, long m, long n, float (&v)[C], float (&up)[C],
+                                       const ColumnBias<C, glu>& bias, const RowPiece<T, C>& res) {
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    v[i] += bias.v[i];
+    if (glu) up[i] += bias.up[glu ? i : 0];
   }
   if (p.z) {
-    T* z = (T*)p.z + m * p.ldz;
-    store_row<T, C>(z, n, p.N, v);
-    if (glu) store_row<T, C>(z + p.N, n, p.N, up);
+    keep_z<C>(p.z, p.M, p.ldz, m, n, p.N, v);
+    if (glu) keep_z<C>(p.z, p.M, p.ldz, m, p.N + n, 2 * p.N, up);
   }
   if (glu) {
 #pragma unroll
     for (int i = 0; i < C; ++i) v[i] = v[i] * sigmoid(v[i]) * up[i];
-  } else if (p.act != kActNone) {
-#pragma unroll
-    for (int i = 0; i < C; ++i) v[i] = act_value(p.act, v[i]);
+  } else if (ACT != kActNone) {
+    act_values<C>(p.act, v);
   }
-  if (p.res) add_row<T, C>((const T*)p.res + m * p.ldr, n, p.N, v);
+  if (with_res)
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] += (float)res.v[i];
   store_row<T, C>((T*)p.out + m * p.ldo, n, p.N, v);
 }
 
@@ -141,15 +279,35 @@ struct Operand {
   long left;         // bytes from there to the operand's end
 };
 __device__ __forceinline__ u32x4 resource(const Operand& o) {
-  // (by words: a 64-bit comparison would leave the scalar unit, and a resource has to come from there)
+  // (compared by words: a 64-bit comparison leaves the scalar unit.  Whatever came from the vector unit all the same
+  // is brought back, and settled is called before such a resource is used.)
   const int hi = (int)(o.left >> 32);
   const unsigned lo = (unsigned)o.left;
   const unsigned n = hi < 0 ? 0u : hi > 0 ? 0x7fffffffu : lo > 0x7fffffffu ? 0x7fffffffu : lo;
-  return u32x4{(unsigned)(size_t)o.base, (unsigned)((size_t)o.base >> 32) & 0xffffu, n, 0x00020000u};
+  return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)(size_t)o.base),
+               (unsigned)__builtin_amdgcn_readfirstlane((int)((size_t)o.base >> 32)) & 0xffffu,
+               (unsigned)__builtin_amdgcn_readfirstlane((int)n), 0x00020000u};
 }
+// A scalar register that the vector unit wrote may be read by a memory instruction five wait states later; the compiler
+// does not look into the instructions below.
+__device__ __forceinline__ void settled(u32x4& r) { asm volatile("s_nop 4" : "+s"(r)); }
 __device__ __forceinline__ void load_piece_lds(const u32x4& r, unsigned off, unsigned m0) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(off), "s"(r) : "memory", "m0");
 }
+// The whole steps of a workgroup, from some step on and round to it again.
+struct StepStream {
+  Operand o;
+  long step, wrap;   // bytes of a step, of all of them
+  int ahead, until;  // steps not yet asked for, steps to the end of the whole ones
+  __device__ u32x4 next() {  // (selects, no branch: it runs between two products; behind the last step loads bring zeros)
+    const u32x4 r = resource({o.base, ahead > 0 ? o.left : 0});
+    --ahead;
+    --until;
+    const long d = step - (until == 0 ? wrap : 0);
+    o = {o.base + d, o.left - d};
+    return r;
+  }
+};
 constexpr unsigned kNowhere = 0x80000000u;  // behind every resource's end
 
 // swizzle of product row r of an operand read in consecutive rows (A), or in the order of column pairs (B)
@@ -199,25 +357,28 @@ __device__ __forceinline__ s16x4_t read_tr4(unsigned at) {
 
 enum : int { kPlain = 0, kEpilogue = 1, kPartial = 2 };
 
-// BM x BN tile of the product by WM x WN waves, two stages of LDS.  Lane l of a wave holds, of each 16x16 tile
+// BM x BN tile of the product by WM x WN waves, three stages of A in LDS and two of B.  Lane l of a wave holds, of each 16x16 tile
 // (it, j) of the wave, row m = 16 it + (l & 15) and four consecutive columns.  Along-the-row B operands (the forward)
 // are read so that the column tiles j = 2 q and 2 q + 1 of a lane are eight consecutive columns, one 16-byte store.
 // swiglu: half of a wave's columns are gates, the other half the ups beside them, so a lane holds both.
 //
 // A step of 64 contraction elements is two halves of 32.  While the matrix cores work on one half's fragments the
 // other half's are read from LDS into registers and the direct loads of the step after next are issued, each
-// between two products (in clumps they keep the one wave of a SIMD from issuing products); the one barrier of a step lies between the halves, where every wave has read
-// the current stage (the loads may overwrite it) and the next stage has landed.
-template <typename T, int BM, int BN, int WM, int WN, bool DA, bool DB, int MODE, bool GLU>
+// between two products (in clumps they keep the one wave of a SIMD from issuing products).  The one barrier of a step
+// lies between the halves, where every wave has read the step's stages (loads may overwrite them) and the next step's
+// have landed.  The 160 KiB of LDS hold two and a half stages: the half goes to A, whose rows come from HBM and are
+// asked for three steps ahead, while B's, which the workgroups of all tile rows share, lie in the caches.
+template <typename T, int BM, int BN, int WM, int WN, bool DA, bool DB, int MODE, int ACT>
 __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs p) {
+  constexpr bool GLU = ACT == kActSwiglu;
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr unsigned kA = BM * kStep * 2, kStage = kA + BN * kStep * 2;
+  constexpr unsigned kA = BM * kStep * 2, kB = BN * kStep * 2, kRing = 3 * kA + 2 * kB;  // bytes of a stage; of all
   constexpr int HALF = BN / WN / 2;  // swiglu: gates of a wave
   static_assert(!GLU || (!DB && MODE == kEpilogue), "gates and ups of one wave");
   static_assert(TM == TN, "one fragment of each operand between two rows of products");
   constexpr int kPass = 64, kRow = TN * 16 + 4;  // rows of a wave in the epilogue at a time, floats a row
   constexpr unsigned kOut = NW * kPass * kRow * 4;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * kStage > kOut ? 2 * kStage : kOut];
+  __shared__ __attribute__((aligned(1024))) char smem[kRing > kOut ? kRing : kOut];
   const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
   constexpr int NT = GLU ? BN / 2 : BN;  // output columns of a tile
@@ -241,7 +402,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
   LoadA la;
   LoadB lb;
   la.init(lds0, wave, l, p.lda);
-  lb.init(lds0 + kA, wave, l, p.ldb);
+  lb.init(lds0 + 3 * kA, wave, l, p.ldb);
   Operand oa, ob;
   {
     // elements of the operands: to the end of the last row's last whole piece
@@ -269,22 +430,11 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
   // those of one tile row keep together and find its operand in the L2.  (8192^3 forward: 849 -> 788 us; contractions
   // of few steps gain nothing and lose the operands' meeting in the L2: 16384 x 5632 over 1024, 187 -> 193 us.)
   const int turn = BM == 256 && whole >= 32 ? 2 * (int)(in % rows) : 0;
-  int ahead = whole, until = whole - turn;  // steps not yet asked for, steps to the end of the whole ones
   const long wrapA = whole * stepA, wrapB = whole * stepB;
   const Operand ta = {oa.base + wrapA, oa.left - wrapA}, tb = {ob.base + wrapB, ob.left - wrapB};  // the end's
-  oa = {oa.base + turn * stepA, oa.left - turn * stepA};
-  ob = {ob.base + turn * stepB, ob.left - turn * stepB};
+  StepStream sa{{oa.base + turn * stepA, oa.left - turn * stepA}, stepA, wrapA, whole, whole - turn};
+  StepStream sb{{ob.base + turn * stepB, ob.left - turn * stepB}, stepB, wrapB, whole, whole - turn};
   u32x4 ra, rb;
-  auto next = [&] {  // (selects, no branch: it runs between two products; behind the last step loads bring zeros)
-    const bool on = ahead > 0;
-    ra = resource({oa.base, on ? oa.left : 0});
-    rb = resource({ob.base, on ? ob.left : 0});
-    --ahead;
-    --until;
-    const long da = stepA - (until == 0 ? wrapA : 0), db = stepB - (until == 0 ? wrapB : 0);
-    oa = {oa.base + da, oa.left - da};
-    ob = {ob.base + db, ob.left - db};
-  };
 
   // fragment addresses of this lane in stage 0
   const int r = l & 15, g = l >> 4;
@@ -303,11 +453,11 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     const int k = 8 * g + (r >> 2), s = wn * TN * 2 + ((r >> 1) & 1);
 #pragma unroll
     for (int j = 0; j < TN; ++j)
-      fb[j] = lds0 + kA + k * (BN * 2) + (((s + 2 * j) ^ (swz_k(k) << 1)) << 4) + 8 * (r & 1);
+      fb[j] = lds0 + 3 * kA + k * (BN * 2) + (((s + 2 * j) ^ (swz_k(k) << 1)) << 4) + 8 * (r & 1);
   } else {
     const int row = wn * TN * 16 + 8 * (r >> 2) + (r & 3);
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) fb[kk] = lds0 + kA + row * 128 + (((4 * kk + g) ^ swz_b(row)) << 4);
+    for (int kk = 0; kk < 2; ++kk) fb[kk] = lds0 + 3 * kA + row * 128 + (((4 * kk + g) ^ swz_b(row)) << 4);
   }
   auto read_a = [&](int it, unsigned stage, int kk) -> s16x8 {
     if constexpr (DA) {
@@ -327,10 +477,10 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
   };
 
   // fragment k of a half in the order that its products need them: a[0], b[0..], a[1..]
-  auto read = [&](s16x8(&a)[TM], s16x8(&b)[TN], int k, unsigned stage, int kk) {
-    if (k == 0) a[0] = read_a(0, stage, kk);
-    else if (k <= TN) b[k - 1] = read_b(k - 1, stage, kk);
-    else a[k - TN] = read_a(k - TN, stage, kk);
+  auto read = [&](s16x8(&a)[TM], s16x8(&b)[TN], int k, unsigned stage_a, unsigned stage_b, int kk) {
+    if (k == 0) a[0] = read_a(0, stage_a, kk);
+    else if (k <= TN) b[k - 1] = read_b(k - 1, stage_b, kk);
+    else a[k - TN] = read_a(k - TN, stage_a, kk);
   };
   // products between two loads, and between two fragment reads: the reads end at three quarters of the half, so that
   // the last ones have arrived by its end
@@ -350,50 +500,65 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
   s16x8 a0[TM], b0[TN], a1[TM], b1[TN];  // fragments of the two halves
 
   if (whole > 0) {
-    next();
+    auto load_a = [&](unsigned stage) {
+      ra = sa.next();
+      settled(ra);
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      la.issue(ra, i, 0, kStep, wave, l);
-      lb.issue(rb, i, 0, kStep, wave, l);
-    }
-    next();
+      for (int i = 0; i < TM; ++i) la.issue(ra, i, stage, kStep, wave, l);
+    };
+    auto load_b = [&](unsigned stage) {
+      rb = sb.next();
+      settled(rb);
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      la.issue(ra, i, kStage, kStep, wave, l);
-      lb.issue(rb, i, kStage, kStep, wave, l);
-    }
+      for (int i = 0; i < TN; ++i) lb.issue(rb, i, stage, kStep, wave, l);
+    };
+    load_a(0);
+    load_b(0);
+    load_a(kA);
+    load_b(kB);
+    load_a(2 * kA);
     clear();  // (while the first loads are on their way)
-    wait_loads<TM + TN>();
+    wait_loads<2 * TM + TN>();
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       b0[i] = read_b(i, 0, 0);
       a0[i] = read_a(i, 0, 0);
     }
-    unsigned stage = 0;
-    for (int s = 0; s < whole; ++s) {
+    unsigned st_a = 0, st_b = 0;  // the step's stages
+    auto step = [&](auto with_loads) {
+      constexpr bool kLoads = decltype(with_loads)::value;
+      const unsigned next_a = st_a == 2 * kA ? 0 : st_a + kA;
 #pragma unroll
       for (int q = 0; q < TM * TN; ++q) {
         product16<T>(b0[q % TN], a0[q / TN], acc[q / TN][q % TN]);
-        if (q == 0) next();
-        if (q % kReadGap == kReadGap - 1 && q / kReadGap < TM + TN) read(a1, b1, q / kReadGap, stage, 1);
+        if (kLoads && q == 0) ra = sa.next();
+        if (kLoads && q == 2) rb = sb.next();
+        if (q % kReadGap == kReadGap - 1 && q / kReadGap < TM + TN) read(a1, b1, q / kReadGap, st_a, st_b, 1);
         __builtin_amdgcn_sched_barrier(0);
       }
-      wait_loads<0>();
-      lds_barrier();  // this stage is read, the next one has landed
+      wait_loads<kLoads ? TM : 0>();
+      lds_barrier();  // this step's stages are read, the next step's have landed (not yet A's behind it)
+      if (kLoads) {
+        settled(ra);
+        settled(rb);
+      }
 #pragma unroll
       for (int q = 0; q < TM * TN; ++q) {
         product16<T>(b1[q % TN], a1[q / TN], acc[q / TN][q % TN]);
-        if (q % kLoadGap == 0) {
-          if (q / kLoadGap % 2) lb.issue(rb, q / kLoadGap / 2, stage, kStep, wave, l);
-          else la.issue(ra, q / kLoadGap / 2, stage, kStep, wave, l);
+        if (kLoads && q % kLoadGap == 0) {
+          if (q / kLoadGap < TN) lb.issue(rb, q / kLoadGap, st_b, kStep, wave, l);
+          else la.issue(ra, q / kLoadGap - TN, st_a, kStep, wave, l);
         }
-        if (q % kReadGap == kReadGap - 1 && q / kReadGap < TM + TN) read(a0, b0, q / kReadGap, stage ^ kStage, 0);
+        if (q % kReadGap == kReadGap - 1 && q / kReadGap < TM + TN) read(a0, b0, q / kReadGap, next_a, st_b ^ kB, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
-      stage ^= kStage;
-    }
-    wait_loads<0>();  // (the last steps' zeros)
+      st_a = next_a;
+      st_b ^= kB;
+    };
+    for (int s = 2; s < whole; ++s) step(std::true_type{});
+    // the last two steps ask for nothing (their last reads are of a stage behind, and not used)
+    for (int s = max(0, whole - 2); s < whole; ++s) step(std::false_type{});
     lds_barrier();
   } else {
     clear();
@@ -401,6 +566,8 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
   if (tail) {
     ra = resource(ta);
     rb = resource(tb);
+    settled(ra);
+    settled(rb);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       la.issue(ra, i, 0, tail, wave, l);
@@ -437,30 +604,55 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
         *(f32x4*)(mine + (16 * i + r) * kRow + (DB ? 16 * j + 4 * g : 32 * (j >> 1) + 4 * (j & 1) + 8 * g)) = acc[4 * h + i][j];
     __builtin_amdgcn_wave_barrier();  // (LDS operations of a wave are in order)
     constexpr int WC = GLU ? HALF : TN * 16, PR = WC / 8;  // output columns of the wave, pieces of a row
+    constexpr int RI = 64 / PR, NG = 4;                    // rows at a time, and how often between the residual's loads
     const int c = l % PR * 8;
-    const long n = n0 + wn * WC + c;
-    for (int i = l / PR; i < kPass; i += 64 / PR) {
-      const long m = m0 + wm * TM * 16 + h * kPass + i;
-      if (m >= p.M || n >= p.N) continue;
+    const long n = n0 + wn * WC + c, mh = m0 + wm * TM * 16 + h * kPass + l / PR;
+    auto row_out = [&](int i, const auto& bias, const RowPiece<T, 8>& res, auto with_res) {
+      const long m = mh + i;
+      if (m >= p.M || n >= p.N) return;
       float v[8], up[8];
-      const float* row = mine + i * kRow + c;
+      const float* row = mine + (i + l / PR) * kRow + c;
 #pragma unroll
       for (int e = 0; e < 8; e += 4) {
         *(f32x4*)(v + e) = *(const f32x4*)(row + e);
         if (GLU) *(f32x4*)(up + e) = *(const f32x4*)(row + HALF + e);
       }
-      if constexpr (MODE == kEpilogue) finish<T, 8, GLU>(p, m, n, v, up);
+      if constexpr (MODE == kEpilogue) finish<T, 8, ACT, decltype(with_res)::value>(p, m, n, v, up, bias, res);
       else if constexpr (MODE == kPlain) store_row<T, 8>((T*)p.out + m * p.ldo, n, p.N, v);
       else store_row<float, 8>(p.part + ((long)blockIdx.y * p.M + m) * p.N, n, p.N, v);
+    };
+    ColumnBias<8, GLU> bias;
+    RowPiece<T, 8> res[NG], next[NG];
+    if constexpr (MODE == kEpilogue) bias.load(p, n);
+    if (MODE == kEpilogue && p.res) {
+      auto fetch = [&](RowPiece<T, 8>(&q)[NG], int i) {
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+          const long m = mh + i + k * RI;
+          if (m < p.M && n < p.N) q[k].load((const T*)p.res + m * p.ldr, n, p.N);
+        }
+      };
+      fetch(res, 0);
+      for (int i = 0; i < kPass; i += NG * RI) {
+        if (i + NG * RI < kPass) fetch(next, i + NG * RI);
+#pragma unroll
+        for (int k = 0; k < NG; ++k) row_out(i + k * RI, bias, res[k], std::true_type{});
+#pragma unroll
+        for (int k = 0; k < NG; ++k) res[k] = next[k];
+      }
+    } else {  // (of its own: waiting for loads that are never made would wait for the stores before them)
+#pragma unroll 2
+      for (int i = 0; i < kPass; i += RI) row_out(i, bias, res[0], std::false_type{});
     }
     __builtin_amdgcn_wave_barrier();
   }
 }
 
 // the parts of the contraction added in their order, then the epilogue
-template <typename T, bool glu>
+template <typename T, int ACT>
 __global__ __launch_bounds__(kThreads) void join_kernel(const ProductArgs p) {
   constexpr int C = 4;
+  constexpr bool glu = ACT == kActSwiglu;
   const long cols = glu ? 2 * p.N : p.N, groups = (p.N + C - 1) / C;
   const long at = (long)blockIdx.x * kThreads + threadIdx.x;
   if (at >= p.M * groups) return;
@@ -473,56 +665,74 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const ProductArgs p) {
     add_row<float, C>(row, n, p.N, v);
     if (glu) add_row<float, C>(row + p.N, n, p.N, up);
   }
-  finish<T, C, glu>(p, m, n, v, up);
+  ColumnBias<C, glu> bias;
+  RowPiece<T, C> res;
+  bias.load(p, n);
+  if (p.res) {
+    res.load((const T*)p.res + m * p.ldr, n, p.N);
+    finish<T, C, ACT, true>(p, m, n, v, up, bias, res);
+  } else {
+    finish<T, C, ACT, false>(p, m, n, v, up, bias, res);
+  }
 }
 
 // ---------------------------------------------------------------------------
-// dz = act'(z) dy, with the bias's gradient: a thread takes 8 columns of the rows of its block
+// dz = act'(z) dy, with the bias's gradient: a wave takes 512 columns, 8 a lane, of a block of rows, four rows loaded
+// together; its sums are one partial row of db.  Bound by HBM bytes.
 // ---------------------------------------------------------------------------
-template <typename T>
+constexpr int kActRows = 4;
+template <typename T, bool glu>
 __global__ __launch_bounds__(kThreads) void act_bwd_kernel(const ActBwdArgs a) {
   constexpr int C = 8;
-  const bool glu = a.act == kActSwiglu;
-  const long n = ((long)blockIdx.x * kThreads + threadIdx.x) * C, width = glu ? a.ldz - a.N : a.ldz;  // (with the columns behind)
-  if (n >= width) return;
-  const long per = (a.M + a.row_blocks - 1) / a.row_blocks, r0 = blockIdx.y * per, r1 = min(a.M, r0 + per);
-  float sum[2][C];
+  typedef T vec __attribute__((ext_vector_type(C)));
+  const long n = ((long)blockIdx.x * 64 + (threadIdx.x & 63)) * C, width = glu ? a.ldz - a.N : a.ldz;  // (with the columns behind)
+  const long rb = (long)blockIdx.y * 4 + (threadIdx.x >> 6);
+  if (n >= width || rb >= a.row_blocks) return;
+  const long per = (a.M + a.row_blocks - 1) / a.row_blocks, r0 = rb * per, r1 = min(a.M, r0 + per);
+  float sum[glu ? 2 : 1][C];
 #pragma unroll
-  for (int i = 0; i < C; ++i) sum[0][i] = sum[1][i] = 0.f;
-  for (long m = r0; m < r1; ++m) {
-    float d[C], z[C], u[C];
+  for (int i = 0; i < C; ++i) sum[0][i] = sum[glu ? 1 : 0][i] = 0.f;
+  for (long m0 = r0; m0 < r1; m0 += kActRows) {
+    vec dy[kActRows];
+    KeptZ<C> z[kActRows], u[kActRows];
 #pragma unroll
-    for (int i = 0; i < C; ++i) d[i] = z[i] = u[i] = 0.f;
-    add_row<T, C>((const T*)a.dy + m * a.ldy, n, a.N, d);
-    if (a.z) add_row<T, C>((const T*)a.z + m * a.ldz, n, a.N, z);
-    if (glu) {
-      add_row<T, C>((const T*)a.z + m * a.ldz + a.N, n, a.N, u);
-      float dg[C], du[C];
+    for (int k = 0; k < kActRows; ++k) {
+      const long m = min(m0 + k, r1 - 1);
+      dy[k] = load_piece((const T*)a.dy + m * a.ldy, (int)n, (int)a.N);
+      if (a.z) z[k].load(a.z, a.M, a.ldz, m, n, a.N);
+      if (glu) u[k].load(a.z, a.M, a.ldz, m, a.N + n, 2 * a.N);
+    }
 #pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const float g = sigmoid(z[i]);
-        dg[i] = d[i] * u[i] * (g * (1.f + z[i] * (1.f - g)));
-        du[i] = d[i] * z[i] * g;
-        sum[0][i] += dg[i];
-        sum[1][i] += du[i];
+    for (int k = 0; k < kActRows; ++k) {
+      const long m = m0 + k;
+      if (m >= r1) break;
+      float d[C], du[C];
+      if constexpr (glu) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          const float gate = z[k][i], g = sigmoid(gate), dd = (float)dy[k][i];
+          // (behind the columns dy and both halves are 0)
+          d[i] = dd * u[k][i] * (g * (1.f + gate * (1.f - g)));
+          du[i] = dd * gate * g;
+          sum[1][i] += du[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < C; ++i) d[i] = (float)dy[k][i];
+        if (a.z) act_slopes<C>(a.act, z[k], d);
       }
+#pragma unroll
+      for (int i = 0; i < C; ++i) sum[0][i] += d[i];
       if (a.dz) {
-        store_row<T, C>((T*)a.dz + m * a.ldz, n, a.N, dg);
-        store_row<T, C>((T*)a.dz + m * a.ldz + a.N, n, a.ldz - a.N, du);  // (du is 0 behind the columns)
+        store_row<T, C>((T*)a.dz + m * a.ldz, n, glu ? a.N : a.ldz, d);
+        if (glu) store_row<T, C>((T*)a.dz + m * a.ldz + a.N, n, a.ldz - a.N, du);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        if (a.z) d[i] *= act_slope(a.act, z[i]);
-        sum[0][i] += d[i];
-      }
-      if (a.dz) store_row<T, C>((T*)a.dz + m * a.ldz, n, a.ldz, d);
     }
   }
   if (a.db_part) {
-    float* row = a.db_part + (long)blockIdx.y * (glu ? 2 * a.N : a.N);
+    float* row = a.db_part + rb * (glu ? 2 * a.N : a.N);
     store_row<float, C>(row, n, a.N, sum[0]);
-    if (glu) store_row<float, C>(row + a.N, n, a.N, sum[1]);
+    if (glu) store_row<float, C>(row + a.N, n, a.N, sum[glu ? 1 : 0]);
   }
 }
 
@@ -561,18 +771,19 @@ __global__ __launch_bounds__(kThreads) void pad_rows_kernel(const PadRowsArgs a)
   *gmem((s16x8*)((short*)a.dst + m * a.ldd + n)) = v;
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool DA, bool DB, int MODE, bool GLU>
+template <typename T, int BM, int BN, int WM, int WN, bool DA, bool DB, int MODE, int ACT>
 hipError_t launch_tiles(const ProductArgs& p, hipStream_t st) {
-  const long tiles = ((p.M + BM - 1) / BM) * ((p.N + (GLU ? BN / 2 : BN) - 1) / (GLU ? BN / 2 : BN));
-  hipLaunchKernelGGL((product_kernel<T, BM, BN, WM, WN, DA, DB, MODE, GLU>), dim3((unsigned)tiles, (unsigned)p.splits),
+  constexpr int NT = ACT == kActSwiglu ? BN / 2 : BN;
+  const long tiles = ((p.M + BM - 1) / BM) * ((p.N + NT - 1) / NT);
+  hipLaunchKernelGGL((product_kernel<T, BM, BN, WM, WN, DA, DB, MODE, ACT>), dim3((unsigned)tiles, (unsigned)p.splits),
                      dim3(WM * WN * 64), 0, st, p);
   return hipGetLastError();
 }
 
-template <typename T, bool DA, bool DB, int MODE, bool GLU>
+template <typename T, bool DA, bool DB, int MODE, int ACT = kActNone>
 hipError_t launch_size(const ProductArgs& p, bool large, hipStream_t st) {
-  if (large) return launch_tiles<T, 256, 256, 2, 2, DA, DB, MODE, GLU>(p, st);
-  return launch_tiles<T, 128, 128, 2, 2, DA, DB, MODE, GLU>(p, st);
+  if (large) return launch_tiles<T, 256, 256, 2, 2, DA, DB, MODE, ACT>(p, st);
+  return launch_tiles<T, 128, 128, 2, 2, DA, DB, MODE, ACT>(p, st);
 }
 
 template <typename T>
@@ -581,21 +792,23 @@ hipError_t launch_typed(int kind, const ProductArgs& p, bool large, hipStream_t 
     ProductArgs q = p;  // partial products of all rows of B
     if (p.act == kActSwiglu) q.N = 2 * p.N;
     q.act = kActNone;
-    const hipError_t e = kind == 0 ? launch_size<T, false, false, kPartial, false>(q, large, st)
-                         : kind == 1 ? launch_size<T, false, true, kPartial, false>(q, large, st)
-                                     : launch_size<T, true, true, kPartial, false>(q, large, st);
+    const hipError_t e = kind == 0 ? launch_size<T, false, false, kPartial>(q, large, st)
+                         : kind == 1 ? launch_size<T, false, true, kPartial>(q, large, st)
+                                     : launch_size<T, true, true, kPartial>(q, large, st);
     if (e != hipSuccess) return e;
     const long threads = p.M * ((p.N + 3) / 4);
     const dim3 grid((unsigned)((threads + kThreads - 1) / kThreads));
-    if (p.act == kActSwiglu) hipLaunchKernelGGL((join_kernel<T, true>), grid, dim3(kThreads), 0, st, p);
-    else hipLaunchKernelGGL((join_kernel<T, false>), grid, dim3(kThreads), 0, st, p);
+    if (p.act == kActSwiglu) hipLaunchKernelGGL((join_kernel<T, kActSwiglu>), grid, dim3(kThreads), 0, st, p);
+    else if (p.act == kActNone) hipLaunchKernelGGL((join_kernel<T, kActNone>), grid, dim3(kThreads), 0, st, p);
+    else hipLaunchKernelGGL((join_kernel<T, kActOther>), grid, dim3(kThreads), 0, st, p);
     return hipGetLastError();
   }
   if (kind == 0)
-    return p.act == kActSwiglu ? launch_size<T, false, false, kEpilogue, true>(p, large, st)
-                               : launch_size<T, false, false, kEpilogue, false>(p, large, st);
-  if (kind == 1) return launch_size<T, false, true, kPlain, false>(p, large, st);
-  return launch_size<T, true, true, kPlain, false>(p, large, st);
+    return p.act == kActSwiglu ? launch_size<T, false, false, kEpilogue, kActSwiglu>(p, large, st)
+           : p.act == kActNone ? launch_size<T, false, false, kEpilogue, kActNone>(p, large, st)
+                               : launch_size<T, false, false, kEpilogue, kActOther>(p, large, st);
+  if (kind == 1) return launch_size<T, false, true, kPlain>(p, large, st);
+  return launch_size<T, true, true, kPlain>(p, large, st);
 }
 
 constexpr int kCus = 256;
@@ -622,9 +835,19 @@ hipError_t launch_product(int kind, const ProductArgs& p, hipStream_t st) {
   return p.dtype == kBf16 ? launch_typed<bf16>(kind, q, large, st) : launch_typed<f16>(kind, q, large, st);
 }
 
+// Blocks of rows, a wave and a partial row of db each: about 16 waves a CU, 4 rows or more a block.
 int act_bwd_row_blocks(long M, long N) {
-  const long cols = (N + 8 * kThreads - 1) / (8 * kThreads);
-  return (int)std::max(1L, std::min((M + 15) / 16, std::max(1L, 2048 / cols)));
+  const long cols = (N + 511) / 512;
+  return (int)std::max(1L, std::min((M + kActRows - 1) / kActRows, std::max(1L, 16 * kCus / cols)));
+}
+
+template <typename T>
+static void launch_act_typed(const ActBwdArgs& a, hipStream_t st) {
+  const bool glu = a.act == kActSwiglu;
+  const long width = glu ? a.ldz - a.N : a.ldz;
+  const dim3 grid((unsigned)((width + 511) / 512), (unsigned)((a.row_blocks + 3) / 4));
+  if (glu) hipLaunchKernelGGL((act_bwd_kernel<T, true>), grid, dim3(kThreads), 0, st, a);
+  else hipLaunchKernelGGL((act_bwd_kernel<T, false>), grid, dim3(kThreads), 0, st, a);
 }
 
 hipError_t launch_act_bwd(const ActBwdArgs& args, hipStream_t st) {
@@ -632,10 +855,8 @@ hipError_t launch_act_bwd(const ActBwdArgs& args, hipStream_t st) {
   const bool glu = a.act == kActSwiglu;
   a.row_blocks = a.M > 0 ? act_bwd_row_blocks(a.M, a.N) : 0;
   if (a.row_blocks) {
-    const long width = glu ? a.ldz - a.N : a.ldz;
-    const dim3 grid((unsigned)((width + 8 * kThreads - 1) / (8 * kThreads)), (unsigned)a.row_blocks);
-    if (a.dtype == kBf16) hipLaunchKernelGGL(act_bwd_kernel<bf16>, grid, dim3(kThreads), 0, st, a);
-    else hipLaunchKernelGGL(act_bwd_kernel<f16>, grid, dim3(kThreads), 0, st, a);
+    if (a.dtype == kBf16) launch_act_typed<bf16>(a, st);
+    else launch_act_typed<f16>(a, st);
   }
   if (a.db)
     hipLaunchKernelGGL(bias_sum_kernel, dim3((unsigned)(((glu ? 2 * a.N : a.N) + 63) / 64)), dim3(1024), 0, st, a);

@@ -43,7 +43,8 @@ def _forward(x, weight, bias, residual, act, keep_z):
     r2 = rows_of(residual) if residual is not None else None
     dev = x.device
     y = torch.empty(*x.shape[:-1], N, device=dev, dtype=x.dtype)
-    z = torch.empty(M, -(-outs // 8) * 8, device=dev, dtype=x.dtype) if keep_z and act else None
+    # what the activation's backward reads, in 24 bits
+    z = torch.empty(3 * M * (-(-outs // 8) * 8), device=dev, dtype=torch.uint8) if keep_z and act else None
     xp, wp = _operand(x2), _operand(w2)
     n = entry("ccq_linear_workspace_bytes")(M, N, K, act)
     ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
