@@ -33,7 +33,7 @@ int norm_bwd_blocks(long rows, int D, int dtype);
 hipError_t launch_norm_fwd(const NormArgs& a, hipStream_t st);
 hipError_t launch_norm_bwd(const NormArgs& a, hipStream_t st);
 hipError_t launch_logprobs(bool bwd, const LogprobArgs& a, hipStream_t st);
-void product_plan(long M, long N, long K, bool* large, int* splits);
+void product_plan(long M, long N, long K, int* side, int* splits);
 hipError_t launch_product(int kind, const ProductArgs& p, hipStream_t st);
 int act_bwd_row_blocks(long M, long N);
 hipError_t launch_act_bwd(const ActBwdArgs& a, hipStream_t st);
@@ -1624,9 +1624,8 @@ constexpr long kMaxSide = 1L << 30;
 long round8(long n) { return (n + 7) & ~7L; }
 long linear_outs(int64_t N, int act) { return act == CCQ_ACT_SWIGLU ? 2 * N : N; }
 size_t partial_bytes(long M, long N, long K) {
-  bool large;
-  int splits;
-  product_plan(M, N, K, &large, &splits);
+  int side, splits;
+  product_plan(M, N, K, &side, &splits);
   return splits > 1 ? (size_t)splits * M * N * sizeof(float) : 0;
 }
 bool rows16(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }

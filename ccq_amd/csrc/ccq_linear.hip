@@ -270,7 +270,7 @@ constexpr int kStep = 64;  // contraction elements a step
 
 // One operand's tile of a step in LDS: R rows of the product by 64 contraction elements.
 //   along the rows (DOWN = false): R rows of 128 bytes, 16-byte piece s of row r at piece s ^ swz(r)
-//   down the rows  (DOWN = true):  64 rows of 2 R bytes, piece s of row k at piece s ^ (swz(k) << 1)
+//   down the rows  (DOWN = true):  64 rows of 2 R bytes, piece s of row k at piece s ^ swz(k)
 // so that the sixteen pieces that a fragment read takes at once lie in different banks.  Direct loads write 1 KiB
 // (64 pieces) each, in LDS order: the swizzle is in the address that a lane reads.
 // A buffer resource bounds every load by the operand's end; what lies behind it comes as zeros.
@@ -313,7 +313,9 @@ constexpr unsigned kNowhere = 0x80000000u;  // behind every resource's end
 // swizzle of product row r of an operand read in consecutive rows (A), or in the order of column pairs (B)
 __device__ __forceinline__ int swz_a(int r) { return (r >> 1) & 7; }
 __device__ __forceinline__ int swz_b(int n) { return ((n >> 1) & 1) | (((n >> 3) & 3) << 1); }
-__device__ __forceinline__ int swz_k(int k) { return (k & 3) | (((k >> 3) & 1) << 2); }
+// of contraction row k of an operand stored down the rows, R columns a row
+template <int R>
+__device__ __forceinline__ int swz_down(int k) { return ((k & 3) | (((k >> 3) & 1) << 2)) << 1 & (R / 8 - 1); }
 
 // Loads of a tile: wave w of NW takes instructions w * PER .. (consecutive pieces of LDS).
 template <int R, bool DOWN, bool B, int NW>
@@ -329,7 +331,7 @@ struct TileLoad {
       const int q = (wave * PER + i) * 64 + l;  // piece of the tile in LDS order
       if (DOWN) {
         const int k = q / (R / 8), s = q % (R / 8);
-        off[i] = (unsigned)(k * ld * 2) + ((s ^ (swz_k(k) << 1)) << 4);
+        off[i] = (unsigned)(k * ld * 2) + ((s ^ swz_down<R>(k)) << 4);
       } else {
         const int r = q >> 3, s = q & 7;
         off[i] = (unsigned)(r * ld * 2) + ((s ^ (B ? swz_b(r) : swz_a(r))) << 4);
@@ -376,7 +378,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
   constexpr int HALF = BN / WN / 2;  // swiglu: gates of a wave
   static_assert(!GLU || (!DB && MODE == kEpilogue), "gates and ups of one wave");
   static_assert(TM == TN, "one fragment of each operand between two rows of products");
-  constexpr int kPass = 64, kRow = TN * 16 + 4;  // rows of a wave in the epilogue at a time, floats a row
+  constexpr int kPass = TM < 4 ? TM * 16 : 64, kRow = TN * 16 + 4;  // rows of a wave in the epilogue at a time, floats a row
   constexpr unsigned kOut = NW * kPass * kRow * 4;
   __shared__ __attribute__((aligned(1024))) char smem[kRing > kOut ? kRing : kOut];
   const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -443,7 +445,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     const int k = 8 * g + (r >> 2), s = wm * TM * 2 + ((r >> 1) & 1);
 #pragma unroll
     for (int it = 0; it < TM; ++it)
-      fa[it] = lds0 + k * (BM * 2) + (((s + 2 * it) ^ (swz_k(k) << 1)) << 4) + 8 * (r & 1);
+      fa[it] = lds0 + k * (BM * 2) + (((s + 2 * it) ^ swz_down<BM>(k)) << 4) + 8 * (r & 1);
   } else {
     const int row = wm * TM * 16 + r;
 #pragma unroll
@@ -453,7 +455,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     const int k = 8 * g + (r >> 2), s = wn * TN * 2 + ((r >> 1) & 1);
 #pragma unroll
     for (int j = 0; j < TN; ++j)
-      fb[j] = lds0 + 3 * kA + k * (BN * 2) + (((s + 2 * j) ^ (swz_k(k) << 1)) << 4) + 8 * (r & 1);
+      fb[j] = lds0 + 3 * kA + k * (BN * 2) + (((s + 2 * j) ^ swz_down<BN>(k)) << 4) + 8 * (r & 1);
   } else {
     const int row = wn * TN * 16 + 8 * (r >> 2) + (r & 3);
 #pragma unroll
@@ -484,7 +486,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
   };
   // products between two loads, and between two fragment reads: the reads end at three quarters of the half, so that
   // the last ones have arrived by its end
-  constexpr int kLoadGap = TM * TN / (TM + TN), kReadGap = TM * TN * 3 / 4 / (TM + TN);
+  constexpr int kLoadGap = TM * TN / (TM + TN), kReadGap = std::max(1, TM * TN * 3 / 4 / (TM + TN));
 
   f32x4 acc[TM][TN];
   auto clear = [&] {
@@ -596,15 +598,15 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
   lds_barrier();
   float* mine = (float*)(smem + wave * kPass * kRow * 4);
 #pragma unroll
-  for (int h = 0; h < TM / 4; ++h) {
+  for (int h = 0; h < TM * 16 / kPass; ++h) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kPass / 16; ++i)
 #pragma unroll
       for (int j = 0; j < TN; ++j)
-        *(f32x4*)(mine + (16 * i + r) * kRow + (DB ? 16 * j + 4 * g : 32 * (j >> 1) + 4 * (j & 1) + 8 * g)) = acc[4 * h + i][j];
+        *(f32x4*)(mine + (16 * i + r) * kRow + (DB ? 16 * j + 4 * g : 32 * (j >> 1) + 4 * (j & 1) + 8 * g)) = acc[h * (kPass / 16) + i][j];
     __builtin_amdgcn_wave_barrier();  // (LDS operations of a wave are in order)
     constexpr int WC = GLU ? HALF : TN * 16, PR = WC / 8;  // output columns of the wave, pieces of a row
-    constexpr int RI = 64 / PR, NG = 4;                    // rows at a time, and how often between the residual's loads
+    constexpr int RI = 64 / PR, NG = kPass / RI < 4 ? kPass / RI : 4;                    // rows at a time, and how often between the residual's loads
     const int c = l % PR * 8;
     const long n = n0 + wn * WC + c, mh = m0 + wm * TM * 16 + h * kPass + l / PR;
     auto row_out = [&](int i, const auto& bias, const RowPiece<T, 8>& res, auto with_res) {
@@ -781,20 +783,21 @@ hipError_t launch_tiles(const ProductArgs& p, hipStream_t st) {
 }
 
 template <typename T, bool DA, bool DB, int MODE, int ACT = kActNone>
-hipError_t launch_size(const ProductArgs& p, bool large, hipStream_t st) {
-  if (large) return launch_tiles<T, 256, 256, 2, 2, DA, DB, MODE, ACT>(p, st);
-  return launch_tiles<T, 128, 128, 2, 2, DA, DB, MODE, ACT>(p, st);
+hipError_t launch_size(const ProductArgs& p, int side, hipStream_t st) {
+  if (side == 256) return launch_tiles<T, 256, 256, 2, 2, DA, DB, MODE, ACT>(p, st);
+  if (side == 128) return launch_tiles<T, 128, 128, 2, 2, DA, DB, MODE, ACT>(p, st);
+  return launch_tiles<T, 64, 64, 2, 2, DA, DB, MODE, ACT>(p, st);
 }
 
 template <typename T>
-hipError_t launch_typed(int kind, const ProductArgs& p, bool large, hipStream_t st) {
+hipError_t launch_typed(int kind, const ProductArgs& p, int side, hipStream_t st) {
   if (p.splits > 1) {
     ProductArgs q = p;  // partial products of all rows of B
     if (p.act == kActSwiglu) q.N = 2 * p.N;
     q.act = kActNone;
-    const hipError_t e = kind == 0 ? launch_size<T, false, false, kPartial>(q, large, st)
-                         : kind == 1 ? launch_size<T, false, true, kPartial>(q, large, st)
-                                     : launch_size<T, true, true, kPartial>(q, large, st);
+    const hipError_t e = kind == 0 ? launch_size<T, false, false, kPartial>(q, side, st)
+                         : kind == 1 ? launch_size<T, false, true, kPartial>(q, side, st)
+                                     : launch_size<T, true, true, kPartial>(q, side, st);
     if (e != hipSuccess) return e;
     const long threads = p.M * ((p.N + 3) / 4);
     const dim3 grid((unsigned)((threads + kThreads - 1) / kThreads));
@@ -804,35 +807,60 @@ hipError_t launch_typed(int kind, const ProductArgs& p, bool large, hipStream_t 
     return hipGetLastError();
   }
   if (kind == 0)
-    return p.act == kActSwiglu ? launch_size<T, false, false, kEpilogue, kActSwiglu>(p, large, st)
-           : p.act == kActNone ? launch_size<T, false, false, kEpilogue, kActNone>(p, large, st)
-                               : launch_size<T, false, false, kEpilogue, kActOther>(p, large, st);
-  if (kind == 1) return launch_size<T, false, true, kPlain>(p, large, st);
-  return launch_size<T, true, true, kPlain>(p, large, st);
+    return p.act == kActSwiglu ? launch_size<T, false, false, kEpilogue, kActSwiglu>(p, side, st)
+           : p.act == kActNone ? launch_size<T, false, false, kEpilogue, kActNone>(p, side, st)
+                               : launch_size<T, false, false, kEpilogue, kActOther>(p, side, st);
+  if (kind == 1) return launch_size<T, false, true, kPlain>(p, side, st);
+  return launch_size<T, true, true, kPlain>(p, side, st);
 }
 
 constexpr int kCus = 256;
 
 }  // namespace
 
-// Tile and parts of the contraction of a product of M x N outputs (swiglu: N = all rows of B) over K.
-void product_plan(long M, long N, long K, bool* large, int* splits) {
-  const long t256 = ((M + 255) / 256) * ((N + 255) / 256), t128 = ((M + 127) / 128) * ((N + 127) / 128);
+// Tile side and parts of the contraction of a product of M x N outputs (swiglu: N = all rows of B) over K, by what a
+// call is expected to take, in us.  A CU holds one workgroup of 256 x 256 (its LDS), two of 128 x 128 or four of 64 x 64;
+// `step` is a step's time beside that many of its kind, `fixed` what a workgroup takes besides (launch, the first
+// loads, the epilogue), measured:
+//   256: 8192 x 4096 over 4096 202 us, 32768 x 1024 over 2816 153, 16384 x 5632 over 1024 189 (128: 243, 191, 193)
+//   128: 2048 x 2048 over 2048 22.5, 8192 x 1024 over 1024 21.8 (256: 42, 30.8; 64: 28, 29.5)
+//    64: 1536 x 784 over 1000 11.3, 16 x 5632 over 1024 8.1 (128 in one part: 14.5, in four: 9.3)
+// Parts of the contraction go through fp32 partial sums: a second launch (3.5), a read of each part, one
+// after the other, and their bytes (10 TB/s: the last-level cache).  2816 x 1024 over 32768 by 256 in five parts 185, by 128 in one 340.
+void product_plan(long M, long N, long K, int* side, int* splits) {
+  static const struct {
+    int side, per_cu;
+    float step0, step1, fixed;
+  } kinds[] = {{256, 1, 0.f, 1.5f, 7.5f}, {128, 2, 0.1f, 0.43f, 4.5f}, {64, 4, 0.1f, 0.19f, 3.5f}};
   const long steps = (K + kStep - 1) / kStep;
-  *large = t256 >= kCus / 2;
+  float best = 0.f;
+  *side = 64;
   *splits = 1;
-  if (!*large && t128 > 0 && t128 < kCus) *splits = (int)std::max(1L, std::min({kCus / t128, steps / 4, 16L}));
+  if (M <= 0 || N <= 0) return;
+  for (const auto& k : kinds) {
+    const long tiles = ((M + k.side - 1) / k.side) * ((N + k.side - 1) / k.side);
+    for (int sp = 1; sp <= 16 && (sp == 1 || sp * 2 <= steps); ++sp) {
+      const long w = (tiles * sp + kCus - 1) / kCus, full = w / k.per_cu, rest = w % k.per_cu, n = (steps + sp - 1) / sp;
+      float t = full * (n * (k.step0 + k.step1 * k.per_cu) + k.fixed);
+      if (rest) t += n * (k.step0 + k.step1 * rest) + k.fixed;
+      if (sp > 1) t += 3.5f + sp * (0.15f + 8e-7f * M * N);
+      if (best == 0.f || t < best) {
+        best = t;
+        *side = k.side;
+        *splits = sp;
+      }
+    }
+  }
 }
 
 // kind 0: y = act(x W^T + b) + r; 1: dx = dz W; 2: dW = dz^T x
 hipError_t launch_product(int kind, const ProductArgs& p, hipStream_t st) {
   if (p.M <= 0 || p.N <= 0) return hipSuccess;
-  bool large;
-  int splits;
-  product_plan(p.M, p.act == kActSwiglu ? 2 * p.N : p.N, p.K, &large, &splits);
+  int side, splits;
+  product_plan(p.M, p.act == kActSwiglu ? 2 * p.N : p.N, p.K, &side, &splits);
   ProductArgs q = p;
   q.splits = splits;
-  return p.dtype == kBf16 ? launch_typed<bf16>(kind, q, large, st) : launch_typed<f16>(kind, q, large, st);
+  return p.dtype == kBf16 ? launch_typed<bf16>(kind, q, side, st) : launch_typed<f16>(kind, q, side, st);
 }
 
 // Blocks of rows, a wave and a partial row of db each: about 16 waves a CU, 4 rows or more a block.
