@@ -66,9 +66,10 @@ def test_norm_abi_refusals():
     assert bwd(ldy=10) == SHAPE and bwd(layer=0) == SHAPE
     assert bwd(x=None) == NULL and bwd(mean=None) == NULL and bwd(rstd=None) == NULL and bwd(ws=None) == NULL
     assert bwd(ws=ctypes.c_void_p(0x1008)) == ALIGN and bwd(dx=ODD) == ALIGN
-    # partial rows of dw and db: one for each workgroup, at most 512
+    # partial rows of dw and db: one for each workgroup, at most 512 (1024 where a lane holds one piece of a row)
     assert lib.ccq_norm_bwd_workspace_bytes(100000, 1024, 0) == 2 * 512 * 1024 * 4
     assert lib.ccq_norm_bwd_workspace_bytes(8, 1024, 0) == 2 * 2 * 1024 * 4
+    assert lib.ccq_norm_bwd_workspace_bytes(100000, 2048, 0) == 2 * 1024 * 2048 * 4
 
 
 def test_token_logprobs_refusals():
