@@ -38,7 +38,7 @@ def stream_on(x: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(x.device.index)
 
 
-def rows_of(x: torch.Tensor) -> torch.Tensor:
+def rows_of(x: torch.Tensor) -> torch.Tensor:  # (host time counts: the common case first)
     """``x [..., D]`` as ``[rows, D]`` with consecutive elements and rows that do not overlap: a view where the
     strides allow one, a copy otherwise."""
     if x.dim() != 2:
@@ -59,6 +59,11 @@ def stride_of(x: torch.Tensor) -> int:
 def current(x: torch.Tensor) -> bool:
     """Whether x's device is the current one, which the C entry points ask for."""
     return x.device.index == torch.cuda.current_device()
+
+
+def like(x: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of x's shape, type and device."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def require_gpu(who: str, x: torch.Tensor) -> None:

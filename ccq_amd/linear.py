@@ -31,7 +31,7 @@ def _operand(x2: torch.Tensor) -> torch.Tensor:
     if K % 8 == 0 and ld % 8 == 0 and ld <= MAX_STRIDE and x2.data_ptr() % 16 == 0:
         return x2
     ldd = -(-K // 8) * 8
-    out = torch.empty(rows, ldd, device=x2.device, dtype=x2.dtype)
+    out = x2.new_empty(rows, ldd)
     call("ccq_pad_rows", x2.data_ptr(), ld, out.data_ptr(), ldd, rows, K, stream_on(x2))
     return out
 
@@ -41,13 +41,12 @@ def _forward(x, weight, bias, residual, act, keep_z):
     (M, K), outs = x2.shape, w2.shape[0]
     N = outs // 2 if act == SWIGLU else outs
     r2 = rows_of(residual) if residual is not None else None
-    dev = x.device
-    y = torch.empty(*x.shape[:-1], N, device=dev, dtype=x.dtype)
+    y = x.new_empty(*x.shape[:-1], N)
     # what the activation's backward reads, in 24 bits
-    z = torch.empty(3 * M * (-(-outs // 8) * 8), device=dev, dtype=torch.uint8) if keep_z and act else None
+    z = x.new_empty(3 * M * (-(-outs // 8) * 8), dtype=torch.uint8) if keep_z and act else None
     xp, wp = _operand(x2), _operand(w2)
     n = entry("ccq_linear_workspace_bytes")(M, N, K, act)
-    ws = torch.empty(n, device=dev, dtype=torch.uint8) if n else None
+    ws = x.new_empty(n, dtype=torch.uint8) if n else None
     call("ccq_linear_fwd", xp.data_ptr(), stride_of(xp), wp.data_ptr(), stride_of(wp), address(bias),
          DTYPES[bias.dtype if bias is not None else x.dtype], address(r2), stride_of(r2) if r2 is not None else 0,
          y.data_ptr(), address(z), address(ws), M, N, K, act, DTYPES[x.dtype], stream_on(x))
@@ -78,15 +77,15 @@ class FusedLinearFunction(torch.autograd.Function):
         dx = dw = db = None
         if need_x or need_w or need_b:
             (M, K), outs = x2.shape, w2.shape[0]
-            dev, dtype = x2.device, x2.dtype
+            dtype = x2.dtype
             d2 = rows_of(dy)
-            dx = torch.empty(shape, device=dev, dtype=dtype) if need_x else None
-            dw = torch.empty(outs, K, device=dev, dtype=dtype) if need_w else None
-            db = torch.empty(outs, device=dev, dtype=bdtype) if need_b else None
+            dx = x2.new_empty(shape) if need_x else None
+            dw = x2.new_empty(outs, K) if need_w else None
+            db = x2.new_empty(outs, dtype=bdtype) if need_b else None
             xp = _operand(x2) if need_w else None
             wp = _operand(w2) if need_x else None
             ld = -(-K // 8) * 8
-            ws = torch.empty(entry("ccq_linear_bwd_workspace_bytes")(M, N, K, act), device=dev, dtype=torch.uint8)
+            ws = x2.new_empty(entry("ccq_linear_bwd_workspace_bytes")(M, N, K, act), dtype=torch.uint8)
             call("ccq_linear_bwd", address(xp), stride_of(xp) if need_w else ld, address(wp),
                  stride_of(wp) if need_x else ld, address(z), d2.data_ptr(), stride_of(d2), address(dx), address(dw),
                  address(db), DTYPES[bdtype if bdtype is not None else dtype], ws.data_ptr(), M, N, K, act,

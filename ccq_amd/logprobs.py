@@ -32,13 +32,12 @@ def _forward(logits, ids, k, ignore, keep):
     maximum and log sum."""
     x2 = rows_of(logits)
     rows, V = x2.shape
-    dev = logits.device
-    i2 = ids.reshape(-1).contiguous()
-    logp = torch.empty(ids.shape, device=dev, dtype=torch.float32)
-    ent = torch.empty(ids.shape, device=dev, dtype=torch.float32)
-    stats = torch.empty(rows, 2, device=dev, dtype=torch.float32) if keep else None
-    top = torch.empty(*ids.shape, k, device=dev, dtype=torch.float32) if k else None
-    top_ids = torch.empty(*ids.shape, k, device=dev, dtype=torch.int64) if k else None
+    i2 = ids.contiguous()
+    logp = x2.new_empty(ids.shape, dtype=torch.float32)
+    ent = x2.new_empty(ids.shape, dtype=torch.float32)
+    stats = x2.new_empty(2 * rows, dtype=torch.float32) if keep else None
+    top = x2.new_empty(*ids.shape, k, dtype=torch.float32) if k else None
+    top_ids = x2.new_empty(*ids.shape, k, dtype=torch.int64) if k else None
     call("ccq_token_logprobs_fwd", x2.data_ptr(), stride_of(x2), i2.data_ptr(), logp.data_ptr(), ent.data_ptr(),
          address(stats), address(top), address(top_ids), rows, V, k, ignore, DTYPES[logits.dtype], stream_on(logits))
     return logp, ent, top, top_ids, x2, i2, stats
@@ -69,7 +68,7 @@ class TokenLogprobsFunction(torch.autograd.Function):
     @staticmethod
     def _backward(ctx, x2, i2, ent, stats, dlogp, dent):
         shape, ignore = ctx.meta
-        dx = torch.empty(shape, device=x2.device, dtype=x2.dtype)
+        dx = x2.new_empty(shape)
         dlogp = dlogp.contiguous() if dlogp is not None else None
         dent = dent.contiguous() if dent is not None else None
         call("ccq_token_logprobs_bwd", x2.data_ptr(), stride_of(x2), i2.data_ptr(), ent.data_ptr(), stats.data_ptr(),

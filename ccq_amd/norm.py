@@ -12,8 +12,8 @@ from typing import Optional, Tuple, Union
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._rows import (DTYPES, address, call, current, entry, needs_grad, require_gpu, require_on, rows_of, stream_on,
-                    stride_of)
+from ._rows import (DTYPES, address, call, current, entry, like, needs_grad, require_gpu, require_on, rows_of,
+                    stream_on, stride_of)
 
 __all__ = ["layer_norm", "rms_norm", "BlockNormFunction"]
 
@@ -26,9 +26,9 @@ def _forward(x, residual, weight, bias, layer, eps, keep):
     x2 = rows_of(x)
     r2 = rows_of(residual) if residual is not None else None
     rows, D = x2.shape
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    s = torch.empty(x.shape, device=x.device, dtype=x.dtype) if r2 is not None else None
-    stats = torch.empty(2 * rows, device=x.device, dtype=torch.float32) if keep else None
+    y = like(x)
+    s = like(x) if r2 is not None else None
+    stats = x.new_empty(2 * rows, dtype=torch.float32) if keep else None
     mean = address(stats)
     wdtype = DTYPES[weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype]
     call("ccq_norm_fwd", x2.data_ptr(), stride_of(x2), address(r2), stride_of(r2) if r2 is not None else 0,
@@ -66,19 +66,18 @@ class BlockNormFunction(torch.autograd.Function):
         need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
         x2 = rows_of(rows_in)
         rows, D = x2.shape
-        dev, dtype = x2.device, x2.dtype
+        dtype = x2.dtype
         if dy is None:
-            dy = torch.zeros(shape, device=dev, dtype=dtype)  # (only the stream was used)
+            dy = x2.new_zeros(shape)  # (only the stream was used)
         d2 = rows_of(dy)
         s2 = rows_of(ds) if ds is not None else None
         wdt = weight.dtype if weight is not None else bdtype if bdtype is not None else dtype
-        dx = torch.empty(shape, device=dev, dtype=dtype) if need_x or need_r else None
-        dw = torch.empty(D, device=dev, dtype=wdt) if need_w else None
-        db = torch.empty(D, device=dev, dtype=wdt) if need_b else None
+        dx = x2.new_empty(shape) if need_x or need_r else None
+        dw = x2.new_empty(D, dtype=wdt) if need_w else None
+        db = x2.new_empty(D, dtype=wdt) if need_b else None
         ws = None
         if need_w or need_b:
-            ws = torch.empty(entry("ccq_norm_bwd_workspace_bytes")(rows, D, DTYPES[dtype]), device=dev,
-                             dtype=torch.uint8)
+            ws = x2.new_empty(entry("ccq_norm_bwd_workspace_bytes")(rows, D, DTYPES[dtype]), dtype=torch.uint8)
         mean = stats.data_ptr()
         call("ccq_norm_bwd", x2.data_ptr(), stride_of(x2), address(weight), mean if layer else 0, mean + 4 * rows,
              d2.data_ptr(), stride_of(d2), address(s2), stride_of(s2) if s2 is not None else 0, address(dx),
