@@ -273,38 +273,41 @@ constexpr int kStep = 64;  // contraction elements a step
 //   down the rows  (DOWN = true):  64 rows of 2 R bytes, piece s of row k at piece s ^ swz(k)
 // so that the sixteen pieces that a fragment read takes at once lie in different banks.  Direct loads write 1 KiB
 // (64 pieces) each, in LDS order: the swizzle is in the address that a lane reads.
-// A buffer resource bounds every load by the operand's end; what lies behind it comes as zeros.
-struct Operand {
-  const char* base;  // first element of the tile in the step
-  long left;         // bytes from there to the operand's end
-};
-__device__ __forceinline__ u32x4 resource(const Operand& o) {
-  // (compared by words: a 64-bit comparison leaves the scalar unit.  Whatever came from the vector unit all the same
-  // is brought back, and settled is called before such a resource is used.)
-  const int hi = (int)(o.left >> 32);
-  const unsigned lo = (unsigned)o.left;
-  const unsigned n = hi < 0 ? 0u : hi > 0 ? 0x7fffffffu : lo > 0x7fffffffu ? 0x7fffffffu : lo;
-  return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)(size_t)o.base),
-               (unsigned)__builtin_amdgcn_readfirstlane((int)((size_t)o.base >> 32)) & 0xffffu,
-               (unsigned)__builtin_amdgcn_readfirstlane((int)n), 0x00020000u};
+// A buffer resource bounds every load by the tile's end (along the rows: of its last row; down them: of the step's last
+// row's columns); what lies behind comes as zeros.
+__device__ __forceinline__ u32x4 resource(size_t base, unsigned bytes) {
+  // (uniform all of it; whatever the compiler left in the vector unit all the same is brought back, and settled is called
+  // before the resource is used)
+  return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)base), (unsigned)__builtin_amdgcn_readfirstlane((int)(base >> 32)),
+               (unsigned)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
 }
 // A scalar register that the vector unit wrote may be read by a memory instruction five wait states later; the compiler
 // does not look into the instructions below.
 __device__ __forceinline__ void settled(u32x4& r) { asm volatile("s_nop 4" : "+s"(r)); }
-__device__ __forceinline__ void load_piece_lds(const u32x4& r, unsigned off, unsigned m0) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(off), "s"(r) : "memory", "m0");
+// A direct load of 64 pieces in two instructions, since M0 is read one wait state after it is written: between them
+// stands a product, or a wait.
+__device__ __forceinline__ void load_to(unsigned lds, int i) { asm volatile("s_add_u32 m0, %0, %1" ::"s"(lds), "i"(i * 1024) : "m0", "scc"); }
+__device__ __forceinline__ void load_from(const u32x4& r, unsigned off) {
+  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r) : "memory");
 }
-// The whole steps of a workgroup, from some step on and round to it again.
+// The whole steps of a workgroup's contraction, from step `turn` on and round to it again; behind the last one the
+// resource is empty.  Few scalar instructions and no branch: it runs between two products.
+template <bool DOWN>
 struct StepStream {
-  Operand o;
-  long step, wrap;   // bytes of a step, of all of them
-  int ahead, until;  // steps not yet asked for, steps to the end of the whole ones
-  __device__ u32x4 next() {  // (selects, no branch: it runs between two products; behind the last step loads bring zeros)
-    const u32x4 r = resource({o.base, ahead > 0 ? o.left : 0});
+  size_t base;           // of the step to come
+  long step, back;       // bytes to the next step, from the last to the first
+  unsigned bytes, last;  // along: to the tile's end, bytes of a round; down: of a step, of the last one
+  int ahead, until;      // steps not yet asked for, steps to the end of the whole ones
+  __device__ StepStream(size_t first, long step, int whole, int turn, unsigned bytes, unsigned last)
+      : base(first + turn * step), step(step), back(-(whole - 1) * step), bytes(DOWN ? bytes : bytes - turn * 128),
+        last(DOWN ? last : (whole - 1) * 128), ahead(whole), until(whole - turn) {}
+  __device__ u32x4 next() {
+    const bool end = until == 1;
+    const u32x4 r = resource(base, ahead <= 0 ? 0u : DOWN && end ? last : bytes);
+    base += end ? back : step;
+    if (!DOWN) bytes += end ? last : -128u;
     --ahead;
     --until;
-    const long d = step - (until == 0 ? wrap : 0);
-    o = {o.base + d, o.left - d};
     return r;
   }
 };
@@ -338,14 +341,19 @@ struct TileLoad {
       }
     }
   }
-  // instruction i of the step at `stage` (bytes); `limit` < 64: contraction elements from there on as zeros
-  __device__ void issue(const u32x4& r, int i, unsigned stage, int limit, int wave, int l) const {
-    unsigned f = off[i];
-    if (!DOWN && limit < kStep) {
-      const int q = (wave * PER + i) * 64 + l, row = q >> 3;
-      if ((((q & 7) ^ (B ? swz_b(row) : swz_a(row))) << 3) >= limit) f = kNowhere;
+  // all of a step at `stage` (bytes); contraction elements at and behind `limit` < 64 of an along operand as zeros
+  __device__ void issue(const u32x4& r, unsigned stage, int limit, int wave, int l) const {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      unsigned f = off[i];
+      if (!DOWN && limit < kStep) {
+        const int q = (wave * PER + i) * 64 + l, row = q >> 3;
+        if ((((q & 7) ^ (B ? swz_b(row) : swz_a(row))) << 3) >= limit) f = kNowhere;
+      }
+      load_to(lds + stage, i);
+      asm volatile("s_nop 0");
+      load_from(r, f);
     }
-    load_piece_lds(r, f, lds + stage + i * 1024);
   }
 };
 
@@ -405,37 +413,34 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
   LoadB lb;
   la.init(lds0, wave, l, p.lda);
   lb.init(lds0 + 3 * kA, wave, l, p.ldb);
-  Operand oa, ob;
-  {
-    // elements of the operands: to the end of the last row's last whole piece
-    const long nb = GLU ? 2 * p.N : p.N;
-    const long ea = ((DA ? p.K : p.M) - 1) * p.lda + (((DA ? p.M : p.K) + 7) & ~7L);
-    const long eb = ((DB ? p.K : nb) - 1) * p.ldb + (((DB ? nb : p.K) + 7) & ~7L);
-    const long fa = DA ? (long)s0 * kStep * p.lda + m0 : m0 * p.lda + (long)s0 * kStep;
-    oa = {(const char*)p.a + fa * 2, (ea - fa) * 2};
-    long fb = DB ? (long)s0 * kStep * p.ldb + n0 : n0 * p.ldb + (long)s0 * kStep;
-    if constexpr (GLU) {
-      // tile row 2 HALF w + c of B: gate n0 + HALF w + c for c < HALF, up n0 + HALF w + c - HALF behind
-      static_assert(LoadB::PER * 8 == HALF, "a wave loads gates or ups");
-      if (wave & 1) fb += p.N * p.ldb;
-#pragma unroll
-      for (int i = 0; i < LoadB::PER; ++i) {
-        const int r = ((wave * LoadB::PER + i) * 64 + l) >> 3;
-        lb.off[i] = (unsigned)((r / (2 * HALF) * HALF + r % HALF) * p.ldb * 2) + (((l & 7) ^ swz_b(r)) << 4);
-      }
-    }
-    ob = {(const char*)p.b + fb * 2, (eb - fb) * 2};
-  }
-  const long stepA = (DA ? kStep * p.lda : kStep) * 2, stepB = (DB ? kStep * p.ldb : kStep) * 2;
   // Rows of an operand that lie a multiple of 4 KiB apart meet in one channel of the L2 at any one step.  So the tile
   // rows of a band begin their contraction at different steps, 256 bytes apart, and come round to them at its end;
   // those of one tile row keep together and find its operand in the L2.  (8192^3 forward: 849 -> 788 us; contractions
   // of few steps gain nothing and lose the operands' meeting in the L2: 16384 x 5632 over 1024, 187 -> 193 us.)
   const int turn = BM == 256 && whole >= 32 ? 2 * (int)(in % rows) : 0;
-  const long wrapA = whole * stepA, wrapB = whole * stepB;
-  const Operand ta = {oa.base + wrapA, oa.left - wrapA}, tb = {ob.base + wrapB, ob.left - wrapB};  // the end's
-  StepStream sa{{oa.base + turn * stepA, oa.left - turn * stepA}, stepA, wrapA, whole, whole - turn};
-  StepStream sb{{ob.base + turn * stepB, ob.left - turn * stepB}, stepB, wrapB, whole, whole - turn};
+  const long stepA = (DA ? kStep * p.lda : kStep) * 2, stepB = (DB ? kStep * p.ldb : kStep) * 2;
+  const size_t pa = (size_t)p.a + (DA ? (long)s0 * kStep * p.lda + m0 : m0 * p.lda + (long)s0 * kStep) * 2;
+  size_t pb = (size_t)p.b + (DB ? (long)s0 * kStep * p.ldb + n0 : n0 * p.ldb + (long)s0 * kStep) * 2;
+  if constexpr (GLU) {
+    // tile row 2 HALF w + c of B: gate n0 + HALF w + c for c < HALF, up n0 + HALF w + c - HALF behind
+    static_assert(LoadB::PER * 8 == HALF, "a wave loads gates or ups");
+    if (wave & 1) pb += p.N * p.ldb * 2;
+#pragma unroll
+    for (int i = 0; i < LoadB::PER; ++i) {
+      const int r = ((wave * LoadB::PER + i) * 64 + l) >> 3;
+      lb.off[i] = (unsigned)((r / (2 * HALF) * HALF + r % HALF) * p.ldb * 2) + (((l & 7) ^ swz_b(r)) << 4);
+    }
+  }
+  // bytes from a tile's first element to the end of the last of `n` rows, which has `cols` columns left and is whole
+  // pieces to its end
+  auto extent = [](long n, long ld, long cols) { return (unsigned)(((n - 1) * ld + ((cols + 7) & ~7L)) * 2); };
+  const long left = p.K - (long)s0 * kStep, end = (long)kStep * (whole - 1);  // contraction from here on; to the last whole step
+  const StepStream<DA> first_a(pa, stepA, whole, turn, DA ? extent(kStep, p.lda, p.M - m0) : extent(min((long)BM, p.M - m0), p.lda, left),
+                               extent(min((long)kStep, left - end), p.lda, p.M - m0));
+  const StepStream<DB> first_b(pb, stepB, whole, turn, DB ? extent(kStep, p.ldb, p.N - n0) : extent(min((long)NT, p.N - n0), p.ldb, left),
+                               extent(min((long)kStep, left - end), p.ldb, p.N - n0));
+  StepStream<DA> sa = first_a;
+  StepStream<DB> sb = first_b;
   u32x4 ra, rb;
 
   // fragment addresses of this lane in stage 0
@@ -505,14 +510,12 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     auto load_a = [&](unsigned stage) {
       ra = sa.next();
       settled(ra);
-#pragma unroll
-      for (int i = 0; i < TM; ++i) la.issue(ra, i, stage, kStep, wave, l);
+      la.issue(ra, stage, kStep, wave, l);
     };
     auto load_b = [&](unsigned stage) {
       rb = sb.next();
       settled(rb);
-#pragma unroll
-      for (int i = 0; i < TN; ++i) lb.issue(rb, i, stage, kStep, wave, l);
+      lb.issue(rb, stage, kStep, wave, l);
     };
     load_a(0);
     load_b(0);
@@ -534,23 +537,32 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
 #pragma unroll
       for (int q = 0; q < TM * TN; ++q) {
         product16<T>(b0[q % TN], a0[q / TN], acc[q / TN][q % TN]);
-        if (kLoads && q == 0) ra = sa.next();
-        if (kLoads && q == 2) rb = sb.next();
+        if (kLoads && q == 0) {
+          ra = sa.next();
+          settled(ra);
+        }
+        if (kLoads && q == 2) {
+          rb = sb.next();
+          settled(rb);
+        }
         if (q % kReadGap == kReadGap - 1 && q / kReadGap < TM + TN) read(a1, b1, q / kReadGap, st_a, st_b, 1);
         __builtin_amdgcn_sched_barrier(0);
       }
       wait_loads<kLoads ? TM : 0>();
       lds_barrier();  // this step's stages are read, the next step's have landed (not yet A's behind it)
-      if (kLoads) {
-        settled(ra);
-        settled(rb);
-      }
+      const unsigned to_a = la.lds + st_a, to_b = lb.lds + st_b;
 #pragma unroll
       for (int q = 0; q < TM * TN; ++q) {
+        constexpr int kGap = kLoadGap;
+        const int k = q / kGap;
+        if (kLoads && q % kGap == 0) {
+          if (k < TN) load_to(to_b, k);
+          else load_to(to_a, k - TN);
+        }
         product16<T>(b1[q % TN], a1[q / TN], acc[q / TN][q % TN]);
-        if (kLoads && q % kLoadGap == 0) {
-          if (q / kLoadGap < TN) lb.issue(rb, q / kLoadGap, st_b, kStep, wave, l);
-          else la.issue(ra, q / kLoadGap - TN, st_a, kStep, wave, l);
+        if (kLoads && q % kGap == 0) {
+          if (k < TN) load_from(rb, lb.off[k < TN ? k : 0]);
+          else load_from(ra, la.off[k < TN ? 0 : k - TN]);
         }
         if (q % kReadGap == kReadGap - 1 && q / kReadGap < TM + TN) read(a0, b0, q / kReadGap, next_a, st_b ^ kB, 0);
         __builtin_amdgcn_sched_barrier(0);
@@ -566,15 +578,13 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     clear();
   }
   if (tail) {
-    ra = resource(ta);
-    rb = resource(tb);
+    const long n = left - (long)kStep * whole;  // elements of the end
+    ra = resource(pa + whole * stepA, DA ? extent(n, p.lda, p.M - m0) : extent(min((long)BM, p.M - m0), p.lda, n));
+    rb = resource(pb + whole * stepB, DB ? extent(n, p.ldb, p.N - n0) : extent(min((long)NT, p.N - n0), p.ldb, n));
     settled(ra);
     settled(rb);
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      la.issue(ra, i, 0, tail, wave, l);
-      lb.issue(rb, i, 0, tail, wave, l);
-    }
+    la.issue(ra, 0, tail, wave, l);
+    lb.issue(rb, 0, tail, wave, l);
     wait_loads<0>();
     lds_barrier();
 #pragma unroll
