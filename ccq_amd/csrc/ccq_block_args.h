@@ -73,7 +73,7 @@ struct ActBwdArgs {
   float* db_part;      // [row blocks, Nz] (nullable)
   void* db;            // [Nz] of bdtype
   long M, N, ldz, ldy;
-  int act, bdtype, dtype, row_blocks;
+  int act, bdtype, dtype, row_blocks, lanes;
 };
 
 struct PadRowsArgs {
