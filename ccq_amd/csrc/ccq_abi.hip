@@ -1632,8 +1632,11 @@ bool rows16(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
 
 int linear_check(const char* who, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ldw, int act, int dtype,
                  int bdtype) {
-  if (M < 0 || N < 1 || K < 1 || M > kMaxSide || N > kMaxSide || linear_outs(N, act) > kMaxStride || K > kMaxStride ||
-      ((M + 127) / 128) * ((linear_outs(N, act) + 127) / 128) > 0x7fffffffL)
+  if (M < 0 || N < 1 || K < 1 || M > kMaxSide || N > kMaxSide || linear_outs(N, act) > kMaxStride || K > kMaxStride)
+    return fail(CCQ_ERR_SHAPE, "%s: M=%lld N=%lld K=%lld", who, (long long)M, (long long)N, (long long)K);
+  const long outs = linear_outs(N, act);
+  auto tiles = [](long m, long n) { return ((m + 255) / 256) * ((n + 255) / 256); };
+  if (std::max({tiles(M, outs), tiles(M, K), tiles(outs, K)}) >= kMaxTiles)
     return fail(CCQ_ERR_SHAPE, "%s: M=%lld N=%lld K=%lld", who, (long long)M, (long long)N, (long long)K);
   if (ldx < round8(K) || ldw < round8(K) || ldx % 8 || ldw % 8 || ldx > kMaxStride || ldw > kMaxStride)
     return fail(CCQ_ERR_SHAPE, "%s: row strides %lld, %lld of K=%lld (multiples of 8, at most 4 Mi)", who, (long long)ldx,

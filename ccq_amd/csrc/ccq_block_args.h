@@ -48,6 +48,9 @@ struct LogprobArgs {
 // Activations of the linear map as the C ABI numbers them (CCQ_ACT_*).
 enum : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4, kActSwiglu = 5 };
 
+// Tiles of a product's launch: workgroups of 256 whose work items in x stay within 32 bits.
+constexpr long kMaxTiles = 1L << 24;
+
 // One product out[M, N] = A B^T over K, its operands stored with the contraction running along the rows
 // (A [M, K], B [N, K]) or down them (A [K, M], B [K, N]), and what is done with the result.
 struct ProductArgs {

@@ -777,19 +777,20 @@ __global__ __launch_bounds__(1024) void bias_sum_kernel(const ActBwdArgs a) {
 }
 
 __global__ __launch_bounds__(kThreads) void pad_rows_kernel(const PadRowsArgs a) {
-  const long pieces = a.ldd / 8, at = (long)blockIdx.x * kThreads + threadIdx.x;
-  if (at >= a.rows * pieces) return;
-  const long m = at / pieces, n = at % pieces * 8;
-  const short* row = (const short*)a.src + m * a.ld;
-  s16x8 v;
-  typedef s16x8 any __attribute__((aligned(2)));
-  if (n + 8 <= a.K) {
-    v = *gmem((const any*)(row + n));
-  } else {
+  const long pieces = a.ldd / 8, end = a.rows * pieces;
+  for (long at = (long)blockIdx.x * kThreads + threadIdx.x; at < end; at += (long)gridDim.x * kThreads) {
+    const long m = at / pieces, n = at % pieces * 8;
+    const short* row = (const short*)a.src + m * a.ld;
+    s16x8 v;
+    typedef s16x8 any __attribute__((aligned(2)));
+    if (n + 8 <= a.K) {
+      v = *gmem((const any*)(row + n));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = n + i < a.K ? *gmem(row + n + i) : (short)0;
+      for (int i = 0; i < 8; ++i) v[i] = n + i < a.K ? *gmem(row + n + i) : (short)0;
+    }
+    *gmem((s16x8*)((short*)a.dst + m * a.ldd + n)) = v;
   }
-  *gmem((s16x8*)((short*)a.dst + m * a.ldd + n)) = v;
 }
 
 template <typename T, int BM, int BN, int WM, int WN, bool DA, bool DB, int MODE, int ACT>
@@ -853,11 +854,12 @@ void product_plan(long M, long N, long K, int* side, int* splits) {
   } kinds[] = {{256, 1, 0.f, 1.5f, 7.5f}, {128, 2, 0.1f, 0.43f, 4.5f}, {64, 4, 0.1f, 0.19f, 3.5f}};
   const long steps = (K + kStep - 1) / kStep;
   float best = 0.f;
-  *side = 64;
+  *side = 256;
   *splits = 1;
   if (M <= 0 || N <= 0) return;
   for (const auto& k : kinds) {
     const long tiles = ((M + k.side - 1) / k.side) * ((N + k.side - 1) / k.side);
+    if (tiles >= kMaxTiles) continue;
     for (int sp = 1; sp <= 16 && (sp == 1 || sp * 2 <= steps); ++sp) {
       const long w = (tiles * sp + kCus - 1) / kCus, full = w / k.per_cu, rest = w % k.per_cu, n = (steps + sp - 1) / sp;
       float t = full * (n * (k.step0 + k.step1 * k.per_cu) + k.fixed);
@@ -920,7 +922,8 @@ hipError_t launch_act_bwd(const ActBwdArgs& args, hipStream_t st) {
 hipError_t launch_pad_rows(const PadRowsArgs& a, hipStream_t st) {
   const long n = a.rows * (a.ldd / 8);
   if (n <= 0) return hipSuccess;
-  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)((n + kThreads - 1) / kThreads)), dim3(kThreads), 0, st, a);
+  const long blocks = std::min((n + kThreads - 1) / kThreads, 1L << 20);
+  hipLaunchKernelGGL(pad_rows_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, a);
   return hipGetLastError();
 }
 

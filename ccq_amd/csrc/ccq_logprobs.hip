@@ -198,13 +198,16 @@ __device__ void top_of_row(TopList<THREADS>& s, const T* row, int V, int k, floa
   }
 }
 
+// grid: (rows up to kRowsX, whole kRowsX of rows), since a launch's work items in x stay within 32 bits
+constexpr long kRowsX = 1L << 20;
 template <typename T, int THREADS, bool TOP>
 __global__ __launch_bounds__(THREADS) void logprob_fwd_kernel(const LogprobArgs a) {
   constexpr int N = Piece<T>::N, W = THREADS / 64;
   __shared__ Part parts[W];
   __shared__ TopList<TOP ? THREADS : 64> top;
   const int tid = threadIdx.x, V = a.V;
-  const long r = blockIdx.x;
+  const long r = (long)blockIdx.y * kRowsX + blockIdx.x;
+  if (r >= a.rows) return;
   const int64_t id = a.ids[r];
   if (id == a.ignore) {
     if (tid == 0) a.logp[r] = a.ent[r] = 0.f;
@@ -340,8 +343,9 @@ void launch_typed(bool bwd, const LogprobArgs& a, hipStream_t st) {
     if (a.k) hipLaunchKernelGGL((logprob_fwd_kernel<T, 1024, true>), dim3((unsigned)a.rows), dim3(1024), 0, st, a);
     else hipLaunchKernelGGL((logprob_fwd_kernel<T, 1024, false>), dim3((unsigned)a.rows), dim3(1024), 0, st, a);
   } else {
-    if (a.k) hipLaunchKernelGGL((logprob_fwd_kernel<T, 256, true>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((logprob_fwd_kernel<T, 256, false>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)std::min(a.rows, kRowsX), (unsigned)((a.rows + kRowsX - 1) / kRowsX));
+    if (a.k) hipLaunchKernelGGL((logprob_fwd_kernel<T, 256, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((logprob_fwd_kernel<T, 256, false>), grid, dim3(256), 0, st, a);
   }
 }
 

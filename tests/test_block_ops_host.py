@@ -169,3 +169,16 @@ def test_linear_abi_refusals():
     # sizes of nothing: no rows, one output
     assert lib.ccq_linear_workspace_bytes(0, 32, 64, 0) == 0
     assert lib.ccq_linear_bwd_workspace_bytes(0, 32, 64, 0) >= 0 and lib.ccq_linear_bwd_workspace_bytes(1, 1, 1, 5) > 0
+
+
+def test_linear_abi_sizes_refused():
+    """Products of more tiles than a launch holds; the longest and widest that fit pass on to the pointers' checks."""
+    lib = _lib.load()
+
+    def fwd(M, N, K):
+        k8 = (K + 7) // 8 * 8
+        return lib.ccq_linear_fwd(None, k8, P, k8, None, 0, None, 0, P, None, P, M, N, K, 0, 0, None)
+
+    assert fwd(1 << 30, 1 << 22, 8) == SHAPE and fwd(1 << 30, 8, 1 << 22) == SHAPE and fwd((1 << 30) + 1, 8, 8) == SHAPE
+    assert fwd(8, (1 << 22) + 1, 8) == SHAPE and fwd(8, 8, (1 << 22) + 1) == SHAPE
+    assert fwd(1 << 30, 1, 1) == NULL and fwd(1, 1 << 22, 8) == NULL and fwd(1, 8, 1 << 22) == NULL

@@ -284,3 +284,22 @@ def test_logprobs_captured_and_other_stream():
         assert all(torch.equal(s, t) for s, t in zip(out, want[k]))
         step(*sets[0])
         torch.cuda.synchronize()
+
+
+def test_logprobs_more_rows_than_a_launch_is_wide():
+    """2^24 + 3 rows of two logits: workgroups of every row would pass 32 bits of work items in one dimension."""
+    from ccq_amd import token_logprobs
+    dev = _cuda()
+    rows = 2 ** 24 + 3
+    x = torch.randn(rows, 2, device=dev, generator=torch.Generator(dev).manual_seed(3)).half().requires_grad_()
+    ids = torch.randint(0, 2, (rows,), device=dev, generator=torch.Generator(dev).manual_seed(4))
+    got = token_logprobs(x, ids)
+    dx = torch.autograd.grad(got.logprobs.sum(), x)[0]
+    d = (x.detach()[:, 1].double() - x.detach()[:, 0].double()) * (2 * ids - 1)    # log odds of the given token
+    want = -torch.log1p(torch.exp(-d))
+    assert ((got.logprobs.double() - want).abs() <= (2 / 256 + 64) * U32 + 4 * U32 * (want.abs() + math.log(2))).all()
+    other = torch.sigmoid(-d)
+    sign = torch.stack([1.0 - 2 * ids, 2 * ids - 1.0], -1)
+    # one rounding to the logits' type (half a step, or half the smallest one), and the relative error of p
+    n = torch.finfo(HF).eps / 2 + (2 / 256 + 64 + 16) * U32
+    assert ((dx.double() - sign * other[:, None]).abs() <= n * other[:, None] + 2.0 ** -25).all()
