@@ -5,7 +5,9 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
@@ -72,6 +74,21 @@ bool needs_grad(std::initializer_list<const Tensor*> xs) {
   return false;
 }
 
+// A leaf that an earlier graph still holds takes its gradients on the stream where that graph was made.  Under capture
+// autograd would wait there for work that is not captured, which ends the process; raised here before it comes to that.
+void check_capture(const Tensor& x) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  const c10::Stream here = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index()).unwrap();
+  for (const auto& edge : node->next_edges()) {
+    if (!dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) continue;
+    const auto stream = edge.function->stream();
+    TORCH_CHECK(!stream || *stream == here, "a backward pass is captured into a graph while a graph of the same leaves from "
+                "another stream is alive: drop that one's outputs first");
+  }
+}
+
 // The kernels have no second derivatives: gradients asked for with a graph of their own carry one that raises.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -135,6 +152,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
       const Tensor ds = grads.size() > 1 ? grads[1] : Tensor();
       if (grads[0].defined() || ds.defined()) {
         c10::DeviceGuard guard(saved[0].device());
+        check_capture(saved[0]);
         const auto shape = ctx->saved_data["shape"].toIntVector();
         const Tensor x = rows_of(saved[0]);
         const auto type = x.scalar_type();
@@ -244,6 +262,7 @@ struct TokenScore : torch::autograd::Function<TokenScore> {
       const auto saved = ctx->get_saved_variables();
       const Tensor& x = saved[0];
       c10::DeviceGuard guard(x.device());
+      check_capture(x);
       const Tensor dlogp = grads[0].defined() ? grads[0].contiguous() : Tensor(),
                    dent = grads[1].defined() ? grads[1].contiguous() : Tensor();
       dx = fresh(x, ctx->saved_data["shape"].toIntVector(), x.scalar_type());
@@ -339,8 +358,9 @@ struct FusedLinear : torch::autograd::Function<FusedLinear> {
       const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
       const bool need_b = present & 1 && ctx->needs_input_grad(++edge);
       const bool need_r = present & 2 && ctx->needs_input_grad(++edge);
+      c10::DeviceGuard guard(x.device());
+      check_capture(x);
       if (need_x || need_w || need_b) {
-        c10::DeviceGuard guard(x.device());
         const int64_t M = x.size(0), K = x.size(1), outs = w.size(0), N = act == CCQ_ACT_SWIGLU ? outs / 2 : outs;
         const int64_t ld = (K + 7) / 8 * 8;
         const auto type = x.scalar_type();

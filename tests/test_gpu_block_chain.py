@@ -136,3 +136,53 @@ def test_two_streams_at_once():
     for k in range(2):
         for got in out[k]:
             assert all(torch.equal(a, b) for a, b in zip(got, want[k]))
+
+
+def each_operator(dev):
+    """Every differentiable operator as a function of one leaf."""
+    import ccq_amd
+    gen = torch.Generator(dev).manual_seed(11)
+    w = torch.randn(64, 64, device=dev, generator=gen).bfloat16()
+    v = torch.ones(64, device=dev)
+    ids = torch.arange(6, device=dev)
+    return {"rms_norm": lambda x: ccq_amd.rms_norm(x, v), "layer_norm": lambda x: ccq_amd.layer_norm(x, v, v),
+            "fused_linear": lambda x: ccq_amd.fused_linear(x, w, activation="silu"),
+            "token_logprobs": lambda x: ccq_amd.token_logprobs(x, ids).logprobs}
+
+
+@pytest.mark.parametrize("name", ["rms_norm", "layer_norm", "fused_linear", "token_logprobs"])
+def test_second_derivative_raises(name):
+    dev = _cuda()
+    x = torch.randn(6, 64, device=dev, generator=torch.Generator(dev).manual_seed(1)).bfloat16().requires_grad_()
+    dx, = torch.autograd.grad(each_operator(dev)[name](x).float().square().sum(), x, create_graph=True)
+    assert torch.isfinite(dx).all()
+    with pytest.raises(RuntimeError, match="twice"):
+        dx.float().square().sum().backward()
+
+
+@pytest.mark.parametrize("name", ["rms_norm", "layer_norm", "fused_linear", "token_logprobs"])
+def test_captured_backward_beside_an_eager_graph_of_its_leaf(name):
+    """Refused where the eager graph is of another stream (autograd would wait for it and end the process); captured and
+    replayed once that graph is gone."""
+    dev = _cuda()
+    f = each_operator(dev)[name]
+    x = torch.randn(6, 64, device=dev, generator=torch.Generator(dev).manual_seed(1)).bfloat16().requires_grad_()
+    y = f(x)
+    dy = torch.randn(y.shape, device=dev, generator=torch.Generator(dev).manual_seed(2)).to(y.dtype)
+    want, = torch.autograd.grad(y, x, dy, retain_graph=True)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="alive"):
+            f(x).backward(dy)
+    del y
+    assert x.grad is None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(f(x), x, dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        got.zero_()
+        f(x.detach())
+        torch.cuda.synchronize()
