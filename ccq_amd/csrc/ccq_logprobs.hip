@@ -12,11 +12,12 @@
 //
 // The alternatives come out of the same pass.  The 64 lanes stand for 64 parts of the row; after a thread's first few
 // pieces, which it holds in registers, the k-th largest of the 64 maxima (k <= 64) is a lower bound of the row's k-th
-// largest logit, and the logits that reach it are listed, those of the pieces behind as they are read: about 24 for
-// k = 20 where the first pieces are the whole row, 24 / f where they are a fraction f.  Every listed logit then counts
-// those before it.  A row that lists more than kTopList is read again with the bound of the whole row's maxima, and one
-// that still does (equal logits) is ranked by k passes over it.  (A second pass for all rows, as first built: 53.8 us
-// against 43.8 with pieces loaded ahead, and this, on 1531 x 32007 fp32 with half the rows skipped, k = 5.)
+// largest logit, and the pieces with a logit that reaches it are listed, those behind as they are read: about 24 for
+// k = 20 where the first pieces are the whole row, 24 / f where they are a fraction f.  Their candidates are listed in
+// turn, and every one counts those before it.  A row with more than kTopPieces is read again with the bound of the whole
+// row's maxima, and one that still has more, or more than kTopList candidates (equal logits), is ranked by k passes over
+// it.  (A second pass for all rows, as first built: 53.8 us against 31 now on 1531 x 32007 fp32 with half the rows
+// skipped, k = 5: 98 MB, whose copy would take 20; the start, the bound and the ranks of a row are about 8.)
 #include <algorithm>
 
 #include "ccq_block_args.h"
@@ -27,7 +28,8 @@ namespace ccq {
 namespace {
 
 constexpr int kTopParts = 64;    // parts of a row, so the largest k
-constexpr int kTopList = 1024;   // listed candidates
+constexpr int kTopPieces = 512;  // pieces that may hold candidates
+constexpr int kTopList = 1024;   // candidates
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFar = -1e4f;    // e^(x - m) is 0 long before: stands for -inf in the products with it
 
@@ -80,40 +82,42 @@ __device__ __forceinline__ unsigned long long rank_key(float x, int i) {
   return (unsigned long long)u << 32 | (unsigned)~i;
 }
 __device__ __forceinline__ int key_index(unsigned long long k) { return (int)~(unsigned)k; }
+__device__ __forceinline__ float key_value(unsigned long long k) {
+  const unsigned u = (unsigned)(k >> 32);
+  return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
+}
 
-// f(column, piece) over the thread's pieces of a row, kAhead of them loaded together
-constexpr int kAhead = 4;
+constexpr int kAhead = 4;  // pieces loaded together
+
+// f(column, piece) over the thread's pieces of a row, one at a time (for rows that are read again: its registers are the
+// main loop's loss)
 template <typename T, typename F>
 __device__ __forceinline__ void over_row(const T* row, int V, int tid, int threads, F&& f) {
   constexpr int N = Piece<T>::N;
-  const int step = threads * N;
-  for (int c = tid * N; c < V; c += kAhead * step) {
-    typename Piece<T>::vec v[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (c + j * step < V) v[j] = load_piece(row, c + j * step, V);
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (c + j * step < V) f(c + j * step, v[j]);
-  }
+#pragma unroll 1
+  for (int c = tid * N; c < V; c += threads * N) f(c, load_piece(row, c, V));
 }
 
-// The candidates of a row: an index's logit in rank order.
+// The candidates of a row: pieces that hold a logit at or above the bound, then those logits in rank order.  (Whole
+// pieces, since a thread that looked at every element there and then took twice the registers: four workgroups a CU for
+// seven, and 50 us for 41 on 2000 x 32000 bf16, k = 5; 29 for 25 on 1000.)
 template <int THREADS>
 struct TopList {
+  u32x4 piece[kTopPieces];
   unsigned long long list[kTopList];
+  int column[kTopPieces];
   float pm[THREADS / 64][kTopParts];
   float bound;
-  int count;
+  int pieces, count;
 };
 
 // the k-th largest of the lanes' maxima over the workgroup's waves
 template <int THREADS>
 __device__ float top_bound(TopList<THREADS>& s, int k, float mine) {
   const int l = threadIdx.x & 63;
-  __syncthreads();  // (the last use of pm and count)
+  __syncthreads();  // (the last use of pm and the counts)
   s.pm[threadIdx.x >> 6][l] = mine;
-  if (threadIdx.x == 0) s.count = 0;
+  if (threadIdx.x == 0) s.pieces = s.count = 0;
   __syncthreads();
   if (threadIdx.x < 64) {  // (one wave: sixteen at once would share the SIMDs for the same answer)
     float v = s.pm[0][l];
@@ -132,17 +136,16 @@ __device__ float top_bound(TopList<THREADS>& s, int k, float mine) {
 }
 
 template <typename T, int THREADS>
-__device__ __forceinline__ void list_piece(TopList<THREADS>& s, const typename Piece<T>::vec& v, int c, int V, float bound) {
-#pragma unroll
-  for (int i = 0; i < Piece<T>::N; ++i)
-    if (c + i < V && (float)v[i] >= bound) {
-      const int at = atomicAdd(&s.count, 1);
-      if (at < kTopList) s.list[at] = rank_key((float)v[i], c + i);
-    }
+__device__ __forceinline__ void list_piece(TopList<THREADS>& s, const typename Piece<T>::vec& v, int c) {
+  const int at = atomicAdd(&s.pieces, 1);
+  if (at < kTopPieces) {
+    s.piece[at] = __builtin_bit_cast(u32x4, v);
+    s.column[at] = c;
+  }
 }
 
-// The k first of the row in rank order, into out / ids.  The list holds every logit that reaches some bound below the
-// k-th largest, unless it overflowed; most: the maximum of this thread's logits; m, logz: the row's.
+// The k first of the row in rank order, into out / ids.  The pieces listed hold every logit that reaches some bound below
+// the k-th largest, unless they overflowed; most: the maximum of this thread's logits; m, logz: the row's.
 template <typename T, int THREADS>
 __device__ void top_of_row(TopList<THREADS>& s, const T* row, int V, int k, float most, float m, float logz, float* out,
                            int64_t* ids) {
@@ -150,25 +153,43 @@ __device__ void top_of_row(TopList<THREADS>& s, const T* row, int V, int k, floa
   const int tid = threadIdx.x;
   const bool bad = logz != logz;  // (a NaN is listed by no comparison)
   __syncthreads();
-  int n = s.count;
-  if (n > kTopList && !bad) {
+  int n = s.pieces;
+  if (n > kTopPieces && !bad) {
     const float bound = top_bound<THREADS>(s, k, most);
-    over_row(row, V, tid, THREADS, [&](int c, const typename Piece<T>::vec& v) { list_piece<T, THREADS>(s, v, c, V, bound); });
+    over_row(row, V, tid, THREADS, [&](int c, const typename Piece<T>::vec& v) {
+      bool reach = false;
+#pragma unroll
+      for (int i = 0; i < N; ++i) reach |= c + i < V && (float)v[i] >= bound;
+      if (reach) list_piece<T, THREADS>(s, v, c);
+    });
     __syncthreads();
-    n = s.count;
+    n = s.pieces;
   }
-  if (n <= kTopList && !bad) {
-    for (int a = tid; a < n; a += THREADS) {
-      const unsigned long long mine = s.list[a];
-      int before = 0;
-      for (int i = 0; i < n; ++i) before += s.list[i] > mine;
-      if (before < k) {
-        const int id = key_index(mine);
-        out[before] = ((float)row[id] - m) - logz;
-        ids[before] = id;
+  if (n <= kTopPieces && !bad) {
+    const float bound = s.bound;
+    for (int a = tid; a < n * N; a += THREADS) {
+      const int c = s.column[a / N] + a % N;
+      const float x = (float)((const T*)s.piece)[a];
+      if (c < V && x >= bound) {
+        const int at = atomicAdd(&s.count, 1);
+        if (at < kTopList) s.list[at] = rank_key(x, c);
       }
     }
-    return;
+    __syncthreads();
+    n = s.count;
+    if (n <= kTopList) {
+      for (int a = tid; a < n; a += THREADS) {
+        const unsigned long long mine = s.list[a];
+        int before = 0;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) before += s.list[i] > mine;
+        if (before < k) {
+          out[before] = (key_value(mine) - m) - logz;
+          ids[before] = key_index(mine);
+        }
+      }
+      return;
+    }
   }
   // the first of the row behind the last one found, k times
   unsigned long long last = ~0ull;
@@ -191,17 +212,20 @@ __device__ void top_of_row(TopList<THREADS>& s, const T* row, int V, int k, floa
     for (int i = 0; i < W; ++i) best = s.list[i] > best ? s.list[i] : best;
     last = best;
     if (tid == 0) {
-      const int id = key_index(best);
-      out[j] = ((float)row[id] - m) - logz;
-      ids[j] = id;
+      out[j] = (key_value(best) - m) - logz;
+      ids[j] = key_index(best);
     }
   }
 }
 
 // grid: (rows up to kRowsX, whole kRowsX of rows), since a launch's work items in x stay within 32 bits
 constexpr long kRowsX = 1L << 20;
+// waves a SIMD that the registers are held to (left to itself the compiler takes LDS for the bound and 121 registers)
+template <typename T, int THREADS>
+constexpr int kFwdWaves = THREADS == 1024 || sizeof(T) == 4 ? 8 : 6;
 template <typename T, int THREADS, bool TOP>
-__global__ __launch_bounds__(THREADS) void logprob_fwd_kernel(const LogprobArgs a) {
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(kFwdWaves<T, THREADS>)))
+void logprob_fwd_kernel(const LogprobArgs a) {
   constexpr int N = Piece<T>::N, W = THREADS / 64;
   __shared__ Part parts[W];
   __shared__ TopList<TOP ? THREADS : 64> top;
@@ -229,9 +253,14 @@ __global__ __launch_bounds__(THREADS) void logprob_fwd_kernel(const LogprobArgs 
       if (c + j * step < V) v[j] = load_piece(row, c + j * step, V);
   };
   fetch(x, tid * N);
+  // a token outside the vocabulary has no log probability
+  const float given = tid == 0 && id >= 0 && id < V ? (float)*gmem(row + id) : NAN;
   for (int c0 = 0; c0 < V; c0 += kAhead * step) {  // (the same rounds for every thread)
     const int c = c0 + tid * N;
     if (kNext) fetch(y, c + kAhead * step);
+    float first[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) first[j] = NAN;  // (reaches no bound)
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int at = c + j * step;
@@ -244,16 +273,16 @@ __global__ __launch_bounds__(THREADS) void logprob_fwd_kernel(const LogprobArgs 
         for (int i = 0; i < N; ++i) v[i] = at + i < V ? v[i] : -INFINITY;
       const float most = add_values<N>(p, v);
       if constexpr (TOP) {
-        if (most >= bound) list_piece<T, THREADS>(top, x[j], at, V, bound);
+        first[j] = most;
+        if (most >= bound) list_piece<T, THREADS>(top, x[j], at);
       }
     }
     if constexpr (TOP) {
       if (c0 == 0) {
         bound = top_bound<THREADS>(top, a.k, p.m);
-        if (p.m >= bound)
 #pragma unroll
-          for (int j = 0; j < kAhead; ++j)
-            if (c + j * step < V) list_piece<T, THREADS>(top, x[j], c + j * step, V, bound);
+        for (int j = 0; j < kAhead; ++j)
+          if (first[j] >= bound) list_piece<T, THREADS>(top, x[j], c + j * step);
       }
     }
     if (!kNext) fetch(x, c + kAhead * step);
@@ -271,8 +300,7 @@ __global__ __launch_bounds__(THREADS) void logprob_fwd_kernel(const LogprobArgs 
   for (int o = 1; o < W; o <<= 1) p = merge(p, Part{__shfl_xor(p.m, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o)});
   const float logz = logf(p.s);
   if (tid == 0) {
-    // a token outside the vocabulary has no log probability
-    a.logp[r] = id >= 0 && id < V ? ((float)row[id] - p.m) - logz : NAN;
+    a.logp[r] = (given - p.m) - logz;
     a.ent[r] = logz - p.t / p.s;
     if (a.stats) {
       a.stats[2 * r] = p.m;
@@ -330,8 +358,10 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(const LogprobArgs
   }
 }
 
-// Fewer rows than fill the chip's 8192 waves with four to a row: sixteen to a row.
-constexpr long kFewRows = 1024;
+// Fewer than two rows a CU: sixteen waves to a row, otherwise four (32000 bf16, k = 5: 16 rows 8.9 us by sixteen and 12.3
+// by four, 256 rows 11.5 and 14.2, 512 16.3 and 17.1, 1000 28 and 25, 2000 50 and 40; without alternatives 16 rows 6.2
+// and 7.7, 512 12.5 and 12.0, 2000 36 and 34).
+constexpr long kFewRows = 512;
 template <typename T>
 void launch_typed(bool bwd, const LogprobArgs& a, hipStream_t st) {
   if (bwd) {

@@ -303,3 +303,27 @@ def test_logprobs_more_rows_than_a_launch_is_wide():
     # one rounding to the logits' type (half a step, or half the smallest one), and the relative error of p
     n = torch.finfo(HF).eps / 2 + (2 / 256 + 64 + 16) * U32
     assert ((dx.double() - sign * other[:, None]).abs() <= n * other[:, None] + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FL], ids=str)
+@pytest.mark.parametrize("rows", [8, 600], ids=str)      # both workgroup sizes
+def test_top_sorted_rows(rows, dtype):
+    """Rows in rising order, whose every later piece reaches the bound of the first ones, and in falling order; runs of
+    equal logits, and the likeliest tokens all in one piece."""
+    V = 40000
+    x = torch.zeros(rows, V)
+    rise = torch.linspace(-20.0, 8.0, V)
+    x[0::8], x[1::8] = rise, rise.flip(0)
+    x[2::8] = rise.round()
+    x[3::8] = rise.round().flip(0)
+    x[4::8, 39990:] = torch.arange(10.0)
+    x[5::8, 20000:20064] = 3.0
+    x[6::8] = -rise.abs()
+    x[7::8, :2000] = 5.0
+    x = x.to(dtype)
+    ids = torch.arange(rows) * 61 % V
+    want = formula(x, ids)
+    for k in (1, 7, 64):
+        got, _ = call(x, ids, k)
+        check_values(got, want, V)
+        check_top(got, x, want, k)
