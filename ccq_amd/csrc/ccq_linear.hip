@@ -367,22 +367,22 @@ __device__ __forceinline__ s16x4_t read_tr4(unsigned at) {
 
 enum : int { kPlain = 0, kEpilogue = 1, kPartial = 2 };
 
-// BM x BN tile of the product by WM x WN waves, three stages of A in LDS and two of B.  Lane l of a wave holds, of each 16x16 tile
-// (it, j) of the wave, row m = 16 it + (l & 15) and four consecutive columns.  Along-the-row B operands (the forward)
+// BM x BN tile of the product by WM x WN waves, NA stages of A in LDS and NB of B.  Lane l of a wave holds, of each 16x16
+// tile (it, j) of the wave, row m = 16 it + (l & 15) and four consecutive columns.  Along-the-row B operands (the forward)
 // are read so that the column tiles j = 2 q and 2 q + 1 of a lane are eight consecutive columns, one 16-byte store.
 // swiglu: half of a wave's columns are gates, the other half the ups beside them, so a lane holds both.
 //
 // A step of 64 contraction elements is two halves of 32.  While the matrix cores work on one half's fragments the
-// other half's are read from LDS into registers and the direct loads of the step after next are issued, each
+// other half's are read from LDS into registers and the direct loads of a later step are issued, each
 // between two products (in clumps they keep the one wave of a SIMD from issuing products).  The one barrier of a step
 // lies between the halves, where every wave has read the step's stages (loads may overwrite them) and the next step's
-// have landed.  The 160 KiB of LDS hold two and a half stages: the half goes to A, whose rows come from HBM and are
+// have landed.  The 160 KiB of LDS hold two and a half stages of 256 x 256: the half goes to A, whose rows come from HBM and are
 // asked for three steps ahead, while B's, which the workgroups of all tile rows share, lie in the caches.
-template <typename T, int BM, int BN, int WM, int WN, bool DA, bool DB, int MODE, int ACT>
+template <typename T, int BM, int BN, int WM, int WN, int NA, int NB, bool DA, bool DB, int MODE, int ACT>
 __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs p) {
   constexpr bool GLU = ACT == kActSwiglu;
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr unsigned kA = BM * kStep * 2, kB = BN * kStep * 2, kRing = 3 * kA + 2 * kB;  // bytes of a stage; of all
+  constexpr unsigned kA = BM * kStep * 2, kB = BN * kStep * 2, kRing = NA * kA + NB * kB;  // bytes of a stage; of all
   constexpr int HALF = BN / WN / 2;  // swiglu: gates of a wave
   static_assert(!GLU || (!DB && MODE == kEpilogue), "gates and ups of one wave");
   static_assert(TM == TN, "one fragment of each operand between two rows of products");
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
   LoadA la;
   LoadB lb;
   la.init(lds0, wave, l, p.lda);
-  lb.init(lds0 + 3 * kA, wave, l, p.ldb);
+  lb.init(lds0 + NA * kA, wave, l, p.ldb);
   // Rows of an operand that lie a multiple of 4 KiB apart meet in one channel of the L2 at any one step.  So the tile
   // rows of a band begin their contraction at different steps, 256 bytes apart, and come round to them at its end;
   // those of one tile row keep together and find its operand in the L2.  (8192^3 forward: 849 -> 788 us; contractions
@@ -460,11 +460,11 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     const int k = 8 * g + (r >> 2), s = wn * TN * 2 + ((r >> 1) & 1);
 #pragma unroll
     for (int j = 0; j < TN; ++j)
-      fb[j] = lds0 + 3 * kA + k * (BN * 2) + (((s + 2 * j) ^ swz_down<BN>(k)) << 4) + 8 * (r & 1);
+      fb[j] = lds0 + NA * kA + k * (BN * 2) + (((s + 2 * j) ^ swz_down<BN>(k)) << 4) + 8 * (r & 1);
   } else {
     const int row = wn * TN * 16 + 8 * (r >> 2) + (r & 3);
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) fb[kk] = lds0 + 3 * kA + row * 128 + (((4 * kk + g) ^ swz_b(row)) << 4);
+    for (int kk = 0; kk < 2; ++kk) fb[kk] = lds0 + NA * kA + row * 128 + (((4 * kk + g) ^ swz_b(row)) << 4);
   }
   auto read_a = [&](int it, unsigned stage, int kk) -> s16x8 {
     if constexpr (DA) {
@@ -517,13 +517,15 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
       settled(rb);
       lb.issue(rb, stage, kStep, wave, l);
     };
-    load_a(0);
-    load_b(0);
-    load_a(kA);
-    load_b(kB);
-    load_a(2 * kA);
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {  // in the order that the steps ask for them
+      if (i >= NA - NB) load_b((i - (NA - NB)) * kB);
+      load_a(i * kA);
+    }
     clear();  // (while the first loads are on their way)
-    wait_loads<2 * TM + TN>();
+    // loads that may be on their way behind those of a step: of the steps asked for later, and A's of the same time
+    constexpr int kBehind = (NB < NA ? TM : 0) + (NB - 2) * (TM + TN);
+    wait_loads<kBehind + TM + TN>();
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
@@ -533,7 +535,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
     unsigned st_a = 0, st_b = 0;  // the step's stages
     auto step = [&](auto with_loads) {
       constexpr bool kLoads = decltype(with_loads)::value;
-      const unsigned next_a = st_a == 2 * kA ? 0 : st_a + kA;
+      const unsigned next_a = st_a == (NA - 1) * kA ? 0 : st_a + kA, next_b = st_b == (NB - 1) * kB ? 0 : st_b + kB;
 #pragma unroll
       for (int q = 0; q < TM * TN; ++q) {
         product16<T>(b0[q % TN], a0[q / TN], acc[q / TN][q % TN]);
@@ -548,7 +550,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
         if (q % kReadGap == kReadGap - 1 && q / kReadGap < TM + TN) read(a1, b1, q / kReadGap, st_a, st_b, 1);
         __builtin_amdgcn_sched_barrier(0);
       }
-      wait_loads<kLoads ? TM : 0>();
+      wait_loads<kLoads ? kBehind : 0>();
       lds_barrier();  // this step's stages are read, the next step's have landed (not yet A's behind it)
       const unsigned to_a = la.lds + st_a, to_b = lb.lds + st_b;
 #pragma unroll
@@ -564,15 +566,15 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(const ProductArgs
           if (k < TN) load_from(rb, lb.off[k < TN ? k : 0]);
           else load_from(ra, la.off[k < TN ? 0 : k - TN]);
         }
-        if (q % kReadGap == kReadGap - 1 && q / kReadGap < TM + TN) read(a0, b0, q / kReadGap, next_a, st_b ^ kB, 0);
+        if (q % kReadGap == kReadGap - 1 && q / kReadGap < TM + TN) read(a0, b0, q / kReadGap, next_a, next_b, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
       st_a = next_a;
-      st_b ^= kB;
+      st_b = next_b;
     };
-    for (int s = 2; s < whole; ++s) step(std::true_type{});
-    // the last two steps ask for nothing (their last reads are of a stage behind, and not used)
-    for (int s = max(0, whole - 2); s < whole; ++s) step(std::false_type{});
+    for (int s = NB; s < whole; ++s) step(std::true_type{});
+    // the last steps ask for nothing (the reads of the very last are of a stage behind, and not used)
+    for (int s = max(0, whole - NB); s < whole; ++s) step(std::false_type{});
     lds_barrier();
   } else {
     clear();
@@ -793,20 +795,29 @@ __global__ __launch_bounds__(kThreads) void pad_rows_kernel(const PadRowsArgs a)
   }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool DA, bool DB, int MODE, int ACT>
+template <typename T, int BM, int BN, int WM, int WN, int NA, int NB, bool DA, bool DB, int MODE, int ACT>
 hipError_t launch_tiles(const ProductArgs& p, hipStream_t st) {
   constexpr int NT = ACT == kActSwiglu ? BN / 2 : BN;
   const long tiles = ((p.M + BM - 1) / BM) * ((p.N + NT - 1) / NT);
-  hipLaunchKernelGGL((product_kernel<T, BM, BN, WM, WN, DA, DB, MODE, ACT>), dim3((unsigned)tiles, (unsigned)p.splits),
+  hipLaunchKernelGGL((product_kernel<T, BM, BN, WM, WN, NA, NB, DA, DB, MODE, ACT>), dim3((unsigned)tiles, (unsigned)p.splits),
                      dim3(WM * WN * 64), 0, st, p);
   return hipGetLastError();
 }
 
+constexpr int kCus = 256;
+// Few tiles of 64 x 64: four stages of both operands in LDS instead of three and two, so two workgroups a CU instead of
+// four, and twice the bytes on their way (operands from HBM: 16 x 5632 over 1024 11.3 -> 7.9 us, 1024^3 9.8 -> 8.2; out of
+// the caches 0.2 slower.  With more tiles four a CU are ahead: 4096 x 2048 over 512 18.6, 23.1 so).
+constexpr int kDeepMost = 2 * kCus;
+
 template <typename T, bool DA, bool DB, int MODE, int ACT = kActNone>
 hipError_t launch_size(const ProductArgs& p, int side, hipStream_t st) {
-  if (side == 256) return launch_tiles<T, 256, 256, 2, 2, DA, DB, MODE, ACT>(p, st);
-  if (side == 128) return launch_tiles<T, 128, 128, 2, 2, DA, DB, MODE, ACT>(p, st);
-  return launch_tiles<T, 64, 64, 2, 2, DA, DB, MODE, ACT>(p, st);
+  if (side == 256) return launch_tiles<T, 256, 256, 2, 2, 3, 2, DA, DB, MODE, ACT>(p, st);
+  if (side == 128) return launch_tiles<T, 128, 128, 2, 2, 3, 2, DA, DB, MODE, ACT>(p, st);
+  constexpr int NT = ACT == kActSwiglu ? 32 : 64;
+  if (((p.M + 63) / 64) * ((p.N + NT - 1) / NT) * p.splits <= kDeepMost)
+    return launch_tiles<T, 64, 64, 2, 2, 4, 4, DA, DB, MODE, ACT>(p, st);
+  return launch_tiles<T, 64, 64, 2, 2, 3, 2, DA, DB, MODE, ACT>(p, st);
 }
 
 template <typename T>
@@ -834,24 +845,26 @@ hipError_t launch_typed(int kind, const ProductArgs& p, int side, hipStream_t st
   return launch_size<T, true, true, kPlain>(p, side, st);
 }
 
-constexpr int kCus = 256;
-
 }  // namespace
 
 // Tile side and parts of the contraction of a product of M x N outputs (swiglu: N = all rows of B) over K, by what a
-// call is expected to take, in us.  A CU holds one workgroup of 256 x 256 (its LDS), two of 128 x 128 or four of 64 x 64;
-// `step` is a step's time beside that many of its kind, `fixed` what a workgroup takes besides (launch, the first
-// loads, the epilogue), measured:
+// call is expected to take, in us.  A CU holds one workgroup of 256 x 256 (its LDS), two of 128 x 128, two of 64 x 64
+// with deep rings or four without; `step1` a step's time for each of them, `step0` what they share, `fixed` what a
+// workgroup takes besides (launch, the first loads, the epilogue), measured:
 //   256: 8192 x 4096 over 4096 202 us, 32768 x 1024 over 2816 153, 16384 x 5632 over 1024 189 (128: 243, 191, 193)
-//   128: 2048 x 2048 over 2048 22.5, 8192 x 1024 over 1024 21.8 (256: 42, 30.8; 64: 28, 29.5)
-//    64: 1536 x 784 over 1000 11.3, 16 x 5632 over 1024 8.1 (128 in one part: 14.5, in four: 9.3)
-// Parts of the contraction go through fp32 partial sums: a second launch (3.5), a read of each part, one
-// after the other, and their bytes (10 TB/s: the last-level cache).  2816 x 1024 over 32768 by 256 in five parts 185, by 128 in one 340.
+//   128: 2048 x 2048 over 2048 21.2, 4096 x 2048 over 1024 20.4 (256: 44, 30.5; 64: 28, 29)
+//    64: 1024 x 1024 over 2048 11.9, 2048 x 1024 over 1024 10.5, over 4096 27.8 (128: 19, 12.2, 33; 128 in two parts: 17.5,
+//        20, 31)
+// Parts of the contraction go through fp32 partial sums: a second launch, and a read of each part, one after the
+// other.  512 x 1024 over 4096 by 64 in one part 19.5, in two or four 16.0; 1024 x 1024 over 2048 11.9 and 17.4;
+// 2816 x 1024 over 32768 by 256 in five 185, by 128 in one 340.
 void product_plan(long M, long N, long K, int* side, int* splits) {
   static const struct {
     int side, per_cu;
     float step0, step1, fixed;
-  } kinds[] = {{256, 1, 0.f, 1.5f, 7.5f}, {128, 2, 0.1f, 0.43f, 4.5f}, {64, 4, 0.1f, 0.19f, 3.5f}};
+    long most;  // workgroups of the launch
+  } kinds[] = {{256, 1, 0.f, 1.5f, 7.5f, kMaxTiles}, {128, 2, 0.1f, 0.43f, 4.5f, kMaxTiles},
+               {64, 2, 0.095f, 0.14f, 3.6f, kDeepMost + 1}, {64, 4, 0.1f, 0.19f, 3.5f, kMaxTiles}};
   const long steps = (K + kStep - 1) / kStep;
   float best = 0.f;
   *side = 256;
@@ -859,12 +872,11 @@ void product_plan(long M, long N, long K, int* side, int* splits) {
   if (M <= 0 || N <= 0) return;
   for (const auto& k : kinds) {
     const long tiles = ((M + k.side - 1) / k.side) * ((N + k.side - 1) / k.side);
-    if (tiles >= kMaxTiles) continue;
-    for (int sp = 1; sp <= 16 && (sp == 1 || sp * 2 <= steps); ++sp) {
+    for (int sp = 1; sp <= 16 && (sp == 1 || sp * 2 <= steps) && tiles * sp < k.most; ++sp) {
       const long w = (tiles * sp + kCus - 1) / kCus, full = w / k.per_cu, rest = w % k.per_cu, n = (steps + sp - 1) / sp;
       float t = full * (n * (k.step0 + k.step1 * k.per_cu) + k.fixed);
       if (rest) t += n * (k.step0 + k.step1 * rest) + k.fixed;
-      if (sp > 1) t += 3.5f + sp * (0.15f + 8e-7f * M * N);
+      if (sp > 1) t += 3.f + sp * (0.1f + 1.2e-6f * M * N);
       if (best == 0.f || t < best) {
         best = t;
         *side = k.side;

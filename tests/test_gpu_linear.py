@@ -101,6 +101,33 @@ def test_linear_whole_numbers(M, N, K, dtype):
         assert torch.equal(plain, got)
 
 
+@pytest.mark.parametrize("K", [40, 64, 100, 128, 192, 250, 256, 320, 384, 448, 600], ids=str)
+@pytest.mark.parametrize("M,N", [(70, 130), (40000, 48), (2600, 2600)], ids=str)
+def test_linear_contraction_lengths(M, N, K):
+    """Contractions from part of a step to ten steps, through every number of stages that a tile's operands have in LDS;
+    few tiles, many narrow ones and wide ones."""
+    print("test_linear_contraction_lengths", M, N, K, flush=True)
+    from ccq_amd import fused_linear
+    dev = _cuda()
+    gen = torch.Generator().manual_seed(M + K)
+    x, w, dy = whole(gen, M, K), whole(gen, N, K), whole(gen, M, N)
+    xg, wg, dg = (t.to(dev, BF) for t in (x, w, dy))
+    got, (dx, dw, _, _) = run(xg, wg, None, None, None, dg)
+    assert torch.equal(got.cpu(), (x @ w.T).to(BF))
+    assert torch.equal(dx.cpu(), (dy @ w).to(BF))
+    assert torch.equal(dw.cpu(), (dy.T @ x).to(BF))
+    # the contraction down the rows of both operands, of the same lengths
+    a, b = whole(gen, K, 72), whole(gen, K, 136)
+    _, (_, dw, _, _) = run(b.to(dev, BF), whole(gen, 72, 136).to(dev, BF), None, None, None, a.to(dev, BF))
+    assert torch.equal(dw.cpu(), (a.T @ b).to(BF))
+    z = x[:5] @ w.T
+    g, u = z.double().chunk(2, -1)
+    y = fused_linear(xg[:5], wg, activation="swiglu").cpu().double()
+    want = g * torch.sigmoid(g) * u
+    # one rounding, and a few units of fp32 of |g| <= 4 K in the exponential
+    assert ((y - want).abs() <= torch.finfo(BF).eps / 2 * want.abs() + U32 * 16 * (g.abs() + 1) * (g * u).abs() + 1e-30).all()
+
+
 @pytest.mark.parametrize("columns", [8, 3], ids=["aligned", "odd"])
 @pytest.mark.parametrize("M,N,K", [(40, 96, 64), (200, 131, 72), (2100, 2048, 136)], ids=str)
 def test_linear_strided_operands(M, N, K, columns):
