@@ -175,6 +175,13 @@ def test_linear_activations(M, N, K, act):
             assert ((have[2].cpu().double() - grads[2]).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("M,N,K", [(5, 44, 4200), (20, 130, 8200)], ids=str)
+@pytest.mark.parametrize("act", ACTS, ids=str)
+def test_linear_few_outputs_of_many_parts(M, N, K, act):
+    """Long contractions of few outputs: the forward adds ten parts and more before its epilogue."""
+    test_linear_activations(M, N, K, act)
+
+
 def test_linear_against_differences():
     """Central differences of the 64-bit formula along random directions; whole numbers and fp16, whose dz rounds by
     2^-11 (the bound), truncation h^2 = 1e-8."""
