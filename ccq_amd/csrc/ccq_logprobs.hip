@@ -311,15 +311,17 @@ void logprob_fwd_kernel(const LogprobArgs a) {
     top_of_row<T, THREADS>(top, row, V, a.k, mine, p.m, logz, a.top + r * a.k, a.top_ids + r * a.k);
 }
 
-// grid: (parts of a row, rows)
+// grid: (parts of a row, rows).  The rows from the last one on, whose logits the forward left in the last-level cache, and
+// neither these nor the gradients put there again: 16384 x 32000 bf16 forward and backward 566 -> 537 us, 4096 rows
+// 160 -> 137 (the products that read the gradients next take what they took).
 constexpr int kBwdPieces = 8;  // 16-byte pieces a thread, all in flight together
 template <typename T>
 __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(const LogprobArgs a) {
   constexpr int N = Piece<T>::N;
   typedef typename Piece<T>::vec vec;
   const int V = a.V;
-  const long r = (long)blockIdx.y + (long)blockIdx.z * 32768;
-  if (r >= a.rows) return;
+  const long r = a.rows - 1 - (long)blockIdx.y - (long)blockIdx.z * 32768;
+  if (r < 0) return;
   const int64_t id = a.ids[r];
   T* out = (T*)a.dx + r * V;
   const int c0 = (blockIdx.x * kBwdPieces * kThreads + threadIdx.x) * N;
@@ -333,7 +335,7 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(const LogprobArgs
   vec x[kBwdPieces];
 #pragma unroll
   for (int j = 0; j < kBwdPieces; ++j)
-    if (c0 + j * step < V) x[j] = load_piece(row, c0 + j * step, V);
+    if (c0 + j * step < V) x[j] = load_last(row, c0 + j * step, V);
   const float m = a.stats[2 * r], logz = a.stats[2 * r + 1], dent = a.dent ? a.dent[r] : 0.f;
   float dlogp = a.dlogp ? a.dlogp[r] : 0.f;
   if (id < 0 || id >= V || logz != logz) dlogp = NAN;  // such a row has no gradient either
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(const LogprobArgs
     vec o;
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = (T)g[i];
-    store_piece(out, at, V, o);
+    store_past(out, at, V, o);
   }
 }
 

@@ -42,6 +42,19 @@ __device__ __forceinline__ void store_piece(T* row, int c, int D, const typename
     if (c + i < D) *gmem(row + c + i) = v[i];
 }
 
+// The same for a row's last use, and for one that is not read soon: the caches keep what is.
+template <typename T>
+__device__ __forceinline__ typename Piece<T>::vec load_last(const T* row, int c, int D) {
+  if (c + Piece<T>::N <= D) return __builtin_nontemporal_load(gmem((const typename Piece<T>::any*)(row + c)));
+  return load_piece(row, c, D);
+}
+template <typename T>
+__device__ __forceinline__ void store_past(T* row, int c, int D, const typename Piece<T>::vec& v) {
+  typedef typename Piece<T>::any any;
+  if (c + Piece<T>::N <= D) __builtin_nontemporal_store((any)v, gmem((any*)(row + c)));
+  else store_piece(row, c, D, v);
+}
+
 // sum over groups of L consecutive lanes (L a power of two <= 64)
 __device__ __forceinline__ float lanes_sum(float x, int L) {
   for (int o = L >> 1; o > 0; o >>= 1) x += __shfl_xor(x, o);
