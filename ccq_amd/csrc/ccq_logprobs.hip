@@ -243,7 +243,7 @@ void logprob_fwd_kernel(const LogprobArgs a) {
   }
   const T* row = (const T*)a.x + r * a.ldx;
   Part p{-INFINITY, 0.f, 0.f};
-  float bound = INFINITY;
+  float bound = NAN;  // (reached by nothing, +inf neither: the list begins with the first bound)
   constexpr int step = THREADS * N;
   constexpr bool kNext = THREADS < 1024;  // the next pieces on their way too (sixteen waves have the registers for one set)
   typename Piece<T>::vec x[kAhead], y[kAhead];

@@ -1,0 +1,43 @@
+"""Rows at the edges of ``ccq_amd.token_logprobs``: infinities and NaN where the alternatives' list begins, rows of
+nothing but -inf with each of the two gradients alone.  Orders and NaN are exact; values beside them keep their bits."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, FL = torch.bfloat16, torch.float16, torch.float32
+
+
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    return torch.device("cuda")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FL], ids=str)
+@pytest.mark.parametrize("rows", [12, 600], ids=str)      # both workgroup sizes
+@pytest.mark.parametrize("V", [9, 1003, 40000], ids=str)
+def test_top_with_positive_infinities(V, rows, dtype):
+    """+inf from the first piece to the last one, alone and in every place: such rows are NaN, their alternatives in the
+    logits' order, and the other rows as they are without them."""
+    print("test_top_with_positive_infinities", V, rows, dtype, flush=True)
+    from ccq_amd import token_logprobs
+    dev = _cuda()
+    gen = torch.Generator().manual_seed(V + rows)
+    x = torch.randn(rows, V, generator=gen).to(dtype)
+    ids = torch.randint(0, V, (rows,), generator=gen).to(dev)
+    k = min(V, 7)
+    good = token_logprobs(x.to(dev), ids, k)
+    x[0, 0] = x[1, 8] = x[2, V - 1] = x[3, V // 2] = math.inf
+    x[4] = math.inf
+    x[5, ::2] = math.inf
+    x[6, ::2], x[6, 1::2] = math.inf, -math.inf
+    got = token_logprobs(x.to(dev), ids, k)
+    order = torch.sort(x.double(), dim=-1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(got.top_ids.cpu(), order)
+    assert got.logprobs[:7].isnan().all() and got.entropy[:7].isnan().all() and got.top_logprobs[:7].isnan().all()
+    for a, b in zip(got, good):
+        assert torch.equal(a[7:], b[7:])
