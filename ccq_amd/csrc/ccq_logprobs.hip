@@ -74,11 +74,12 @@ __device__ __forceinline__ float add_values(Part& p, const float (&v)[N]) {
   return m;
 }
 
-// Order of the alternatives: NaN before any number, the larger logit first, the lower index first.
+// Order of the alternatives: NaN before any number, the larger logit first, the lower index first.  A key lies above 0
+// and below 2^64 - 1, where the passes over a row begin: +inf's upper half is 0xff800000, -inf's 0x007fffff.
 __device__ __forceinline__ unsigned long long rank_key(float x, int i) {
   const int b = __float_as_int(x + 0.f);  // (-0 as +0)
   unsigned u = b < 0 ? ~(unsigned)b : (unsigned)b | 0x80000000u;
-  if (x != x) u = 0xffffffffu;
+  if (x != x) u = 0xfffffffeu;
   return (unsigned long long)u << 32 | (unsigned)~i;
 }
 __device__ __forceinline__ int key_index(unsigned long long k) { return (int)~(unsigned)k; }

@@ -41,3 +41,31 @@ def test_top_with_positive_infinities(V, rows, dtype):
     assert got.logprobs[:7].isnan().all() and got.entropy[:7].isnan().all() and got.top_logprobs[:7].isnan().all()
     for a, b in zip(got, good):
         assert torch.equal(a[7:], b[7:])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FL], ids=str)
+@pytest.mark.parametrize("rows", [6, 600], ids=str)
+@pytest.mark.parametrize("V", [1, 2, 64, 1003], ids=str)
+def test_top_with_nan_logits(V, rows, dtype):
+    """A NaN stands before every number, the lowest index first: at token 0, at the last one, all over the row, beside
+    +inf; with as many alternatives as tokens each of them once."""
+    print("test_top_with_nan_logits", V, rows, dtype, flush=True)
+    from ccq_amd import token_logprobs
+    dev = _cuda()
+    gen = torch.Generator().manual_seed(V + rows)
+    x = torch.randn(rows, V, generator=gen).to(dtype)
+    x[0, 0] = x[1, V - 1] = math.nan
+    x[2] = math.nan
+    x[3, 0], x[3, V // 2] = math.inf, math.nan
+    x[4, 0], x[4, V // 2] = math.nan, math.inf
+    ids = torch.randint(0, V, (rows,), generator=gen).to(dev)
+    key = torch.where(x.isnan(), math.inf, x.double()) + 0.0
+    # NaN first: a stable sort by the number, then one by being a NaN
+    order = torch.sort(key, dim=-1, descending=True, stable=True).indices
+    nan = x.isnan().gather(1, order).int()
+    order = order.gather(1, torch.sort(nan, dim=-1, descending=True, stable=True).indices)
+    for k in sorted({1, min(V, 5), min(V, 64)}):
+        got = token_logprobs(x.to(dev), ids, k)
+        assert torch.equal(got.top_ids.cpu(), order[:, :k]), k
+        assert got.top_logprobs[:5].isnan().all() and got.logprobs[:5].isnan().all()
+        assert torch.isfinite(got.top_logprobs[5:]).all()
