@@ -339,7 +339,8 @@ __global__ __launch_bounds__(kThreads) void logprob_bwd_kernel(const LogprobArgs
     if (c0 + j * step < V) x[j] = load_last(row, c0 + j * step, V);
   const float m = a.stats[2 * r], logz = a.stats[2 * r + 1], dent = a.dent ? a.dent[r] : 0.f;
   float dlogp = a.dlogp ? a.dlogp[r] : 0.f;
-  if (id < 0 || id >= V || logz != logz) dlogp = NAN;  // such a row has no gradient either
+  // such a row has no gradient either (log Z is NaN beside a NaN or +inf, -inf where nothing but -inf is)
+  if (id < 0 || id >= V || !(logz > -INFINITY)) dlogp = NAN;
   const float c = -(dlogp + dent * (dent != 0.f ? a.ent[r] : 0.f));
 #pragma unroll
   for (int j = 0; j < kBwdPieces; ++j) {

@@ -69,3 +69,37 @@ def test_top_with_nan_logits(V, rows, dtype):
         assert torch.equal(got.top_ids.cpu(), order[:, :k]), k
         assert got.top_logprobs[:5].isnan().all() and got.logprobs[:5].isnan().all()
         assert torch.isfinite(got.top_logprobs[5:]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FL], ids=str)
+@pytest.mark.parametrize("rows", [9, 600], ids=str)
+def test_gradient_of_rows_without_a_logit(rows, dtype):
+    """Nothing but -inf, a NaN, +inf, a token outside: NaN gradients whichever of the two results they come from, the
+    entropy's alone only where the entropy is NaN; the other rows as they are without them."""
+    print("test_gradient_of_rows_without_a_logit", rows, dtype, flush=True)
+    from ccq_amd import token_logprobs
+    dev = _cuda()
+    gen = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, 777, generator=gen).to(dtype)
+    ids = torch.randint(0, 777, (rows,), generator=gen)
+    good_ids = ids.clone()
+    bad = x.clone()
+    bad[0] = -math.inf
+    bad[1] = -math.inf
+    bad[2, 5], bad[3, 700] = math.nan, math.inf
+    bad[4] = -math.inf
+    ids[0], ids[4], ids[5] = 0, -100, 777
+    one, some, none = torch.ones(rows), torch.randn(rows, generator=gen), torch.zeros(rows)
+
+    def grad(x, ids, dlogp, dent):
+        leaf = x.to(dev).requires_grad_()
+        got = token_logprobs(leaf, ids.to(dev))
+        outs = [(o, g.to(dev)) for o, g in ((got.logprobs, dlogp), (got.entropy, dent)) if g is not None]
+        return torch.autograd.grad([o for o, _ in outs], leaf, [g for _, g in outs])[0]
+
+    for dlogp, dent in ((one, None), (one, none), (none, None), (None, some), (some, some), (None, none)):
+        dx, want = grad(bad, ids, dlogp, dent), grad(x, good_ids, dlogp, dent)
+        assert dx[:4].isnan().all(), (dlogp is None, dent is None)
+        assert dx[5].isnan().all()
+        assert (dx[4] == 0).all()
+        assert torch.equal(dx[6:], want[6:])
