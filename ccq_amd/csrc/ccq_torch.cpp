@@ -4,6 +4,7 @@
 // without waiting for the interpreter.
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -72,6 +73,14 @@ bool needs_grad(std::initializer_list<const Tensor*> xs) {
   for (const Tensor* x : xs)
     if (x->defined() && x->requires_grad()) return true;
   return false;
+}
+
+// The kernels have no forward-mode derivatives: an input or an arriving gradient with a tangent is refused, since results
+// without one would stand for a derivative of zero.
+void refuse_tangents(const std::string& who, std::initializer_list<const Tensor*> xs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* x : xs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!x->defined() || !x->_fw_grad(0).defined(), who, " has no forward-mode derivatives");
 }
 
 // A leaf that an earlier graph still holds takes its gradients on the stream where that graph was made.  Under capture
@@ -150,6 +159,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
       const bool need_w = present & 2 && ctx->needs_input_grad(++edge);
       const bool need_b = present & 4 && ctx->needs_input_grad(++edge);
       const Tensor ds = grads.size() > 1 ? grads[1] : Tensor();
+      refuse_tangents(layer ? "layer_norm" : "rms_norm", {&grads[0], &ds});
       if (grads[0].defined() || ds.defined()) {
         c10::DeviceGuard guard(saved[0].device());
         check_capture(saved[0]);
@@ -204,9 +214,10 @@ variable_list norm(const std::string& who, const Tensor& x, const OptTensor& wei
   require_on(who, "residual", residual, x);
   TORCH_CHECK_VALUE(!has(residual) || (residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type()), who,
                     ": residual: expected x's shape ", x.sizes(), " and type ", x.scalar_type());
-  require_gpu(who, x);
   const Tensor r = value(residual), w = has(weight) ? weight->contiguous() : Tensor(),
                b = has(bias) ? bias->contiguous() : Tensor();
+  refuse_tangents(who, {&x, &r, &w, &b});
+  require_gpu(who, x);
   if (needs_grad({&x, &r, &w, &b})) {
     auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     return BlockNorm::apply(x, opt(r), opt(w), opt(b), layer, eps);
@@ -257,6 +268,7 @@ struct TokenScore : torch::autograd::Function<TokenScore> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     Tensor dx;
+    refuse_tangents("token_logprobs", {&grads[0], &grads[1]});
     if (grads[0].defined() || grads[1].defined()) {
       at::NoGradGuard no_grad;
       const auto saved = ctx->get_saved_variables();
@@ -286,6 +298,7 @@ variable_list token_logprobs(const Tensor& logits, const Tensor& ids, int64_t to
   require_on(who, "ids", ids, logits);
   const int64_t most = std::min(kMaxTop, logits.size(-1));
   TORCH_CHECK_VALUE(top_k >= 0 && top_k <= most, who, ": top_k=", top_k, " must lie in [0, ", most, "]");
+  refuse_tangents(who, {&logits});
   require_gpu(who, logits);
   const Tensor i = ids.to(at::kLong);
   if (needs_grad({&logits})) return TokenScore::apply(logits, i, top_k, ignore);
@@ -355,6 +368,7 @@ struct FusedLinear : torch::autograd::Function<FusedLinear> {
       const int64_t present = ctx->saved_data["has"].toInt();
       const auto btype = (at::ScalarType)ctx->saved_data["bias"].toInt();
       int edge = 1;
+      refuse_tangents("fused_linear", {&dy});
       const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
       const bool need_b = present & 1 && ctx->needs_input_grad(++edge);
       const bool need_r = present & 2 && ctx->needs_input_grad(++edge);
@@ -401,8 +415,9 @@ Tensor fused_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias
   shape.back() = N;
   TORCH_CHECK_VALUE(!has(residual) || (residual->sizes() == at::IntArrayRef(shape) && residual->scalar_type() == x.scalar_type()),
                     who, ": residual: expected ", at::IntArrayRef(shape), " ", x.scalar_type());
-  require_gpu(who, x);
   const Tensor b = has(bias) ? bias->contiguous() : Tensor(), r = value(residual);
+  refuse_tangents(who, {&x, &weight, &b, &r});
+  require_gpu(who, x);
   if (needs_grad({&x, &weight, &b, &r})) {
     auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     return FusedLinear::apply(x, weight, opt(b), opt(r), act)[0];
