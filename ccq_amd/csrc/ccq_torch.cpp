@@ -27,7 +27,7 @@ using torch::autograd::Variable;
 using torch::autograd::variable_list;
 using OptTensor = std::optional<Tensor>;
 
-constexpr int64_t kMaxNorm = 8192, kMaxTop = 64, kMaxStride = int64_t(1) << 22;
+constexpr int64_t kMaxNorm = 8192, kMaxTop = 64, kMaxVocabulary = int64_t(1) << 30, kMaxStride = int64_t(1) << 22;
 
 bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
 const void* address(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
@@ -295,6 +295,8 @@ variable_list token_logprobs(const Tensor& logits, const Tensor& ids, int64_t to
                    " takes int64 or int32 ids (got ", ids.scalar_type(), ")");
   TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1 && ids.sizes() == logits.sizes().slice(0, logits.dim() - 1),
                     who, ": ids ", ids.sizes(), ": expected the positions of logits ", logits.sizes());
+  TORCH_CHECK_VALUE(logits.size(-1) <= kMaxVocabulary, who, ": logits ", logits.sizes(), ": needs a last dimension of at most ",
+                    kMaxVocabulary);
   require_on(who, "ids", ids, logits);
   const int64_t most = std::min(kMaxTop, logits.size(-1));
   TORCH_CHECK_VALUE(top_k >= 0 && top_k <= most, who, ": top_k=", top_k, " must lie in [0, ", most, "]");

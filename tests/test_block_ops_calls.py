@@ -41,3 +41,13 @@ def test_forward_mode_is_refused(name, leaf):
             call(dual)
         with pytest.raises(RuntimeError, match="GPU only"):     # its value alone
             call(fwAD.unpack_dual(dual).primal)
+
+
+@pytest.mark.parametrize("V", [(1 << 30) + 1, (1 << 32) + 8, 1 << 40])
+def test_vocabularies_that_a_row_cannot_count_are_refused(V):
+    """Above 2^30 tokens, which the kernels' columns count to; a size that 32 bits would cut to a small one among them."""
+    x = torch.zeros(1, 1, dtype=BF).expand(2, V)
+    with pytest.raises(ValueError, match="last dimension"):
+        token_logprobs(x, torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="GPU only"):
+        token_logprobs(x[:, :1 << 30], torch.zeros(2, dtype=torch.int64))
