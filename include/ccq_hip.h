@@ -519,7 +519,7 @@ int ccq_token_logprobs_bwd(const void* logits, int64_t ldx, const int64_t* ids, 
  * with zeros behind column K (ccq_pad_rows makes such a copy of any rows); bias [N] (swiglu: [2 N]) of
  * bdtype, dtype or F32 (nullable); r [M, N] (row stride ldr, nullable); y [M, N] contiguous.
  * z (nullable): x W^T + b for the backward of an activation, 3 M ldz bytes, ldz = N (swiglu: 2 N) rounded
- * up to a multiple of 8: the upper 16 bits of the fp32 values [M, ldz], then the 8 below them [M, ldz].
+ * up to a multiple of 8: of the fp32 values rounded to 24 bits, the upper 16 [M, ldz], then the 8 below them [M, ldz].
  * fp32 accumulation, bias, activation and residual; y rounds once.  act: CCQ_ACT_*:
  * none, relu, silu, gelu (erf), gelu with tanh, swiglu (silu(gate) up).  workspace:
  * ccq_linear_workspace_bytes bytes (partial sums where few tiles split the contraction).

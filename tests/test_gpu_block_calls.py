@@ -38,3 +38,69 @@ def test_forward_mode_through_a_gradient_is_refused(name):
             call(fwAD.make_dual(x.detach(), torch.ones_like(x)))
         got, = torch.autograd.grad(y, x, fwAD.unpack_dual(dual).primal, retain_graph=True)
         assert torch.equal(got, want) and torch.equal(call(x.detach()), y)
+
+
+def kept_z(x, w, act, bias=None):
+    """What a training forward keeps of x W^T + b (b fp32) for the activation's backward: 16 bits, then 8, of every value."""
+    from ccq_amd import _lib
+    lib = _lib.load()
+    M, K, outs = x.shape[0], x.shape[1], w.shape[0]
+    N, ld = outs // 2 if act == 5 else outs, (outs + 7) // 8 * 8
+    y = torch.empty(M, N, device=x.device, dtype=x.dtype)
+    z = torch.zeros(3 * M * ld, device=x.device, dtype=torch.uint8)
+    ws = torch.empty(max(16, lib.ccq_linear_workspace_bytes(M, N, K, act)), device=x.device, dtype=torch.uint8)
+    status = lib.ccq_linear_fwd(x.data_ptr(), K, w.data_ptr(), K, None if bias is None else bias.data_ptr(), 2, None, 0,
+                                y.data_ptr(), z.data_ptr(), ws.data_ptr(), M, N, K, act, 0,
+                                torch.cuda.current_stream().cuda_stream)
+    assert status == 0, lib.ccq_last_error()
+    z = z.cpu()
+    hi = z[:2 * M * ld].view(torch.int16).view(M, ld)[:, :outs].int()
+    lo = z[2 * M * ld:].view(M, ld)[:, :outs].int()
+    return (hi << 16 | lo << 8).view(torch.float32)
+
+
+@pytest.mark.parametrize("act", [2, 5], ids=["silu", "swiglu"])
+@pytest.mark.parametrize("M,N,K", [(40, 70, 8), (700, 301, 64), (3000, 1500, 128), (6, 44, 4200)], ids=str)
+def test_kept_values_round_to_nearest(M, N, K, act):
+    """Whole numbers of 24 bits: at most half a step of 16 bits, and the 4 units of 2^-24 that the products may err by
+    (4 / 256 of a step).  (6 x 44 over 4200 adds parts of the contraction.)"""
+    print("test_kept_values_round_to_nearest", M, N, K, act, flush=True)
+    dev = _cuda()
+    gen = torch.Generator().manual_seed(M + K)
+    outs = 2 * N if act == 5 else N
+    x = torch.zeros(M, K)
+    x[:, 0], x[:, 1], x[:, K - 1] = 65536, 256, 1
+    x *= torch.randint(0, 2, (M, 1), generator=gen) * 2 - 1
+    w = torch.zeros(outs, K)
+    w[:, [0, 1, K - 1]] = torch.randint(0, 256, (outs, 3), generator=gen).float()
+    z = x.double() @ w.double().T
+    kept = kept_z(x.to(dev, BF), w.to(dev, BF), act).double()
+    step = torch.exp2(torch.floor(torch.log2(z.abs().clamp_min(1))) - 15)
+    worst = ((kept - z).abs() / step).max().item()
+    assert worst <= 0.5 + 4 / 256, worst
+
+
+def test_kept_values_at_the_ends():
+    """The largest finite value stays finite, infinities and NaN stay, zeros keep their sign."""
+    dev = _cuda()
+    x = torch.zeros(8, 8, device=dev, dtype=BF)
+    x[:, :3] = torch.tensor([torch.finfo(BF).max, 255 * 2.0 ** 112, 255 * 2.0 ** 104], dtype=BF)
+    x[1] = -x[1]
+    x[2, 1:] = 0
+    x[3] = float("inf")
+    x[4] = -float("inf")
+    x[5, 0] = float("nan")
+    x[6] = 0
+    x[7] = 2.0 ** -120
+    w = torch.ones(16, 8, device=dev, dtype=BF)
+    kept = kept_z(x, w, 2)
+    big = torch.finfo(FL).max
+    assert torch.isfinite(kept[:3]).all() and torch.isfinite(kept[6:]).all()
+    assert ((kept[0] - big).abs() <= big * 2.0 ** -15).all() and ((kept[1] + big).abs() <= big * 2.0 ** -15).all()
+    assert (kept[2] == torch.finfo(BF).max).all()
+    assert (kept[3] == float("inf")).all() and (kept[4] == -float("inf")).all() and kept[5].isnan().all()
+    assert (kept[6] == 0).all() and (kept[7] == 2.0 ** -117).all()
+    # NaN of any payload: of the lowest bit alone, of all of them, of either sign
+    bits = torch.tensor([0x7f800001, 0x7fffffff, 0x800001 - 2 ** 31 + 0x7f000000, -1] * 4, dtype=torch.int32)
+    assert bits.view(FL).isnan().all()
+    assert kept_z(x[6:], w, 2, bits.to(dev).view(FL)).isnan().all()
