@@ -74,6 +74,7 @@ SIGNATURES = {
     "ccq_norm_bwd": (_I, [_P, _I64] + [_P] * 4 + [_I64, _P, _I64] + [_P] * 4 + [_I64] + [_I] * 4 + [_P]),
     "ccq_token_logprobs_fwd": (_I, [_P, _I64] + [_P] * 6 + [_I64, _I, _I, _I64, _I, _P]),
     "ccq_token_logprobs_bwd": (_I, [_P, _I64] + [_P] * 6 + [_I64, _I, _I64, _I, _P]),
+    "ccq_linear_plan": (_I, [_I64] * 3 + [_P] * 2),
     "ccq_linear_workspace_bytes": (_SZ, [_I64] * 3 + [_I]),
     "ccq_linear_fwd": (_I, [_P, _I64] * 2 + [_P, _I, _P, _I64] + [_P] * 3 + [_I64] * 3 + [_I, _I, _P]),
     "ccq_linear_bwd_workspace_bytes": (_SZ, [_I64] * 3 + [_I]),

@@ -1668,6 +1668,15 @@ size_t carve_linear_bwd(char* base, int64_t M, int64_t N, int64_t K, int act, Li
 
 extern "C" {
 
+int ccq_linear_plan(int64_t M, int64_t N, int64_t K, int* side, int* parts) {
+  const char* who = "ccq_linear_plan";
+  if (M < 1 || N < 1 || K < 1 || M > kMaxSide || N > kMaxSide || K > kMaxSide)
+    return fail(CCQ_ERR_SHAPE, "%s: M=%lld N=%lld K=%lld", who, (long long)M, (long long)N, (long long)K);
+  if (!side || !parts) return fail(CCQ_ERR_NULL, "%s: side and parts are required", who);
+  product_plan(M, N, K, side, parts);
+  return CCQ_OK;
+}
+
 size_t ccq_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int act) {
   return M > 0 && N > 0 && K > 0 ? partial_bytes(M, linear_outs(N, act), K) : 0;
 }

@@ -534,6 +534,9 @@ int ccq_token_logprobs_bwd(const void* logits, int64_t ldx, const int64_t* ids, 
 #define CCQ_ACT_GELU 3
 #define CCQ_ACT_GELU_TANH 4
 #define CCQ_ACT_SWIGLU 5
+/* How a product of M x N outputs (swiglu: N all 2 N rows of the weight; backward: dx is M x K over N, dw N x K over M) over
+ * K runs: sides of its square tiles (256, 128 or 64) and parts of the contraction, added through the workspace. */
+int ccq_linear_plan(int64_t M, int64_t N, int64_t K, int* side, int* parts);
 size_t ccq_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int act);
 int ccq_linear_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias, int bdtype,
                    const void* r, int64_t ldr, void* y, void* z, void* workspace, int64_t M, int64_t N, int64_t K,

@@ -1,6 +1,8 @@
 """Calls of the operators around the mixers that are refused on any device: derivatives that the kernels do not have,
 sizes that they cannot count."""
 
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -51,3 +53,12 @@ def test_vocabularies_that_a_row_cannot_count_are_refused(V):
         token_logprobs(x, torch.zeros(2, dtype=torch.int64))
     with pytest.raises(RuntimeError, match="GPU only"):
         token_logprobs(x[:, :1 << 30], torch.zeros(2, dtype=torch.int64))
+
+
+def test_linear_plan_refusals():
+    from ccq_amd import _lib
+    lib = _lib.load()
+    a, b = ctypes.c_int(), ctypes.c_int()
+    for size in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (1 << 31, 1, 1)):
+        assert lib.ccq_linear_plan(*size, ctypes.byref(a), ctypes.byref(b)) == -1
+    assert lib.ccq_linear_plan(1, 1, 1, None, ctypes.byref(b)) == -2
