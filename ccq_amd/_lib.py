@@ -78,6 +78,7 @@ SIGNATURES = {
     "ccq_linear_workspace_bytes": (_SZ, [_I64] * 3 + [_I]),
     "ccq_linear_fwd": (_I, [_P, _I64] * 2 + [_P, _I, _P, _I64] + [_P] * 3 + [_I64] * 3 + [_I, _I, _P]),
     "ccq_linear_bwd_workspace_bytes": (_SZ, [_I64] * 3 + [_I]),
+    "ccq_linear_bwd_call_workspace_bytes": (_SZ, [_I64] * 3 + [_I, _P, _I64] + [_I] * 3),
     "ccq_linear_bwd": (_I, [_P, _I64] * 2 + [_P, _P, _I64] + [_P] * 3 + [_I, _P] + [_I64] * 3 + [_I, _I, _P]),
     "ccq_pad_rows": (_I, [_P, _I64, _P] + [_I64] * 3 + [_P]),
     "ccq_timing_enable": (_I, [_I]),

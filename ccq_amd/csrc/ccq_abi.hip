@@ -1647,19 +1647,28 @@ int linear_check(const char* who, int64_t M, int64_t N, int64_t K, int64_t ldx, 
   return CCQ_OK;
 }
 
+// What a backward call makes: dz in a buffer of its own where a product needs one, and which gradients.
+struct LinearBwdParts {
+  bool dz, dx, dw, db;
+};
+// Without an activation dz is dy itself, where its rows can be read as an operand's.
+LinearBwdParts linear_bwd_parts(const void* dy, int64_t ldy, int64_t N, int act, bool dx, bool dw, bool db) {
+  const bool direct = act == CCQ_ACT_NONE && N % 8 == 0 && rows16(dy, ldy) && ldy <= kMaxStride;
+  return {(dx || dw) && !direct, dx, dw, db};
+}
 // Sub-buffers of the backward's workspace: dz, the partial sums of db and of a product.
 struct LinearBwd {
   char* dz;
   float* db_part;
   float* part;
 };
-size_t carve_linear_bwd(char* base, int64_t M, int64_t N, int64_t K, int act, LinearBwd* out) {
+size_t carve_linear_bwd(char* base, int64_t M, int64_t N, int64_t K, int act, const LinearBwdParts& p, LinearBwd* out) {
   Slicer sl{base};
   const long Nz = linear_outs(N, act);
   LinearBwd t;
-  t.dz = sl.take<char>((size_t)M * round8(Nz) * 2);
-  t.db_part = sl.take<float>((size_t)(M > 0 ? act_bwd_row_blocks(M, N) : 0) * Nz);
-  t.part = (float*)sl.take<char>(std::max(partial_bytes(M, K, Nz), partial_bytes(Nz, K, M)));
+  t.dz = sl.take<char>(p.dz ? (size_t)M * round8(Nz) * 2 : 0);
+  t.db_part = sl.take<float>((size_t)(p.db && M > 0 ? act_bwd_row_blocks(M, N) : 0) * Nz);
+  t.part = (float*)sl.take<char>(std::max(p.dx ? partial_bytes(M, K, Nz) : 0, p.dw ? partial_bytes(Nz, K, M) : 0));
   if (out) *out = t;
   return sl.off;
 }
@@ -1704,7 +1713,12 @@ int ccq_linear_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, 
 }
 
 size_t ccq_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int act) {
-  return M >= 0 && N > 0 && K > 0 ? carve_linear_bwd(nullptr, M, N, K, act, nullptr) : 0;
+  return M >= 0 && N > 0 && K > 0 ? carve_linear_bwd(nullptr, M, N, K, act, {true, true, true, true}, nullptr) : 0;
+}
+size_t ccq_linear_bwd_call_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, const void* dy, int64_t ldy, int dx,
+                                           int dw, int db) {
+  if (M < 0 || N < 1 || K < 1) return 0;
+  return carve_linear_bwd(nullptr, M, N, K, act, linear_bwd_parts(dy, ldy, N, act, dx, dw, db), nullptr);
 }
 
 int ccq_linear_bwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* z, const void* dy,
@@ -1714,7 +1728,8 @@ int ccq_linear_bwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, 
   if (int e = linear_check(who, M, N, K, ldx, ldw, act, dtype, bdtype)) return e;
   if (ldy < N) return fail(CCQ_ERR_SHAPE, "%s: dy's row stride %lld is below N=%lld", who, (long long)ldy, (long long)N);
   if (!dx && !dw && !db) return CCQ_OK;
-  if ((!workspace && ccq_linear_bwd_workspace_bytes(M, N, K, act)) || (M > 0 && (!dy || (dw && !x) || (dx && !weight) || (act != CCQ_ACT_NONE && !z))))
+  const LinearBwdParts parts = linear_bwd_parts(dy, ldy, N, act, dx, dw, db);
+  if ((!workspace && carve_linear_bwd(nullptr, M, N, K, act, parts, nullptr)) || (M > 0 && (!dy || (dw && !x) || (dx && !weight) || (act != CCQ_ACT_NONE && !z))))
     return fail(CCQ_ERR_NULL, "%s: dy, x (for dw), weight (for dx), z (with an activation) and the workspace are required", who);
   if (!aligned16(x) || !aligned16(weight) || !aligned16(z) || !aligned16(workspace))
     return fail(CCQ_ERR_ALIGN, "%s: x, weight, z and the workspace must be 16-byte aligned", who);
@@ -1722,19 +1737,17 @@ int ccq_linear_bwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, 
     return fail(CCQ_ERR_ALIGN, "%s: dy, dx, dw and db must be aligned to their elements", who);
   if (int e = check_stream_device(stream, who)) return e;
   LinearBwd ws;
-  carve_linear_bwd((char*)workspace, M, N, K, act, &ws);
+  carve_linear_bwd((char*)workspace, M, N, K, act, parts, &ws);
   const long Nz = linear_outs(N, act), ldz = round8(Nz);
   hipStream_t st = (hipStream_t)stream;
-  // without an activation dz is dy itself, where its rows can be read as an operand's
-  const bool direct = act == CCQ_ACT_NONE && N % 8 == 0 && rows16(dy, ldy) && ldy <= kMaxStride;
-  if (!direct || db) {
+  if (parts.dz || db) {
     ActBwdArgs a{};
-    a.z = act == CCQ_ACT_NONE ? nullptr : z; a.dy = dy; a.dz = direct ? nullptr : ws.dz; a.db_part = db ? ws.db_part : nullptr;
+    a.z = act == CCQ_ACT_NONE ? nullptr : z; a.dy = dy; a.dz = parts.dz ? ws.dz : nullptr; a.db_part = db ? ws.db_part : nullptr;
     a.db = db; a.M = M; a.N = N; a.ldz = ldz; a.ldy = ldy; a.act = act; a.bdtype = bdtype; a.dtype = dtype;
     if (int e = hip_status(timed("linear_dz", st, [&] { return launch_act_bwd(a, st); }), who)) return e;
   }
   ProductArgs p{};
-  p.a = direct ? dy : ws.dz; p.lda = direct ? ldy : ldz; p.part = ws.part; p.act = CCQ_ACT_NONE; p.dtype = dtype;
+  p.a = parts.dz ? ws.dz : dy; p.lda = parts.dz ? ldz : ldy; p.part = ws.part; p.act = CCQ_ACT_NONE; p.dtype = dtype;
   p.bdtype = dtype; p.N = K; p.ldo = K;
   if (dx) {
     p.b = weight; p.ldb = ldw; p.M = M; p.K = Nz; p.out = dx;

@@ -385,7 +385,8 @@ struct FusedLinear : torch::autograd::Function<FusedLinear> {
         if (need_w) dw = fresh(x, {outs, K}, type);
         if (need_b) db = fresh(x, {outs}, btype);
         const Tensor a = need_w ? operand(x) : Tensor(), b = need_x ? operand(w) : Tensor();
-        const Tensor ws = bytes(x, ccq_linear_bwd_workspace_bytes(M, N, K, act));
+        const size_t n = ccq_linear_bwd_call_workspace_bytes(M, N, K, act, address(d), stride_of(d), need_x, need_w, need_b);
+        const Tensor ws = n ? bytes(x, n) : Tensor();
         check(ccq_linear_bwd(address(a), need_w ? stride_of(a) : ld, address(b), need_x ? stride_of(b) : ld,
                              address(saved[2]), address(d), stride_of(d), out_address(dx), out_address(dw),
                              out_address(db), code(btype), out_address(ws), M, N, K, act, code(type), stream_on(x)),

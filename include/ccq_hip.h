@@ -526,7 +526,10 @@ int ccq_token_logprobs_bwd(const void* logits, int64_t ldx, const int64_t* ids, 
  * Backward: dz = act'(z) dy (rounded to dtype once, as it enters two products), dx = dz W [M, K],
  * dw = dz^T x (weight's shape), both contiguous, db = the sum of dz's rows in fp32, rounded to bdtype
  * (each nullable); dy [M, N] (row stride ldy); z as the forward left it (not for act none).  The residual's
- * gradient is dy.  workspace: ccq_linear_bwd_workspace_bytes bytes.  All sums run in a fixed order.
+ * gradient is dy.  workspace: ccq_linear_bwd_workspace_bytes bytes hold any call of the sizes (dz [M, N rounded up], its
+ * sums and a product's); ccq_linear_bwd_call_workspace_bytes is what the call with this dy, ldy and these gradients (not 0:
+ * wanted) needs, nothing for dz where dy is read in its place (no activation, N and ldy multiples of 8, dy 16-byte
+ * aligned).  All sums run in a fixed order.
  */
 #define CCQ_ACT_NONE 0
 #define CCQ_ACT_RELU 1
@@ -542,6 +545,8 @@ int ccq_linear_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, 
                    const void* r, int64_t ldr, void* y, void* z, void* workspace, int64_t M, int64_t N, int64_t K,
                    int act, int dtype, void* stream);
 size_t ccq_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int act);
+size_t ccq_linear_bwd_call_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, const void* dy, int64_t ldy, int dx,
+                                           int dw, int db);
 int ccq_linear_bwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* z, const void* dy,
                    int64_t ldy, void* dx, void* dw, void* db, int bdtype, void* workspace, int64_t M, int64_t N,
                    int64_t K, int act, int dtype, void* stream);

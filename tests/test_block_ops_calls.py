@@ -7,7 +7,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
-from ccq_amd import fused_linear, layer_norm, rms_norm, token_logprobs
+from ccq_amd import _lib, fused_linear, layer_norm, rms_norm, token_logprobs
 
 BF = torch.bfloat16
 
@@ -56,9 +56,29 @@ def test_vocabularies_that_a_row_cannot_count_are_refused(V):
 
 
 def test_linear_plan_refusals():
-    from ccq_amd import _lib
     lib = _lib.load()
     a, b = ctypes.c_int(), ctypes.c_int()
     for size in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (1 << 31, 1, 1)):
         assert lib.ccq_linear_plan(*size, ctypes.byref(a), ctypes.byref(b)) == -1
     assert lib.ccq_linear_plan(1, 1, 1, None, ctypes.byref(b)) == -2
+
+
+def test_linear_backward_workspace_of_a_call():
+    """dz has no place where dy is read itself, the bias's partial sums none without its gradient."""
+    lib = _lib.load()
+
+    def need(M, N, K, act=0, dy=0x1000, ldy=None, dx=1, dw=1, db=0):
+        return lib.ccq_linear_bwd_call_workspace_bytes(M, N, K, act, ctypes.c_void_p(dy), N if ldy is None else ldy, dx, dw, db)
+
+    parts = max(lib.ccq_linear_workspace_bytes(16384, 1024, 32000, 0), lib.ccq_linear_workspace_bytes(32000, 1024, 16384, 0))
+    dz = 16384 * 32000 * 2
+    assert need(16384, 32000, 1024) <= parts + 256
+    for case in (dict(dy=0x1008), dict(ldy=32004), dict(ldy=(1 << 22) + 8), dict(act=2)):
+        assert dz <= need(16384, 32000, 1024, **case) <= dz + parts + 512, case
+    assert need(16384, 32000, 1024, act=2, dx=0, dw=0, db=1) < dz    # (db alone: no product reads dz)
+    assert need(16384, 31999, 1024) >= dz - 16384 * 2
+    assert 0 < need(64, 64, 64, db=1) <= lib.ccq_linear_bwd_workspace_bytes(64, 64, 64, 0)
+    assert need(64, 64, 64) == 0 and need(0, 64, 64, act=2) == 0 and need(-1, 64, 64) == 0
+    for act in range(6):
+        for M, N, K in ((1, 1, 1), (16384, 2816, 1024), (37, 4200, 24), (128, 128, 262144)):
+            assert need(M, N, K, act, dy=0x1002, db=1) <= lib.ccq_linear_bwd_workspace_bytes(M, N, K, act)

@@ -104,3 +104,51 @@ def test_kept_values_at_the_ends():
     bits = torch.tensor([0x7f800001, 0x7fffffff, 0x800001 - 2 ** 31 + 0x7f000000, -1] * 4, dtype=torch.int32)
     assert bits.view(FL).isnan().all()
     assert kept_z(x[6:], w, 2, bits.to(dev).view(FL)).isnan().all()
+
+
+@pytest.mark.parametrize("bias", [False, True], ids=["plain", "bias"])
+def test_linear_backward_memory_of_a_head(bias):
+    """A head's backward reads the logits' gradient where it lies: beside the gradients it allocates the products' and
+    the bias's partial sums, nothing of the logits' size."""
+    from ccq_amd import _lib, fused_linear
+    dev, lib = _cuda(), _lib.load()
+    M, N, K = 4096, 32000, 256
+    gen = torch.Generator(dev).manual_seed(4)
+    x = torch.randint(-2, 3, (M, K), generator=gen, device=dev).to(BF).requires_grad_()
+    w = torch.randint(-2, 3, (N, K), generator=gen, device=dev).to(BF).requires_grad_()
+    leaves = [x, w] + ([torch.zeros(N, device=dev, requires_grad=True)] if bias else [])
+    y = fused_linear(*leaves)
+    dy = torch.randint(-2, 3, (M, N), generator=gen, device=dev).to(BF)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    grads = torch.autograd.grad(y, leaves, dy)
+    peak = torch.cuda.max_memory_allocated() - before
+    most = lib.ccq_linear_bwd_call_workspace_bytes(M, N, K, 0, dy.data_ptr(), N, 1, 1, int(bias))
+    assert peak <= sum(2 * g.numel() for g in grads[:2]) + 4 * N + most + (8 << 20), peak    # (blocks of whole MiB)
+    assert bias or most < M * N
+    assert torch.equal(grads[0], (dy.float() @ w.detach().float()).to(BF))
+    assert torch.equal(grads[1], (dy.float().T @ x.detach().float()).to(BF))
+    if bias:
+        assert torch.equal(grads[2], dy.float().sum(0))
+
+
+@pytest.mark.parametrize("act", [None, "silu", "swiglu"])
+@pytest.mark.parametrize("wanted", range(1, 8))
+def test_linear_gradients_one_by_one(act, wanted):
+    """Any set of the gradients of x, weight and bias: each call's own workspace, the same bits as of all together; from
+    rows of dy that are read in place, padded ones and ones inside wider rows."""
+    from ccq_amd import fused_linear
+    dev = _cuda()
+    gen = torch.Generator(dev).manual_seed(5)
+    for M, N, K, pad in ((300, 136, 200, 0), (300, 136, 200, 8), (300, 131, 72, 0), (70, 44, 4200, 0), (2100, 64, 64, 1)):
+        outs = 2 * N if act == "swiglu" else N
+        x, w, b = (torch.randn(*s, generator=gen, device=dev).to(BF) for s in ((M, K), (outs, K), (outs,)))
+        dy = torch.randn(M, N + pad, generator=gen, device=dev).to(BF)[:, :N]
+
+        def grads(which):
+            leaves = [t.detach().requires_grad_(bool(which >> i & 1)) for i, t in enumerate((x, w / K ** 0.5, b))]
+            return torch.autograd.grad(fused_linear(*leaves, activation=act), [t for t in leaves if t.requires_grad], dy)
+
+        want = [g for i, g in enumerate(grads(7)) if wanted >> i & 1]
+        assert all(torch.equal(s, t) for s, t in zip(grads(wanted), want))
