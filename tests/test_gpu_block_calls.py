@@ -152,3 +152,50 @@ def test_linear_gradients_one_by_one(act, wanted):
 
         want = [g for i, g in enumerate(grads(7)) if wanted >> i & 1]
         assert all(torch.equal(s, t) for s, t in zip(grads(wanted), want))
+
+
+def test_more_than_2_31_elements():
+    """Rows whose offsets pass 32 bits, forward and backward: the last rows as in a call of them alone (600 rows and more
+    take the same workgroups), whole numbers for the linear map."""
+    from ccq_amd import fused_linear, rms_norm, token_logprobs
+    dev = _cuda()
+    gen = torch.Generator(dev).manual_seed(6)
+    tail = slice(-700, None)
+
+    def norm(x, r, dy):
+        x = x.detach().requires_grad_()
+        y, s = rms_norm(x, None, residual=r)
+        return [y, s, torch.autograd.grad(y, x, dy)[0]]
+
+    def score(x, ids):
+        x = x.detach().requires_grad_()
+        got = token_logprobs(x, ids, 3)
+        return [*got, torch.autograd.grad(got.logprobs.sum(), x)[0]]
+
+    rows = 2 ** 31 // 8192 + 1000
+    x, dy = (torch.empty(rows, 8192, device=dev, dtype=BF).normal_(generator=gen) for _ in range(2))
+    print("norm", flush=True)
+    for a, b in zip(norm(x, dy, dy), norm(x[tail], dy[tail], dy[tail])):
+        assert torch.equal(a[tail], b)
+    del x, dy, a, b
+    rows = 2 ** 31 // 32000 + 1000
+    x = torch.empty(rows, 32000, device=dev, dtype=BF).normal_(generator=gen)
+    ids = torch.randint(0, 32000, (rows,), generator=gen, device=dev)
+    print("logprobs", flush=True)
+    for a, b in zip(score(x, ids), score(x[tail], ids[tail])):
+        assert torch.equal(a[tail], b)
+    del x, ids, a, b
+    M, N, K = 2 ** 31 // 4096 + 1000, 4096, 64
+    x, w, dy = (torch.randint(-2, 3, s, generator=gen, device=dev, dtype=torch.int8).to(BF) for s in ((M, K), (N, K), (M, N)))
+    x.requires_grad_(), w.requires_grad_()
+    print("linear", flush=True)
+    y = fused_linear(x, w, activation="relu")
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    z = x[tail].detach().float() @ w.detach().float().T
+    dz = dy[tail].float() * (z > 0)
+    assert torch.equal(y[tail], z.relu().to(BF)) and torch.equal(dx[tail], (dz @ w.detach().float()).to(BF))
+    want = torch.zeros(N, K, device=dev)
+    for part in range(0, M, 65536):     # (sums of whole numbers below 2^24)
+        p, q = x[part:part + 65536].detach().float(), dy[part:part + 65536].float()
+        want += (q * (p @ w.detach().float().T > 0)).T @ p
+    assert torch.equal(dw, want.to(BF))
