@@ -38,9 +38,9 @@ constexpr float kTanhA = 0.7978845608028654f, kTanhB = 0.044715f;  // gelu_tanh:
 __device__ __forceinline__ float exp_(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp_(-z)); }
 
-// erfc(x) = t e^(P(t) - x^2), t = 1 / (1 + x / 2), for x >= 0, and 2 - erfc(-x): P the polynomial of degree 9 nearest
-// to log(erfc(x) e^(x^2) / t) over t in (0, 1] in the largest error (1.0e-7; fitted at 400 Chebyshev nodes with
-// weights that even the errors out).  In fp32 within 4e-7.
+// erfc(x) = t e^(P(t) - x^2), t = 1 / (1 + x / 2), for x >= 0, and 2 - erfc(-x): the form of Numerical Recipes (section
+// 6.2), its P of degree 9 fitted anew, the polynomial nearest to log(erfc(x) e^(x^2) / t) over t in (0, 1] in the largest
+// error (1.0e-7; at 400 Chebyshev nodes with weights that even the errors out).  In fp32 within 4e-7.
 __device__ __forceinline__ float erfc_(float x) {
   const float a = fabsf(x), t = __builtin_amdgcn_rcpf(1.f + 0.5f * a);
   float p = 0.168761006f;
@@ -720,7 +720,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const ProductArgs p) {
 // ---------------------------------------------------------------------------
 // dz = act'(z) dy, with the bias's gradient: a wave takes up to 512 columns, 8 a lane, of a block of rows (narrower
 // maps: several rows at once), two rows a lane loaded together; its sums are one partial row of db.  Bound by HBM bytes
-// (16384 x 2816 swiglu 106 us, 5.2 TB/s).
+// (16384 x 2816 swiglu 104 us, 5.3 TB/s).
 // ---------------------------------------------------------------------------
 constexpr int kActRows = 2;
 template <typename T, bool glu>
@@ -833,8 +833,8 @@ hipError_t launch_tiles(const ProductArgs& p, hipStream_t st) {
 
 constexpr int kCus = 256;
 // Few tiles of 64 x 64: four stages of both operands in LDS instead of three and two, so two workgroups a CU instead of
-// four, and twice the bytes on their way (operands from HBM: 16 x 5632 over 1024 11.3 -> 7.9 us, 1024^3 9.8 -> 8.2; out of
-// the caches 0.2 slower.  With more tiles four a CU are ahead: 4096 x 2048 over 512 18.6, 23.1 so).
+// four, and twice the bytes on their way (operands from HBM: 16 x 5632 over 1024 12.2 -> 7.7 us, 1024^3 10.5 -> 7.9; out
+// of the caches 0.2 slower.  With more tiles four a CU are ahead: 4096 x 2048 over 512 18.6, 23.1 so).
 constexpr int kDeepMost = 2 * kCus;
 
 template <typename T, bool DA, bool DB, int MODE, int ACT = kActNone>
@@ -847,8 +847,8 @@ hipError_t launch_size(const ProductArgs& p, int side, hipStream_t st) {
   return launch_tiles<T, 64, 64, 2, 2, 3, 2, DA, DB, MODE, ACT>(p, st);
 }
 
-// Eight threads an output where there are few outputs and many parts (16 x 1024 over 2816 in nine, both kernels: 8.5 ->
-// 6.1 us; 128 x 128 over 262144 in 64: 63 -> 47).
+// Eight threads an output where there are few outputs and many parts (both kernels, beside one thread: 16 x 1024 over 2816
+// 9.2 -> 7.6 us, 64 x 64 over 65536 25 -> 13, 128 x 128 over 262144 61 -> 46).
 template <typename T, int ACT>
 hipError_t launch_join(const ProductArgs& p, hipStream_t st) {
   const long threads = p.M * ((p.N + 3) / 4);

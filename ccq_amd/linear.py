@@ -25,9 +25,10 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     activation one of None, "relu", "silu" ("swish"), "gelu" (erf), "gelu_tanh", or "swiglu", where ``weight``
     ``[2 N, K]`` (and ``bias`` ``[2 N]``) hold the gate rows, then the up rows, and ``act(z) = silu(gate) * up``.
     ``bias`` in x's type or fp32; ``residual`` of the output's shape.  Products accumulate in fp32, and bias,
-    activation and residual are applied there: one rounding of the output.  Gradients of all four tensors (first derivatives); the
-    gradient of ``x @ weight.T + bias`` is rounded to x's type once, where it enters the products.  Rows that are
-    not 16-byte aligned or an odd width are copied to padded rows first."""
+    activation and residual are applied there: one rounding of the output.  Gradients of all four tensors (first derivatives,
+    reverse mode); the gradient of ``x @ weight.T + bias`` is rounded to x's type once, where it enters the products.  Rows
+    that are not 16-byte aligned or an odd width are copied to padded rows first, in each direction; leading dimensions
+    whose strides are not those of rows one after the other are copied too."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"fused_linear: activation {activation!r} is unknown (expected one of "

@@ -24,10 +24,12 @@ class TokenLogprobs(NamedTuple):
 
 
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, ignore_index: int = -100) -> TokenLogprobs:
-    """Of ``logits [..., V]`` (bf16, fp16 or fp32 on the GPU, any row stride) and tokens ``ids [...]`` (int64 or
-    int32): fp32 ``log_softmax(logits)[ids]`` and the entropy of every position, both differentiable (first
-    derivatives), and with ``top_k`` (at most 64) the log probabilities and ids of its likeliest tokens, ties to the
-    lowest id (not differentiable).  A position whose id is ``ignore_index`` is skipped: its logits are not read, its
-    results are 0 (ids -1) and its gradient is 0.  An id outside the vocabulary has the log probability NaN (nothing
-    is read out of bounds); a logit of -inf masks its token."""
+    """Of ``logits [..., V]`` (bf16, fp16 or fp32 on the GPU, V at most 2^30, any stride between rows) and tokens
+    ``ids [...]`` (int64 or int32): fp32 ``log_softmax(logits)[ids]`` and the entropy of every position, both
+    differentiable (first derivatives, reverse mode), and with ``top_k`` (at most 64) the log probabilities and ids of
+    its likeliest tokens, ties to the lowest id (not differentiable).  A position whose id is ``ignore_index`` is
+    skipped: its logits are not read, its results are 0 (ids -1) and its gradient is 0.  An id outside the vocabulary
+    has the log probability NaN (nothing is read out of bounds); a logit of -inf masks its token.  Positions that do not lie at one stride, such as
+    ``logits[:, :-1]`` of ``[B, T, V]``, are copied first and the copy is kept for the backward: of all positions, with
+    ``ids`` of ``ignore_index`` at the last ones, nothing is."""
     return TokenLogprobs(*ops().token_logprobs(logits, ids, top_k, ignore_index))

@@ -20,10 +20,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5, residual: Optional[torch.Tensor] = None
                ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension (bf16, fp16 or fp32 on the GPU, 1 to
-    8192 wide, any row stride); ``weight`` and ``bias`` ``[D]`` in x's type or fp32, each optional.  With
-    ``residual`` (x's shape and type) the rows are ``s = x + residual``, rounded to their type as the residual
-    stream holds them, and it returns ``(y, s)``.  Statistics and sums in fp32, one rounding of y.  Gradients of x,
-    residual, weight and bias (first derivatives)."""
+    8192 wide, any stride between rows; leading dimensions without one such stride are copied); ``weight`` and ``bias``
+    ``[D]`` in x's type or fp32, each optional.  With ``residual`` (x's shape and type) the rows are ``s = x + residual``,
+    rounded to their type as the residual stream holds them, and it returns ``(y, s)``.  Statistics and sums in fp32, one
+    rounding of y.  Gradients of x, residual, weight and bias (first derivatives, reverse mode)."""
     if residual is None:
         return ops().norm("layer_norm", x, weight, bias, eps, True)
     return ops().norm_residual("layer_norm", x, weight, bias, eps, residual, True)

@@ -492,7 +492,7 @@ int ccq_norm_bwd(const void* x, int64_t ldx, const void* w, const float* mean, c
                  int64_t rows, int D, int dtype, int wdtype, int layer, void* stream);
 
 /*
- * Log probabilities of given tokens: of logits [rows, V] of dtype (row stride ldx >= V) and tokens
+ * Log probabilities of given tokens: of logits [rows, V] of dtype (V at most 2^30, row stride ldx >= V) and tokens
  * ids [rows], fp32 log softmax(logits)[id] into logp [rows], the entropy of each row's distribution into
  * entropy [rows], each row's maximum and log sum exp(logits - maximum) into stats [rows, 2] (for the
  * backward; nullable), and the k likeliest tokens of each row (0 <= k <= min(V, 64); ties to the lowest index, a NaN logit before any number) into top
