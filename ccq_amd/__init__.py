@@ -10,6 +10,7 @@ from .ccq_gdn import (chunk_ccq_gdn, chunk_gated_delta_rule, fused_ccq_clean, fu
                       fused_recurrent_ccq_gdn)
 from .ccq_gla import chunk_ccq_gla, chunk_gla, fused_chunk_ccq_gla, fused_recurrent_ccq_gla
 from .clean import FusedCCQCleanRead, _ccq_compute_z_and_sum_kk, _CCQCleanQ, fused_ccq_clean_read
+from .fp8 import Fp8Rows, fp8_linear, quantize_fp8, rms_norm_fp8
 from .l2norm import l2norm
 from .layers import CCQGDN, CCQGLA, LayerCache
 from .linear import fused_linear
@@ -39,4 +40,8 @@ __all__ = [
     "fused_linear",
     "token_logprobs",
     "TokenLogprobs",
+    "Fp8Rows",
+    "quantize_fp8",
+    "rms_norm_fp8",
+    "fp8_linear",
 ]

@@ -81,6 +81,9 @@ SIGNATURES = {
     "ccq_linear_bwd_call_workspace_bytes": (_SZ, [_I64] * 3 + [_I, _P, _I64] + [_I] * 3),
     "ccq_linear_bwd": (_I, [_P, _I64] * 2 + [_P, _P, _I64] + [_P] * 3 + [_I, _P] + [_I64] * 3 + [_I, _I, _P]),
     "ccq_pad_rows": (_I, [_P, _I64, _P] + [_I64] * 3 + [_P]),
+    "ccq_quantize_fp8": (_I, [_P, _I64] * 3 + [_I64] * 2 + [_I, _P]),
+    "ccq_norm_fp8_fwd": (_I, [_P, _I64] * 2 + [_P] + [_P, _I64] * 2 + [_P, _I64] + [_I] * 3 + [_F, _P]),
+    "ccq_fp8_linear": (_I, [_P, _I64] * 4 + [_P, _I] + [_P, _I64] * 3 + [_I64] * 3 + [_I, _I, _P]),
     "ccq_timing_enable": (_I, [_I]),
     "ccq_timing_reset": (_I, []),
     "ccq_timing_select": (_I, [ctypes.c_char_p]),
@@ -132,7 +135,8 @@ KERNELS = ("conv_fwd", "conv_bwd", "gnorm_fwd", "gnorm_bwd",
            "gdn_prep", "gdn_fwd_state", "gdn_fwd_o", "gdn_bwd_state", "gdn_bwd_dqkw", "gdn_bwd_wy",
            "gla_intra", "gla_fwd_state", "gla_fwd_o", "gla_bwd_state", "gla_bwd_dv", "gla_bwd_dqk",
            "clean_z_fwd", "clean_z_bwd", "narrow_fwd", "narrow_bwd", "norm_fwd", "norm_bwd",
-           "logprobs_fwd", "logprobs_bwd", "linear_fwd", "linear_dz", "linear_dx", "linear_dw")
+           "logprobs_fwd", "logprobs_bwd", "linear_fwd", "linear_dz", "linear_dx", "linear_dw",
+           "quantize_fp8", "norm_fp8", "linear_fp8")
 
 
 def timing_enable(on: bool) -> None:

@@ -14,7 +14,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libccq_hip.so")
 SOURCES = ["ccq_abi.hip", "ccq_cwalk.hip", "ccq_gdn.hip", "ccq_gwalk.hip", "ccq_gla.hip", "ccq_decode.hip", "ccq_zclean.hip", "ccq_misc.hip", "ccq_cseg.hip", "ccq_prologue.hip",
-           "ccq_linear.hip", "ccq_norm.hip", "ccq_logprobs.hip"]
+           "ccq_linear.hip", "ccq_norm.hip", "ccq_logprobs.hip", "ccq_fp8.hip"]
 TORCH_SOURCE = "ccq_torch.cpp"
 TORCH_LIB = os.path.join(HERE, "_ccq_torch.so")
 CXX = os.environ.get("CXX", "g++")

@@ -35,6 +35,8 @@ hipError_t launch_norm_bwd(const NormArgs& a, hipStream_t st);
 hipError_t launch_logprobs(bool bwd, const LogprobArgs& a, hipStream_t st);
 void product_plan(long M, long N, long K, int* side, int* splits);
 hipError_t launch_product(int kind, const ProductArgs& p, hipStream_t st);
+hipError_t launch_quantize(const QuantizeArgs& a, hipStream_t st);
+hipError_t launch_fp8_product(const Fp8ProductArgs& p, hipStream_t st);
 int act_bwd_row_blocks(long M, long N);
 hipError_t launch_act_bwd(const ActBwdArgs& a, hipStream_t st);
 hipError_t launch_pad_rows(const PadRowsArgs& a, hipStream_t st);
@@ -1771,6 +1773,89 @@ int ccq_pad_rows(const void* src, int64_t ld, void* dst, int64_t ldd, int64_t ro
   if (int e = check_stream_device(stream, who)) return e;
   PadRowsArgs a{src, dst, (long)rows, (long)K, (long)ld, (long)ldd};
   return hip_status(launch_pad_rows(a, (hipStream_t)stream), who);
+}
+
+}  // extern "C"
+
+// ---- serving in 8 bits ----
+namespace {
+
+// rows of e4m3 values and of their scales, as the kernels read and write them
+int fp8_rows_check(const char* who, const char* what, const void* v, int64_t ldv, const void* s, int64_t lds, int64_t D) {
+  if (ldv < ((D + 15) & ~15L) || ldv % 16 || ldv > kMaxStride || lds < (((D + 127) / 128 + 3) & ~3L) || lds % 4 || lds > kMaxStride)
+    return fail(CCQ_ERR_SHAPE, "%s: %s: row strides %lld of the values, %lld of the scales of D=%lld (multiples of 16 and 4, at most 4 Mi)",
+                who, what, (long long)ldv, (long long)lds, (long long)D);
+  if (!aligned16(v) || (reinterpret_cast<uintptr_t>(s) & 3))
+    return fail(CCQ_ERR_ALIGN, "%s: %s: values must be 16-byte aligned, scales 4-byte aligned", who, what);
+  return CCQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ccq_quantize_fp8(const void* x, int64_t ldx, void* values, int64_t ldv, void* scales, int64_t lds, int64_t rows,
+                     int64_t D, int dtype, void* stream) {
+  const char* who = "ccq_quantize_fp8";
+  if (rows < 0 || rows > kMaxSide || D < 1 || D > kMaxStride || ldx < D || !dtype_ok(dtype))
+    return fail(CCQ_ERR_SHAPE, "%s: rows=%lld D=%lld ldx=%lld dtype=%d", who, (long long)rows, (long long)D, (long long)ldx, dtype);
+  if (int e = fp8_rows_check(who, "output", values, ldv, scales, lds, D)) return e;
+  if (rows == 0) return CCQ_OK;
+  if (!x || !values || !scales) return fail(CCQ_ERR_NULL, "%s: x, values and scales are required", who);
+  if (!element_aligned(x, dtype)) return fail(CCQ_ERR_ALIGN, "%s: x must be aligned to its elements", who);
+  if (int e = check_stream_device(stream, who)) return e;
+  QuantizeArgs a{x, (unsigned char*)values, (unsigned char*)scales, (long)rows, (long)D, (long)ldx, (long)ldv, (long)lds, dtype};
+  hipStream_t st = (hipStream_t)stream;
+  return hip_status(timed("quantize_fp8", st, [&] { return launch_quantize(a, st); }), who);
+}
+
+int ccq_norm_fp8_fwd(const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w, void* values, int64_t ldv,
+                     void* scales, int64_t lds, void* s, int64_t rows, int D, int dtype, int wdtype, float eps,
+                     void* stream) {
+  const char* who = "ccq_norm_fp8_fwd";
+  if (int e = norm_check(who, rows, D, dtype, wdtype, 0, nullptr)) return e;
+  if (ldx < D || (r && ldr < D)) return fail(CCQ_ERR_SHAPE, "%s: row strides %lld, %lld below D=%d", who, (long long)ldx, (long long)ldr, D);
+  if (int e = fp8_rows_check(who, "output", values, ldv, scales, lds, D)) return e;
+  if (rows == 0) return CCQ_OK;
+  if (!x || !values || !scales || !r != !s)
+    return fail(CCQ_ERR_NULL, "%s: x, values and scales are required, r and s go together", who);
+  for (const void* p : {x, r, (const void*)s})
+    if (!element_aligned(p, dtype)) return fail(CCQ_ERR_ALIGN, "%s: rows must be aligned to their elements", who);
+  if (!element_aligned(w, wdtype)) return fail(CCQ_ERR_ALIGN, "%s: w must be aligned to its elements", who);
+  if (int e = check_stream_device(stream, who)) return e;
+  NormArgs a{};
+  a.x = x; a.ldx = ldx; a.r = r; a.ldr = ldr; a.w = w; a.y = values; a.ldy = ldv; a.scales = (unsigned char*)scales;
+  a.lds = lds; a.s = s; a.rows = rows; a.D = D; a.dtype = dtype; a.wdtype = wdtype; a.eps = eps;
+  hipStream_t st = (hipStream_t)stream;
+  return hip_status(timed("norm_fp8", st, [&] { return launch_norm_fwd(a, st); }), who);
+}
+
+int ccq_fp8_linear(const void* x, int64_t ldx, const void* xs, int64_t ldxs, const void* weight, int64_t ldw,
+                   const void* ws, int64_t ldws, const void* bias, int bdtype, const void* r, int64_t ldr, void* y,
+                   int64_t ldy, void* ys, int64_t ldys, int64_t M, int64_t N, int64_t K, int act, int dtype, void* stream) {
+  const char* who = "ccq_fp8_linear";
+  if (M < 0 || N < 1 || K < 1 || M > kMaxSide || N > kMaxSide || linear_outs(N, act) > kMaxStride || K > kMaxStride ||
+      ((M + 63) / 64) * ((linear_outs(N, act) + 63) / 64) > kMaxTiles)
+    return fail(CCQ_ERR_SHAPE, "%s: M=%lld N=%lld K=%lld", who, (long long)M, (long long)N, (long long)K);
+  if (act < CCQ_ACT_NONE || act > CCQ_ACT_SWIGLU || !dtype_ok(bdtype) || (!ys && !dtype_ok(dtype)))
+    return fail(CCQ_ERR_SHAPE, "%s: act=%d dtype=%d bdtype=%d", who, act, dtype, bdtype);
+  if (r && (ys || ldr < N)) return fail(CCQ_ERR_SHAPE, "%s: a residual of row stride %lld (N=%lld; none of an output in 8 bits)", who, (long long)ldr, (long long)N);
+  if (int e = fp8_rows_check(who, "x", x, ldx, xs, ldxs, K)) return e;
+  if (int e = fp8_rows_check(who, "weight", weight, ldw, ws, ldws, K)) return e;
+  if (ys)
+    if (int e = fp8_rows_check(who, "y", y, ldy, ys, ldys, N)) return e;
+  if (M == 0) return CCQ_OK;
+  if (!x || !xs || !weight || !ws || !y) return fail(CCQ_ERR_NULL, "%s: x, xs, weight, ws and y are required", who);
+  if ((!ys && !element_aligned(y, dtype)) || !element_aligned(r, dtype) || !element_aligned(bias, bdtype))
+    return fail(CCQ_ERR_ALIGN, "%s: y, r and bias must be aligned to their elements", who);
+  if (int e = check_stream_device(stream, who)) return e;
+  Fp8ProductArgs p{};
+  p.a = (const unsigned char*)x; p.lda = ldx; p.sa = (const unsigned char*)xs; p.lsa = ldxs;
+  p.b = (const unsigned char*)weight; p.ldb = ldw; p.sb = (const unsigned char*)ws; p.lsb = ldws;
+  p.M = M; p.N = N; p.K = K; p.out = y; p.ldo = ys ? ldy : N; p.os = (unsigned char*)ys; p.los = ldys;
+  p.bias = bias; p.bdtype = bdtype; p.res = r; p.ldr = ldr; p.act = act; p.dtype = dtype;
+  hipStream_t st = (hipStream_t)stream;
+  return hip_status(timed("linear_fp8", st, [&] { return launch_fp8_product(p, st); }), who);
 }
 
 }  // extern "C"

@@ -1,5 +1,5 @@
 // Arguments of the kernels around the token mixers: block norms (ccq_norm.hip), log probabilities of given
-// tokens (ccq_logprobs.hip), projections with an epilogue (ccq_linear.hip).
+// tokens (ccq_logprobs.hip), projections with an epilogue (ccq_linear.hip; on 8-bit rows ccq_fp8.hip).
 #pragma once
 
 #include <stdint.h>
@@ -28,6 +28,8 @@ struct NormArgs {
   long rows, ldx, ldr, ldy, ldds;
   int D, dtype, wdtype, layer;
   float eps;
+  unsigned char* scales;  // forward into 8 bits: [rows, D / 128 rounded up] row stride lds, y's row stride ldy bytes
+  long lds;
 };
 
 struct LogprobArgs {
@@ -83,6 +85,31 @@ struct PadRowsArgs {
   const void* src;     // [rows, K] row stride ld
   void* dst;           // [rows, ldd], zeros behind the K columns
   long rows, K, ld, ldd;
+};
+
+struct QuantizeArgs {
+  const void* x;           // [rows, D] row stride ldx
+  unsigned char* values;   // [rows, D] row stride ldv bytes
+  unsigned char* scales;   // [rows, D / 128 rounded up] row stride lds
+  long rows, D, ldx, ldv, lds;
+  int dtype;
+};
+
+// out[M, N] = act(A B^T + bias) + res over K, A [M, K] and B [N, K] (swiglu: [2 N, K]) e4m3 with a scale for each 128 of K.
+struct Fp8ProductArgs {
+  const unsigned char* a;   // row stride lda bytes, 16-byte aligned rows
+  const unsigned char* b;   // row stride ldb
+  const unsigned char* sa;  // scales of A, row stride lsa, 4-byte aligned rows
+  const unsigned char* sb;  // scales of B, row stride lsb
+  long lda, ldb, lsa, lsb;
+  long M, N, K;
+  void* out;                // [M, N] of dtype, or e4m3 with a row stride of ldo bytes
+  unsigned char* os;        // the output's scales, row stride los (nullable: not in 8 bits)
+  long ldo, los;
+  const void* bias;         // [N] (swiglu: [2 N]) of bdtype (nullable)
+  const void* res;          // [M, N] of dtype, row stride ldr (nullable)
+  long ldr;
+  int act, bdtype, dtype;
 };
 
 }  // namespace ccq

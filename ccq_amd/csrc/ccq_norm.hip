@@ -15,6 +15,7 @@
 #include <algorithm>
 
 #include "ccq_block_args.h"
+#include "ccq_fp8.h"
 #include "ccq_rows.h"
 
 namespace ccq {
@@ -103,7 +104,8 @@ __device__ __forceinline__ void keep_packed(V& v) {
   v = __builtin_bit_cast(V, u);
 }
 
-template <typename T, bool LAYER, int WPR, int P>
+// Q8: y in 8 bits (ccq_fp8.h); 128 / N consecutive lanes hold a block, all of the team where it has fewer.
+template <typename T, bool LAYER, int WPR, int P, bool Q8>
 __global__ __launch_bounds__(WPR > 4 ? WPR * 64 : kThreads) void norm_fwd_kernel(const NormArgs a, int lanes) {
   constexpr int N = Piece<T>::N;
   typedef typename Piece<T>::vec vec;
@@ -174,7 +176,27 @@ __global__ __launch_bounds__(WPR > 4 ? WPR * 64 : kThreads) void norm_fwd_kernel
       }
     team_sum<WPR, 1>(s2, t.L, tid, slots, phase);
     const float rstd = 1.f / sqrtf(s2[0] * inv + a.eps);
-    if (row < a.rows) {
+    if constexpr (Q8) {
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const int c = c0 + j * step, block = kFp8Block / N;
+        float v[N];
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {  // (zeros behind D)
+          v[i] = f[j][i] * rstd * w[j][i];
+          m = max(m, magnitude(v[i]));
+        }
+        const unsigned byte = scale_byte(lanes_max(m, min(t.L, block)));
+        if (row >= a.rows || c >= D) continue;
+        typedef unsigned words __attribute__((ext_vector_type(N / 4)));
+        words o;
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) o[i] = fp8_word(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], byte);
+        *gmem((words*)((unsigned char*)a.y + row * a.ldy + c)) = o;
+        if ((t.li & (block - 1)) == 0) a.scales[row * a.lds + c / kFp8Block] = (unsigned char)byte;
+      }
+    } else if (row < a.rows) {
 #pragma unroll
       for (int j = 0; j < P; ++j) {
         vec y;
@@ -352,8 +374,10 @@ void launch_typed(bool bwd, const NormArgs& a, const NormShape& s, unsigned bloc
   if (s.wpr == W && s.p == PP) {                                                                               \
     if (bwd)                                                                                                   \
       hipLaunchKernelGGL((norm_bwd_kernel<T, LAYER, W, PP>), dim3(blocks), block, 0, st, a, s.lanes);          \
+    else if (LAYER || !a.scales)                                                                               \
+      hipLaunchKernelGGL((norm_fwd_kernel<T, LAYER, W, PP, false>), dim3(blocks), block, 0, st, a, s.lanes);   \
     else                                                                                                       \
-      hipLaunchKernelGGL((norm_fwd_kernel<T, LAYER, W, PP>), dim3(blocks), block, 0, st, a, s.lanes);          \
+      hipLaunchKernelGGL((norm_fwd_kernel<T, LAYER, W, PP, !LAYER>), dim3(blocks), block, 0, st, a, s.lanes);  \
   }
   CCQ_NORM(1, 1) CCQ_NORM(1, 2) CCQ_NORM(4, 1) CCQ_NORM(4, 2) CCQ_NORM(16, 1)
   if constexpr (sizeof(T) == 4) {  // (8192 of two bytes are one piece a thread)

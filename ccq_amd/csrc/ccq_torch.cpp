@@ -192,8 +192,8 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
   }
 };
 
-variable_list norm(const std::string& who, const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps,
-                   const OptTensor& residual, bool layer) {
+void check_norm(const std::string& who, const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps,
+                const OptTensor& residual) {
   TORCH_CHECK_TYPE(known(x.scalar_type()), who, " takes bf16, fp16 or fp32 rows (got ", x.scalar_type(), ")");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= kMaxNorm, who, ": x ", x.sizes(),
                     ": needs a last dimension in [1, ", kMaxNorm, "]");
@@ -214,6 +214,11 @@ variable_list norm(const std::string& who, const Tensor& x, const OptTensor& wei
   require_on(who, "residual", residual, x);
   TORCH_CHECK_VALUE(!has(residual) || (residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type()), who,
                     ": residual: expected x's shape ", x.sizes(), " and type ", x.scalar_type());
+}
+
+variable_list norm(const std::string& who, const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps,
+                   const OptTensor& residual, bool layer) {
+  check_norm(who, x, weight, bias, eps, residual);
   const Tensor r = value(residual), w = has(weight) ? weight->contiguous() : Tensor(),
                b = has(bias) ? bias->contiguous() : Tensor();
   refuse_tangents(who, {&x, &r, &w, &b});
@@ -428,6 +433,142 @@ Tensor fused_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias
   return linear_forward(x, weight, b, r, (int)act, false).y;
 }
 
+// ---------------------------------------------------------------------------
+// serving in 8 bits
+// ---------------------------------------------------------------------------
+constexpr int64_t kFp8Block = 128;
+int64_t blocks_of(int64_t D) { return (D + kFp8Block - 1) / kFp8Block; }
+int64_t up_to(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
+
+void refuse_gradients(const std::string& who, std::initializer_list<const Tensor*> xs) {
+  TORCH_CHECK(!needs_grad(xs), who, " has no gradients: call it under torch.no_grad(), or on tensors that need none");
+  refuse_tangents(who, xs);
+}
+
+// New rows in 8 bits: both parts views of rows that the products read in place.
+Tensor fresh_bytes(const Tensor& x, at::IntArrayRef shape, int64_t unit, at::ScalarType type) {
+  auto room = shape.vec();
+  room.back() = up_to(shape.back(), unit);
+  return fresh(x, room, type).narrow(-1, 0, shape.back());
+}
+struct Rows8 {
+  Tensor values, scales;
+};
+Rows8 fresh_rows(const Tensor& x, at::IntArrayRef shape) {
+  auto scales = shape.vec();
+  scales.back() = blocks_of(shape.back());
+  return {fresh_bytes(x, shape, 16, at::kFloat8_e4m3fn), fresh_bytes(x, scales, 4, at::kFloat8_e8m0fnu)};
+}
+
+// Rows of bytes at multiples of `unit` and readable to the next multiple behind their end: a view where the storage has
+// that, a copy otherwise.
+struct ByteRows {
+  Tensor t;
+  int64_t ld;
+};
+ByteRows byte_rows(const Tensor& x, int64_t unit) {
+  const Tensor t = rows_of(x.view(at::kByte));
+  const int64_t n = t.size(0), D = t.size(1), room = up_to(D, unit), ld = n > 1 ? t.stride(0) : room;
+  const int64_t end = t.storage_offset() + (n - 1) * ld + room;
+  if (n == 0 || (ld >= room && ld % unit == 0 && ld <= kMaxStride && (size_t)address(t) % unit == 0 &&
+                 end <= (int64_t)t.storage().nbytes()))
+    return {t, std::max(ld, room)};
+  Tensor out = fresh(t, {n, room}, at::kByte);
+  out.narrow(1, 0, D).copy_(t);
+  return {out, room};
+}
+int64_t row_stride(const Tensor& t, int64_t unit) {  // of rows that fresh_bytes made
+  return up_to(t.size(-1), unit);
+}
+
+std::tuple<Tensor, Tensor> quantize_fp8(const Tensor& x) {
+  const char* who = "quantize_fp8";
+  TORCH_CHECK_TYPE(known(x.scalar_type()), who, " takes bf16, fp16 or fp32 rows (got ", x.scalar_type(), ")");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= kMaxStride, who, ": x ", x.sizes(),
+                    ": needs a last dimension in [1, ", kMaxStride, "]");
+  refuse_gradients(who, {&x});
+  require_gpu(who, x);
+  c10::DeviceGuard guard(x.device());
+  const Tensor rows = rows_of(x);
+  Rows8 o = fresh_rows(x, x.sizes());
+  check(ccq_quantize_fp8(address(rows), stride_of(rows), out_address(o.values), row_stride(o.values, 16),
+                         out_address(o.scales), row_stride(o.scales, 4), rows.size(0), rows.size(1),
+                         code(x.scalar_type()), stream_on(x)),
+        "ccq_quantize_fp8");
+  return {o.values, o.scales};
+}
+
+std::tuple<Tensor, Tensor, OptTensor> rms_norm_fp8(const Tensor& x, const OptTensor& weight, double eps,
+                                                   const OptTensor& residual) {
+  const char* who = "rms_norm_fp8";
+  check_norm(who, x, weight, OptTensor(), eps, residual);
+  const Tensor w = has(weight) ? weight->contiguous() : Tensor(), res = value(residual);
+  refuse_gradients(who, {&x, &res, &w});
+  require_gpu(who, x);
+  c10::DeviceGuard guard(x.device());
+  const Tensor rows = rows_of(x), r = res.defined() ? rows_of(res) : Tensor();
+  Rows8 o = fresh_rows(x, x.sizes());
+  const Tensor s = r.defined() ? like(x) : Tensor();
+  check(ccq_norm_fp8_fwd(address(rows), stride_of(rows), address(r), stride_of(r), address(w), out_address(o.values),
+                         row_stride(o.values, 16), out_address(o.scales), row_stride(o.scales, 4), out_address(s),
+                         rows.size(0), (int)rows.size(1), code(x.scalar_type()),
+                         code(w.defined() ? w.scalar_type() : x.scalar_type()), (float)eps, stream_on(x)),
+        "ccq_norm_fp8_fwd");
+  return {o.values, o.scales, s.defined() ? OptTensor(s) : OptTensor()};
+}
+
+void check_rows8(const char* who, const char* name, const Tensor& values, const Tensor& scales, const Tensor& x) {
+  TORCH_CHECK_TYPE(values.scalar_type() == at::kFloat8_e4m3fn && scales.scalar_type() == at::kFloat8_e8m0fnu, who, ": ", name,
+                   " needs values in float8_e4m3fn and scales in float8_e8m0fnu (got ", values.scalar_type(), ", ",
+                   scales.scalar_type(), ")");
+  TORCH_CHECK_VALUE(values.dim() >= 1 && values.size(-1) >= 1 && values.size(-1) <= kMaxStride, who, ": ", name, " values ",
+                    values.sizes(), ": need a last dimension in [1, ", kMaxStride, "]");
+  auto shape = values.sizes().vec();
+  shape.back() = blocks_of(shape.back());
+  TORCH_CHECK_VALUE(scales.sizes() == at::IntArrayRef(shape), who, ": ", name, " scales ", scales.sizes(), ": expected ",
+                    at::IntArrayRef(shape), ", one for each 128 elements of a row");
+  for (const Tensor* t : {&values, &scales})
+    TORCH_CHECK_VALUE(t->device() == x.device(), who, ": ", name, " must be on ", x.device().str(), " (got ", t->device().str(), ")");
+}
+
+std::tuple<Tensor, OptTensor> fp8_linear(const Tensor& x, const Tensor& xs, const Tensor& weight, const Tensor& ws,
+                                         const OptTensor& bias, int64_t act, const OptTensor& residual,
+                                         at::ScalarType dtype, bool quantize) {
+  const char* who = "fp8_linear";
+  check_rows8(who, "x", x, xs, x);
+  check_rows8(who, "weight", weight, ws, x);
+  TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.size(0) >= 1 && weight.size(0) <= kMaxStride,
+                    who, ": x ", x.sizes(), " and weight ", weight.sizes(),
+                    ": expected [..., K] and [outputs, K], at least one output and at most ", kMaxStride);
+  const int64_t K = x.size(-1), outs = weight.size(0), N = act == CCQ_ACT_SWIGLU ? outs / 2 : outs;
+  TORCH_CHECK_VALUE(act != CCQ_ACT_SWIGLU || outs % 2 == 0, who, ": swiglu needs as many gate as up rows (weight has ", outs, ")");
+  TORCH_CHECK_TYPE(quantize || known(dtype), who, ": dtype must be bf16, fp16 or fp32 (got ", dtype, ")");
+  require_on(who, "bias", bias, x);
+  require_on(who, "residual", residual, x);
+  TORCH_CHECK_VALUE(!has(bias) || (bias->dim() == 1 && bias->size(0) == outs), who, ": bias: expected [", outs, "]");
+  TORCH_CHECK_TYPE(!has(bias) || known(bias->scalar_type()), who, ": bias: expected bf16, fp16 or fp32");
+  auto shape = x.sizes().vec();
+  shape.back() = N;
+  TORCH_CHECK_VALUE(!quantize || !has(residual), who, ": residual: an output in 8 bits has none");
+  TORCH_CHECK_VALUE(!has(residual) || (residual->sizes() == at::IntArrayRef(shape) && residual->scalar_type() == dtype),
+                    who, ": residual: expected ", at::IntArrayRef(shape), " ", dtype);
+  const Tensor b = has(bias) ? bias->contiguous() : Tensor(), res = value(residual);
+  refuse_gradients(who, {&x, &xs, &weight, &ws, &b, &res});
+  require_gpu(who, x);
+  c10::DeviceGuard guard(x.device());
+  const ByteRows xv = byte_rows(x, 16), xe = byte_rows(xs, 4), wv = byte_rows(weight, 16), we = byte_rows(ws, 4);
+  const Tensor r = res.defined() ? rows_of(res) : Tensor();
+  Rows8 o;
+  if (quantize) o = fresh_rows(x, shape);
+  else o.values = fresh(x, shape, dtype);
+  check(ccq_fp8_linear(address(xv.t), xv.ld, address(xe.t), xe.ld, address(wv.t), wv.ld, address(we.t), we.ld, address(b),
+                       code(b.defined() ? b.scalar_type() : at::kFloat), address(r), stride_of(r), out_address(o.values),
+                       quantize ? row_stride(o.values, 16) : N, out_address(o.scales), quantize ? row_stride(o.scales, 4) : 0,
+                       xv.t.size(0), N, K, (int)act, quantize ? CCQ_DTYPE_BF16 : code(dtype), stream_on(x)),
+        "ccq_fp8_linear");
+  return {o.values, quantize ? OptTensor(o.scales) : OptTensor()};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -441,4 +582,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   });
   m.def("token_logprobs", &token_logprobs);
   m.def("fused_linear", &fused_linear);
+  m.def("quantize_fp8", &quantize_fp8);
+  m.def("rms_norm_fp8", &rms_norm_fp8);
+  m.def("fp8_linear", &fp8_linear);
 }

@@ -555,6 +555,35 @@ int ccq_linear_bwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, 
 int ccq_pad_rows(const void* src, int64_t ld, void* dst, int64_t ldd, int64_t rows, int64_t K, void* stream);
 
 /*
+ * Serving in 8 bits (inference; the reference runs its projections in the activations' type).  Rows in 8 bits are e4m3
+ * values [rows, D] (row stride ldv bytes) with one scale for each 128 consecutive elements of a row, e8m0 [rows, D / 128
+ * rounded up] (row stride lds bytes): element k stands for value[k] * 2^(scale[k / 128] - 127).  The scale of a block is
+ * the least power of two from 2^-126 on that brings its largest magnitude to 448 (the largest e4m3) or below; the values
+ * are rounded once, to the nearest, ties to even.  A block with an infinity or NaN has scale 255 (NaN) and NaN for its
+ * values.  Value rows are 16-byte aligned (base and stride) and readable to the next multiple of 16 bytes behind D,
+ * scale rows 4-byte aligned and readable to the next multiple of 4; what lies there does not matter, and what a call
+ * writes there is no result.  Strides of values and scales at most 4 Mi.
+ *
+ * ccq_quantize_fp8: x [rows, D] of dtype (any element-aligned address, stride ldx >= D) into that form; D at most 4 Mi.
+ * ccq_norm_fp8_fwd: ccq_norm_fwd's RMS norm (x, r, s, w as there) with y in 8 bits.
+ */
+int ccq_quantize_fp8(const void* x, int64_t ldx, void* values, int64_t ldv, void* scales, int64_t lds, int64_t rows,
+                     int64_t D, int dtype, void* stream);
+int ccq_norm_fp8_fwd(const void* x, int64_t ldx, const void* r, int64_t ldr, const void* w, void* values, int64_t ldv,
+                     void* scales, int64_t lds, void* s, int64_t rows, int D, int dtype, int wdtype, float eps,
+                     void* stream);
+/*
+ * y = act(x W^T + b) + r over rows in 8 bits: x [M, K] (values x, ldx; scales xs, ldxs), weight [N, K] (swiglu: [2 N, K], gate
+ * rows, then up rows; values weight, ldw; scales ws, ldws), bias [N] (swiglu: [2 N]) of bdtype (nullable), r [M, N] of
+ * dtype (row stride ldr, nullable), act CCQ_ACT_*.  Products, bias, activation and residual in fp32.  y [M, N] of dtype,
+ * contiguous, rounded once; or, with ys not NULL, y [M, N] (row stride ldy) and ys (ldys) in 8 bits (no r then; dtype is
+ * not looked at).
+ */
+int ccq_fp8_linear(const void* x, int64_t ldx, const void* xs, int64_t ldxs, const void* weight, int64_t ldw,
+                   const void* ws, int64_t ldws, const void* bias, int bdtype, const void* r, int64_t ldr, void* y,
+                   int64_t ldy, void* ys, int64_t ldys, int64_t M, int64_t N, int64_t K, int act, int dtype, void* stream);
+
+/*
  * Kernel timing (measurement facility; no counterpart in the reference).  While enabled, each
  * entry point records a HIP event pair around every launch of its kernels on the caller's
  * stream.  ccq_timing_read waits for the recorded events of `kernel` (names: conv_fwd, conv_bwd,
@@ -562,7 +591,7 @@ int ccq_pad_rows(const void* src, int64_t ld, void* dst, int64_t ldd, int64_t ro
  * clean_bwd_dk, clean_bwd_gate, gdn_prep, gdn_fwd_state, gdn_fwd_o, gdn_bwd_state, gdn_bwd_dqkw,
  * gdn_bwd_wy, gla_intra, gla_fwd_state, gla_fwd_o, gla_bwd_state, gla_bwd_dv, gla_bwd_dqk,
  * clean_z_fwd, clean_z_bwd, narrow_fwd, narrow_bwd, norm_fwd, norm_bwd, logprobs_fwd, logprobs_bwd,
- * linear_fwd, linear_dz, linear_dx, linear_dw) and returns the summed
+ * linear_fwd, linear_dz, linear_dx, linear_dw, quantize_fp8, norm_fp8, linear_fp8) and returns the summed
  * milliseconds and the number of launches since the last ccq_timing_reset.  ccq_timing_select
  * restricts the events to the kernel of that name (NULL: every kernel), so that a timed loop carries
  * one event pair per step instead of one per kernel.

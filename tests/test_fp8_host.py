@@ -1,0 +1,162 @@
+"""Refusals of the operators of serving in 8 bits that need no GPU, in the Python entry points and at the C ABI, and the
+tests' own 64-bit definition of the format against torch's conversions."""
+
+import ctypes
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+from _fp8 import exponent, quantized, to_e4m3
+from ccq_amd import Fp8Rows, _lib, fp8_linear, quantize_fp8, rms_norm_fp8
+
+SHAPE, NULL, ALIGN = -1, -2, -3
+P = ctypes.c_void_p(0x1000)     # never dereferenced: the checks fail first
+ODD = ctypes.c_void_p(0x1001)
+BF = torch.bfloat16
+
+
+def _rows(rows, K, lead=()):
+    return Fp8Rows(torch.zeros(*lead, rows, K).to(torch.float8_e4m3fn),
+                   torch.ones(*lead, rows, -(-K // 128)).to(torch.float8_e8m0fnu))
+
+
+def test_definition():
+    every = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    every = every[torch.isfinite(every)]
+    assert torch.equal(to_e4m3(every), every)
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn(4000, generator=gen) * torch.exp(3 * torch.randn(4000, generator=gen))
+    x = x.clamp(-448, 448)
+    assert torch.equal(to_e4m3(x.double()).float(), x.to(torch.float8_e4m3fn).float())
+    ties = (every.sort().values[1:] + every.sort().values[:-1]) / 2
+    assert torch.equal(to_e4m3(ties).float(), ties.float().to(torch.float8_e4m3fn).float())
+    m = torch.tensor([0.0, 448.0, 448.0001, 896.0, 1.0, 1.75, 1.7500001, 2.0 ** -140], dtype=torch.float64)
+    assert exponent(m).tolist() == [-126, 0, 1, 1, -8, -8, -7, -126]
+    v, s = quantized(torch.randn(3, 300, generator=gen))
+    assert v.shape == (3, 300) and s.shape == (3, 3) and float(v.abs().max()) <= 448
+
+
+def test_quantize_refusals():
+    x = torch.zeros(4, 64, dtype=BF)
+    with pytest.raises(RuntimeError, match="GPU"):
+        quantize_fp8(x)
+    with pytest.raises(TypeError, match="bf16, fp16 or fp32"):
+        quantize_fp8(x.double())
+    with pytest.raises(TypeError, match="bf16, fp16 or fp32"):
+        quantize_fp8(x.to(torch.float8_e4m3fn))
+    with pytest.raises(ValueError, match="last dimension"):
+        quantize_fp8(x[:, :0])
+    with pytest.raises(ValueError, match="last dimension"):
+        quantize_fp8(torch.zeros((), dtype=BF))
+    with pytest.raises(ValueError, match="last dimension"):
+        quantize_fp8(torch.zeros(1, dtype=BF).expand((1 << 22) + 1))
+    with pytest.raises(RuntimeError, match="no gradients"):
+        quantize_fp8(x.float().requires_grad_())
+
+
+def test_norm_refusals():
+    x, w = torch.zeros(4, 64, dtype=BF), torch.ones(64, dtype=BF)
+    with pytest.raises(RuntimeError, match="GPU"):
+        rms_norm_fp8(x, w)
+    with pytest.raises(TypeError, match="bf16, fp16 or fp32"):
+        rms_norm_fp8(x.double(), w)
+    with pytest.raises(ValueError, match="last dimension"):
+        rms_norm_fp8(torch.zeros(2, 8193, dtype=BF))
+    with pytest.raises(ValueError, match="weight"):
+        rms_norm_fp8(x, w[:32])
+    with pytest.raises(TypeError, match="weight"):
+        rms_norm_fp8(x, w.half())
+    with pytest.raises(ValueError, match="residual"):
+        rms_norm_fp8(x, w, residual=x[:1])
+    with pytest.raises(ValueError, match="eps"):
+        rms_norm_fp8(x, w, eps=-1.0)
+    for call in (lambda: rms_norm_fp8(x.clone().requires_grad_(), w), lambda: rms_norm_fp8(x, w.clone().requires_grad_()),
+                 lambda: rms_norm_fp8(x, w, residual=x.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
+            call()
+    with fwAD.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+        rms_norm_fp8(fwAD.make_dual(x.float(), torch.ones(4, 64)))
+
+
+def test_linear_refusals():
+    x, w = _rows(4, 200), _rows(32, 200)
+    with pytest.raises(RuntimeError, match="GPU"):
+        fp8_linear(x, w)
+    with pytest.raises(ValueError, match="activation"):
+        fp8_linear(x, w, activation="tanh")
+    with pytest.raises(TypeError, match="float8_e4m3fn"):
+        fp8_linear((x.values.float(), x.scales), w)
+    with pytest.raises(TypeError, match="float8_e8m0fnu"):
+        fp8_linear(x, (w.values, w.scales.float()))
+    with pytest.raises(ValueError, match="x scales"):
+        fp8_linear((x.values, x.scales[:, :1]), w)
+    with pytest.raises(ValueError, match="weight scales"):
+        fp8_linear(x, (w.values, w.scales[:31]))
+    with pytest.raises(ValueError, match="weight"):
+        fp8_linear(x, _rows(32, 201))
+    with pytest.raises(ValueError, match="weight"):
+        fp8_linear(x, _rows(32, 200, (2,)))
+    with pytest.raises(ValueError, match="at least one"):
+        fp8_linear(x, _rows(0, 200))
+    with pytest.raises(ValueError, match="last dimension"):
+        fp8_linear(_rows(4, 0), w)
+    with pytest.raises(ValueError, match="up rows"):
+        fp8_linear(x, _rows(31, 200), activation="swiglu")
+    with pytest.raises(TypeError, match="dtype"):
+        fp8_linear(x, w, dtype=torch.float64)
+    with pytest.raises(ValueError, match="bias"):
+        fp8_linear(x, w, torch.zeros(31))
+    with pytest.raises(TypeError, match="bias"):
+        fp8_linear(x, w, torch.zeros(32, dtype=torch.float64))
+    with pytest.raises(ValueError, match="residual"):
+        fp8_linear(x, w, residual=torch.zeros(1, 32, dtype=BF))
+    with pytest.raises(ValueError, match="residual"):
+        fp8_linear(x, w, residual=torch.zeros(4, 32))
+    with pytest.raises(ValueError, match="residual"):
+        fp8_linear(x, w, residual=torch.zeros(4, 32, dtype=BF), quantize=True)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        fp8_linear(x, w, torch.zeros(32, requires_grad=True))
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
+        fp8_linear(x, w, torch.zeros(32, requires_grad=True))
+
+
+def test_abi_refusals():
+    lib = _lib.load()
+
+    def quant(x=P, ldx=200, v=P, ldv=208, s=P, lds=4, rows=4, D=200, dtype=0):
+        return lib.ccq_quantize_fp8(x, ldx, v, ldv, s, lds, rows, D, dtype, None)
+
+    assert quant(D=0) == SHAPE and quant(ldx=199) == SHAPE and quant(dtype=3) == SHAPE and quant(rows=-1) == SHAPE
+    assert quant(ldv=200) == SHAPE and quant(ldv=192) == SHAPE and quant(lds=2) == SHAPE and quant(lds=6) == SHAPE
+    assert quant(D=600, ldx=600, ldv=608) == SHAPE      # five scales a row need 8 bytes
+    assert quant(D=(1 << 22) + 1, ldx=1 << 23, ldv=1 << 23) == SHAPE and quant(ldv=(1 << 22) + 16) == SHAPE
+    assert quant(x=None) == NULL and quant(v=None) == NULL and quant(s=None) == NULL
+    assert quant(x=ODD) == ALIGN and quant(v=ctypes.c_void_p(0x1008)) == ALIGN and quant(s=ctypes.c_void_p(0x1002)) == ALIGN
+    assert quant(rows=0) == 0
+
+    def norm(x=P, ldx=200, r=None, ldr=0, w=P, v=P, ldv=208, s=P, lds=4, stream=None, D=200, dtype=0, wdtype=0):
+        return lib.ccq_norm_fp8_fwd(x, ldx, r, ldr, w, v, ldv, s, lds, stream, 4, D, dtype, wdtype, 1e-5, None)
+
+    assert norm(D=0) == SHAPE and norm(D=8193, ldx=9000, ldv=9008, lds=80) == SHAPE and norm(ldx=199) == SHAPE
+    assert norm(wdtype=1) == SHAPE and norm(r=P, ldr=199, stream=P) == SHAPE and norm(ldv=200) == SHAPE
+    assert norm(x=None) == NULL and norm(v=None) == NULL and norm(s=None) == NULL and norm(r=P, ldr=200) == NULL
+    assert norm(x=ODD) == ALIGN and norm(v=ODD) == ALIGN and norm(w=ODD) == ALIGN
+
+    def linear(x=P, ldx=208, xs=P, ldxs=4, w=P, ldw=208, ws=P, ldws=4, b=None, bd=0, r=None, ldr=0, y=P, ldy=32, ys=None,
+               ldys=0, M=4, N=32, K=200, act=0, dt=0):
+        return lib.ccq_fp8_linear(x, ldx, xs, ldxs, w, ldw, ws, ldws, b, bd, r, ldr, y, ldy, ys, ldys, M, N, K, act, dt, None)
+
+    assert linear(M=-1) == SHAPE and linear(N=0) == SHAPE and linear(K=0) == SHAPE and linear(act=6) == SHAPE
+    assert linear(dt=3) == SHAPE and linear(bd=3) == SHAPE and linear(r=P, ldr=31) == SHAPE
+    assert linear(ldx=200) == SHAPE and linear(ldw=192) == SHAPE and linear(ldxs=3) == SHAPE and linear(ldws=0) == SHAPE
+    assert linear(ys=P, ldys=4, ldy=24) == SHAPE and linear(ys=P, ldys=2) == SHAPE
+    assert linear(ys=P, ldys=4, r=P, ldr=32) == SHAPE
+    assert linear(M=1 << 30, N=1 << 22) == SHAPE and linear(N=(1 << 21) + 1, act=5) == SHAPE
+    assert linear(x=None) == NULL and linear(xs=None) == NULL and linear(w=None) == NULL and linear(ws=None) == NULL
+    assert linear(y=None) == NULL
+    assert linear(x=ctypes.c_void_p(0x1008)) == ALIGN and linear(xs=ODD) == ALIGN and linear(ws=ODD) == ALIGN
+    assert linear(y=ODD) == ALIGN and linear(b=ODD) == ALIGN and linear(r=ODD, ldr=32) == ALIGN
+    assert linear(M=0) == 0
