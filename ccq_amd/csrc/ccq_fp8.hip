@@ -71,6 +71,20 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ int slot_row(int s, int G) { return s / (16 * G) * (16 * G) + (s & 15) * G + s / 16 % G; }
 __device__ __forceinline__ int swz(int s) { return (s >> 1) & 7; }
 
+// c += a b 2^(ea + eb - 254) on the matrix cores, the accumulator kept where it is (left to itself the register allocator
+// moves the accumulators about between the products).  Two wait states lie between a vector instruction that wrote an
+// operand and this one, which the compiler does not know of: the operands come straight out of LDS, or operand_settled.
+__device__ __forceinline__ void product128(const i32x8& a, int ea, const i32x8& b, int eb, f32x4& c) {
+  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]"
+               : "+a"(c) : "v"(a), "v"(b), "v"(ea), "v"(eb));
+}
+__device__ __forceinline__ void operand_settled(i32x8& v) { asm volatile("s_nop 1" : "+v"(v)); }
+__device__ __forceinline__ void accumulator(f32x4& c) { asm volatile("" : "+a"(c)); }
+// direct load of 4 bytes a lane from its own address to LDS byte lds + 4 * lane
+__device__ __forceinline__ void load4_to(unsigned lds, const void* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
+}
+
 // eight e4m3 (bytes 8 c .. of a fragment) in bf16, exactly
 __device__ __forceinline__ bf16x8 widen(const i32x8& f, int c) {
   bf16x8 o;
@@ -84,139 +98,235 @@ __device__ __forceinline__ bf16x8 widen(const i32x8& f, int c) {
   return o;
 }
 
+// BM x BN tile of the product by WM x WN waves, two stages of both operands in LDS.  A lane of a wave holds, of each 16 x 16
+// tile (i, j), row r = l & 15 of A's fragment and the columns 4 (l >> 4) .. + 3 of B's.
+//
+// A step is one block of 128.  Its products go in quarters of the wave's tile, (A0, B0), (A0, B1), (A1, B1), (A1, B0), each
+// while the half that the next one needs is read from LDS: B1, A1, then the next step's A0 and, into B1's registers, its B0, so that
+// the halves of B change places from step to step.  At the middle of a step every wave has read all of it and the next
+// step has landed: the one barrier stands there, and the loads of the step after next follow it, between products.
 template <int BM, int BN, int WM, int WN, int ACT, bool EXACT>
 __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8ProductArgs p) {
   constexpr bool GLU = ACT == kActSwiglu;
-  constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, HALF = BN / WN / 2;
+  constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, HALF = BN / WN / 2, HM = TM / 2, HN = TN / 2;
   constexpr int GA = std::min(TM, 4), GB = std::min(GLU ? TN / 2 : TN, 4);
-  constexpr unsigned kA = BM * kStep, kB = BN * kStep;
+  constexpr unsigned kA = BM * kStep, kStage = (BM + BN) * kStep, kScales = (BM + BN) * 4;  // of a step; of four steps
   constexpr int kPass = std::min(TM * 16, 64), kPitch = BN + 4;
-  constexpr unsigned kRing = 2 * (kA + kB), kOut = WM * kPass * kPitch * 4;
+  constexpr unsigned kRing = 2 * (kStage + kScales), kOut = WM * kPass * kPitch * 4;
   constexpr int NT = GLU ? BN / 2 : BN;  // output columns of a tile
-  constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;
+  constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, PS = ((BM + BN) / 64 + NW - 1) / NW;
   static_assert(PA >= 1 && PB >= 1 && (!GLU || PB * 8 == HALF), "whole loads a wave, of gates or ups");
+  static_assert(TM % 2 == 0 && TN % 2 == 0, "halves");
   __shared__ __attribute__((aligned(1024))) char smem[std::max(kRing, kOut)];
   const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN, r = l & 15, g = l >> 4;
+  // tile of this workgroup: each XCD (workgroups are handed out round-robin over the 8) takes consecutive tiles, in
+  // column order within bands of 8 tile rows, so that its L2 holds what its workgroups share
   const int tm = (int)((p.M + BM - 1) / BM), tn = (int)((p.N + NT - 1) / NT), tiles = tm * tn;
   const int xcd = blockIdx.x & 7, q8 = tiles >> 3, r8 = tiles & 7;
   const int t = xcd * q8 + min(xcd, r8) + (blockIdx.x >> 3);
   const int band = t / (8 * tn), in = t - band * 8 * tn, band_rows = min(8, tm - band * 8);
   const long m0 = (long)(band * 8 + in % band_rows) * BM, n0 = (long)(in / band_rows) * NT;
+  const int steps = (int)((p.K + kStep - 1) / kStep), tail = (int)(p.K & (kStep - 1)), whole = steps - (tail ? 1 : 0);
 
-  const unsigned lds0 = lds_addr(smem);
+  // row of B in slot s: swiglu: the gates of a wave's columns, then their ups
+  auto b_row = [&](int s) { return GLU ? s / (2 * HALF) * HALF + slot_row(s % HALF, GB) : slot_row(s, GB); };
+  auto b_up = [&](int s) { return GLU && s % (2 * HALF) >= HALF; };
+  const unsigned lds0 = lds_addr(smem), lds_scales = lds0 + 2 * kStage;
   unsigned offa[PA], offb[PB];
+  const unsigned char* scales[PS];
 #pragma unroll
   for (int i = 0; i < PA; ++i) {
     const int s = (wave * PA + i) * 8 + (l >> 3), row = slot_row(s, GA);
     offa[i] = m0 + row < p.M ? (unsigned)(row * p.lda) + (((l & 7) ^ swz(s)) << 4) : kNowhere;
   }
-  // row of B in slot s: swiglu: the gates of a wave's columns, then their ups
-  auto b_row = [&](int s) { return GLU ? s / (2 * HALF) * HALF + slot_row(s % HALF, GB) : slot_row(s, GB); };
-  auto b_up = [&](int s) { return GLU && s % (2 * HALF) >= HALF; };
 #pragma unroll
   for (int i = 0; i < PB; ++i) {
     const int s = (wave * PB + i) * 8 + (l >> 3), row = b_row(s);
     offb[i] = n0 + row < p.N ? (unsigned)(row * p.ldb) + (((l & 7) ^ swz(s)) << 4) : kNowhere;
   }
-  const size_t pa = (size_t)p.a + m0 * p.lda, pb = (size_t)p.b + (n0 + (GLU && (wave & 1) ? p.N : 0)) * p.ldb;
-  const int steps = (int)((p.K + kStep - 1) / kStep), tail = (int)(p.K & (kStep - 1));
-  auto load = [&](int s) {
-    const unsigned stage = (s & 1) * (kA + kB);
-    u32x4 ra = resource(pa + (long)s * kStep, 0x7fffffffu), rb = resource(pb + (long)s * kStep, 0x7fffffffu);
-    settled(ra);
-    settled(rb);
-    const int left = tail && s == steps - 1 ? tail : kStep;
-    auto issue = [&](const u32x4& rs, unsigned off, unsigned to, int i) {
-      load_to(to, i);
-      asm volatile("s_nop 0");
-      load_from(rs, off);
-    };
+  // scales: A's slots, then B's, 64 a load (of fewer than the waves have, some load the same ones)
+  auto scale_slot = [&](int i) { return (wave * PS + i) % ((BM + BN) / 64) * 64; };
 #pragma unroll
-    for (int i = 0; i < PA; ++i) {
-      const int slot = (wave * PA + i) * 8 + (l >> 3);
-      issue(ra, ((l & 7) ^ swz(slot)) * 16 < left ? offa[i] : kNowhere, lds0 + stage + wave * PA * 1024, i);
-    }
-#pragma unroll
-    for (int i = 0; i < PB; ++i) {
-      const int slot = (wave * PB + i) * 8 + (l >> 3);
-      issue(rb, ((l & 7) ^ swz(slot)) * 16 < left ? offb[i] : kNowhere, lds0 + stage + kA + wave * PB * 1024, i);
-    }
-  };
-  // rows of this lane's scales
-  const unsigned char *sa[TM], *sb[TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) sa[i] = p.sa + std::min(m0 + slot_row((wm * TM + i) * 16 + r, GA), p.M - 1) * p.lsa;
-#pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int s = (wn * TN + j) * 16 + r;
-    sb[j] = p.sb + (std::min(n0 + b_row(s), p.N - 1) + (b_up(s) ? p.N : 0)) * p.lsb;
+  for (int i = 0; i < PS; ++i) {  // (rows behind the last one: the last one's)
+    const int s = scale_slot(i) + l;
+    if (s < BM) scales[i] = p.sa + min(m0 + slot_row(s, GA), p.M - 1) * p.lsa;
+    else scales[i] = p.sb + (min(n0 + b_row(s - BM), p.N - 1) + (b_up(s - BM) ? p.N : 0)) * p.lsb;
   }
-  unsigned ea[TM], eb[TN];
+  const size_t pa = (size_t)p.a + m0 * p.lda, pb = (size_t)p.b + (n0 + (GLU && (wave & 1) ? p.N : 0)) * p.ldb;
+  auto load_scales = [&](int quad) {  // of steps 4 quad .. + 3
+    if (quad * 4 >= steps) return;
+#pragma unroll
+    for (int i = 0; i < PS; ++i)
+      load4_to(lds_scales + (quad & 1) * kScales + scale_slot(i) * 4, scales[i] + 4 * quad);
+  };
+  auto step_resource = [&](size_t base, int s) { return resource(base + (size_t)s * kStep, s < whole ? 0x7fffffffu : 0u); };
+
+  // fragment addresses of this lane in stage 0, and of its scales
+  unsigned fa[2], fb[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    fa[h] = lds0 + (wm * TM * 16 + r) * 128 + (((g + 4 * h) ^ swz(r)) << 4);
+    fb[h] = lds0 + kA + (wn * TN * 16 + r) * 128 + (((g + 4 * h) ^ swz(r)) << 4);
+  }
+  const unsigned ea0 = lds_scales + (wm * TM * 16 + r) * 4, eb0 = lds_scales + (BM + wn * TN * 16 + r) * 4;
+  struct Frag {
+    i32x8 v;
+    int e;
+  };
+  auto read = [&](Frag& f, const unsigned (&at)[2], unsigned e0, int i, unsigned stage, unsigned scale) {
+    const i32x4 x = __builtin_bit_cast(i32x4, read16(at[0] + stage + i * 2048)), y = __builtin_bit_cast(i32x4, read16(at[1] + stage + i * 2048));
+    f.v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    typedef __attribute__((address_space(3))) const unsigned char lds_byte;
+    f.e = *(lds_byte*)(size_t)(e0 + scale + i * 64);
+  };
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto frag = [&](unsigned at, int slot) {
-    const s16x8 lo = read16(at + slot * 128 + ((g ^ swz(slot)) << 4)), hi = read16(at + slot * 128 + (((g + 4) ^ swz(slot)) << 4));
-    const i32x4 x = __builtin_bit_cast(i32x4, lo), y = __builtin_bit_cast(i32x4, hi);
-    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-  };
-  load(0);
-  for (int s = 0; s < steps; ++s) {
-    if ((s & 3) == 0) {
-#pragma unroll
-      for (int i = 0; i < TM; ++i) ea[i] = *gmem((const unsigned*)(sa[i] + s));
-#pragma unroll
-      for (int j = 0; j < TN; ++j) eb[j] = *gmem((const unsigned*)(sb[j] + s));
+    for (int j = 0; j < TN; ++j) {
+      acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (!EXACT) accumulator(acc[i][j]);
     }
+  acc_settled();
+  auto product = [&](const Frag& a, const Frag& b, f32x4& c) {
+    if constexpr (!EXACT) {
+      product128(b.v, b.e, a.v, a.e, c);
+    } else {
+      f32x4 sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum = mfma16(widen(b.v, k), widen(a.v, k), sum);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // the scale of column 4 g + q lies in lane 4 g + q
+        const int y = __shfl(b.e, 4 * g + q);
+        c[q] += a.e == (int)kFp8Nan || y == (int)kFp8Nan ? NAN : __builtin_ldexpf(sum[q], a.e + y - 254);
+      }
+    }
+  };
+
+  Frag a0[HM], a1[HM], b0[HN], b1[HN];
+  u32x4 ra, rb;
+  // a quarter of the products, with `reads` between them; f(k) for each k < n, spread over the quarter
+  auto quarter = [&](int ih, int jh, const Frag (&a)[HM], const Frag (&b)[HN], auto&& between) {
+#pragma unroll
+    for (int q = 0; q < HM * HN; ++q) {
+      product(a[q / HN], b[q % HN], acc[ih * HM + q / HN][jh * HN + q % HN]);
+      between(q);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  constexpr int Q = HM * HN;
+  auto step = [&](int s, Frag (&x0)[HN], Frag (&x1)[HN]) {  // x0: this step's B0; x1: its B1, then the next step's B0
+    const unsigned stage = (s & 1) * kStage, next = kStage - stage;
+    const unsigned scale = (s >> 2 & 1) * kScales + (s & 3), scale_next = ((s + 1) >> 2 & 1) * kScales + ((s + 1) & 3);
+    quarter(0, 0, a0, x0, [&](int q) {
+#pragma unroll
+      for (int k = q * HN / Q; k < (q + 1) * HN / Q; ++k) read(x1[k], fb, eb0, HN + k, stage, scale);
+    });
+    quarter(0, 1, a0, x1, [&](int q) {
+#pragma unroll
+      for (int k = q * HM / Q; k < (q + 1) * HM / Q; ++k) read(a1[k], fa, ea0, HM + k, stage, scale);
+    });
     wait_loads<0>();
     lds_barrier();
-    if (s + 1 < steps) load(s + 1);
-    const unsigned at = lds0 + (s & 1) * (kA + kB);
-    i32x8 mask;
-    const bool part = tail & 15 && s == steps - 1;
-    if (part)
+    ra = step_resource(pa, s + 2);
+    rb = step_resource(pb, s + 2);
+    settled(ra);
+    settled(rb);
+    if ((s & 3) == 0) load_scales((s >> 2) + 1);
+    const unsigned to_a = lds0 + stage + wave * PA * 1024, to_b = lds0 + stage + kA + wave * PB * 1024;
+    quarter(1, 1, a1, x1, [&](int q) {
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {  // bytes of the end: the row's storage goes on behind them
-        const int n = tail - (16 * (g + d / 4 * 4) + d % 4 * 4);
-        mask[d] = n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1;
+      for (int k = q * (PA + PB) / Q; k < (q + 1) * (PA + PB) / Q; ++k) {
+        if (k < PA) {
+          load_to(to_a, k);
+          asm volatile("s_nop 0");
+          load_from(ra, offa[k < PA ? k : 0]);
+        } else {
+          load_to(to_b, k - PA);
+          asm volatile("s_nop 0");
+          load_from(rb, offb[k < PA ? 0 : k - PA]);
+        }
       }
-    i32x8 b[TN];
+#pragma unroll
+      for (int k = q * HM / Q; k < (q + 1) * HM / Q; ++k) read(a0[k], fa, ea0, k, next, scale_next);
+    });
+    quarter(1, 0, a1, x0, [&](int q) {
+#pragma unroll
+      for (int k = q * HN / Q; k < (q + 1) * HN / Q; ++k) read(x1[k], fb, eb0, k, next, scale_next);
+    });
+  };
+  auto load_step = [&](int s, int left) {  // all of a step; its elements at and behind `left` as zeros
+    const unsigned stage = (s & 1) * kStage;
+    ra = resource(pa + (size_t)s * kStep, 0x7fffffffu);
+    rb = resource(pb + (size_t)s * kStep, 0x7fffffffu);
+    settled(ra);
+    settled(rb);
+#pragma unroll
+    for (int i = 0; i < PA; ++i) {
+      const int slot = (wave * PA + i) * 8 + (l >> 3);
+      load_to(lds0 + stage + wave * PA * 1024, i);
+      asm volatile("s_nop 0");
+      load_from(ra, ((l & 7) ^ swz(slot)) * 16 < left ? offa[i] : kNowhere);
+    }
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+      const int slot = (wave * PB + i) * 8 + (l >> 3);
+      load_to(lds0 + stage + kA + wave * PB * 1024, i);
+      asm volatile("s_nop 0");
+      load_from(rb, ((l & 7) ^ swz(slot)) * 16 < left ? offb[i] : kNowhere);
+    }
+  };
+  load_scales(0);
+  if (whole > 0) {
+    load_step(0, kStep);
+    if (whole > 1) load_step(1, kStep);
+    if (whole > 1) wait_loads<PA + PB>();
+    else wait_loads<0>();
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < HM; ++i) read(a0[i], fa, ea0, i, 0, 0);
+#pragma unroll
+    for (int j = 0; j < HN; ++j) read(b0[j], fb, eb0, j, 0, 0);
+    int s = 0;
+    for (; s + 2 <= whole; s += 2) {
+      step(s, b0, b1);
+      step(s + 1, b1, b0);
+    }
+    if (s < whole) step(s, b0, b1);
+    wait_loads<0>();
+    lds_barrier();
+  }
+  if (tail) {
+    load_step(whole, tail);
+    wait_loads<0>();
+    lds_barrier();
+    i32x8 mask;
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {  // bytes of the end: the row's storage goes on behind them
+      const int n = tail - (16 * (g + d / 4 * 4) + d % 4 * 4);
+      mask[d] = n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1;
+    }
+    const unsigned stage = (whole & 1) * kStage, scale = (whole >> 2 & 1) * kScales + (whole & 3);
+    Frag b[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      b[j] = frag(at + kA, (wn * TN + j) * 16 + r);
-      if (part) b[j] &= mask;
+      read(b[j], fb, eb0, j, stage, scale);
+      b[j].v &= mask;
+      operand_settled(b[j].v);
     }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      i32x8 a = frag(at, (wm * TM + i) * 16 + r);
-      if (part) a &= mask;
+      Frag a;
+      read(a, fa, ea0, i, stage, scale);
+      a.v &= mask;
+      operand_settled(a.v);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        if constexpr (!EXACT) {
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a, acc[i][j], 0, 0, 0, eb[j], 0, ea[i]);
-        } else {
-          f32x4 sum{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 4; ++c) sum = mfma16(widen(b[j], c), widen(a, c), sum);
-          // the columns' scales lie in the lanes that hold their fragment's rows: column 4 g + q in lane 4 g + q
-          const unsigned x = ea[i] & 0xff;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const unsigned y = (unsigned)__shfl((int)eb[j], 4 * g + q) & 0xff;
-            acc[i][j][q] += x == kFp8Nan || y == kFp8Nan ? NAN : __builtin_ldexpf(sum[q], (int)(x + y) - 254);
-          }
-        }
-      }
+      for (int j = 0; j < TN; ++j) product(a, b[j], acc[i][j]);
     }
-#pragma unroll
-    for (int i = 0; i < TM; ++i) ea[i] >>= 8;
-#pragma unroll
-    for (int j = 0; j < TN; ++j) eb[j] >>= 8;
   }
 
+  acc_settled();
   float* tile = (float*)smem;
   constexpr int PR = NT / 8, RP = NW * 64 / PR;  // threads of a row, rows at a time
   const int c = tid % PR * 8, cw = c / (GLU ? HALF : NT), cs = GLU ? cw * 2 * HALF + c % HALF : c;
