@@ -79,6 +79,14 @@ __device__ __forceinline__ void product128(const i32x8& a, int ea, const i32x8& 
                : "+a"(c) : "v"(a), "v"(b), "v"(ea), "v"(eb));
 }
 __device__ __forceinline__ void operand_settled(i32x8& v) { asm volatile("s_nop 1" : "+v"(v)); }
+// an accumulator's value, read where the program says so (left to itself the compiler copies all 256 at once, and spills)
+template <bool PINNED>
+__device__ __forceinline__ float value_of(float c) {
+  if (!PINNED) return c;
+  float v;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(c));
+  return v;
+}
 __device__ __forceinline__ void accumulator(f32x4& c) { asm volatile("" : "+a"(c)); }
 // direct load of 4 bytes a lane from its own address to LDS byte lds + 4 * lane
 __device__ __forceinline__ void load4_to(unsigned lds, const void* from) {
@@ -98,24 +106,27 @@ __device__ __forceinline__ bf16x8 widen(const i32x8& f, int c) {
   return o;
 }
 
+enum : int { kOut16 = 0, kOut32 = 1, kOut8 = 2 };  // bf16 or fp16 (dtype), fp32, e4m3 with scales
+
 // BM x BN tile of the product by WM x WN waves, two stages of both operands in LDS.  A lane of a wave holds, of each 16 x 16
 // tile (i, j), row r = l & 15 of A's fragment and the columns 4 (l >> 4) .. + 3 of B's.
 //
 // A step is one block of 128.  Its products go in quarters of the wave's tile, (A0, B0), (A0, B1), (A1, B1), (A1, B0), each
 // while the half that the next one needs is read from LDS: B1, A1, then the next step's A0 and, into B1's registers, its B0, so that
-// the halves of B change places from step to step.  At the middle of a step every wave has read all of it and the next
-// step has landed: the one barrier stands there, and the loads of the step after next follow it, between products.
-template <int BM, int BN, int WM, int WN, int ACT, bool EXACT>
+// the halves of B change places from step to step.  So A0 and B0 of a step have been read when it begins, A1 and B1 at its
+// middle: there stand the barriers, and behind each of them those halves of the step after next are loaded, between
+// products, a step and a half before they are read.
+template <int BM, int BN, int WM, int WN, int ACT, int OUT>
 __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8ProductArgs p) {
-  constexpr bool GLU = ACT == kActSwiglu;
+  constexpr bool GLU = ACT == kActSwiglu, EXACT = OUT == kOut32;
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, HALF = BN / WN / 2, HM = TM / 2, HN = TN / 2;
   constexpr int GA = std::min(TM, 4), GB = std::min(GLU ? TN / 2 : TN, 4);
   constexpr unsigned kA = BM * kStep, kStage = (BM + BN) * kStep, kScales = (BM + BN) * 4;  // of a step; of four steps
   constexpr int kPass = std::min(TM * 16, 64), kPitch = BN + 4;
   constexpr unsigned kRing = 2 * (kStage + kScales), kOut = WM * kPass * kPitch * 4;
   constexpr int NT = GLU ? BN / 2 : BN;  // output columns of a tile
-  constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW, PS = ((BM + BN) / 64 + NW - 1) / NW;
-  static_assert(PA >= 1 && PB >= 1 && (!GLU || PB * 8 == HALF), "whole loads a wave, of gates or ups");
+  constexpr int PA = BM / 16 / NW, PB = BN / 16 / NW, PS = ((BM + BN) / 64 + NW - 1) / NW;
+  static_assert(PA >= 1 && PB >= 1, "whole loads a wave of each half");
   static_assert(TM % 2 == 0 && TN % 2 == 0, "halves");
   __shared__ __attribute__((aligned(1024))) char smem[std::max(kRing, kOut)];
   const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -133,17 +144,24 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
   auto b_row = [&](int s) { return GLU ? s / (2 * HALF) * HALF + slot_row(s % HALF, GB) : slot_row(s, GB); };
   auto b_up = [&](int s) { return GLU && s % (2 * HALF) >= HALF; };
   const unsigned lds0 = lds_addr(smem), lds_scales = lds0 + 2 * kStage;
-  unsigned offa[PA], offb[PB];
+  // Loads of half h of a step: 8 slots each; a wave's i-th one of A and of B begins at these slots.
+  auto slot_a = [&](int h, int i) { const int k = wave * PA + i; return k / (2 * HM) * (TM * 16) + h * (HM * 16) + k % (2 * HM) * 8; };
+  auto slot_b = [&](int h, int i) { const int k = wave * PB + i; return k / (2 * HN) * (TN * 16) + h * (HN * 16) + k % (2 * HN) * 8; };
+  auto piece = [&](int slot) { return (l & 7) ^ swz(slot + (l >> 3)); };
+  unsigned offa[2][PA], offb[2][PB];
   const unsigned char* scales[PS];
 #pragma unroll
-  for (int i = 0; i < PA; ++i) {
-    const int s = (wave * PA + i) * 8 + (l >> 3), row = slot_row(s, GA);
-    offa[i] = m0 + row < p.M ? (unsigned)(row * p.lda) + (((l & 7) ^ swz(s)) << 4) : kNowhere;
-  }
+  for (int h = 0; h < 2; ++h) {
 #pragma unroll
-  for (int i = 0; i < PB; ++i) {
-    const int s = (wave * PB + i) * 8 + (l >> 3), row = b_row(s);
-    offb[i] = n0 + row < p.N ? (unsigned)(row * p.ldb) + (((l & 7) ^ swz(s)) << 4) : kNowhere;
+    for (int i = 0; i < PA; ++i) {
+      const int s = slot_a(h, i), row = slot_row(s + (l >> 3), GA);
+      offa[h][i] = m0 + row < p.M ? (unsigned)(row * p.lda) + (piece(s) << 4) : kNowhere;
+    }
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {  // (swiglu: half 0 holds gates, half 1 ups)
+      const int s = slot_b(h, i), row = b_row(s + (l >> 3));
+      offb[h][i] = n0 + row < p.N ? (unsigned)(row * p.ldb) + (piece(s) << 4) : kNowhere;
+    }
   }
   // scales: A's slots, then B's, 64 a load (of fewer than the waves have, some load the same ones)
   auto scale_slot = [&](int i) { return (wave * PS + i) % ((BM + BN) / 64) * 64; };
@@ -153,14 +171,16 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     if (s < BM) scales[i] = p.sa + min(m0 + slot_row(s, GA), p.M - 1) * p.lsa;
     else scales[i] = p.sb + (min(n0 + b_row(s - BM), p.N - 1) + (b_up(s - BM) ? p.N : 0)) * p.lsb;
   }
-  const size_t pa = (size_t)p.a + m0 * p.lda, pb = (size_t)p.b + (n0 + (GLU && (wave & 1) ? p.N : 0)) * p.ldb;
+  const size_t pa = (size_t)p.a + m0 * p.lda, pb = (size_t)p.b + n0 * p.ldb, up = GLU ? p.N * p.ldb : 0;
   auto load_scales = [&](int quad) {  // of steps 4 quad .. + 3
     if (quad * 4 >= steps) return;
 #pragma unroll
     for (int i = 0; i < PS; ++i)
       load4_to(lds_scales + (quad & 1) * kScales + scale_slot(i) * 4, scales[i] + 4 * quad);
   };
-  auto step_resource = [&](size_t base, int s) { return resource(base + (size_t)s * kStep, s < whole ? 0x7fffffffu : 0u); };
+  auto step_resource = [&](size_t base, int s) {  // (empty behind the last whole step)
+    return resource(base + (size_t)s * kStep, s < whole ? 0x7fffffffu : 0u);
+  };
 
   // fragment addresses of this lane in stage 0, and of its scales
   unsigned fa[2], fb[2];
@@ -205,7 +225,6 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
   };
 
   Frag a0[HM], a1[HM], b0[HN], b1[HN];
-  u32x4 ra, rb;
   // a quarter of the products, with `reads` between them; f(k) for each k < n, spread over the quarter
   auto quarter = [&](int ih, int jh, const Frag (&a)[HM], const Frag (&b)[HN], auto&& between) {
 #pragma unroll
@@ -215,74 +234,71 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  constexpr int Q = HM * HN;
+  constexpr int Q = HM * HN, PL = PA + PB;
+  // the loads of half h of the step whose resources are given, one at a time
+  auto load = [&](int h, int k, unsigned stage, const u32x4& ra, const u32x4& rb) {
+    if (k < PA) {
+      load_to(lds0 + stage + slot_a(h, k) * 128, 0);
+      asm volatile("s_nop 0");
+      load_from(ra, offa[h][k < PA ? k : 0]);
+    } else {
+      load_to(lds0 + stage + kA + slot_b(h, k - PA) * 128, 0);
+      asm volatile("s_nop 0");
+      load_from(rb, offb[h][k < PA ? 0 : k - PA]);
+    }
+  };
+  auto spread = [&](int q, int n, auto&& f) {  // f(0) .. f(n - 1) over the first three quarters of Q products
+#pragma unroll
+    for (int k = 0; k < n; ++k)
+      if (q == k * Q * 3 / 4 / n) f(k);
+  };
   auto step = [&](int s, Frag (&x0)[HN], Frag (&x1)[HN]) {  // x0: this step's B0; x1: its B1, then the next step's B0
     const unsigned stage = (s & 1) * kStage, next = kStage - stage;
     const unsigned scale = (s >> 2 & 1) * kScales + (s & 3), scale_next = ((s + 1) >> 2 & 1) * kScales + ((s + 1) & 3);
+    wait_loads<2 * PL>();
+    lds_barrier();
+    if ((s & 3) == 0) load_scales((s >> 2) + 1);
+    u32x4 ra = step_resource(pa, s + 2), rb = step_resource(pb, s + 2);
+    settled(ra);
+    settled(rb);
     quarter(0, 0, a0, x0, [&](int q) {
-#pragma unroll
-      for (int k = q * HN / Q; k < (q + 1) * HN / Q; ++k) read(x1[k], fb, eb0, HN + k, stage, scale);
+      spread(q, HN, [&](int k) { read(x1[k], fb, eb0, HN + k, stage, scale); });
+      spread(q, PA, [&](int k) { load(0, k, stage, ra, rb); });
     });
     quarter(0, 1, a0, x1, [&](int q) {
-#pragma unroll
-      for (int k = q * HM / Q; k < (q + 1) * HM / Q; ++k) read(a1[k], fa, ea0, HM + k, stage, scale);
+      spread(q, HM, [&](int k) { read(a1[k], fa, ea0, HM + k, stage, scale); });
+      spread(q, PB, [&](int k) { load(0, PA + k, stage, ra, rb); });
     });
-    wait_loads<0>();
+    wait_loads<2 * PL>();
     lds_barrier();
-    ra = step_resource(pa, s + 2);
-    rb = step_resource(pb, s + 2);
-    settled(ra);
-    settled(rb);
-    if ((s & 3) == 0) load_scales((s >> 2) + 1);
-    const unsigned to_a = lds0 + stage + wave * PA * 1024, to_b = lds0 + stage + kA + wave * PB * 1024;
+    if (GLU) {
+      rb = step_resource(pb + up, s + 2);
+      settled(rb);
+    }
     quarter(1, 1, a1, x1, [&](int q) {
-#pragma unroll
-      for (int k = q * (PA + PB) / Q; k < (q + 1) * (PA + PB) / Q; ++k) {
-        if (k < PA) {
-          load_to(to_a, k);
-          asm volatile("s_nop 0");
-          load_from(ra, offa[k < PA ? k : 0]);
-        } else {
-          load_to(to_b, k - PA);
-          asm volatile("s_nop 0");
-          load_from(rb, offb[k < PA ? 0 : k - PA]);
-        }
-      }
-#pragma unroll
-      for (int k = q * HM / Q; k < (q + 1) * HM / Q; ++k) read(a0[k], fa, ea0, k, next, scale_next);
+      spread(q, HM, [&](int k) { read(a0[k], fa, ea0, k, next, scale_next); });
+      spread(q, PA, [&](int k) { load(1, k, stage, ra, rb); });
     });
     quarter(1, 0, a1, x0, [&](int q) {
-#pragma unroll
-      for (int k = q * HN / Q; k < (q + 1) * HN / Q; ++k) read(x1[k], fb, eb0, k, next, scale_next);
+      spread(q, HN, [&](int k) { read(x1[k], fb, eb0, k, next, scale_next); });
+      spread(q, PB, [&](int k) { load(1, PA + k, stage, ra, rb); });
     });
   };
-  auto load_step = [&](int s, int left) {  // all of a step; its elements at and behind `left` as zeros
-    const unsigned stage = (s & 1) * kStage;
-    ra = resource(pa + (size_t)s * kStep, 0x7fffffffu);
-    rb = resource(pb + (size_t)s * kStep, 0x7fffffffu);
-    settled(ra);
-    settled(rb);
+  auto load_step = [&](int s) {  // all of a whole step
 #pragma unroll
-    for (int i = 0; i < PA; ++i) {
-      const int slot = (wave * PA + i) * 8 + (l >> 3);
-      load_to(lds0 + stage + wave * PA * 1024, i);
-      asm volatile("s_nop 0");
-      load_from(ra, ((l & 7) ^ swz(slot)) * 16 < left ? offa[i] : kNowhere);
-    }
+    for (int h = 0; h < 2; ++h) {
+      u32x4 ra = step_resource(pa, s), rb = step_resource(pb + h * up, s);
+      settled(ra);
+      settled(rb);
 #pragma unroll
-    for (int i = 0; i < PB; ++i) {
-      const int slot = (wave * PB + i) * 8 + (l >> 3);
-      load_to(lds0 + stage + kA + wave * PB * 1024, i);
-      asm volatile("s_nop 0");
-      load_from(rb, ((l & 7) ^ swz(slot)) * 16 < left ? offb[i] : kNowhere);
+      for (int k = 0; k < PL; ++k) load(h, k, s * kStage, ra, rb);
     }
   };
   load_scales(0);
   if (whole > 0) {
-    load_step(0, kStep);
-    if (whole > 1) load_step(1, kStep);
-    if (whole > 1) wait_loads<PA + PB>();
-    else wait_loads<0>();
+    load_step(0);
+    load_step(1);
+    wait_loads<3 * PL>();
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < HM; ++i) read(a0[i], fa, ea0, i, 0, 0);
@@ -297,8 +313,22 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     wait_loads<0>();
     lds_barrier();
   }
-  if (tail) {
-    load_step(whole, tail);
+  if (tail) {  // the end of the rows: its elements at and behind `tail` as zeros
+    const unsigned stage = (whole & 1) * kStage, scale = (whole >> 2 & 1) * kScales + (whole & 3);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      u32x4 ra = resource(pa + (size_t)whole * kStep, 0x7fffffffu), rb = resource(pb + h * up + (size_t)whole * kStep, 0x7fffffffu);
+      settled(ra);
+      settled(rb);
+#pragma unroll
+      for (int k = 0; k < PL; ++k) {
+        const bool of_a = k < PA;
+        const int slot = of_a ? slot_a(h, k) : slot_b(h, k - PA);
+        load_to(lds0 + stage + (of_a ? 0 : kA) + slot * 128, 0);
+        asm volatile("s_nop 0");
+        load_from(of_a ? ra : rb, piece(slot) * 16 < tail ? (of_a ? offa[h][of_a ? k : 0] : offb[h][of_a ? 0 : k - PA]) : kNowhere);
+      }
+    }
     wait_loads<0>();
     lds_barrier();
     i32x8 mask;
@@ -307,7 +337,6 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
       const int n = tail - (16 * (g + d / 4 * 4) + d % 4 * 4);
       mask[d] = n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1;
     }
-    const unsigned stage = (whole & 1) * kStage, scale = (whole >> 2 & 1) * kScales + (whole & 3);
     Frag b[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
@@ -327,8 +356,120 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
   }
 
   acc_settled();
+  // Tiles that end within the columns: straight from the accumulators.  A lane holds, of each of its rows, W consecutive
+  // columns of each group.
+  constexpr int W = 4 * GB, JG = TN / GB / (GLU ? 2 : 1), COLS = GLU ? HALF : TN * 16;
+  if constexpr (ACT != kActOther) {
+    if (n0 + NT <= p.N) {
+      const long nw = n0 + wn * COLS + g * W;
+      auto row_of = [&](int i) { return m0 + wm * TM * 16 + slot_row(i * 16 + r, GA); };
+      float bias[TN / GB][W];
+#pragma unroll
+      for (int j = 0; j < TN / GB; ++j)
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+          bias[j][e] = p.bias ? bias_at(p.bias, p.bdtype, (j >= JG ? p.N : 0) + nw + j % JG * 16 * GB + e) : 0.f;
+      auto values = [&](int i, int j, float (&v)[W]) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          v[e] = value_of<!EXACT>(acc[i][j * GB + e % GB][e / GB]) + bias[j][e];
+          if (GLU) {
+            constexpr int U = GLU ? JG : 0;
+            v[e] = v[e] * sigmoid(v[e]) * (value_of<!EXACT>(acc[i][(j + U) * GB + e % GB][e / GB]) + bias[j + U][e]);
+          }
+        }
+      };
+      if constexpr (OUT == kOut8) {
+        // a block's columns lie in the four lanes of a row, and with swiglu in two waves
+        static_assert(COLS == kFp8Block || (GLU && COLS * 2 == kFp8Block), "blocks of a wave, or of two");
+        auto largest = [&](const float (&v)[JG][W]) {
+          unsigned most = 0;
+#pragma unroll
+          for (int j = 0; j < JG; ++j)
+#pragma unroll
+            for (int e = 0; e < W; ++e) most = max(most, magnitude(v[j][e]));
+          most = max(most, (unsigned)__shfl_xor((int)most, 16));
+          return max(most, (unsigned)__shfl_xor((int)most, 32));
+        };
+        auto emit = [&](int i, const float (&v)[JG][W], unsigned most) {
+          const unsigned byte = scale_byte(most);
+          const long m = row_of(i);
+          if (m >= p.M) return;
+#pragma unroll
+          for (int j = 0; j < JG; ++j) {
+            typedef unsigned words __attribute__((ext_vector_type(W / 4)));
+            words o;
+#pragma unroll
+            for (int e = 0; e < W / 4; ++e) o[e] = fp8_word(v[j][4 * e], v[j][4 * e + 1], v[j][4 * e + 2], v[j][4 * e + 3], byte);
+            *gmem((words*)((unsigned char*)p.out + m * p.ldo + nw + j * 16 * GB)) = o;
+          }
+          if (g == 0 && (!GLU || (wn & 1) == 0)) p.os[m * p.los + (n0 + wn * COLS) / kFp8Block] = (unsigned char)byte;
+        };
+        if constexpr (!GLU) {
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+            float v[JG][W];
+#pragma unroll
+            for (int j = 0; j < JG; ++j) values(i, j, v[j]);
+            emit(i, v, largest(v));
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        } else {
+          __shared__ unsigned block_most[WN][BM];
+          float v[TM][JG][W];
+          unsigned most[TM];
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+            values(i, 0, v[i][0]);
+            most[i] = largest(v[i]);
+            if (g == 0) block_most[wn][(wm * TM + i) * 16 + r] = most[i];
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          __syncthreads();
+#pragma unroll
+          for (int i = 0; i < TM; ++i) emit(i, v[i], max(most[i], block_most[wn ^ 1][(wm * TM + i) * 16 + r]));
+        }
+      } else {
+        // all of the residual on its way at once: the fragments' registers are free
+        auto emit = [&](auto type) {
+          typedef decltype(type) T;
+          RowPiece<T, W> res[TM][JG];
+          if (p.res)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+              for (int j = 0; j < JG; ++j)
+                if (row_of(i) < p.M) res[i][j].v = *gmem((const typename RowPiece<T, W>::any*)((const T*)p.res + row_of(i) * p.ldr + nw + j * 16 * GB));
+#pragma unroll
+          for (int i = 0; i < TM; ++i) {
+            const long m = row_of(i);
+            if (m >= p.M) continue;
+#pragma unroll
+            for (int j = 0; j < JG; ++j) {
+              float v[W];
+              values(i, j, v);
+              if (p.res)
+#pragma unroll
+                for (int e = 0; e < W; ++e) v[e] += (float)res[i][j].v[e];
+              typename RowPiece<T, W>::vec o;
+#pragma unroll
+              for (int e = 0; e < W; ++e) o[e] = (T)v[e];
+              *gmem((typename RowPiece<T, W>::any*)((T*)p.out + m * p.ldo + nw + j * 16 * GB)) = o;
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+        };
+        if constexpr (OUT == kOut32) emit(0.f);
+        else if (p.dtype == kBf16) emit((bf16)0.f);
+        else emit((f16)0.f);
+      }
+      return;
+    }
+  }
+
+  // The others, and the activations that are code of some size, through LDS: a thread takes eight consecutive columns.
   float* tile = (float*)smem;
-  constexpr int PR = NT / 8, RP = NW * 64 / PR;  // threads of a row, rows at a time
+  constexpr int PR = NT / 8, RP = NW * 64 / PR, NG = 4;  // threads of a row, rows at a time, how often before the next loads
   const int c = tid % PR * 8, cw = c / (GLU ? HALF : NT), cs = GLU ? cw * 2 * HALF + c % HALF : c;
   const long n = n0 + c;
   float bias[8], bias_up[8];
@@ -337,6 +478,54 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     bias[i] = p.bias && n + i < p.N ? bias_at(p.bias, p.bdtype, n + i) : 0.f;
     bias_up[i] = GLU && p.bias && n + i < p.N ? bias_at(p.bias, p.bdtype, p.N + n + i) : 0.f;
   }
+  auto through = [&](auto type, int h) {
+    typedef decltype(type) T;
+    for (int i0 = tid / PR; i0 < WM * kPass; i0 += NG * RP) {
+      RowPiece<T, 8> res[NG];
+      long m[NG];
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        const int i = i0 + k * RP;
+        m[k] = i < WM * kPass ? m0 + i / kPass * (TM * 16) + slot_row(h * kPass + i % kPass, GA) : p.M;
+        if (p.res && m[k] < p.M && n < p.N) res[k].load((const T*)p.res + m[k] * p.ldr, n, p.N);
+      }
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        const int i = i0 + k * RP;
+        if (m[k] >= p.M || (n >= p.N && OUT != kOut8)) continue;
+        float v[8], up[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] = tile[i * kPitch + cs + e] + bias[e];
+          if (GLU) up[e] = tile[i * kPitch + cs + HALF + e] + bias_up[e];
+        }
+        if (GLU) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = v[e] * sigmoid(v[e]) * up[e];
+        } else if (ACT != kActNone) {
+          act_values<8>(p.act, v);
+        }
+        if constexpr (OUT == kOut8) {  // a row's 16 lanes of a block go together
+          unsigned most = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (n + e >= p.N) v[e] = 0.f;
+            most = max(most, magnitude(v[e]));
+          }
+          const unsigned byte = scale_byte(lanes_max(most, 16));
+          if (n >= p.N) continue;
+          *gmem((u32x2*)((unsigned char*)p.out + m[k] * p.ldo + n)) =
+              u32x2{fp8_word(v[0], v[1], v[2], v[3], byte), fp8_word(v[4], v[5], v[6], v[7], byte)};
+          if ((tid & 15) == 0) p.os[m[k] * p.los + n / kFp8Block] = (unsigned char)byte;
+        } else {
+          if (p.res)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += (float)res[k].v[e];
+          store_row<T, 8>((T*)p.out + m[k] * p.ldo, n, p.N, v);
+        }
+      }
+    }
+  };
 #pragma unroll
   for (int h = 0; h < TM * 16 / kPass; ++h) {
     lds_barrier();
@@ -348,58 +537,25 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
         for (int q = 0; q < 4; ++q)
 #pragma unroll
           for (int k = 0; k < GB; ++k)
-            tile[(wm * kPass + i * 16 + r) * kPitch + (wn * TN + j) * 16 + (4 * g + q) * GB + k] = acc[h * (kPass / 16) + i][j + k][q];
+            tile[(wm * kPass + i * 16 + r) * kPitch + (wn * TN + j) * 16 + (4 * g + q) * GB + k] =
+                value_of<!EXACT>(acc[h * (kPass / 16) + i][j + k][q]);
     __syncthreads();
-    for (int i = tid / PR; i < WM * kPass; i += RP) {
-      const long m = m0 + i / kPass * (TM * 16) + slot_row(h * kPass + i % kPass, GA);
-      if (m >= p.M || (n >= p.N && !p.os)) continue;
-      float v[8], up[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] = tile[i * kPitch + cs + e] + bias[e];
-        if (GLU) up[e] = tile[i * kPitch + cs + HALF + e] + bias_up[e];
-      }
-      if (GLU) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = v[e] * sigmoid(v[e]) * up[e];
-      } else if (ACT != kActNone) {
-        act_values<8>(p.act, v);
-      }
-      if (p.os) {  // a row's 16 lanes of a block go together
-        unsigned most = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (n + e >= p.N) v[e] = 0.f;
-          most = max(most, magnitude(v[e]));
-        }
-        const unsigned byte = scale_byte(lanes_max(most, 16));
-        if (n >= p.N) continue;
-        *gmem((u32x2*)((unsigned char*)p.out + m * p.ldo + n)) =
-            u32x2{fp8_word(v[0], v[1], v[2], v[3], byte), fp8_word(v[4], v[5], v[6], v[7], byte)};
-        if ((tid & 15) == 0) p.os[m * p.los + n / kFp8Block] = (unsigned char)byte;
-        continue;
-      }
-      if (p.dtype == kF32) {
-        if (p.res) add_row<float, 8>((const float*)p.res + m * p.ldr, n, p.N, v);
-        store_row<float, 8>((float*)p.out + m * p.ldo, n, p.N, v);
-      } else if (p.dtype == kBf16) {
-        if (p.res) add_row<bf16, 8>((const bf16*)p.res + m * p.ldr, n, p.N, v);
-        store_row<bf16, 8>((bf16*)p.out + m * p.ldo, n, p.N, v);
-      } else {
-        if (p.res) add_row<f16, 8>((const f16*)p.res + m * p.ldr, n, p.N, v);
-        store_row<f16, 8>((f16*)p.out + m * p.ldo, n, p.N, v);
-      }
+    if constexpr (OUT == kOut16) {
+      if (p.dtype == kBf16) through((bf16)0.f, h);
+      else through((f16)0.f, h);
+    } else {
+      through(0.f, h);
     }
   }
 }
 
-template <int BM, int BN, int WM, int WN, bool EXACT>
+template <int BM, int BN, int WM, int WN, int OUT>
 hipError_t launch_tiles(const Fp8ProductArgs& p, hipStream_t st) {
   const int NT = p.act == kActSwiglu ? BN / 2 : BN;
   const dim3 grid((unsigned)(((p.M + BM - 1) / BM) * ((p.N + NT - 1) / NT))), block(WM * WN * 64);
-  if (p.act == kActSwiglu) hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActSwiglu, EXACT>), grid, block, 0, st, p);
-  else if (p.act == kActNone) hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActNone, EXACT>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActOther, EXACT>), grid, block, 0, st, p);
+  if (p.act == kActSwiglu) hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActSwiglu, OUT>), grid, block, 0, st, p);
+  else if (p.act == kActNone) hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActNone, OUT>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActOther, OUT>), grid, block, 0, st, p);
   return hipGetLastError();
 }
 
@@ -422,9 +578,10 @@ hipError_t launch_quantize(const QuantizeArgs& a, hipStream_t st) {
 hipError_t launch_fp8_product(const Fp8ProductArgs& p, hipStream_t st) {
   if (p.M <= 0) return hipSuccess;
   const long outs = p.act == kActSwiglu ? 2 * p.N : p.N;
-  if (!p.os && p.dtype == kF32) return launch_tiles<64, 64, 2, 2, true>(p, st);
-  if (p.os || ((p.M + 255) / 256) * ((outs + 255) / 256) >= kCus / 2) return launch_tiles<256, 256, 2, 2, false>(p, st);
-  return launch_tiles<64, 64, 2, 2, false>(p, st);
+  if (!p.os && p.dtype == kF32) return launch_tiles<64, 64, 2, 2, kOut32>(p, st);
+  if (p.os) return launch_tiles<256, 256, 2, 2, kOut8>(p, st);
+  if (((p.M + 255) / 256) * ((outs + 255) / 256) >= kCus / 2) return launch_tiles<256, 256, 2, 2, kOut16>(p, st);
+  return launch_tiles<64, 64, 2, 2, kOut16>(p, st);
 }
 
 }  // namespace ccq
