@@ -106,6 +106,27 @@ __device__ __forceinline__ bf16x8 widen(const i32x8& f, int c) {
   return o;
 }
 
+// stores that a step lets go on, in its first half alone or throughout
+template <int STORES, bool FIRST_HALF>
+struct Spare {
+  static constexpr int stores = STORES;
+  static constexpr bool first_half = FIRST_HALF;
+};
+
+// The kernel's arguments, read again where they are used: kept over the loop over tiles they and what follows from them
+// would not fit the scalar registers.
+typedef const __attribute__((address_space(4))) Fp8ProductArgs* ArgsAgain;
+__device__ __forceinline__ ArgsAgain args_again() {
+  ArgsAgain p = (ArgsAgain)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+// the same of a value that follows from the lane
+__device__ __forceinline__ int again(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 enum : int { kOut16 = 0, kOut32 = 1, kOut8 = 2 };  // bf16 or fp16 (dtype), fp32, e4m3 with scales
 
 // BM x BN tile of the product by WM x WN waves, two stages of both operands in LDS.  A lane of a wave holds, of each 16 x 16
@@ -131,55 +152,72 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
   __shared__ __attribute__((aligned(1024))) char smem[std::max(kRing, kOut)];
   const int tid = threadIdx.x, l = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN, r = l & 15, g = l >> 4;
-  // tile of this workgroup: each XCD (workgroups are handed out round-robin over the 8) takes consecutive tiles, in
-  // column order within bands of 8 tile rows, so that its L2 holds what its workgroups share
-  const int tm = (int)((p.M + BM - 1) / BM), tn = (int)((p.N + NT - 1) / NT), tiles = tm * tn;
-  const int xcd = blockIdx.x & 7, q8 = tiles >> 3, r8 = tiles & 7;
-  const int t = xcd * q8 + min(xcd, r8) + (blockIdx.x >> 3);
-  const int band = t / (8 * tn), in = t - band * 8 * tn, band_rows = min(8, tm - band * 8);
-  const long m0 = (long)(band * 8 + in % band_rows) * BM, n0 = (long)(in / band_rows) * NT;
   const int steps = (int)((p.K + kStep - 1) / kStep), tail = (int)(p.K & (kStep - 1)), whole = steps - (tail ? 1 : 0);
 
   // row of B in slot s: swiglu: the gates of a wave's columns, then their ups
   auto b_row = [&](int s) { return GLU ? s / (2 * HALF) * HALF + slot_row(s % HALF, GB) : slot_row(s, GB); };
   auto b_up = [&](int s) { return GLU && s % (2 * HALF) >= HALF; };
   const unsigned lds0 = lds_addr(smem), lds_scales = lds0 + 2 * kStage;
-  // Loads of half h of a step: 8 slots each; a wave's i-th one of A and of B begins at these slots.
-  auto slot_a = [&](int h, int i) { const int k = wave * PA + i; return k / (2 * HM) * (TM * 16) + h * (HM * 16) + k % (2 * HM) * 8; };
-  auto slot_b = [&](int h, int i) { const int k = wave * PB + i; return k / (2 * HN) * (TN * 16) + h * (HN * 16) + k % (2 * HN) * 8; };
-  auto piece = [&](int slot) { return (l & 7) ^ swz(slot + (l >> 3)); };
-  unsigned offa[2][PA], offb[2][PB];
-  const unsigned char* scales[PS];
+  // Loads of half h of a step take 8 slots each, a wave's i-th one those from first + 16 H h + 8 i on (H fragments of the
+  // operand's wave in a half).  A lane takes piece (l & 7) ^ swz of row l >> 3 of them; of the swizzle two forms occur, as the
+  // slot is 0 or 8 in 16.  The rows of a load lie at a distance from the first one's that no wave differs in.
+  const int first_a = wave * PA / (2 * HM) * (TM * 16) + wave * PA % (2 * HM) * 8;
+  const int first_b = wave * PB / (2 * HN) * (TN * 16) + wave * PB % (2 * HN) * 8;
+  constexpr int FA = std::min(PA, 2), FB = std::min(PB, 2);
+  int piece_a[FA], piece_b[FB];
+  unsigned lane_a[FA], lane_b[FB];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int i = 0; i < PA; ++i) {
-      const int s = slot_a(h, i), row = slot_row(s + (l >> 3), GA);
-      offa[h][i] = m0 + row < p.M ? (unsigned)(row * p.lda) + (piece(s) << 4) : kNowhere;
-    }
-#pragma unroll
-    for (int i = 0; i < PB; ++i) {  // (swiglu: half 0 holds gates, half 1 ups)
-      const int s = slot_b(h, i), row = b_row(s + (l >> 3));
-      offb[h][i] = n0 + row < p.N ? (unsigned)(row * p.ldb) + (piece(s) << 4) : kNowhere;
-    }
+  for (int i = 0; i < FA; ++i) {
+    piece_a[i] = 16 * ((l & 7) ^ swz(first_a + 8 * i + (l >> 3)));
+    lane_a[i] = (unsigned)((slot_row(first_a, GA) + GA * (l >> 3)) * p.lda) + piece_a[i];
   }
-  // scales: A's slots, then B's, 64 a load (of fewer than the waves have, some load the same ones)
+#pragma unroll
+  for (int i = 0; i < FB; ++i) {
+    piece_b[i] = 16 * ((l & 7) ^ swz(first_b + 8 * i + (l >> 3)));
+    lane_b[i] = (unsigned)((b_row(first_b) + GB * (l >> 3)) * p.ldb) + piece_b[i];
+  }
+  const unsigned lds_a = lds0 + first_a * 128, lds_b = lds0 + kA + first_b * 128;
   auto scale_slot = [&](int i) { return (wave * PS + i) % ((BM + BN) / 64) * 64; };
+  long m0, n0;  // the tile whose operands are loaded
+  size_t pa, pb;
+  unsigned enda, endb;  // bytes from there to the end of its last row
+  const size_t up = GLU ? p.N * p.ldb : 0;
+  const unsigned char* scales[PS];
+  // Tiles: each XCD (workgroups are handed out round-robin over the 8) takes consecutive ones, in column order within
+  // bands of 8 tile rows, so that its L2 holds what its workgroups share.  A workgroup takes every `stride`-th of its XCD's.
+  const int tiles = (int)((p.M + BM - 1) / BM) * (int)((p.N + NT - 1) / NT);
+  const int xcd = blockIdx.x & 7, mine = (tiles >> 3) + (xcd < (tiles & 7)), stride = (gridDim.x + 7) >> 3;
+  auto place = [&](int k) {
+    const ArgsAgain p = args_again();
+    const int l = again(tid & 63);
+    const int tm = (int)((p->M + BM - 1) / BM), tn = (int)((p->N + NT - 1) / NT), tiles = tm * tn, q8 = tiles >> 3, r8 = tiles & 7;
+    const int t = xcd * q8 + min(xcd, r8) + k;
+    const int band = t / (8 * tn), in = t - band * 8 * tn, band_rows = min(8, tm - band * 8);
+    m0 = (long)(band * 8 + in % band_rows) * BM;
+    n0 = (long)(in / band_rows) * NT;
+    pa = (size_t)p->a + m0 * p->lda;
+    pb = (size_t)p->b + n0 * p->ldb;
+    const long row = (p->K + 15) & ~15L;
+    enda = (unsigned)((min((long)BM, p->M - m0) - 1) * p->lda + row);
+    endb = (unsigned)((min((long)NT, p->N - n0) - 1) * p->ldb + row);
+    // scales: A's slots, then B's, 64 a load (of fewer than the waves have, some load the same ones)
 #pragma unroll
-  for (int i = 0; i < PS; ++i) {  // (rows behind the last one: the last one's)
-    const int s = scale_slot(i) + l;
-    if (s < BM) scales[i] = p.sa + min(m0 + slot_row(s, GA), p.M - 1) * p.lsa;
-    else scales[i] = p.sb + (min(n0 + b_row(s - BM), p.N - 1) + (b_up(s - BM) ? p.N : 0)) * p.lsb;
-  }
-  const size_t pa = (size_t)p.a + m0 * p.lda, pb = (size_t)p.b + n0 * p.ldb, up = GLU ? p.N * p.ldb : 0;
+    for (int i = 0; i < PS; ++i) {  // (rows behind the last one: the last one's)
+      const int s = scale_slot(i) + l;
+      if (s < BM) scales[i] = p->sa + min(m0 + slot_row(s, GA), p->M - 1) * p->lsa;
+      else scales[i] = p->sb + (min(n0 + b_row(s - BM), p->N - 1) + (b_up(s - BM) ? p->N : 0)) * p->lsb;
+    }
+  };
   auto load_scales = [&](int quad) {  // of steps 4 quad .. + 3
     if (quad * 4 >= steps) return;
 #pragma unroll
     for (int i = 0; i < PS; ++i)
       load4_to(lds_scales + (quad & 1) * kScales + scale_slot(i) * 4, scales[i] + 4 * quad);
   };
-  auto step_resource = [&](size_t base, int s) {  // (empty behind the last whole step)
-    return resource(base + (size_t)s * kStep, s < whole ? 0x7fffffffu : 0u);
+  // A buffer resource bounds every load by the end of the tile's last row; what lies behind comes as zeros, and all of it
+  // behind the last whole step.
+  auto step_resource = [&](size_t base, unsigned end, int s) {
+    return resource(base + (size_t)s * kStep, s < whole ? end - s * kStep : 0u);
   };
 
   // fragment addresses of this lane in stage 0, and of its scales
@@ -201,14 +239,6 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     f.e = *(lds_byte*)(size_t)(e0 + scale + i * 64);
   };
   f32x4 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (!EXACT) accumulator(acc[i][j]);
-    }
-  acc_settled();
   auto product = [&](const Frag& a, const Frag& b, f32x4& c) {
     if constexpr (!EXACT) {
       product128(b.v, b.e, a.v, a.e, c);
@@ -235,81 +265,120 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     }
   };
   constexpr int Q = HM * HN, PL = PA + PB;
-  // the loads of half h of the step whose resources are given, one at a time
-  auto load = [&](int h, int k, unsigned stage, const u32x4& ra, const u32x4& rb) {
-    if (k < PA) {
-      load_to(lds0 + stage + slot_a(h, k) * 128, 0);
-      asm volatile("s_nop 0");
-      load_from(ra, offa[h][k < PA ? k : 0]);
-    } else {
-      load_to(lds0 + stage + kA + slot_b(h, k - PA) * 128, 0);
-      asm volatile("s_nop 0");
-      load_from(rb, offb[h][k < PA ? 0 : k - PA]);
-    }
+  // a load of half h of the step whose resource is given, where the lane is `on` (zeros elsewhere)
+  auto load_a = [&](int h, int i, unsigned stage, const u32x4& ra, bool on) {
+    load_to(lds_a + stage, (h * HM * 16 + 8 * i) / 8);
+    const unsigned off = lane_a[i % FA] + (unsigned)(slot_row(h * HM * 16 + 8 * i, GA) * p.lda);
+    asm volatile("s_nop 0");
+    load_from(ra, on ? off : kNowhere);
+  };
+  auto load_b = [&](int h, int i, unsigned stage, const u32x4& rb, bool on) {  // (swiglu: half 0 holds gates, half 1 ups)
+    load_to(lds_b + stage, (h * HN * 16 + 8 * i) / 8);
+    const unsigned off = lane_b[i % FB] + (unsigned)(b_row(h * HN * 16 + 8 * i) * p.ldb);
+    asm volatile("s_nop 0");
+    load_from(rb, on ? off : kNowhere);
   };
   auto spread = [&](int q, int n, auto&& f) {  // f(0) .. f(n - 1) over the first three quarters of Q products
 #pragma unroll
     for (int k = 0; k < n; ++k)
       if (q == k * Q * 3 / 4 / n) f(k);
   };
-  auto step = [&](int s, Frag (&x0)[HN], Frag (&x1)[HN]) {  // x0: this step's B0; x1: its B1, then the next step's B0
+  // (spare: the last tile's stores may be on their way behind the loads)
+  auto step = [&](auto spare, int s, Frag (&x0)[HN], Frag (&x1)[HN]) {  // x0: this step's B0; x1: its B1, then the next step's B0
     const unsigned stage = (s & 1) * kStage, next = kStage - stage;
     const unsigned scale = (s >> 2 & 1) * kScales + (s & 3), scale_next = ((s + 1) >> 2 & 1) * kScales + ((s + 1) & 3);
-    wait_loads<2 * PL>();
+    constexpr int kWait = 2 * PL + decltype(spare)::stores;
+    wait_loads<kWait>();
     lds_barrier();
     if ((s & 3) == 0) load_scales((s >> 2) + 1);
-    u32x4 ra = step_resource(pa, s + 2), rb = step_resource(pb, s + 2);
+    u32x4 ra = step_resource(pa, enda, s + 2), rb = step_resource(pb, endb, s + 2);
     settled(ra);
     settled(rb);
     quarter(0, 0, a0, x0, [&](int q) {
       spread(q, HN, [&](int k) { read(x1[k], fb, eb0, HN + k, stage, scale); });
-      spread(q, PA, [&](int k) { load(0, k, stage, ra, rb); });
+      spread(q, PA, [&](int k) { load_a(0, k, stage, ra, true); });
     });
     quarter(0, 1, a0, x1, [&](int q) {
       spread(q, HM, [&](int k) { read(a1[k], fa, ea0, HM + k, stage, scale); });
-      spread(q, PB, [&](int k) { load(0, PA + k, stage, ra, rb); });
+      spread(q, PB, [&](int k) { load_b(0, k, stage, rb, true); });
     });
-    wait_loads<2 * PL>();
+    wait_loads<decltype(spare)::first_half ? 2 * PL : kWait>();
     lds_barrier();
     if (GLU) {
-      rb = step_resource(pb + up, s + 2);
+      rb = step_resource(pb + up, endb, s + 2);
       settled(rb);
     }
     quarter(1, 1, a1, x1, [&](int q) {
       spread(q, HM, [&](int k) { read(a0[k], fa, ea0, k, next, scale_next); });
-      spread(q, PA, [&](int k) { load(1, k, stage, ra, rb); });
+      spread(q, PA, [&](int k) { load_a(1, k, stage, ra, true); });
     });
     quarter(1, 0, a1, x0, [&](int q) {
       spread(q, HN, [&](int k) { read(x1[k], fb, eb0, k, next, scale_next); });
-      spread(q, PB, [&](int k) { load(1, PA + k, stage, ra, rb); });
+      spread(q, PB, [&](int k) { load_b(1, k, stage, rb, true); });
     });
   };
   auto load_step = [&](int s) {  // all of a whole step
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      u32x4 ra = step_resource(pa, s), rb = step_resource(pb + h * up, s);
+      u32x4 ra = step_resource(pa, enda, s), rb = step_resource(pb + h * up, endb, s);
       settled(ra);
       settled(rb);
 #pragma unroll
-      for (int k = 0; k < PL; ++k) load(h, k, s * kStage, ra, rb);
+      for (int k = 0; k < PL; ++k)
+        if (k < PA) load_a(h, k, s * kStage, ra, true);
+        else load_b(h, k - PA, s * kStage, rb, true);
     }
   };
-  load_scales(0);
-  if (whole > 0) {
+  // Stores of a whole tile, at the least: they follow the next tile's first loads, and go on while its first steps run.
+  constexpr int W = 4 * GB, JG = TN / GB / (GLU ? 2 : 1), COLS = GLU ? HALF : TN * 16;
+  constexpr int kStores = TM * JG * W * (OUT == kOut8 ? 1 : OUT == kOut32 ? 4 : 2) / 16;
+  static_assert(3 * PL + kStores < 64, "operations that a wait can count");
+  auto begin = [&] {
+    load_scales(0);
+    if (whole == 0) return;
     load_step(0);
     load_step(1);
-    wait_loads<3 * PL>();
-    lds_barrier();
+  };
+  place(blockIdx.x >> 3);
+  begin();
+  bool counted = false;  // kStores stores or more follow the loads
+  for (int k = blockIdx.x >> 3; k < mine; k += stride) {
+  {  // the sums begin with the bias
+    const ArgsAgain p = args_again();
+    const long nb = n0 + wn * COLS + (again(tid & 63) >> 4) * W;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      f32x4 b{0.f, 0.f, 0.f, 0.f};
+      if (p->bias)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const long n = nb + j / GB % JG * 16 * GB + q * GB + j % GB;
+          if (n < p->N) b[q] = bias_at(p->bias, p->bdtype, (j / GB >= JG ? p->N : 0) + n);
+        }
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        acc[i][j] = b;
+        if (!EXACT) accumulator(acc[i][j]);
+      }
+    }
+  }
+  acc_settled();
+  if (counted) wait_loads<3 * PL + kStores>();
+  else wait_loads<0>();
+  lds_barrier();
+  if (whole > 0) {
 #pragma unroll
     for (int i = 0; i < HM; ++i) read(a0[i], fa, ea0, i, 0, 0);
 #pragma unroll
     for (int j = 0; j < HN; ++j) read(b0[j], fb, eb0, j, 0, 0);
-    int s = 0;
+    step(Spare<kStores, false>{}, 0, b0, b1);
+    if (whole > 1) step(Spare<kStores, true>{}, 1, b1, b0);
+    int s = 2;
     for (; s + 2 <= whole; s += 2) {
-      step(s, b0, b1);
-      step(s + 1, b1, b0);
+      step(Spare<0, true>{}, s, b0, b1);
+      step(Spare<0, true>{}, s + 1, b1, b0);
     }
-    if (s < whole) step(s, b0, b1);
+    if (s < whole) step(Spare<0, true>{}, s, b0, b1);
     wait_loads<0>();
     lds_barrier();
   }
@@ -317,17 +386,14 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     const unsigned stage = (whole & 1) * kStage, scale = (whole >> 2 & 1) * kScales + (whole & 3);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      u32x4 ra = resource(pa + (size_t)whole * kStep, 0x7fffffffu), rb = resource(pb + h * up + (size_t)whole * kStep, 0x7fffffffu);
+      const size_t at = (size_t)whole * kStep;
+      u32x4 ra = resource(pa + at, enda - (unsigned)at), rb = resource(pb + h * up + at, endb - (unsigned)at);
       settled(ra);
       settled(rb);
 #pragma unroll
-      for (int k = 0; k < PL; ++k) {
-        const bool of_a = k < PA;
-        const int slot = of_a ? slot_a(h, k) : slot_b(h, k - PA);
-        load_to(lds0 + stage + (of_a ? 0 : kA) + slot * 128, 0);
-        asm volatile("s_nop 0");
-        load_from(of_a ? ra : rb, piece(slot) * 16 < tail ? (of_a ? offa[h][of_a ? k : 0] : offb[h][of_a ? 0 : k - PA]) : kNowhere);
-      }
+      for (int k = 0; k < PL; ++k)
+        if (k < PA) load_a(h, k, stage, ra, piece_a[k % FA] < tail);
+        else load_b(h, k - PA, stage, rb, piece_b[(k - PA) % FB] < tail);
     }
     wait_loads<0>();
     lds_barrier();
@@ -353,29 +419,32 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
 #pragma unroll
       for (int j = 0; j < TN; ++j) product(a, b[j], acc[i][j]);
     }
+    lds_barrier();
   }
 
   acc_settled();
+  const ArgsAgain p = args_again();
+  const int tid = again(threadIdx.x), l = tid & 63, r = l & 15, g = l >> 4;
+  const long cm = m0, cn = n0;  // this tile, while the next one's operands are loaded
+  const bool direct = ACT != kActOther && cn + NT <= p->N, more = k + stride < mine;
+  if (direct && more) {
+    place(k + stride);
+    begin();
+  }
+  counted = direct && cm + BM <= p->M;
   // Tiles that end within the columns: straight from the accumulators.  A lane holds, of each of its rows, W consecutive
-  // columns of each group.
-  constexpr int W = 4 * GB, JG = TN / GB / (GLU ? 2 : 1), COLS = GLU ? HALF : TN * 16;
+  // columns of each group->
   if constexpr (ACT != kActOther) {
-    if (n0 + NT <= p.N) {
-      const long nw = n0 + wn * COLS + g * W;
-      auto row_of = [&](int i) { return m0 + wm * TM * 16 + slot_row(i * 16 + r, GA); };
-      float bias[TN / GB][W];
-#pragma unroll
-      for (int j = 0; j < TN / GB; ++j)
-#pragma unroll
-        for (int e = 0; e < W; ++e)
-          bias[j][e] = p.bias ? bias_at(p.bias, p.bdtype, (j >= JG ? p.N : 0) + nw + j % JG * 16 * GB + e) : 0.f;
+    if (direct) {
+      const long nw = cn + wn * COLS + g * W;
+      auto row_of = [&](int i) { return cm + wm * TM * 16 + slot_row(i * 16 + r, GA); };
       auto values = [&](int i, int j, float (&v)[W]) {
 #pragma unroll
         for (int e = 0; e < W; ++e) {
-          v[e] = value_of<!EXACT>(acc[i][j * GB + e % GB][e / GB]) + bias[j][e];
+          v[e] = value_of<!EXACT>(acc[i][j * GB + e % GB][e / GB]);
           if (GLU) {
             constexpr int U = GLU ? JG : 0;
-            v[e] = v[e] * sigmoid(v[e]) * (value_of<!EXACT>(acc[i][(j + U) * GB + e % GB][e / GB]) + bias[j + U][e]);
+            v[e] = v[e] * sigmoid(v[e]) * value_of<!EXACT>(acc[i][(j + U) * GB + e % GB][e / GB]);
           }
         }
       };
@@ -394,16 +463,16 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
         auto emit = [&](int i, const float (&v)[JG][W], unsigned most) {
           const unsigned byte = scale_byte(most);
           const long m = row_of(i);
-          if (m >= p.M) return;
+          if (m >= p->M) return;
 #pragma unroll
           for (int j = 0; j < JG; ++j) {
             typedef unsigned words __attribute__((ext_vector_type(W / 4)));
             words o;
 #pragma unroll
             for (int e = 0; e < W / 4; ++e) o[e] = fp8_word(v[j][4 * e], v[j][4 * e + 1], v[j][4 * e + 2], v[j][4 * e + 3], byte);
-            *gmem((words*)((unsigned char*)p.out + m * p.ldo + nw + j * 16 * GB)) = o;
+            *gmem((words*)((unsigned char*)p->out + m * p->ldo + nw + j * 16 * GB)) = o;
           }
-          if (g == 0 && (!GLU || (wn & 1) == 0)) p.os[m * p.los + (n0 + wn * COLS) / kFp8Block] = (unsigned char)byte;
+          if (g == 0 && (!GLU || (wn & 1) == 0)) p->os[m * p->los + (cn + wn * COLS) / kFp8Block] = (unsigned char)byte;
         };
         if constexpr (!GLU) {
 #pragma unroll
@@ -434,36 +503,36 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
         auto emit = [&](auto type) {
           typedef decltype(type) T;
           RowPiece<T, W> res[TM][JG];
-          if (p.res)
+          if (p->res)
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
               for (int j = 0; j < JG; ++j)
-                if (row_of(i) < p.M) res[i][j].v = *gmem((const typename RowPiece<T, W>::any*)((const T*)p.res + row_of(i) * p.ldr + nw + j * 16 * GB));
+                if (row_of(i) < p->M) res[i][j].v = *gmem((const typename RowPiece<T, W>::any*)((const T*)p->res + row_of(i) * p->ldr + nw + j * 16 * GB));
 #pragma unroll
           for (int i = 0; i < TM; ++i) {
             const long m = row_of(i);
-            if (m >= p.M) continue;
+            if (m >= p->M) continue;
 #pragma unroll
             for (int j = 0; j < JG; ++j) {
               float v[W];
               values(i, j, v);
-              if (p.res)
+              if (p->res)
 #pragma unroll
                 for (int e = 0; e < W; ++e) v[e] += (float)res[i][j].v[e];
               typename RowPiece<T, W>::vec o;
 #pragma unroll
               for (int e = 0; e < W; ++e) o[e] = (T)v[e];
-              *gmem((typename RowPiece<T, W>::any*)((T*)p.out + m * p.ldo + nw + j * 16 * GB)) = o;
+              *gmem((typename RowPiece<T, W>::any*)((T*)p->out + m * p->ldo + nw + j * 16 * GB)) = o;
               __builtin_amdgcn_sched_barrier(0);
             }
           }
         };
         if constexpr (OUT == kOut32) emit(0.f);
-        else if (p.dtype == kBf16) emit((bf16)0.f);
+        else if (p->dtype == kBf16) emit((bf16)0.f);
         else emit((f16)0.f);
       }
-      return;
+      continue;
     }
   }
 
@@ -471,13 +540,7 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
   float* tile = (float*)smem;
   constexpr int PR = NT / 8, RP = NW * 64 / PR, NG = 4;  // threads of a row, rows at a time, how often before the next loads
   const int c = tid % PR * 8, cw = c / (GLU ? HALF : NT), cs = GLU ? cw * 2 * HALF + c % HALF : c;
-  const long n = n0 + c;
-  float bias[8], bias_up[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    bias[i] = p.bias && n + i < p.N ? bias_at(p.bias, p.bdtype, n + i) : 0.f;
-    bias_up[i] = GLU && p.bias && n + i < p.N ? bias_at(p.bias, p.bdtype, p.N + n + i) : 0.f;
-  }
+  const long n = cn + c;
   auto through = [&](auto type, int h) {
     typedef decltype(type) T;
     for (int i0 = tid / PR; i0 < WM * kPass; i0 += NG * RP) {
@@ -486,42 +549,42 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         const int i = i0 + k * RP;
-        m[k] = i < WM * kPass ? m0 + i / kPass * (TM * 16) + slot_row(h * kPass + i % kPass, GA) : p.M;
-        if (p.res && m[k] < p.M && n < p.N) res[k].load((const T*)p.res + m[k] * p.ldr, n, p.N);
+        m[k] = i < WM * kPass ? cm + i / kPass * (TM * 16) + slot_row(h * kPass + i % kPass, GA) : p->M;
+        if (p->res && m[k] < p->M && n < p->N) res[k].load((const T*)p->res + m[k] * p->ldr, n, p->N);
       }
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         const int i = i0 + k * RP;
-        if (m[k] >= p.M || (n >= p.N && OUT != kOut8)) continue;
+        if (m[k] >= p->M || (n >= p->N && OUT != kOut8)) continue;
         float v[8], up[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          v[e] = tile[i * kPitch + cs + e] + bias[e];
-          if (GLU) up[e] = tile[i * kPitch + cs + HALF + e] + bias_up[e];
+          v[e] = tile[i * kPitch + cs + e];
+          if (GLU) up[e] = tile[i * kPitch + cs + HALF + e];
         }
         if (GLU) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = v[e] * sigmoid(v[e]) * up[e];
         } else if (ACT != kActNone) {
-          act_values<8>(p.act, v);
+          act_values<8>(p->act, v);
         }
         if constexpr (OUT == kOut8) {  // a row's 16 lanes of a block go together
           unsigned most = 0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            if (n + e >= p.N) v[e] = 0.f;
+            if (n + e >= p->N) v[e] = 0.f;
             most = max(most, magnitude(v[e]));
           }
           const unsigned byte = scale_byte(lanes_max(most, 16));
-          if (n >= p.N) continue;
-          *gmem((u32x2*)((unsigned char*)p.out + m[k] * p.ldo + n)) =
+          if (n >= p->N) continue;
+          *gmem((u32x2*)((unsigned char*)p->out + m[k] * p->ldo + n)) =
               u32x2{fp8_word(v[0], v[1], v[2], v[3], byte), fp8_word(v[4], v[5], v[6], v[7], byte)};
-          if ((tid & 15) == 0) p.os[m[k] * p.los + n / kFp8Block] = (unsigned char)byte;
+          if ((tid & 15) == 0) p->os[m[k] * p->los + n / kFp8Block] = (unsigned char)byte;
         } else {
-          if (p.res)
+          if (p->res)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += (float)res[k].v[e];
-          store_row<T, 8>((T*)p.out + m[k] * p.ldo, n, p.N, v);
+          store_row<T, 8>((T*)p->out + m[k] * p->ldo, n, p->N, v);
         }
       }
     }
@@ -541,25 +604,33 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
                 value_of<!EXACT>(acc[h * (kPass / 16) + i][j + k][q]);
     __syncthreads();
     if constexpr (OUT == kOut16) {
-      if (p.dtype == kBf16) through((bf16)0.f, h);
+      if (p->dtype == kBf16) through((bf16)0.f, h);
       else through((f16)0.f, h);
     } else {
       through(0.f, h);
     }
   }
+  if (more) {
+    lds_barrier();
+    place(k + stride);
+    begin();
+  }
+  }
 }
+
+constexpr int kCus = 256;
 
 template <int BM, int BN, int WM, int WN, int OUT>
 hipError_t launch_tiles(const Fp8ProductArgs& p, hipStream_t st) {
   const int NT = p.act == kActSwiglu ? BN / 2 : BN;
-  const dim3 grid((unsigned)(((p.M + BM - 1) / BM) * ((p.N + NT - 1) / NT))), block(WM * WN * 64);
+  const long tiles = ((p.M + BM - 1) / BM) * ((p.N + NT - 1) / NT);
+  const dim3 grid((unsigned)(BM == 256 ? std::min<long>(tiles, kCus) : tiles)), block(WM * WN * 64);
   if (p.act == kActSwiglu) hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActSwiglu, OUT>), grid, block, 0, st, p);
   else if (p.act == kActNone) hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActNone, OUT>), grid, block, 0, st, p);
   else hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActOther, OUT>), grid, block, 0, st, p);
   return hipGetLastError();
 }
 
-constexpr int kCus = 256;
 
 }  // namespace
 

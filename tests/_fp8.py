@@ -113,17 +113,18 @@ def linear64(x, w, bias=None, act=None, residual=None, exact=False):
 
     Products of two e4m3 are exact in fp32.  exact (an output in fp32): a block's 128 products are added in fp32, then the
     blocks: at most 128 + K / 128 roundings, each 2^-24 of the magnitudes' sum.  Otherwise what the 8-bit instruction cuts
-    off, and the fp32 additions of its eights and of the blocks.  Bias and residual round once more each, an activation within
-    8 roundings of its argument and result (exponential, reciprocal, products; the error function within 4e-7)."""
+    off, and the fp32 additions of its eights and of the blocks.  A residual rounds once more, an
+    activation within 8 roundings of its argument and result (exponential, reciprocal, products; the error function within
+    4e-7)."""
     a, b = meant(*x), meant(*w)
     K = a.shape[-1]
     z, size = a @ b.T, a.abs() @ b.abs().T
+    if bias is not None:  # the sums begin with it
+        z = z + bias.cpu().double()
+        size = size + bias.cpu().double().abs()
     err = ((128 if exact else 16) + K / 128) * 2.0 ** -24 * size
     if not exact:
         err = err + cut_off(x, w)
-    if bias is not None:
-        z = z + bias.cpu().double()
-        err = err + 2.0 ** -24 * (z.abs() + size)
     if act == "swiglu":
         n = z.shape[-1] // 2
         y, slope = act64("silu", z[:, :n])
