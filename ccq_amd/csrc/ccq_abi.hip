@@ -36,7 +36,8 @@ hipError_t launch_logprobs(bool bwd, const LogprobArgs& a, hipStream_t st);
 void product_plan(long M, long N, long K, int* side, int* splits);
 hipError_t launch_product(int kind, const ProductArgs& p, hipStream_t st);
 hipError_t launch_quantize(const QuantizeArgs& a, hipStream_t st);
-hipError_t launch_fp8_product(const Fp8ProductArgs& p, hipStream_t st);
+long fp8_product_workspace(long M, long N, long K, int act, int dtype, bool into8);
+hipError_t launch_fp8_product(const Fp8ProductArgs& p, float* workspace, hipStream_t st);
 int act_bwd_row_blocks(long M, long N);
 hipError_t launch_act_bwd(const ActBwdArgs& a, hipStream_t st);
 hipError_t launch_pad_rows(const PadRowsArgs& a, hipStream_t st);
@@ -1830,9 +1831,13 @@ int ccq_norm_fp8_fwd(const void* x, int64_t ldx, const void* r, int64_t ldr, con
   return hip_status(timed("norm_fp8", st, [&] { return launch_norm_fwd(a, st); }), who);
 }
 
+size_t ccq_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, int dtype, int into8) {
+  return M > 0 && N > 0 && K > 0 ? (size_t)fp8_product_workspace(M, N, K, act, dtype, into8 != 0) * sizeof(float) : 0;
+}
+
 int ccq_fp8_linear(const void* x, int64_t ldx, const void* xs, int64_t ldxs, const void* weight, int64_t ldw,
                    const void* ws, int64_t ldws, const void* bias, int bdtype, const void* r, int64_t ldr, void* y,
-                   int64_t ldy, void* ys, int64_t ldys, int64_t M, int64_t N, int64_t K, int act, int dtype, void* stream) {
+                   int64_t ldy, void* ys, int64_t ldys, void* workspace, int64_t M, int64_t N, int64_t K, int act, int dtype, void* stream) {
   const char* who = "ccq_fp8_linear";
   if (M < 0 || N < 1 || K < 1 || M > kMaxSide || N > kMaxSide || linear_outs(N, act) > kMaxStride || K > kMaxStride ||
       ((M + 63) / 64) * ((linear_outs(N, act) + 63) / 64) > kMaxTiles)
@@ -1845,9 +1850,11 @@ int ccq_fp8_linear(const void* x, int64_t ldx, const void* xs, int64_t ldxs, con
   if (ys)
     if (int e = fp8_rows_check(who, "y", y, ldy, ys, ldys, N)) return e;
   if (M == 0) return CCQ_OK;
-  if (!x || !xs || !weight || !ws || !y) return fail(CCQ_ERR_NULL, "%s: x, xs, weight, ws and y are required", who);
+  if (!x || !xs || !weight || !ws || !y || (!workspace && fp8_product_workspace(M, N, K, act, dtype, ys != nullptr)))
+    return fail(CCQ_ERR_NULL, "%s: x, xs, weight, ws, y and the workspace are required", who);
   if ((!ys && !element_aligned(y, dtype)) || !element_aligned(r, dtype) || !element_aligned(bias, bdtype))
     return fail(CCQ_ERR_ALIGN, "%s: y, r and bias must be aligned to their elements", who);
+  if (!aligned16(workspace)) return fail(CCQ_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", who);
   if (int e = check_stream_device(stream, who)) return e;
   Fp8ProductArgs p{};
   p.a = (const unsigned char*)x; p.lda = ldx; p.sa = (const unsigned char*)xs; p.lsa = ldxs;
@@ -1855,7 +1862,7 @@ int ccq_fp8_linear(const void* x, int64_t ldx, const void* xs, int64_t ldxs, con
   p.M = M; p.N = N; p.K = K; p.out = y; p.ldo = ys ? ldy : N; p.os = (unsigned char*)ys; p.los = ldys;
   p.bias = bias; p.bdtype = bdtype; p.res = r; p.ldr = ldr; p.act = act; p.dtype = dtype;
   hipStream_t st = (hipStream_t)stream;
-  return hip_status(timed("linear_fp8", st, [&] { return launch_fp8_product(p, st); }), who);
+  return hip_status(timed("linear_fp8", st, [&] { return launch_fp8_product(p, (float*)workspace, st); }), who);
 }
 
 }  // extern "C"

@@ -106,6 +106,18 @@ __device__ __forceinline__ bf16x8 widen(const i32x8& f, int c) {
   return o;
 }
 
+// c += a b 2^(ea + eb - 254), exactly but for fp32's additions; lane l holds the scales of rows l & 15 of both
+__device__ __forceinline__ void exact_product(const i32x8& a, int ea, const i32x8& b, int eb, f32x4& c) {
+  f32x4 sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) sum = mfma16(widen(a, k), widen(b, k), sum);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {  // (row 4 g + q of the result: its scale lies in lane 4 g + q)
+    const int y = __shfl(ea, 4 * (lane_id() >> 4) + q);
+    c[q] += eb == (int)kFp8Nan || y == (int)kFp8Nan ? NAN : __builtin_ldexpf(sum[q], eb + y - 254);
+  }
+}
+
 // stores that a step lets go on, in its first half alone or throughout
 template <int STORES, bool FIRST_HALF>
 struct Spare {
@@ -127,7 +139,8 @@ __device__ __forceinline__ int again(int x) {
   return x;
 }
 
-enum : int { kOut16 = 0, kOut32 = 1, kOut8 = 2 };  // bf16 or fp16 (dtype), fp32, e4m3 with scales
+// bf16 or fp16 (dtype; of tiles below 256 fp32 too, of 8-bit products, for a workspace); fp32 exactly; e4m3 with scales
+enum : int { kOut16 = 0, kOut32 = 1, kOut8 = 2 };
 
 // BM x BN tile of the product by WM x WN waves, two stages of both operands in LDS.  A lane of a wave holds, of each 16 x 16
 // tile (i, j), row r = l & 15 of A's fragment and the columns 4 (l >> 4) .. + 3 of B's.
@@ -239,54 +252,101 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     f.e = *(lds_byte*)(size_t)(e0 + scale + i * 64);
   };
   f32x4 acc[TM][TN];
-  auto product = [&](const Frag& a, const Frag& b, f32x4& c) {
-    if constexpr (!EXACT) {
-      product128(b.v, b.e, a.v, a.e, c);
-    } else {
-      f32x4 sum{0.f, 0.f, 0.f, 0.f};
+  // Exactly: the columns' scales of a fragment of B, those of 4 g + q (with the byte of the step in their words)
+  struct ColumnScales {
+    i32x4 word;
+  };
+  constexpr int kScaleSets = EXACT ? TN : 1;
+  auto read_columns = [&](ColumnScales (&c)[kScaleSets], unsigned scale) {
+    if constexpr (EXACT) {
+      typedef __attribute__((address_space(3))) const i32x4 lds_words;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum = mfma16(widen(b.v, k), widen(a.v, k), sum);
+      for (int j = 0; j < TN; ++j) {
+        c[j].word = *(lds_words*)(size_t)(lds_scales + (BM + (wn * TN + j) * 16 + 4 * g) * 4 + (scale & ~3u));
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {  // the scale of column 4 g + q lies in lane 4 g + q
-        const int y = __shfl(b.e, 4 * g + q);
-        c[q] += a.e == (int)kFp8Nan || y == (int)kFp8Nan ? NAN : __builtin_ldexpf(sum[q], a.e + y - 254);
+        for (int q = 0; q < 4; ++q) c[j].word[q] = c[j].word[q] >> (8 * (scale & 3)) & 0xff;
       }
+    }
+  };
+  bool nan_row[EXACT ? TM : 1], nan_column[kScaleSets][4];  // a scale that is NaN was met
+  // all products of a step, exactly
+  auto multiply = [&](const Frag (&a)[TM], const Frag (&b)[TN], const ColumnScales (&c)[kScaleSets]) {
+    if constexpr (EXACT) {
+      bf16x8 wide[TN][4];
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) wide[j][k] = widen(b[j].v, k);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        bf16x8 row[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) row[k] = widen(a[i].v, k);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          f32x4 sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sum = mfma16(wide[j][k], row[k], sum);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[i][j][q] += __builtin_ldexpf(sum[q], a[i].e + c[j].word[q] - 254);
+        }
+        nan_row[i] |= a[i].e == (int)kFp8Nan;
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) nan_column[j][q] |= c[j].word[q] == (int)kFp8Nan;
     }
   };
 
   Frag a0[HM], a1[HM], b0[HN], b1[HN];
   // a quarter of the products, with `reads` between them; f(k) for each k < n, spread over the quarter
-  auto quarter = [&](int ih, int jh, const Frag (&a)[HM], const Frag (&b)[HN], auto&& between) {
+  auto quarter = [&](int ih, int jh, const Frag (&a)[HM], const Frag (&b)[HN], auto&& before, auto&& between) {
 #pragma unroll
     for (int q = 0; q < HM * HN; ++q) {
-      product(a[q / HN], b[q % HN], acc[ih * HM + q / HN][jh * HN + q % HN]);
+      before(q);
+      product128(b[q % HN].v, b[q % HN].e, a[q / HN].v, a[q / HN].e, acc[ih * HM + q / HN][jh * HN + q % HN]);
       between(q);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
   constexpr int Q = HM * HN, PL = PA + PB;
-  // a load of half h of the step whose resource is given, where the lane is `on` (zeros elsewhere)
-  auto load_a = [&](int h, int i, unsigned stage, const u32x4& ra, bool on) {
-    load_to(lds_a + stage, (h * HM * 16 + 8 * i) / 8);
-    const unsigned off = lane_a[i % FA] + (unsigned)(slot_row(h * HM * 16 + 8 * i, GA) * p.lda);
-    asm volatile("s_nop 0");
-    load_from(ra, on ? off : kNowhere);
+  // A load of half h of a step in two parts, since M0 is read one wait state after it is written: between them stands a
+  // product, or a wait.  (swiglu: half 0 of B holds gates, half 1 ups)
+  auto to_a = [&](int h, int i, unsigned stage) { load_to(lds_a + stage, (h * HM * 16 + 8 * i) / 8); };
+  auto to_b = [&](int h, int i, unsigned stage) { load_to(lds_b + stage, (h * HN * 16 + 8 * i) / 8); };
+  auto off_a = [&](int h, int i) { return lane_a[i % FA] + (unsigned)(slot_row(h * HM * 16 + 8 * i, GA) * p.lda); };
+  auto off_b = [&](int h, int i) { return lane_b[i % FB] + (unsigned)(b_row(h * HN * 16 + 8 * i) * p.ldb); };
+  auto load_half = [&](int h, unsigned stage, const u32x4& ra, const u32x4& rb, int left) {  // zeros from `left` on
+#pragma unroll
+    for (int k = 0; k < PL; ++k) {
+      const int i = k < PA ? k : k - PA;
+      if (k < PA) to_a(h, i, stage);
+      else to_b(h, i, stage);
+      const unsigned off = k < PA ? off_a(h, i) : off_b(h, i);
+      const bool on = (k < PA ? piece_a[i % FA] : piece_b[i % FB]) < left;
+      asm volatile("s_nop 0");
+      load_from(k < PA ? ra : rb, on ? off : kNowhere);
+    }
   };
-  auto load_b = [&](int h, int i, unsigned stage, const u32x4& rb, bool on) {  // (swiglu: half 0 holds gates, half 1 ups)
-    load_to(lds_b + stage, (h * HN * 16 + 8 * i) / 8);
-    const unsigned off = lane_b[i % FB] + (unsigned)(b_row(h * HN * 16 + 8 * i) * p.ldb);
-    asm volatile("s_nop 0");
-    load_from(rb, on ? off : kNowhere);
-  };
-  auto spread = [&](int q, int n, auto&& f) {  // f(0) .. f(n - 1) over the first three quarters of Q products
+  // Between which of a quarter's products its n reads and its n loads stand: f(k) for the k-th one (where exactly matters
+  // little; with the loads beside the reads 8192^3 took 2 to 3 % longer).
+  auto reads = [&](int q, int n, auto&& f) {
 #pragma unroll
     for (int k = 0; k < n; ++k)
       if (q == k * Q * 3 / 4 / n) f(k);
   };
+  static_assert(PA == PB && (PA == 1 || (PA - 2) * Q / PA + 2 < Q - 1), "one load between two products");
+  auto loads = [&](int q, int n, auto&& f) {
+#pragma unroll
+    for (int k = 0; k < n; ++k)
+      if (q == std::min(k * Q / n + 2, Q - 1)) f(k);
+  };
+  auto scale_at = [&](int s) { return (s >> 2 & 1) * kScales + (s & 3); };
   // (spare: the last tile's stores may be on their way behind the loads)
   auto step = [&](auto spare, int s, Frag (&x0)[HN], Frag (&x1)[HN]) {  // x0: this step's B0; x1: its B1, then the next step's B0
     const unsigned stage = (s & 1) * kStage, next = kStage - stage;
-    const unsigned scale = (s >> 2 & 1) * kScales + (s & 3), scale_next = ((s + 1) >> 2 & 1) * kScales + ((s + 1) & 3);
+    const unsigned scale = scale_at(s), scale_next = scale_at(s + 1);
     constexpr int kWait = 2 * PL + decltype(spare)::stores;
     wait_loads<kWait>();
     lds_barrier();
@@ -295,12 +355,16 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     settled(ra);
     settled(rb);
     quarter(0, 0, a0, x0, [&](int q) {
-      spread(q, HN, [&](int k) { read(x1[k], fb, eb0, HN + k, stage, scale); });
-      spread(q, PA, [&](int k) { load_a(0, k, stage, ra, true); });
+      loads(q, PA, [&](int k) { to_a(0, k, stage); });
+    }, [&](int q) {
+      reads(q, HN, [&](int k) { read(x1[k], fb, eb0, HN + k, stage, scale); });
+      loads(q, PA, [&](int k) { load_from(ra, off_a(0, k)); });
     });
     quarter(0, 1, a0, x1, [&](int q) {
-      spread(q, HM, [&](int k) { read(a1[k], fa, ea0, HM + k, stage, scale); });
-      spread(q, PB, [&](int k) { load_b(0, k, stage, rb, true); });
+      loads(q, PB, [&](int k) { to_b(0, k, stage); });
+    }, [&](int q) {
+      reads(q, HM, [&](int k) { read(a1[k], fa, ea0, HM + k, stage, scale); });
+      loads(q, PB, [&](int k) { load_from(rb, off_b(0, k)); });
     });
     wait_loads<decltype(spare)::first_half ? 2 * PL : kWait>();
     lds_barrier();
@@ -309,12 +373,16 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
       settled(rb);
     }
     quarter(1, 1, a1, x1, [&](int q) {
-      spread(q, HM, [&](int k) { read(a0[k], fa, ea0, k, next, scale_next); });
-      spread(q, PA, [&](int k) { load_a(1, k, stage, ra, true); });
+      loads(q, PA, [&](int k) { to_a(1, k, stage); });
+    }, [&](int q) {
+      reads(q, HM, [&](int k) { read(a0[k], fa, ea0, k, next, scale_next); });
+      loads(q, PA, [&](int k) { load_from(ra, off_a(1, k)); });
     });
     quarter(1, 0, a1, x0, [&](int q) {
-      spread(q, HN, [&](int k) { read(x1[k], fb, eb0, k, next, scale_next); });
-      spread(q, PB, [&](int k) { load_b(1, k, stage, rb, true); });
+      loads(q, PB, [&](int k) { to_b(1, k, stage); });
+    }, [&](int q) {
+      reads(q, HN, [&](int k) { read(x1[k], fb, eb0, k, next, scale_next); });
+      loads(q, PB, [&](int k) { load_from(rb, off_b(1, k)); });
     });
   };
   auto load_step = [&](int s) {  // all of a whole step
@@ -323,16 +391,14 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
       u32x4 ra = step_resource(pa, enda, s), rb = step_resource(pb + h * up, endb, s);
       settled(ra);
       settled(rb);
-#pragma unroll
-      for (int k = 0; k < PL; ++k)
-        if (k < PA) load_a(h, k, s * kStage, ra, true);
-        else load_b(h, k - PA, s * kStage, rb, true);
+      load_half(h, (s & 1) * kStage, ra, rb, kStep);
     }
   };
   // Stores of a whole tile, at the least: they follow the next tile's first loads, and go on while its first steps run.
   constexpr int W = 4 * GB, JG = TN / GB / (GLU ? 2 : 1), COLS = GLU ? HALF : TN * 16;
   constexpr int kStores = TM * JG * W * (OUT == kOut8 ? 1 : OUT == kOut32 ? 4 : 2) / 16;
-  static_assert(3 * PL + kStores < 64, "operations that a wait can count");
+  constexpr bool kMany = BM == 256;  // a workgroup goes over several tiles
+  static_assert(3 * PL + (kMany ? kStores : 0) < 64, "operations that a wait can count");
   auto begin = [&] {
     load_scales(0);
     if (whole == 0) return;
@@ -363,37 +429,77 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     }
   }
   acc_settled();
-  if (counted) wait_loads<3 * PL + kStores>();
-  else wait_loads<0>();
-  lds_barrier();
-  if (whole > 0) {
-#pragma unroll
-    for (int i = 0; i < HM; ++i) read(a0[i], fa, ea0, i, 0, 0);
-#pragma unroll
-    for (int j = 0; j < HN; ++j) read(b0[j], fb, eb0, j, 0, 0);
-    step(Spare<kStores, false>{}, 0, b0, b1);
-    if (whole > 1) step(Spare<kStores, true>{}, 1, b1, b0);
-    int s = 2;
-    for (; s + 2 <= whole; s += 2) {
-      step(Spare<0, true>{}, s, b0, b1);
-      step(Spare<0, true>{}, s + 1, b1, b0);
-    }
-    if (s < whole) step(Spare<0, true>{}, s, b0, b1);
-    wait_loads<0>();
+  if constexpr (EXACT) {
+    for (int i = 0; i < TM; ++i) nan_row[i] = false;
+    for (int j = 0; j < kScaleSets; ++j)
+      for (int q = 0; q < 4; ++q) nan_column[j][q] = false;
+    // A step's fragments are read whole while the step before is multiplied, which keeps the vector unit busy.
+    wait_loads<2 * PL>();
     lds_barrier();
+    if (whole > 0) {
+      Frag a[2][TM], b[2][TN];
+      ColumnScales c[2][kScaleSets];
+      auto read_step = [&](int s, Frag (&a)[TM], Frag (&b)[TN], ColumnScales (&c)[kScaleSets]) {
+        const unsigned stage = (s & 1) * kStage, scale = scale_at(s);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          read(b[i], fb, eb0, i, stage, scale);
+          read(a[i], fa, ea0, i, stage, scale);
+        }
+        read_columns(c, scale);
+      };
+      auto plain_step = [&](int s, int now) {
+        wait_loads<0>();
+        lds_barrier();
+        if ((s & 3) == 0) load_scales((s >> 2) + 1);
+        read_step(s + 1, a[now ^ 1], b[now ^ 1], c[now ^ 1]);
+        load_step(s + 2);
+        multiply(a[now], b[now], c[now]);
+      };
+      read_step(0, a[0], b[0], c[0]);
+      int s = 0;
+      for (; s + 2 <= whole; s += 2) {
+        plain_step(s, 0);
+        plain_step(s + 1, 1);
+      }
+      if (s < whole) plain_step(s, 0);
+      wait_loads<0>();
+      lds_barrier();
+    }
+  } else {
+    if (!kMany) wait_loads<3 * PL>();
+    else if (counted) wait_loads<3 * PL + kStores>();
+    else wait_loads<0>();
+    lds_barrier();
+    if (whole > 0) {
+#pragma unroll
+      for (int i = 0; i < HM; ++i) read(a0[i], fa, ea0, i, 0, 0);
+#pragma unroll
+      for (int j = 0; j < HN; ++j) read(b0[j], fb, eb0, j, 0, 0);
+      int s = 0;
+      if constexpr (kMany) {
+        step(Spare<kStores, false>{}, 0, b0, b1);
+        if (whole > 1) step(Spare<kStores, true>{}, 1, b1, b0);
+        s = 2;
+      }
+      for (; s + 2 <= whole; s += 2) {
+        step(Spare<0, true>{}, s, b0, b1);
+        step(Spare<0, true>{}, s + 1, b1, b0);
+      }
+      if (s < whole) step(Spare<0, true>{}, s, b0, b1);
+      wait_loads<0>();
+      lds_barrier();
+    }
   }
   if (tail) {  // the end of the rows: its elements at and behind `tail` as zeros
-    const unsigned stage = (whole & 1) * kStage, scale = (whole >> 2 & 1) * kScales + (whole & 3);
+    const unsigned stage = (whole & 1) * kStage, scale = scale_at(whole);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const size_t at = (size_t)whole * kStep;
       u32x4 ra = resource(pa + at, enda - (unsigned)at), rb = resource(pb + h * up + at, endb - (unsigned)at);
       settled(ra);
       settled(rb);
-#pragma unroll
-      for (int k = 0; k < PL; ++k)
-        if (k < PA) load_a(h, k, stage, ra, piece_a[k % FA] < tail);
-        else load_b(h, k - PA, stage, rb, piece_b[(k - PA) % FB] < tail);
+      load_half(h, stage, ra, rb, tail);
     }
     wait_loads<0>();
     lds_barrier();
@@ -410,23 +516,43 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
       b[j].v &= mask;
       operand_settled(b[j].v);
     }
+    if constexpr (EXACT) {
+      Frag a[TM];
+      ColumnScales c[kScaleSets];
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      Frag a;
-      read(a, fa, ea0, i, stage, scale);
-      a.v &= mask;
-      operand_settled(a.v);
+      for (int i = 0; i < TM; ++i) {
+        read(a[i], fa, ea0, i, stage, scale);
+        a[i].v &= mask;
+      }
+      read_columns(c, scale);
+      multiply(a, b, c);
+    } else {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) product(a, b[j], acc[i][j]);
+      for (int i = 0; i < TM; ++i) {
+        Frag a;
+        read(a, fa, ea0, i, stage, scale);
+        a.v &= mask;
+        operand_settled(a.v);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) product128(b[j].v, b[j].e, a.v, a.e, acc[i][j]);
+      }
     }
     lds_barrier();
   }
 
+  if constexpr (EXACT)
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (nan_row[i] || nan_column[j][q]) acc[i][j][q] = NAN;
   acc_settled();
   const ArgsAgain p = args_again();
   const int tid = again(threadIdx.x), l = tid & 63, r = l & 15, g = l >> 4;
   const long cm = m0, cn = n0;  // this tile, while the next one's operands are loaded
-  const bool direct = ACT != kActOther && cn + NT <= p->N, more = k + stride < mine;
+  const bool direct = ACT != kActOther && cn + NT <= p->N, more = kMany && k + stride < mine;
   if (direct && more) {
     place(k + stride);
     begin();
@@ -449,8 +575,9 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
         }
       };
       if constexpr (OUT == kOut8) {
-        // a block's columns lie in the four lanes of a row, and with swiglu in two waves
-        static_assert(COLS == kFp8Block || (GLU && COLS * 2 == kFp8Block), "blocks of a wave, or of two");
+        // a block's columns lie in the four lanes of a row, of one wave or of two
+        constexpr bool kTwo = COLS * 2 == kFp8Block;
+        static_assert((kTwo && JG == 1) || COLS == kFp8Block, "blocks of a wave, or of two");
         auto largest = [&](const float (&v)[JG][W]) {
           unsigned most = 0;
 #pragma unroll
@@ -472,9 +599,9 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
             for (int e = 0; e < W / 4; ++e) o[e] = fp8_word(v[j][4 * e], v[j][4 * e + 1], v[j][4 * e + 2], v[j][4 * e + 3], byte);
             *gmem((words*)((unsigned char*)p->out + m * p->ldo + nw + j * 16 * GB)) = o;
           }
-          if (g == 0 && (!GLU || (wn & 1) == 0)) p->os[m * p->los + (cn + wn * COLS) / kFp8Block] = (unsigned char)byte;
+          if (g == 0 && (!kTwo || (wn & 1) == 0)) p->os[m * p->los + (cn + wn * COLS) / kFp8Block] = (unsigned char)byte;
         };
-        if constexpr (!GLU) {
+        if constexpr (!kTwo) {
 #pragma unroll
           for (int i = 0; i < TM; ++i) {
             float v[JG][W];
@@ -530,9 +657,11 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
         };
         if constexpr (OUT == kOut32) emit(0.f);
         else if (p->dtype == kBf16) emit((bf16)0.f);
-        else emit((f16)0.f);
+        else if (kMany || p->dtype == kF16) emit((f16)0.f);
+        else emit(0.f);
       }
-      continue;
+      if (kMany) continue;
+      return;
     }
   }
 
@@ -605,11 +734,13 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     __syncthreads();
     if constexpr (OUT == kOut16) {
       if (p->dtype == kBf16) through((bf16)0.f, h);
-      else through((f16)0.f, h);
+      else if (kMany || p->dtype == kF16) through((f16)0.f, h);
+      else through(0.f, h);
     } else {
       through(0.f, h);
     }
   }
+  if (!kMany) return;
   if (more) {
     lds_barrier();
     place(k + stride);
@@ -618,19 +749,203 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
   }
 }
 
+// ---------------------------------------------------------------------------
+// few rows: the weight's bytes
+// ---------------------------------------------------------------------------
+// 16 columns (swiglu: 16 gates and their ups) of 16 rows by a group of `parts` waves, each over its part of the
+// contraction, from memory straight into the matrix instruction's operands: a wave waits for nothing but its own loads,
+// four steps of them at once.  The parts' sums meet in LDS, in their order.
+struct ThinArgs {
+  Fp8ProductArgs p;
+  int parts;  // waves to a group: 1, 2, 4 or 8
+};
+constexpr int kThinWaves = 8;
+template <int N>
+struct Count {
+  static constexpr int value = N;
+};
+template <int ACT, int OUT>
+__global__ __launch_bounds__(kThinWaves * 64) void fp8_thin_kernel(const ThinArgs a) {
+  constexpr bool GLU = ACT == kActSwiglu, EXACT = OUT == kOut32;
+  constexpr int C = GLU ? 2 : 1, kAhead = 4;
+  const Fp8ProductArgs& p = a.p;
+  __shared__ f32x4 sums[kThinWaves][C][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, r = l & 15, g = l >> 4;
+  const int part = wave & (a.parts - 1), first = wave - part;
+  const long n0 = ((long)blockIdx.x * (kThinWaves / a.parts) + first / a.parts) * 16, m0 = (long)blockIdx.y * 16;
+  const int steps = (int)((p.K + kStep - 1) / kStep), tail = (int)(p.K & (kStep - 1));
+  const int per = (steps + a.parts - 1) / a.parts, s0 = min(part * per, steps), s1 = min(s0 + per, steps);
+  // this lane's rows (behind the last one: the last one's, which nothing is made of)
+  const long m = min(m0 + r, p.M - 1);
+  const unsigned char *av = p.a + m * p.lda + 16 * g, *ae = p.sa + m * p.lsa, *bv[C], *be[C];
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+    const long n = min(n0 + r, p.N - 1) + j * p.N;
+    bv[j] = p.b + n * p.ldb + 16 * g;
+    be[j] = p.sb + n * p.lsb;
+  }
+  struct Frag {
+    i32x8 v;
+    int e;
+  };
+  // pieces g and g + 4 of a step; `end`: the contraction's end, with zeros behind it
+  auto load = [&](Frag& f, const unsigned char* v, const unsigned char* e, int s, bool end) {
+    const int left = end ? tail : kStep;
+    i32x4 x{0, 0, 0, 0}, y{0, 0, 0, 0};
+    if (16 * g < left) x = *gmem((const i32x4*)(v + (long)s * kStep));
+    if (16 * g + 64 < left) y = *gmem((const i32x4*)(v + (long)s * kStep + 64));
+    if (end)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int n = tail - 16 * g - 4 * d;
+        x[d] &= n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1;
+        y[d] &= n >= 68 ? -1 : n <= 64 ? 0 : (1 << (8 * (n - 64))) - 1;
+      }
+    f.v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    f.e = *gmem(e + s);
+  };
+  f32x4 acc[C];
+#pragma unroll
+  for (int j = 0; j < C; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // (no branch between the loads of a batch: they would be waited for there)
+  auto run = [&](int s, auto count, auto end) {
+    constexpr int B = decltype(count)::value;
+    Frag x[B], w[B][C];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+      const bool last = decltype(end)::value && b == B - 1;
+#pragma unroll
+      for (int j = 0; j < C; ++j) load(w[b][j], bv[j], be[j], s + b, last);
+      load(x[b], av, ae, s + b, last);
+    }
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        if constexpr (!EXACT)
+          acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[b][j].v, x[b].v, acc[j], 0, 0, 0, w[b][j].e, 0, x[b].e);
+        else
+          exact_product(w[b][j].v, w[b][j].e, x[b].v, x[b].e, acc[j]);
+      }
+  };
+  const bool ends = tail && s1 == steps && s0 < s1;
+  int s = s0;
+  for (; s + kAhead + (ends ? 1 : 0) <= s1; s += kAhead) run(s, Count<kAhead>{}, Count<false>{});
+  auto rest = [&](auto end) {
+    switch (s1 - s) {
+      case 1: run(s, Count<1>{}, end); break;
+      case 2: run(s, Count<2>{}, end); break;
+      case 3: run(s, Count<3>{}, end); break;
+      case 4: run(s, Count<4>{}, end); break;
+      default: break;
+    }
+  };
+  if (ends) rest(Count<true>{});
+  else rest(Count<false>{});
+
+  if (a.parts > 1) {
+#pragma unroll
+    for (int j = 0; j < C; ++j) sums[wave][j][l] = acc[j];
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+      for (int k = 1; k < a.parts; ++k) acc[j] += sums[first + k][j][l];
+  }
+  const long n = n0 + 4 * g, row = m0 + r;
+  if (row >= p.M || n >= p.N) return;
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const long c = min(n + e, p.N - 1);
+    v[e] = acc[0][e] + (p.bias ? bias_at(p.bias, p.bdtype, c) : 0.f);
+    if (GLU) v[e] = v[e] * sigmoid(v[e]) * (acc[C - 1][e] + (p.bias ? bias_at(p.bias, p.bdtype, p.N + c) : 0.f));
+  }
+  if (!GLU && ACT != kActNone) act_values<4>(p.act, v);
+  auto emit = [&](auto type) {
+    typedef decltype(type) T;
+    if (p.res) add_row<T, 4>((const T*)p.res + row * p.ldr, n, p.N, v);
+    store_row<T, 4>((T*)p.out + row * p.ldo, n, p.N, v);
+  };
+  if (OUT == kOut32 || p.dtype == kF32) emit(0.f);
+  else if (p.dtype == kBf16) emit((bf16)0.f);
+  else emit((f16)0.f);
+}
+
 constexpr int kCus = 256;
 
-template <int BM, int BN, int WM, int WN, int OUT>
-hipError_t launch_tiles(const Fp8ProductArgs& p, hipStream_t st) {
-  const int NT = p.act == kActSwiglu ? BN / 2 : BN;
-  const long tiles = ((p.M + BM - 1) / BM) * ((p.N + NT - 1) / NT);
-  const dim3 grid((unsigned)(BM == 256 ? std::min<long>(tiles, kCus) : tiles)), block(WM * WN * 64);
-  if (p.act == kActSwiglu) hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActSwiglu, OUT>), grid, block, 0, st, p);
-  else if (p.act == kActNone) hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActNone, OUT>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActOther, OUT>), grid, block, 0, st, p);
+template <int OUT>
+hipError_t launch_thin(const Fp8ProductArgs& p, int parts, hipStream_t st) {
+  const long groups = (p.N + 15) / 16, per = kThinWaves / parts;
+  const dim3 grid((unsigned)((groups + per - 1) / per), (unsigned)((p.M + 15) / 16)), block(kThinWaves * 64);
+  const ThinArgs a{p, parts};
+  if (p.act == kActSwiglu) hipLaunchKernelGGL((fp8_thin_kernel<kActSwiglu, OUT>), grid, block, 0, st, a);
+  else if (p.act == kActNone) hipLaunchKernelGGL((fp8_thin_kernel<kActNone, OUT>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((fp8_thin_kernel<kActOther, OUT>), grid, block, 0, st, a);
   return hipGetLastError();
 }
 
+template <int BM, int OUT>
+hipError_t launch_tiles(const Fp8ProductArgs& p, hipStream_t st) {
+  constexpr int BN = BM, WM = 2, WN = 2;
+  const int NT = p.act == kActSwiglu ? BN / 2 : BN;
+  const long tiles = ((p.M + BM - 1) / BM) * ((p.N + NT - 1) / NT);
+  const dim3 grid((unsigned)(BM == 256 ? std::min<long>(tiles, kCus) : tiles)), block(WM * WN * 64);
+  if (p.act == kActSwiglu) {
+    if constexpr (OUT != kOut8 || BN == 256) hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActSwiglu, OUT>), grid, block, 0, st, p);
+  } else if (p.act == kActNone) {
+    hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActNone, OUT>), grid, block, 0, st, p);
+  } else {
+    hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActOther, OUT>), grid, block, 0, st, p);
+  }
+  return hipGetLastError();
+}
+
+// How a product runs.
+struct Fp8Plan {
+  int side;      // of its tiles: 256, 128, 64; 0: 16 rows by 16 columns at a time (fp8_thin_kernel)
+  int parts;     // of the contraction (side 0)
+  bool through;  // an output in 8 bits is written in fp32 first, and quantised by a second launch
+};
+// By what a call is expected to take, in us, out of measured times (`steps` of 128):
+//   side 0: 3.6 for one step a wave and 0.8 for each more (4096 x 4096, 16 rows: 6.7, 64 tiles 12.2; 1024 over 2816, 16 rows
+//     5.4 and 8.6; 1024 over 1024, 64 rows 3.7 and 5.4), 2050 tiles of 16 x 16 and a step in a us (32000 over 1024, 16 rows
+//     11.0 and 7.9)
+//   64: 0.28 a step where the CUs have few tiles (1024 over 1024, 512 rows: 5.8, 128 tiles 7.4, 256 16.6), 1450 tiles and
+//     steps a us (2816 over 1024, 2048 rows 14.5, 128 tiles 12.3, 256 18.5); exactly: 0.83 and 480
+//   128: 0.42, and 600 (4096 x 4096, 2048 rows 31, 256 tiles 42 - 47, 64 52)
+//   256: a round of all CUs 1.4 a step (8192^3 365; fewer workgroups 1.0) and 5 (swiglu into 8 bits 6) for the outputs
+//   through fp32: the second launch, and 8 bytes an output to and fro
+Fp8Plan fp8_plan(long M, long N, long K, int act, int out) {
+  const bool glu = act == kActSwiglu;
+  const long outs = glu ? 2 * N : N, steps = (K + kStep - 1) / kStep;
+  Fp8Plan best{256, 1, false};
+  float least = 0.f;
+  auto offer = [&](int side, int parts, bool through, float t) {
+    if (through) t += 2.2f + 1.3e-6f * M * N;
+    if (least == 0.f || t < least) {
+      least = t;
+      best = {side, parts, through};
+    }
+  };
+  auto tiles = [&](long side) { return (float)(((M + side - 1) / side) * ((outs + side - 1) / side)); };
+  const bool exact = out == kOut32, through = out == kOut8;
+  if (M <= 1024) {
+    const long groups = (N + 15) / 16 * ((M + 15) / 16);
+    int parts = 1;
+    while (parts < kThinWaves && parts * 2 <= steps && groups * parts * 2 <= 16384) parts *= 2;
+    offer(0, parts, through, 2.8f + std::max(0.8f * ((steps + parts - 1) / parts), groups * steps * (glu ? 1.7f : 1.f) / 2050.f));
+  }
+  if (exact) {
+    offer(64, 1, false, 2.5f + std::max(0.83f * steps, tiles(64) * (steps + 2) / 480.f));
+    return best;
+  }
+  offer(64, 1, through, 3.f + std::max(0.28f * steps, tiles(64) * (steps + 4) / 1450.f));
+  offer(128, 1, through && glu, 3.4f + std::max(0.42f * steps, tiles(128) * (steps + 8) / 600.f));
+  const long t = (long)tiles(256), full = t / kCus, rest = t % kCus;
+  offer(256, 1, false, 4.f + full * (1.4f * steps + 5.f) + (rest ? (1.f + 0.4f * rest / kCus) * steps + 5.f : 0.f));
+  return best;
+}
 
 }  // namespace
 
@@ -646,13 +961,32 @@ hipError_t launch_quantize(const QuantizeArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-hipError_t launch_fp8_product(const Fp8ProductArgs& p, hipStream_t st) {
-  if (p.M <= 0) return hipSuccess;
-  const long outs = p.act == kActSwiglu ? 2 * p.N : p.N;
-  if (!p.os && p.dtype == kF32) return launch_tiles<64, 64, 2, 2, kOut32>(p, st);
-  if (p.os) return launch_tiles<256, 256, 2, 2, kOut8>(p, st);
-  if (((p.M + 255) / 256) * ((outs + 255) / 256) >= kCus / 2) return launch_tiles<256, 256, 2, 2, kOut16>(p, st);
-  return launch_tiles<64, 64, 2, 2, kOut16>(p, st);
+static int out_kind(const Fp8ProductArgs& p) { return p.os ? kOut8 : p.dtype == kF32 ? kOut32 : kOut16; }
+
+// fp32 elements of the workspace that such a call needs
+long fp8_product_workspace(long M, long N, long K, int act, int dtype, bool into8) {
+  return M > 0 && fp8_plan(M, N, K, act, into8 ? kOut8 : dtype == kF32 ? kOut32 : kOut16).through ? M * N : 0;
+}
+
+hipError_t launch_fp8_product(const Fp8ProductArgs& args, float* workspace, hipStream_t st) {
+  if (args.M <= 0) return hipSuccess;
+  const int out = out_kind(args);
+  const Fp8Plan plan = fp8_plan(args.M, args.N, args.K, args.act, out);
+  Fp8ProductArgs p = args;
+  if (plan.through) {
+    p.out = workspace;
+    p.ldo = p.N;
+    p.dtype = kF32;
+    p.os = nullptr;
+  }
+  hipError_t e;
+  if (plan.side == 0) e = out == kOut32 ? launch_thin<kOut32>(p, plan.parts, st) : launch_thin<kOut16>(p, plan.parts, st);
+  else if (out == kOut32) e = launch_tiles<64, kOut32>(p, st);
+  else if (plan.side == 64) e = launch_tiles<64, kOut16>(p, st);
+  else if (plan.side == 128) e = p.os ? launch_tiles<128, kOut8>(p, st) : launch_tiles<128, kOut16>(p, st);
+  else e = p.os ? launch_tiles<256, kOut8>(p, st) : launch_tiles<256, kOut16>(p, st);
+  if (e != hipSuccess || !plan.through) return e;
+  return launch_quantize({workspace, (unsigned char*)args.out, args.os, args.M, args.N, args.N, args.ldo, args.los, kF32}, st);
 }
 
 }  // namespace ccq

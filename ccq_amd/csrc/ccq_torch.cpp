@@ -447,9 +447,12 @@ void refuse_gradients(const std::string& who, std::initializer_list<const Tensor
 
 // New rows in 8 bits: both parts views of rows that the products read in place.
 Tensor fresh_bytes(const Tensor& x, at::IntArrayRef shape, int64_t unit, at::ScalarType type) {
+  if (shape.back() % unit == 0) return fresh(x, shape, type);
   auto room = shape.vec();
   room.back() = up_to(shape.back(), unit);
-  return fresh(x, room, type).narrow(-1, 0, shape.back());
+  Tensor t = fresh(x, room, type);
+  t.unsafeGetTensorImpl()->set_sizes_and_strides(shape, c10::DimVector(t.strides()));  // (narrow, without its host work)
+  return t;
 }
 struct Rows8 {
   Tensor values, scales;
@@ -561,10 +564,14 @@ std::tuple<Tensor, OptTensor> fp8_linear(const Tensor& x, const Tensor& xs, cons
   Rows8 o;
   if (quantize) o = fresh_rows(x, shape);
   else o.values = fresh(x, shape, dtype);
+  const int64_t M = xv.t.size(0);
+  const int type = quantize ? CCQ_DTYPE_BF16 : code(dtype);
+  const size_t n = ccq_fp8_linear_workspace_bytes(M, N, K, (int)act, type, quantize);
+  const Tensor workspace = n ? bytes(x, n) : Tensor();
   check(ccq_fp8_linear(address(xv.t), xv.ld, address(xe.t), xe.ld, address(wv.t), wv.ld, address(we.t), we.ld, address(b),
                        code(b.defined() ? b.scalar_type() : at::kFloat), address(r), stride_of(r), out_address(o.values),
                        quantize ? row_stride(o.values, 16) : N, out_address(o.scales), quantize ? row_stride(o.scales, 4) : 0,
-                       xv.t.size(0), N, K, (int)act, quantize ? CCQ_DTYPE_BF16 : code(dtype), stream_on(x)),
+                       out_address(workspace), M, N, K, (int)act, type, stream_on(x)),
         "ccq_fp8_linear");
   return {o.values, quantize ? OptTensor(o.scales) : OptTensor()};
 }

@@ -577,11 +577,14 @@ int ccq_norm_fp8_fwd(const void* x, int64_t ldx, const void* r, int64_t ldr, con
  * rows, then up rows; values weight, ldw; scales ws, ldws), bias [N] (swiglu: [2 N]) of bdtype (nullable), r [M, N] of
  * dtype (row stride ldr, nullable), act CCQ_ACT_*.  Products, bias, activation and residual in fp32.  y [M, N] of dtype,
  * contiguous, rounded once; or, with ys not NULL, y [M, N] (row stride ldy) and ys (ldys) in 8 bits (no r then; dtype is
- * not looked at).
+ * not looked at).  workspace: ccq_fp8_linear_workspace_bytes bytes (into8 not 0: the output in 8 bits), for outputs in 8
+ * bits of few rows.
  */
+size_t ccq_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, int dtype, int into8);
 int ccq_fp8_linear(const void* x, int64_t ldx, const void* xs, int64_t ldxs, const void* weight, int64_t ldw,
                    const void* ws, int64_t ldws, const void* bias, int bdtype, const void* r, int64_t ldr, void* y,
-                   int64_t ldy, void* ys, int64_t ldys, int64_t M, int64_t N, int64_t K, int act, int dtype, void* stream);
+                   int64_t ldy, void* ys, int64_t ldys, void* workspace, int64_t M, int64_t N, int64_t K, int act,
+                   int dtype, void* stream);
 
 /*
  * Kernel timing (measurement facility; no counterpart in the reference).  While enabled, each

@@ -146,8 +146,8 @@ def test_abi_refusals():
     assert norm(x=ODD) == ALIGN and norm(v=ODD) == ALIGN and norm(w=ODD) == ALIGN
 
     def linear(x=P, ldx=208, xs=P, ldxs=4, w=P, ldw=208, ws=P, ldws=4, b=None, bd=0, r=None, ldr=0, y=P, ldy=32, ys=None,
-               ldys=0, M=4, N=32, K=200, act=0, dt=0):
-        return lib.ccq_fp8_linear(x, ldx, xs, ldxs, w, ldw, ws, ldws, b, bd, r, ldr, y, ldy, ys, ldys, M, N, K, act, dt, None)
+               ldys=0, work=P, M=4, N=32, K=200, act=0, dt=0):
+        return lib.ccq_fp8_linear(x, ldx, xs, ldxs, w, ldw, ws, ldws, b, bd, r, ldr, y, ldy, ys, ldys, work, M, N, K, act, dt, None)
 
     assert linear(M=-1) == SHAPE and linear(N=0) == SHAPE and linear(K=0) == SHAPE and linear(act=6) == SHAPE
     assert linear(dt=3) == SHAPE and linear(bd=3) == SHAPE and linear(r=P, ldr=31) == SHAPE
@@ -159,4 +159,9 @@ def test_abi_refusals():
     assert linear(y=None) == NULL
     assert linear(x=ctypes.c_void_p(0x1008)) == ALIGN and linear(xs=ODD) == ALIGN and linear(ws=ODD) == ALIGN
     assert linear(y=ODD) == ALIGN and linear(b=ODD) == ALIGN and linear(r=ODD, ldr=32) == ALIGN
+    assert linear(ys=P, ldys=4, K=2000, ldx=2000, ldw=2000, ldxs=16, ldws=16, work=None) == NULL  # (few rows: through fp32)
+    assert linear(work=ODD) == ALIGN
     assert linear(M=0) == 0
+    size = lib.ccq_fp8_linear_workspace_bytes
+    assert size(4, 32, 2000, 0, 0, 1) == 4 * 32 * 4 and size(4, 32, 2000, 0, 0, 0) == 0 and size(0, 32, 2000, 0, 0, 1) == 0
+    assert size(32768, 4096, 4096, 0, 0, 1) == 0
