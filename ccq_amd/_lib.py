@@ -83,6 +83,7 @@ SIGNATURES = {
     "ccq_pad_rows": (_I, [_P, _I64, _P] + [_I64] * 3 + [_P]),
     "ccq_quantize_fp8": (_I, [_P, _I64] * 3 + [_I64] * 2 + [_I, _P]),
     "ccq_norm_fp8_fwd": (_I, [_P, _I64] * 2 + [_P] + [_P, _I64] * 2 + [_P, _I64] + [_I] * 3 + [_F, _P]),
+    "ccq_fp8_linear_plan": (_I, [_I64] * 3 + [_I] * 3 + [_P] * 3),
     "ccq_fp8_linear_workspace_bytes": (_SZ, [_I64] * 3 + [_I] * 3),
     "ccq_fp8_linear": (_I, [_P, _I64] * 4 + [_P, _I] + [_P, _I64] * 3 + [_P] + [_I64] * 3 + [_I, _I, _P]),
     "ccq_timing_enable": (_I, [_I]),

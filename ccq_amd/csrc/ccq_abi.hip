@@ -36,6 +36,7 @@ hipError_t launch_logprobs(bool bwd, const LogprobArgs& a, hipStream_t st);
 void product_plan(long M, long N, long K, int* side, int* splits);
 hipError_t launch_product(int kind, const ProductArgs& p, hipStream_t st);
 hipError_t launch_quantize(const QuantizeArgs& a, hipStream_t st);
+void fp8_product_plan(long M, long N, long K, int act, int dtype, bool into8, int* side, int* parts, int* through);
 long fp8_product_workspace(long M, long N, long K, int act, int dtype, bool into8);
 hipError_t launch_fp8_product(const Fp8ProductArgs& p, float* workspace, hipStream_t st);
 int act_bwd_row_blocks(long M, long N);
@@ -1829,6 +1830,17 @@ int ccq_norm_fp8_fwd(const void* x, int64_t ldx, const void* r, int64_t ldr, con
   a.lds = lds; a.s = s; a.rows = rows; a.D = D; a.dtype = dtype; a.wdtype = wdtype; a.eps = eps;
   hipStream_t st = (hipStream_t)stream;
   return hip_status(timed("norm_fp8", st, [&] { return launch_norm_fwd(a, st); }), who);
+}
+
+int ccq_fp8_linear_plan(int64_t M, int64_t N, int64_t K, int act, int dtype, int into8, int* side, int* parts, int* through) {
+  const char* who = "ccq_fp8_linear_plan";
+  if (M < 1 || N < 1 || K < 1 || M > kMaxSide || N > kMaxSide || K > kMaxSide)
+    return fail(CCQ_ERR_SHAPE, "%s: M=%lld N=%lld K=%lld", who, (long long)M, (long long)N, (long long)K);
+  if (act < CCQ_ACT_NONE || act > CCQ_ACT_SWIGLU || (!into8 && !dtype_ok(dtype)))
+    return fail(CCQ_ERR_SHAPE, "%s: act=%d dtype=%d", who, act, dtype);
+  if (!side || !parts || !through) return fail(CCQ_ERR_NULL, "%s: side, parts and through are required", who);
+  fp8_product_plan(M, N, K, act, dtype, into8 != 0, side, parts, through);
+  return CCQ_OK;
 }
 
 size_t ccq_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, int dtype, int into8) {

@@ -31,8 +31,20 @@ __device__ __forceinline__ unsigned fp8_word(float a, float b, float c, float d,
   return byte == kFp8Nan ? 0x7f7f7f7fu : (unsigned)w;
 }
 
-// maximum over groups of L consecutive lanes (L a power of two <= 64)
+// maximum over 16 consecutive lanes, by rotations within them
+__device__ __forceinline__ unsigned lanes_max16(unsigned x) {
+  x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, true));  // row_ror:8, 4, 2, 1
+  x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, true));
+  x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, true));
+  return max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, true));
+}
+// over groups of L consecutive lanes (L a power of two <= 64)
 __device__ __forceinline__ unsigned lanes_max(unsigned x, int L) {
+  if (L >= 16) {
+    x = lanes_max16(x);
+    for (int o = 16; o < L; o <<= 1) x = max(x, (unsigned)__shfl_xor((int)x, o));
+    return x;
+  }
   for (int o = L >> 1; o > 0; o >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, o));
   return x;
 }

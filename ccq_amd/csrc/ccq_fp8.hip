@@ -50,7 +50,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const QuantizeArgs a
     unsigned m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = max(m, magnitude(v[i]));
-    const unsigned byte = scale_byte(lanes_max(m, 16));
+    const unsigned byte = scale_byte(lanes_max16(m));
     if (c < a.D) {  // (a whole piece: the rows are multiples of 16)
       *gmem((u32x2*)(a.values + row * a.ldv + c)) =
           u32x2{fp8_word(v[0], v[1], v[2], v[3], byte), fp8_word(v[4], v[5], v[6], v[7], byte)};
@@ -665,9 +665,11 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     }
   }
 
-  // The others, and the activations that are code of some size, through LDS: a thread takes eight consecutive columns.
+  // The others, and the activations that are code of some size, through LDS: a thread takes eight consecutive columns of NG
+  // rows at a time.
   float* tile = (float*)smem;
-  constexpr int PR = NT / 8, RP = NW * 64 / PR, NG = 4;  // threads of a row, rows at a time, how often before the next loads
+  constexpr int PR = NT / 8, RP = NW * 64 / PR, NG = std::min(4, WM * kPass / RP);  // threads of a row, rows at a time
+  static_assert(WM * kPass % (NG * RP) == 0, "whole groups of rows");
   const int c = tid % PR * 8, cw = c / (GLU ? HALF : NT), cs = GLU ? cw * 2 * HALF + c % HALF : c;
   const long n = cn + c;
   auto through = [&](auto type, int h) {
@@ -675,45 +677,47 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     for (int i0 = tid / PR; i0 < WM * kPass; i0 += NG * RP) {
       RowPiece<T, 8> res[NG];
       long m[NG];
+      float v[NG * 8], up[8];
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
         const int i = i0 + k * RP;
-        m[k] = i < WM * kPass ? cm + i / kPass * (TM * 16) + slot_row(h * kPass + i % kPass, GA) : p->M;
+        m[k] = cm + i / kPass * (TM * 16) + slot_row(h * kPass + i % kPass, GA);
         if (p->res && m[k] < p->M && n < p->N) res[k].load((const T*)p->res + m[k] * p->ldr, n, p->N);
       }
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
-        const int i = i0 + k * RP;
-        if (m[k] >= p->M || (n >= p->N && OUT != kOut8)) continue;
-        float v[8], up[8];
+        const float* row = tile + (i0 + k * RP) * kPitch + cs;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] = tile[i * kPitch + cs + e];
-          if (GLU) up[e] = tile[i * kPitch + cs + HALF + e];
+        for (int e = 0; e < 8; e += 4) {
+          *(f32x4*)(v + 8 * k + e) = *(const f32x4*)(row + e);
+          if (GLU) *(f32x4*)(up + e) = *(const f32x4*)(row + HALF + e);
         }
-        if (GLU) {
+        if (GLU)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = v[e] * sigmoid(v[e]) * up[e];
-        } else if (ACT != kActNone) {
-          act_values<8>(p->act, v);
-        }
+          for (int e = 0; e < 8; ++e) v[8 * k + e] = v[8 * k + e] * sigmoid(v[8 * k + e]) * up[e];
+      }
+      if (!GLU && ACT != kActNone) act_values<NG * 8>(p->act, v);
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        float(&w)[8] = *(float(*)[8])(v + 8 * k);
         if constexpr (OUT == kOut8) {  // a row's 16 lanes of a block go together
           unsigned most = 0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            if (n + e >= p->N) v[e] = 0.f;
-            most = max(most, magnitude(v[e]));
+            if (n + e >= p->N) w[e] = 0.f;
+            most = max(most, magnitude(w[e]));
           }
-          const unsigned byte = scale_byte(lanes_max(most, 16));
-          if (n >= p->N) continue;
-          *gmem((u32x2*)((unsigned char*)p->out + m[k] * p->ldo + n)) =
-              u32x2{fp8_word(v[0], v[1], v[2], v[3], byte), fp8_word(v[4], v[5], v[6], v[7], byte)};
-          if ((tid & 15) == 0) p->os[m[k] * p->los + n / kFp8Block] = (unsigned char)byte;
-        } else {
+          const unsigned byte = scale_byte(lanes_max16(most));
+          const u32x2 o = {fp8_word(w[0], w[1], w[2], w[3], byte), fp8_word(w[4], w[5], w[6], w[7], byte)};
+          if (m[k] < p->M && n < p->N) {
+            *gmem((u32x2*)((unsigned char*)p->out + m[k] * p->ldo + n)) = o;
+            if ((tid & 15) == 0) p->os[m[k] * p->los + n / kFp8Block] = (unsigned char)byte;
+          }
+        } else if (m[k] < p->M && n < p->N) {
           if (p->res)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += (float)res[k].v[e];
-          store_row<T, 8>((T*)p->out + m[k] * p->ldo, n, p->N, v);
+            for (int e = 0; e < 8; ++e) w[e] += (float)res[k].v[e];
+          store_row<T, 8>((T*)p->out + m[k] * p->ldo, n, p->N, w);
         }
       }
     }
@@ -753,107 +757,126 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
 // few rows: the weight's bytes
 // ---------------------------------------------------------------------------
 // 16 columns (swiglu: 16 gates and their ups) of 16 rows by a group of `parts` waves, each over its part of the
-// contraction, from memory straight into the matrix instruction's operands: a wave waits for nothing but its own loads,
-// four steps of them at once.  The parts' sums meet in LDS, in their order.
+// contraction, through LDS of its own: a wave waits for nothing but its own loads, some steps of which are on their way.
+// (Straight into registers a lane's neighbours would lie in other rows, and 16 bytes take a request each: 16 bytes a cycle
+// and CU, 64 so.)  The parts' sums meet in LDS, in their order.  An output in 8 bits needs its blocks' largest magnitudes:
+// its workgroup is eight groups of one wave, 128 columns.
 struct ThinArgs {
   Fp8ProductArgs p;
   int parts;  // waves to a group: 1, 2, 4 or 8
 };
 constexpr int kThinWaves = 8;
-template <int N>
-struct Count {
-  static constexpr int value = N;
-};
 template <int ACT, int OUT>
 __global__ __launch_bounds__(kThinWaves * 64) void fp8_thin_kernel(const ThinArgs a) {
   constexpr bool GLU = ACT == kActSwiglu, EXACT = OUT == kOut32;
-  constexpr int C = GLU ? 2 : 1, kAhead = 4;
+  constexpr int NW = kThinWaves, C = GLU ? 2 : 1, kAhead = GLU ? 3 : 4, kLoads = 2 * (C + 1);  // of a step
+  constexpr unsigned kTile = 16 * kStep, kSlot = (C + 1) * kTile, kMine = kAhead * kSlot + 512;
   const Fp8ProductArgs& p = a.p;
-  __shared__ f32x4 sums[kThinWaves][C][64];
+  const int parts = OUT == kOut8 ? 1 : a.parts;
+  __shared__ __attribute__((aligned(1024))) char smem[NW * kMine];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63, r = l & 15, g = l >> 4;
-  const int part = wave & (a.parts - 1), first = wave - part;
-  const long n0 = ((long)blockIdx.x * (kThinWaves / a.parts) + first / a.parts) * 16, m0 = (long)blockIdx.y * 16;
+  const int part = wave & (parts - 1), first = wave - part;
+  const long n0 = ((long)blockIdx.x * (NW / parts) + first / parts) * 16, m0 = (long)blockIdx.y * 16;
   const int steps = (int)((p.K + kStep - 1) / kStep), tail = (int)(p.K & (kStep - 1));
-  const int per = (steps + a.parts - 1) / a.parts, s0 = min(part * per, steps), s1 = min(s0 + per, steps);
-  // this lane's rows (behind the last one: the last one's, which nothing is made of)
-  const long m = min(m0 + r, p.M - 1);
-  const unsigned char *av = p.a + m * p.lda + 16 * g, *ae = p.sa + m * p.lsa, *bv[C], *be[C];
+  const int per = (steps + parts - 1) / parts, s0 = min(part * per, steps), s1 = min(s0 + per, steps);
+  const unsigned lds = lds_addr(smem) + wave * kMine, lds_scales = lds + kAhead * kSlot;
+  // rows behind the last one: the last one's, which nothing is made of; operand 0: x, then the weight's gates and ups
+  const long na = min(n0, p.N - 1);
+  unsigned off[2][2];  // of a lane's piece in a load of x, of the weight
 #pragma unroll
-  for (int j = 0; j < C; ++j) {
-    const long n = min(n0 + r, p.N - 1) + j * p.N;
-    bv[j] = p.b + n * p.ldb + 16 * g;
-    be[j] = p.sb + n * p.lsb;
+  for (int i = 0; i < 2; ++i) {
+    const int slot = 8 * i + (l >> 3), piece = ((l & 7) ^ swz(slot)) << 4;
+    off[0][i] = (unsigned)(min((long)slot, p.M - 1 - m0) * p.lda) + piece;
+    off[1][i] = (unsigned)(min((long)slot, p.N - 1 - na) * p.ldb) + piece;
   }
+  size_t base[C + 1];
+  base[0] = (size_t)p.a + m0 * p.lda;
+#pragma unroll
+  for (int j = 0; j < C; ++j) base[1 + j] = (size_t)p.b + (na + j * p.N) * p.ldb;
+  // scales: 16 rows of each operand, a word of four steps a lane (the fourth 16 lanes as the first)
+  const int op = g <= C ? g : 0;
+  const unsigned char* scales = op ? p.sb + (min(na + r, p.N - 1) + (op - 1) * p.N) * p.lsb : p.sa + min(m0 + r, p.M - 1) * p.lsa;
+  auto load_scales = [&](int quad) {
+    if (quad * 4 < steps) load4_to(lds_scales + (quad & 1) * 256, scales + 4 * quad);
+  };
+  auto load_step = [&](int s, int slot) {  // (nothing but zeros behind the part's end)
+    const int left = tail && s == steps - 1 ? tail : kStep;
+#pragma unroll
+    for (int o = 0; o <= C; ++o) {
+      u32x4 rs = resource(base[o] + (size_t)s * kStep, s < s1 ? 0x7fffffffu : 0u);
+      settled(rs);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        load_to(lds + slot * kSlot + o * kTile, i);
+        const unsigned f = off[o ? 1 : 0][i];
+        const bool on = (((l & 7) ^ swz(8 * i + (l >> 3))) << 4) < left;
+        asm volatile("s_nop 0");
+        load_from(rs, on ? f : kNowhere);
+      }
+    }
+  };
   struct Frag {
     i32x8 v;
     int e;
   };
-  // pieces g and g + 4 of a step; `end`: the contraction's end, with zeros behind it
-  auto load = [&](Frag& f, const unsigned char* v, const unsigned char* e, int s, bool end) {
-    const int left = end ? tail : kStep;
-    i32x4 x{0, 0, 0, 0}, y{0, 0, 0, 0};
-    if (16 * g < left) x = *gmem((const i32x4*)(v + (long)s * kStep));
-    if (16 * g + 64 < left) y = *gmem((const i32x4*)(v + (long)s * kStep + 64));
-    if (end)
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const int n = tail - 16 * g - 4 * d;
-        x[d] &= n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1;
-        y[d] &= n >= 68 ? -1 : n <= 64 ? 0 : (1 << (8 * (n - 64))) - 1;
-      }
+  auto read = [&](Frag& f, int o, int s, int slot) {
+    const unsigned at = lds + slot * kSlot + o * kTile + r * kStep;
+    const i32x4 x = __builtin_bit_cast(i32x4, read16(at + ((g ^ swz(r)) << 4))),
+                y = __builtin_bit_cast(i32x4, read16(at + (((g + 4) ^ swz(r)) << 4)));
     f.v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-    f.e = *gmem(e + s);
+    typedef __attribute__((address_space(3))) const unsigned char lds_byte;
+    f.e = *(lds_byte*)(size_t)(lds_scales + (s >> 2 & 1) * 256 + (16 * o + r) * 4 + (s & 3));
   };
   f32x4 acc[C];
 #pragma unroll
   for (int j = 0; j < C; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  // (no branch between the loads of a batch: they would be waited for there)
-  auto run = [&](int s, auto count, auto end) {
-    constexpr int B = decltype(count)::value;
-    Frag x[B], w[B][C];
+  if (s0 < s1) {
+    load_scales(s0 >> 2);
+    load_scales((s0 >> 2) + 1);
 #pragma unroll
-    for (int b = 0; b < B; ++b) {
-      const bool last = decltype(end)::value && b == B - 1;
+    for (int i = 0; i < kAhead; ++i) load_step(s0 + i, i);
+    int slot = 0;
+    for (int s = s0; s < s1; ++s) {
+      wait_loads<(kAhead - 1) * kLoads>();
+      Frag x, w[C];
+      read(x, 0, s, slot);
 #pragma unroll
-      for (int j = 0; j < C; ++j) load(w[b][j], bv[j], be[j], s + b, last);
-      load(x[b], av, ae, s + b, last);
-    }
+      for (int j = 0; j < C; ++j) read(w[j], 1 + j, s, slot);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next load arrives there
+      if ((s & 3) == 3) load_scales((s >> 2) + 2);
+      load_step(s + kAhead, slot);
+      slot = slot == kAhead - 1 ? 0 : slot + 1;
+      if (tail & 15 && s == steps - 1)
 #pragma unroll
-    for (int b = 0; b < B; ++b)
+        for (int d = 0; d < 8; ++d) {  // bytes of the end: the rows' storage goes on behind them
+          const int n = tail - (16 * (g + d / 4 * 4) + d % 4 * 4);
+          const int mask = n >= 4 ? -1 : n <= 0 ? 0 : (1 << (8 * n)) - 1;
+          x.v[d] &= mask;
+#pragma unroll
+          for (int j = 0; j < C; ++j) w[j].v[d] &= mask;
+        }
 #pragma unroll
       for (int j = 0; j < C; ++j) {
-        if constexpr (!EXACT)
-          acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[b][j].v, x[b].v, acc[j], 0, 0, 0, w[b][j].e, 0, x[b].e);
-        else
-          exact_product(w[b][j].v, w[b][j].e, x[b].v, x[b].e, acc[j]);
+        if constexpr (!EXACT) acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[j].v, x.v, acc[j], 0, 0, 0, w[j].e, 0, x.e);
+        else exact_product(w[j].v, w[j].e, x.v, x.e, acc[j]);
       }
-  };
-  const bool ends = tail && s1 == steps && s0 < s1;
-  int s = s0;
-  for (; s + kAhead + (ends ? 1 : 0) <= s1; s += kAhead) run(s, Count<kAhead>{}, Count<false>{});
-  auto rest = [&](auto end) {
-    switch (s1 - s) {
-      case 1: run(s, Count<1>{}, end); break;
-      case 2: run(s, Count<2>{}, end); break;
-      case 3: run(s, Count<3>{}, end); break;
-      case 4: run(s, Count<4>{}, end); break;
-      default: break;
     }
-  };
-  if (ends) rest(Count<true>{});
-  else rest(Count<false>{});
+    wait_loads<0>();
+  }
 
-  if (a.parts > 1) {
+  if (parts > 1) {
+    f32x4* sums = (f32x4*)smem;
+    __syncthreads();  // (the sums lie where other waves' steps lay)
 #pragma unroll
-    for (int j = 0; j < C; ++j) sums[wave][j][l] = acc[j];
+    for (int j = 0; j < C; ++j) sums[(wave * C + j) * 64 + l] = acc[j];
     __syncthreads();
     if (part) return;
 #pragma unroll
     for (int j = 0; j < C; ++j)
-      for (int k = 1; k < a.parts; ++k) acc[j] += sums[first + k][j][l];
+      for (int k = 1; k < parts; ++k) acc[j] += sums[((first + k) * C + j) * 64 + l];
   }
   const long n = n0 + 4 * g, row = m0 + r;
-  if (row >= p.M || n >= p.N) return;
+  if (OUT != kOut8 && (row >= p.M || n >= p.N)) return;
   float v[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -862,6 +885,26 @@ __global__ __launch_bounds__(kThinWaves * 64) void fp8_thin_kernel(const ThinArg
     if (GLU) v[e] = v[e] * sigmoid(v[e]) * (acc[C - 1][e] + (p.bias ? bias_at(p.bias, p.bdtype, p.N + c) : 0.f));
   }
   if (!GLU && ACT != kActNone) act_values<4>(p.act, v);
+  if constexpr (OUT == kOut8) {
+    __shared__ unsigned block_most[NW][16];
+    unsigned most = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (n + e >= p.N) v[e] = 0.f;
+      most = max(most, magnitude(v[e]));
+    }
+    most = max(most, (unsigned)__shfl_xor((int)most, 16));
+    most = max(most, (unsigned)__shfl_xor((int)most, 32));
+    if (g == 0) block_most[wave][r] = most;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NW; ++k) most = max(most, block_most[k][r]);
+    if (row >= p.M || n >= p.N) return;
+    const unsigned byte = scale_byte(most);
+    *gmem((unsigned*)((unsigned char*)p.out + row * p.ldo + n)) = fp8_word(v[0], v[1], v[2], v[3], byte);
+    if (wave == 0 && g == 0) p.os[row * p.los + n / kFp8Block] = (unsigned char)byte;
+    return;
+  }
   auto emit = [&](auto type) {
     typedef decltype(type) T;
     if (p.res) add_row<T, 4>((const T*)p.res + row * p.ldr, n, p.N, v);
@@ -907,43 +950,53 @@ struct Fp8Plan {
   int parts;     // of the contraction (side 0)
   bool through;  // an output in 8 bits is written in fp32 first, and quantised by a second launch
 };
-// By what a call is expected to take, in us, out of measured times (`steps` of 128):
-//   side 0: 3.6 for one step a wave and 0.8 for each more (4096 x 4096, 16 rows: 6.7, 64 tiles 12.2; 1024 over 2816, 16 rows
-//     5.4 and 8.6; 1024 over 1024, 64 rows 3.7 and 5.4), 2050 tiles of 16 x 16 and a step in a us (32000 over 1024, 16 rows
-//     11.0 and 7.9)
-//   64: 0.28 a step where the CUs have few tiles (1024 over 1024, 512 rows: 5.8, 128 tiles 7.4, 256 16.6), 1450 tiles and
-//     steps a us (2816 over 1024, 2048 rows 14.5, 128 tiles 12.3, 256 18.5); exactly: 0.83 and 480
-//   128: 0.42, and 600 (4096 x 4096, 2048 rows 31, 256 tiles 42 - 47, 64 52)
-//   256: a round of all CUs 1.4 a step (8192^3 365; fewer workgroups 1.0) and 5 (swiglu into 8 bits 6) for the outputs
-//   through fp32: the second launch, and 8 bytes an output to and fro
+// By what a call is expected to take, in us, out of measured times (`steps` of 128; an activation without a gate is code
+// that a tile's outputs pass through: `act`):
+//   side 0: a workgroup a CU, 0.29 a step of a wave (swiglu 0.45, exactly 0.52), or the weight's bytes.  1024 over 1024, 64
+//     rows: 4.3 in eight parts, 5.9 in one, by 64 tiles 5.5; 4064 over 1728, 40 rows 10.9, 7.8 (two parts 6.0), 7.4; 2816
+//     over 1024, 600 rows 78, 20, 6.8
+//   64: 0.28 a step where the CUs have few tiles (1024 over 1024, 300 rows: 5.5, 128 tiles 7.3, 256 16.5), 1450 tiles and
+//     steps a us (1024 over 1024, 2000 rows 6.9, 128 tiles 7.8; 2188 over 959, 4363 rows 25, 22); exactly: 0.83 and 480
+//   128: half a step's microsecond for each tile of a CU (2816 over 1024, 16384 rows 57.3, silu 71, gelu 84; 256 tiles 57.9,
+//     90, 111; 3520 over 3008, 25960 rows 316, 317, 344; 255, 302, 350; 2188 over 959, 4363 rows 22, 25, 29; 30, 35, 42)
+//   256: a round of all CUs 1.4 a step (8192^3 365; fewer workgroups 1.0) and 5 for the outputs, more where they end inside
+//     a tile
+//   through fp32: the second launch (its host time too), and 8 bytes an output to and fro
 Fp8Plan fp8_plan(long M, long N, long K, int act, int out) {
-  const bool glu = act == kActSwiglu;
+  const bool glu = act == kActSwiglu, other = !glu && act != kActNone;
   const long outs = glu ? 2 * N : N, steps = (K + kStep - 1) / kStep;
   Fp8Plan best{256, 1, false};
   float least = 0.f;
   auto offer = [&](int side, int parts, bool through, float t) {
-    if (through) t += 2.2f + 1.3e-6f * M * N;
+    if (through) t += 4.f + 1.3e-6f * M * N;
     if (least == 0.f || t < least) {
       least = t;
       best = {side, parts, through};
     }
   };
-  auto tiles = [&](long side) { return (float)(((M + side - 1) / side) * ((outs + side - 1) / side)); };
+  auto tiles = [&](long side) { return ((M + side - 1) / side) * ((outs + side - 1) / side); };
   const bool exact = out == kOut32, through = out == kOut8;
   if (M <= 1024) {
     const long groups = (N + 15) / 16 * ((M + 15) / 16);
-    int parts = 1;
-    while (parts < kThinWaves && parts * 2 <= steps && groups * parts * 2 <= 16384) parts *= 2;
-    offer(0, parts, through, 2.8f + std::max(0.8f * ((steps + parts - 1) / parts), groups * steps * (glu ? 1.7f : 1.f) / 2050.f));
+    const float step = exact ? 0.52f : glu ? 0.45f : 0.29f, bytes = 1.5f + outs * K / 5e6f;
+    auto time = [&](int parts) {
+      const long wgs = (groups * parts + kThinWaves - 1) / kThinWaves, rounds = (wgs + kCus - 1) / kCus;
+      const float part = step * ((steps + parts - 1) / parts);
+      return std::max(bytes, 2.4f + (rounds == 1 ? 1.6f + part : rounds * (2.3f + part)));
+    };
+    for (int parts = 1; parts <= kThinWaves && (parts == 1 || parts <= steps); parts *= 2) offer(0, parts, through, time(parts));
+    if (through) offer(0, 1, false, time(1));
   }
   if (exact) {
     offer(64, 1, false, 2.5f + std::max(0.83f * steps, tiles(64) * (steps + 2) / 480.f));
     return best;
   }
-  offer(64, 1, through, 3.f + std::max(0.28f * steps, tiles(64) * (steps + 4) / 1450.f));
-  offer(128, 1, through && glu, 3.4f + std::max(0.42f * steps, tiles(128) * (steps + 8) / 600.f));
-  const long t = (long)tiles(256), full = t / kCus, rest = t % kCus;
-  offer(256, 1, false, 4.f + full * (1.4f * steps + 5.f) + (rest ? (1.f + 0.4f * rest / kCus) * steps + 5.f : 0.f));
+  offer(64, 1, through, 3.f + std::max(0.28f * steps, tiles(64) * (steps + 4) / 1450.f) + (other ? 0.7f : 0.f));
+  const long on_one = (tiles(128) + kCus - 1) / kCus;
+  offer(128, 1, through && glu, 3.4f + on_one * 0.5f * (steps + (on_one > 1 ? 1 : 0)) + (other ? 1.f + on_one * 1.8f : 0.f));
+  const long full = tiles(256) / kCus, rest = tiles(256) % kCus;
+  const float ends = 6.f + (other ? 12.f : 0.f) + (N % 256 || M % 256 ? 3.f : 0.f);
+  offer(256, 1, false, 4.f + full * (1.4f * steps + ends) + (rest ? (1.f + 0.4f * rest / kCus) * steps + ends : 0.f));
   return best;
 }
 
@@ -961,16 +1014,23 @@ hipError_t launch_quantize(const QuantizeArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-static int out_kind(const Fp8ProductArgs& p) { return p.os ? kOut8 : p.dtype == kF32 ? kOut32 : kOut16; }
+static int out_kind(int dtype, bool into8) { return into8 ? kOut8 : dtype == kF32 ? kOut32 : kOut16; }
 
 // fp32 elements of the workspace that such a call needs
 long fp8_product_workspace(long M, long N, long K, int act, int dtype, bool into8) {
-  return M > 0 && fp8_plan(M, N, K, act, into8 ? kOut8 : dtype == kF32 ? kOut32 : kOut16).through ? M * N : 0;
+  return M > 0 && fp8_plan(M, N, K, act, out_kind(dtype, into8)).through ? M * N : 0;
+}
+
+void fp8_product_plan(long M, long N, long K, int act, int dtype, bool into8, int* side, int* parts, int* through) {
+  const Fp8Plan plan = fp8_plan(M, N, K, act, out_kind(dtype, into8));
+  *side = plan.side;
+  *parts = plan.parts;
+  *through = plan.through;
 }
 
 hipError_t launch_fp8_product(const Fp8ProductArgs& args, float* workspace, hipStream_t st) {
   if (args.M <= 0) return hipSuccess;
-  const int out = out_kind(args);
+  const int out = out_kind(args.dtype, args.os != nullptr);
   const Fp8Plan plan = fp8_plan(args.M, args.N, args.K, args.act, out);
   Fp8ProductArgs p = args;
   if (plan.through) {
@@ -980,7 +1040,8 @@ hipError_t launch_fp8_product(const Fp8ProductArgs& args, float* workspace, hipS
     p.os = nullptr;
   }
   hipError_t e;
-  if (plan.side == 0) e = out == kOut32 ? launch_thin<kOut32>(p, plan.parts, st) : launch_thin<kOut16>(p, plan.parts, st);
+  if (plan.side == 0)
+    e = out == kOut32 ? launch_thin<kOut32>(p, plan.parts, st) : p.os ? launch_thin<kOut8>(p, 1, st) : launch_thin<kOut16>(p, plan.parts, st);
   else if (out == kOut32) e = launch_tiles<64, kOut32>(p, st);
   else if (plan.side == 64) e = launch_tiles<64, kOut16>(p, st);
   else if (plan.side == 128) e = p.os ? launch_tiles<128, kOut8>(p, st) : launch_tiles<128, kOut16>(p, st);

@@ -580,6 +580,9 @@ int ccq_norm_fp8_fwd(const void* x, int64_t ldx, const void* r, int64_t ldr, con
  * not looked at).  workspace: ccq_fp8_linear_workspace_bytes bytes (into8 not 0: the output in 8 bits), for outputs in 8
  * bits of few rows.
  */
+/* How such a product runs: sides of its square tiles (256, 128, 64; 0: 16 columns of 16 rows to a wave, in parts of the
+ * contraction), and whether it goes through the workspace. */
+int ccq_fp8_linear_plan(int64_t M, int64_t N, int64_t K, int act, int dtype, int into8, int* side, int* parts, int* through);
 size_t ccq_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, int dtype, int into8);
 int ccq_fp8_linear(const void* x, int64_t ldx, const void* xs, int64_t ldxs, const void* weight, int64_t ldw,
                    const void* ws, int64_t ldws, const void* bias, int bdtype, const void* r, int64_t ldr, void* y,
