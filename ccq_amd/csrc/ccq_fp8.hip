@@ -958,9 +958,11 @@ struct Fp8Plan {
 //   64: 0.28 a step where the CUs have few tiles (1024 over 1024, 300 rows: 5.5, 128 tiles 7.3, 256 16.5), 1450 tiles and
 //     steps a us (1024 over 1024, 2000 rows 6.9, 128 tiles 7.8; 2188 over 959, 4363 rows 25, 22); exactly: 0.83 and 480
 //   128: half a step's microsecond for each tile of a CU (2816 over 1024, 16384 rows 57.3, silu 71, gelu 84; 256 tiles 57.9,
-//     90, 111; 3520 over 3008, 25960 rows 316, 317, 344; 255, 302, 350; 2188 over 959, 4363 rows 22, 25, 29; 30, 35, 42)
-//   256: a round of all CUs 1.4 a step (8192^3 365; fewer workgroups 1.0) and 5 for the outputs, more where they end inside
-//     a tile
+//     90, 111; 3520 over 3008, 25960 rows 316, 317, 344; 255, 302, 350; 2188 over 959, 4363 rows 22, 25, 29; 30, 35, 42;
+//     4096 over 4096, 2048 rows 35, 4096 rows 66; 47, 62), more where outputs end inside a tile (1100 over 700, 600 rows
+//     9.6, 1024 over 1024 7.8)
+//   256: a round of all CUs 1.4 a step (8192^3 365; fewer workgroups 1.0), and the outputs, more where they end inside a tile
+//     (swiglu 2816 over 1024, 9000 rows 74, 128 tiles 63; 16384 rows 104, 108; 1024 over 2816, 30000 rows 78, 91)
 //   through fp32: the second launch (its host time too), and 8 bytes an output to and fro
 Fp8Plan fp8_plan(long M, long N, long K, int act, int out) {
   const bool glu = act == kActSwiglu, other = !glu && act != kActNone;
@@ -968,7 +970,7 @@ Fp8Plan fp8_plan(long M, long N, long K, int act, int out) {
   Fp8Plan best{256, 1, false};
   float least = 0.f;
   auto offer = [&](int side, int parts, bool through, float t) {
-    if (through) t += 4.f + 1.3e-6f * M * N;
+    if (through) t += 5.f + 1.3e-6f * M * N;
     if (least == 0.f || t < least) {
       least = t;
       best = {side, parts, through};
@@ -993,7 +995,7 @@ Fp8Plan fp8_plan(long M, long N, long K, int act, int out) {
   }
   offer(64, 1, through, 3.f + std::max(0.28f * steps, tiles(64) * (steps + 4) / 1450.f) + (other ? 0.7f : 0.f));
   const long on_one = (tiles(128) + kCus - 1) / kCus;
-  offer(128, 1, through && glu, 3.4f + on_one * 0.5f * (steps + (on_one > 1 ? 1 : 0)) + (other ? 1.f + on_one * 1.8f : 0.f));
+  offer(128, 1, through && glu, 4.f + (N % 128 || M % 128 ? 2.f : 0.f) + on_one * 0.5f * (steps + (on_one > 1 ? 1 : 0)) + (other ? 1.f + on_one * 1.8f : 0.f));
   const long full = tiles(256) / kCus, rest = tiles(256) % kCus;
   const float ends = 6.f + (other ? 12.f : 0.f) + (N % 256 || M % 256 ? 3.f : 0.f);
   offer(256, 1, false, 4.f + full * (1.4f * steps + ends) + (rest ? (1.f + 0.4f * rest / kCus) * steps + ends : 0.f));

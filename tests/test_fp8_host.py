@@ -159,9 +159,42 @@ def test_abi_refusals():
     assert linear(y=None) == NULL
     assert linear(x=ctypes.c_void_p(0x1008)) == ALIGN and linear(xs=ODD) == ALIGN and linear(ws=ODD) == ALIGN
     assert linear(y=ODD) == ALIGN and linear(b=ODD) == ALIGN and linear(r=ODD, ldr=32) == ALIGN
-    assert linear(ys=P, ldys=4, K=2000, ldx=2000, ldw=2000, ldxs=16, ldws=16, work=None) == NULL  # (few rows: through fp32)
+    # few rows, long: through fp32 (which sizes go that way is the plan's, and asked first)
+    K = 16384
+    assert lib.ccq_fp8_linear_workspace_bytes(4, 32, K, 0, 0, 1) > 0
+    assert linear(ys=P, ldys=4, K=K, ldx=K, ldw=K, ldxs=K // 128, ldws=K // 128, work=None) == NULL
     assert linear(work=ODD) == ALIGN
     assert linear(M=0) == 0
     size = lib.ccq_fp8_linear_workspace_bytes
-    assert size(4, 32, 2000, 0, 0, 1) == 4 * 32 * 4 and size(4, 32, 2000, 0, 0, 0) == 0 and size(0, 32, 2000, 0, 0, 1) == 0
+    assert size(4, 32, K, 0, 0, 1) == 4 * 32 * 4 and size(4, 32, K, 0, 0, 0) == 0 and size(0, 32, K, 0, 0, 1) == 0
     assert size(32768, 4096, 4096, 0, 0, 1) == 0
+
+
+def test_plan_refusals():
+    lib = _lib.load()
+    a, b, c = (ctypes.byref(ctypes.c_int()) for _ in range(3))
+    for size in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (1 << 31, 1, 1)):
+        assert lib.ccq_fp8_linear_plan(*size, 0, 0, 0, a, b, c) == -1
+    assert lib.ccq_fp8_linear_plan(1, 1, 1, 9, 0, 0, a, b, c) == -1
+    assert lib.ccq_fp8_linear_plan(1, 1, 1, 0, 9, 0, a, b, c) == -1
+    assert lib.ccq_fp8_linear_plan(1, 1, 1, 0, 0, 0, a, b, None) == -2
+    assert lib.ccq_fp8_linear_plan(1, 1, 1, 0, 9, 1, a, b, c) == 0
+
+
+def test_plan_and_workspace_agree():
+    """An output goes through the workspace where the plan says so, and only one in 8 bits does."""
+    lib = _lib.load()
+    seen = set()
+    for M in (1, 5, 16, 64, 300, 1000, 1100, 5000, 70000):
+        for N in (1, 129, 700, 4096, 40000):
+            for K in (1, 130, 1000, 8192):
+                for act in (0, 3, 5):
+                    for dtype, into8 in ((0, 0), (2, 0), (0, 1)):
+                        a, b, c = (ctypes.c_int() for _ in range(3))
+                        assert lib.ccq_fp8_linear_plan(M, N, K, act, dtype, into8, *map(ctypes.byref, (a, b, c))) == 0
+                        room = lib.ccq_fp8_linear_workspace_bytes(M, N, K, act, dtype, into8)
+                        assert room == (4 * M * N if c.value else 0) and (into8 or not c.value)
+                        assert a.value in (0, 64, 128, 256) and (b.value == 1 or a.value == 0 and b.value in (2, 4, 8))
+                        assert a.value or M <= 1024
+                        seen.add((a.value, dtype, into8, c.value))
+    assert {s[0] for s in seen} == {0, 64, 128, 256} and {s[3] for s in seen} == {0, 1}
