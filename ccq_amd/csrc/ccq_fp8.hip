@@ -93,22 +93,34 @@ __device__ __forceinline__ void load4_to(unsigned lds, const void* from) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(from) : "memory", "m0");
 }
 
-// eight e4m3 (bytes 8 c .. of a fragment) in bf16, exactly
-__device__ __forceinline__ bf16x8 widen(const i32x8& f, int c) {
+// eight e4m3 (bytes 8 c .. of a fragment) times a power of two in bf16, exactly (within bf16's range)
+__device__ __forceinline__ bf16x8 widen(const i32x8& f, int c, float scale = 1.f) {
   bf16x8 o;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const bf16x2 v = (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * c + i / 2], 1.f, true)
-                             : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * c + i / 2], 1.f, false);
+    const bf16x2 v = (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * c + i / 2], scale, true)
+                             : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f[2 * c + i / 2], scale, false);
     o[2 * i] = v[0];
     o[2 * i + 1] = v[1];
   }
   return o;
 }
 
+// The scale of a byte, 2^(e - 127).  Those of bytes 77 .. 177 may go into the widened values: 2^-59 .. 2^59 with them in
+// bf16, and their products 2^-118 .. 2^118 in fp32.
+constexpr int kNearOne = 77;
+constexpr unsigned kNearMost = 100;
+__device__ __forceinline__ float scale_of(int byte) { return __uint_as_float((unsigned)byte << 23); }
+
 // c += a b 2^(ea + eb - 254), exactly but for fp32's additions; lane l holds the scales of rows l & 15 of both
 __device__ __forceinline__ void exact_product(const i32x8& a, int ea, const i32x8& b, int eb, f32x4& c) {
   f32x4 sum{0.f, 0.f, 0.f, 0.f};
+  if (__all(max((unsigned)(ea - kNearOne), (unsigned)(eb - kNearOne)) <= kNearMost)) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum = mfma16(widen(a, k, scale_of(ea)), widen(b, k, scale_of(eb)), sum);
+    c += sum;
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < 4; ++k) sum = mfma16(widen(a, k), widen(b, k), sum);
 #pragma unroll
@@ -151,7 +163,7 @@ enum : int { kOut16 = 0, kOut32 = 1, kOut8 = 2 };
 // middle: there stand the barriers, and behind each of them those halves of the step after next are loaded, between
 // products, a step and a half before they are read.
 template <int BM, int BN, int WM, int WN, int ACT, int OUT>
-__global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8ProductArgs p) {
+__global__ __launch_bounds__(WM * WN * 64, OUT == kOut32 ? 3 : 1) void fp8_product_kernel(const Fp8ProductArgs p) {
   constexpr bool GLU = ACT == kActSwiglu, EXACT = OUT == kOut32;
   constexpr int NW = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, HALF = BN / WN / 2, HM = TM / 2, HN = TN / 2;
   constexpr int GA = std::min(TM, 4), GB = std::min(GLU ? TN / 2 : TN, 4);
@@ -269,9 +281,38 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     }
   };
   bool nan_row[EXACT ? TM : 1], nan_column[kScaleSets][4];  // a scale that is NaN was met
-  // all products of a step, exactly
-  auto multiply = [&](const Frag (&a)[TM], const Frag (&b)[TN], const ColumnScales (&c)[kScaleSets]) {
+  // All products of a step, exactly.  Scales near one go into the widened values (4096^3 218 -> 184 us), others are applied
+  // to the block's sums.
+  auto multiply = [&](const Frag (&a)[TM], const Frag (&b)[TN], unsigned scale) {
     if constexpr (EXACT) {
+      unsigned off = 0;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) off = max(off, (unsigned)(a[i].e - kNearOne));
+#pragma unroll
+      for (int j = 0; j < TN; ++j) off = max(off, (unsigned)(b[j].e - kNearOne));
+      if (__all(off <= kNearMost)) {
+        bf16x8 wide[TN][4];
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) wide[j][k] = widen(b[j].v, k, scale_of(b[j].e));
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          bf16x8 row[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) row[k] = widen(a[i].v, k, scale_of(a[i].e));
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            f32x4 sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum = mfma16(wide[j][k], row[k], sum);
+            acc[i][j] += sum;
+          }
+        }
+        return;
+      }
+      ColumnScales c[kScaleSets];
+      read_columns(c, scale);
       bf16x8 wide[TN][4];
 #pragma unroll
       for (int j = 0; j < TN; ++j)
@@ -433,36 +474,21 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     for (int i = 0; i < TM; ++i) nan_row[i] = false;
     for (int j = 0; j < kScaleSets; ++j)
       for (int q = 0; q < 4; ++q) nan_column[j][q] = false;
-    // A step's fragments are read whole while the step before is multiplied, which keeps the vector unit busy.
-    wait_loads<2 * PL>();
-    lds_barrier();
-    if (whole > 0) {
-      Frag a[2][TM], b[2][TN];
-      ColumnScales c[2][kScaleSets];
-      auto read_step = [&](int s, Frag (&a)[TM], Frag (&b)[TN], ColumnScales (&c)[kScaleSets]) {
-        const unsigned stage = (s & 1) * kStage, scale = scale_at(s);
+    for (int s = 0; s < whole; ++s) {
+      const unsigned stage = (s & 1) * kStage, scale = scale_at(s);
+      Frag a[TM], b[TN];
+      wait_loads<2 * PL>();
+      lds_barrier();
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          read(b[i], fb, eb0, i, stage, scale);
-          read(a[i], fa, ea0, i, stage, scale);
-        }
-        read_columns(c, scale);
-      };
-      auto plain_step = [&](int s, int now) {
-        wait_loads<0>();
-        lds_barrier();
-        if ((s & 3) == 0) load_scales((s >> 2) + 1);
-        read_step(s + 1, a[now ^ 1], b[now ^ 1], c[now ^ 1]);
-        load_step(s + 2);
-        multiply(a[now], b[now], c[now]);
-      };
-      read_step(0, a[0], b[0], c[0]);
-      int s = 0;
-      for (; s + 2 <= whole; s += 2) {
-        plain_step(s, 0);
-        plain_step(s + 1, 1);
-      }
-      if (s < whole) plain_step(s, 0);
+      for (int j = 0; j < TN; ++j) read(b[j], fb, eb0, j, stage, scale);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) read(a[i], fa, ea0, i, stage, scale);
+      lds_barrier();
+      if ((s & 3) == 0) load_scales((s >> 2) + 1);
+      load_step(s + 2);
+      multiply(a, b, scale);
+    }
+    if (whole > 0) {
       wait_loads<0>();
       lds_barrier();
     }
@@ -518,14 +544,12 @@ __global__ __launch_bounds__(WM * WN * 64) void fp8_product_kernel(const Fp8Prod
     }
     if constexpr (EXACT) {
       Frag a[TM];
-      ColumnScales c[kScaleSets];
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         read(a[i], fa, ea0, i, stage, scale);
         a[i].v &= mask;
       }
-      read_columns(c, scale);
-      multiply(a, b, c);
+      multiply(a, b, scale);
     } else {
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
@@ -952,11 +976,11 @@ struct Fp8Plan {
 };
 // By what a call is expected to take, in us, out of measured times (`steps` of 128; an activation without a gate is code
 // that a tile's outputs pass through: `act`):
-//   side 0: a workgroup a CU, 0.29 a step of a wave (swiglu 0.45, exactly 0.52), or the weight's bytes.  1024 over 1024, 64
+//   side 0: a workgroup a CU, 0.29 a step of a wave (swiglu 0.45, exactly 0.46), or the weight's bytes.  1024 over 1024, 64
 //     rows: 4.3 in eight parts, 5.9 in one, by 64 tiles 5.5; 4064 over 1728, 40 rows 10.9, 7.8 (two parts 6.0), 7.4; 2816
 //     over 1024, 600 rows 78, 20, 6.8
 //   64: 0.28 a step where the CUs have few tiles (1024 over 1024, 300 rows: 5.5, 128 tiles 7.3, 256 16.5), 1450 tiles and
-//     steps a us (1024 over 1024, 2000 rows 6.9, 128 tiles 7.8; 2188 over 959, 4363 rows 25, 22); exactly: 0.83 and 480
+//     steps a us (1024 over 1024, 2000 rows 6.9, 128 tiles 7.8; 2188 over 959, 4363 rows 25, 22); exactly: 0.62 and 740
 //   128: half a step's microsecond for each tile of a CU (2816 over 1024, 16384 rows 57.3, silu 71, gelu 84; 256 tiles 57.9,
 //     90, 111; 3520 over 3008, 25960 rows 316, 317, 344; 255, 302, 350; 2188 over 959, 4363 rows 22, 25, 29; 30, 35, 42;
 //     4096 over 4096, 2048 rows 35, 4096 rows 66; 47, 62), more where outputs end inside a tile (1100 over 700, 600 rows
@@ -980,7 +1004,7 @@ Fp8Plan fp8_plan(long M, long N, long K, int act, int out) {
   const bool exact = out == kOut32, through = out == kOut8;
   if (M <= 1024) {
     const long groups = (N + 15) / 16 * ((M + 15) / 16);
-    const float step = exact ? 0.52f : glu ? 0.45f : 0.29f, bytes = 1.5f + outs * K / 5e6f;
+    const float step = exact ? 0.46f : glu ? 0.45f : 0.29f, bytes = 1.5f + outs * K / 5e6f;
     auto time = [&](int parts) {
       const long wgs = (groups * parts + kThinWaves - 1) / kThinWaves, rounds = (wgs + kCus - 1) / kCus;
       const float part = step * ((steps + parts - 1) / parts);
@@ -990,7 +1014,7 @@ Fp8Plan fp8_plan(long M, long N, long K, int act, int out) {
     if (through) offer(0, 1, false, time(1));
   }
   if (exact) {
-    offer(64, 1, false, 2.5f + std::max(0.83f * steps, tiles(64) * (steps + 2) / 480.f));
+    offer(64, 1, false, 3.5f + std::max(0.62f * steps, tiles(64) * (steps + 2) / 740.f));
     return best;
   }
   offer(64, 1, through, 3.f + std::max(0.28f * steps, tiles(64) * (steps + 4) / 1450.f) + (other ? 0.7f : 0.f));

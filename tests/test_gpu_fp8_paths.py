@@ -51,7 +51,7 @@ CASES = [((3, 37, 1000), "0/8 0/8 0/8 0/8 0/1 0/1 0/1"),
          ((30, 1030, 513), "64 0/4 64 0/4 0/1 0/1 0/1"),
          ((33, 4100, 2000), "0/2 0/2 64 0/2 0/1 0/1 0/1"),
          ((900, 300, 600), "64 64 64 0/1 0/1 0/1 0/1"),
-         ((250, 530, 300), "64 64 64 64 0/1 0/1 0/1"),
+         ((250, 530, 300), "64 64 64 0/2 0/1 0/1 0/1"),
          ((600, 1100, 700), "64 64 64 64 128 0/1 64t"),
          ((1, 129, 4100), "0/8 0/8 0/8 0/8 0/8t 0/8t 0/8t"),
          ((1100, 520, 90), "64 64 64 64 128 128 64t"),
