@@ -111,6 +111,14 @@ def test_norm(rows, D, dtype, wdtype, residual):
     check_rounded(got.values, got.scales, y, ((D + 2) / 2 + 6) * 2.0 ** -24 * y.abs())
 
 
+@pytest.mark.parametrize("residual", [False, True], ids=["", "residual"])
+@pytest.mark.parametrize("dtype,rows,D", [(BF, 5, 4104), (HF, 3, 7271), (FL, 3, 2052), (FL, 2, 4096), (FL, 2, 5003), (BF, 1500, 5000)],
+                         ids=str)
+def test_norm_wide(dtype, rows, D, residual):
+    """Rows of more than two pieces a lane, and more of them than workgroups."""
+    test_norm(rows, D, dtype, FL, residual)
+
+
 def test_norm_without_weight_strides_and_other_shapes():
     from ccq_amd import quantize_fp8, rms_norm, rms_norm_fp8
     dev = _cuda()
