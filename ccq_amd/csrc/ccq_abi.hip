@@ -1852,7 +1852,7 @@ int ccq_fp8_linear(const void* x, int64_t ldx, const void* xs, int64_t ldxs, con
                    int64_t ldy, void* ys, int64_t ldys, void* workspace, int64_t M, int64_t N, int64_t K, int act, int dtype, void* stream) {
   const char* who = "ccq_fp8_linear";
   if (M < 0 || N < 1 || K < 1 || M > kMaxSide || N > kMaxSide || linear_outs(N, act) > kMaxStride || K > kMaxStride ||
-      ((M + 63) / 64) * ((linear_outs(N, act) + 63) / 64) > kMaxTiles)
+      ((M + 63) / 64) * ((linear_outs(N, act) + 63) / 64) >= kMaxTiles)
     return fail(CCQ_ERR_SHAPE, "%s: M=%lld N=%lld K=%lld", who, (long long)M, (long long)N, (long long)K);
   if (act < CCQ_ACT_NONE || act > CCQ_ACT_SWIGLU || !dtype_ok(bdtype) || (!ys && !dtype_ok(dtype)))
     return fail(CCQ_ERR_SHAPE, "%s: act=%d dtype=%d bdtype=%d", who, act, dtype, bdtype);

@@ -154,6 +154,7 @@ def test_abi_refusals():
     assert linear(ldx=200) == SHAPE and linear(ldw=192) == SHAPE and linear(ldxs=3) == SHAPE and linear(ldws=0) == SHAPE
     assert linear(ys=P, ldys=4, ldy=24) == SHAPE and linear(ys=P, ldys=2) == SHAPE
     assert linear(ys=P, ldys=4, r=P, ldr=32) == SHAPE
+    assert linear(M=1 << 18, N=1 << 18) == SHAPE    # 2^24 tiles of 64: 2^32 work items, one more than a launch holds
     assert linear(M=1 << 30, N=1 << 22) == SHAPE and linear(N=(1 << 21) + 1, act=5) == SHAPE
     assert linear(x=None) == NULL and linear(xs=None) == NULL and linear(w=None) == NULL and linear(ws=None) == NULL
     assert linear(y=None) == NULL
