@@ -110,6 +110,7 @@ struct Fp8ProductArgs {
   const void* res;          // [M, N] of dtype, row stride ldr (nullable)
   long ldr;
   int act, bdtype, dtype;
+  int later;  // of tiles of 256: by how much some workgroups begin later (set at the launch)
 };
 
 }  // namespace ccq

@@ -453,6 +453,13 @@ __global__ __launch_bounds__(WM * WN * 64, OUT == kOut32 ? 3 : 1) void fp8_produ
     load_step(0);
     load_step(1);
   };
+  // Some workgroups begin half a tile later, so that not all of them multiply at once and store at once: where the last
+  // round is not full those that have a tile less, otherwise every other one.
+  if constexpr (kMany) {
+    const int k0 = blockIdx.x >> 3, rounds = (tiles + (int)gridDim.x - 1) / (int)gridDim.x;
+    const bool later = tiles % (int)gridDim.x ? k0 + (rounds - 1) * stride >= mine : k0 & 1;
+    for (int i = later ? 0 : p.later; i < p.later; ++i) __builtin_amdgcn_s_sleep(16);  // (1024 cycles)
+  }
   place(blockIdx.x >> 3);
   begin();
   bool counted = false;  // kStores stores or more follow the loads
@@ -961,11 +968,24 @@ hipError_t launch_thin(const Fp8ProductArgs& p, int parts, hipStream_t st) {
   return hipGetLastError();
 }
 
+// Half a tile of 256 in units of 1024 cycles, by which some workgroups begin later; 0 where that costs more than it gives.
+// Where the last round is not full it costs nothing: 16384 x 2816 swiglu over 1024 into 8 bits 111 -> 104 us, into bf16 109 ->
+// 106, 16384 x 2816 58.6 -> 55.0.  Full rounds end half a tile later: 65536 x 2816 swiglu over 1024 into 8 bits (22 rounds)
+// 413 -> 365, into bf16 390 -> 363, 16384 x 4096 over 1024 (4) 79.9 -> 76.9, but 8192^3 (4) 384 -> 395, 65536 x 1024 over 2816
+// (4) 165 -> 177.
+int half_tile(long tiles, long steps) {
+  const long rounds = (tiles + kCus - 1) / kCus;
+  const float tile = 1.4f * steps + 6.f;  // us, each of 2 units
+  return rounds > 1 && (tiles % kCus || rounds * 4.5f > tile) ? (int)std::min(tile, 1000.f) : 0;
+}
+
 template <int BM, int OUT>
-hipError_t launch_tiles(const Fp8ProductArgs& p, hipStream_t st) {
+hipError_t launch_tiles(const Fp8ProductArgs& args, hipStream_t st) {
   constexpr int BN = BM, WM = 2, WN = 2;
+  Fp8ProductArgs p = args;
   const int NT = p.act == kActSwiglu ? BN / 2 : BN;
   const long tiles = ((p.M + BM - 1) / BM) * ((p.N + NT - 1) / NT);
+  p.later = BM == 256 ? half_tile(tiles, (p.K + kStep - 1) / kStep) : 0;
   const dim3 grid((unsigned)(BM == 256 ? std::min<long>(tiles, kCus) : tiles)), block(WM * WN * 64);
   if (p.act == kActSwiglu) {
     if constexpr (OUT != kOut8 || BN == 256) hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActSwiglu, OUT>), grid, block, 0, st, p);
