@@ -166,7 +166,7 @@ enum : int { kOut16 = 0, kOut32 = 1, kOut8 = 2 };
 //
 // Bound by the matrix cores: a step of a 256 tile takes 1.4 us, its instructions alone 1.1.  8192^3 365 - 400 us (2.75 - 3.0
 // PFLOP/s; fragments read a whole step at a time 727, halves loaded a step ahead 440); 32768 x 1024 over 2816 with residual
-// 92; 16384 x 2816 swiglu over 1024 into 8 bits 104 - 111, of which the outputs' arithmetic, with one wave a SIMD, is a third.
+// 92; 16384 x 2816 swiglu over 1024 into 8 bits 99 - 104, of which the outputs' arithmetic, with one wave a SIMD, is a third.
 // In fp32 (exactly) the conversions bound it, 64 a step and wave at half rate: 4096^3 184 us; fragments are held once and
 // read between two barriers, so that three workgroups share a CU.
 template <int BM, int BN, int WM, int WN, int ACT, int OUT>
