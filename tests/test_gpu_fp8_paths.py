@@ -63,7 +63,9 @@ CASES = [((3, 37, 1000), "0/8 0/8 0/8 0/8 0/1 0/1 0/1"),
          ((16300, 2040, 2100), "256 128 256 64 256 128 256"),
          ((16301, 2047, 4100), "256 256 256 64 256 256 256"),
          ((16384, 2048, 2176), "256 256 256 64 256 256 256"),
-         ((8190, 4097, 1100), "128 128 128 64 128 128 256")]
+         ((8190, 4097, 1100), "128 128 128 64 128 128 256"),
+         ((16384, 4096, 1040), "256 128 256 64 256 128 256"),
+         ((8192, 4096, 300), "128 128 128 64 128 128 256")]
 
 
 @pytest.mark.parametrize("size,ways", CASES, ids=lambda c: "x".join(map(str, c)) if isinstance(c, tuple) else "")
