@@ -1857,6 +1857,7 @@ int ccq_fp8_linear(const void* x, int64_t ldx, const void* xs, int64_t ldxs, con
   if (act < CCQ_ACT_NONE || act > CCQ_ACT_SWIGLU || !dtype_ok(bdtype) || (!ys && !dtype_ok(dtype)))
     return fail(CCQ_ERR_SHAPE, "%s: act=%d dtype=%d bdtype=%d", who, act, dtype, bdtype);
   if (r && (ys || ldr < N)) return fail(CCQ_ERR_SHAPE, "%s: a residual of row stride %lld (N=%lld; none of an output in 8 bits)", who, (long long)ldr, (long long)N);
+  if (!ys && ldy && ldy < N) return fail(CCQ_ERR_SHAPE, "%s: row stride %lld of y below N=%lld", who, (long long)ldy, (long long)N);
   if (int e = fp8_rows_check(who, "x", x, ldx, xs, ldxs, K)) return e;
   if (int e = fp8_rows_check(who, "weight", weight, ldw, ws, ldws, K)) return e;
   if (ys)
@@ -1871,7 +1872,7 @@ int ccq_fp8_linear(const void* x, int64_t ldx, const void* xs, int64_t ldxs, con
   Fp8ProductArgs p{};
   p.a = (const unsigned char*)x; p.lda = ldx; p.sa = (const unsigned char*)xs; p.lsa = ldxs;
   p.b = (const unsigned char*)weight; p.ldb = ldw; p.sb = (const unsigned char*)ws; p.lsb = ldws;
-  p.M = M; p.N = N; p.K = K; p.out = y; p.ldo = ys ? ldy : N; p.os = (unsigned char*)ys; p.los = ldys;
+  p.M = M; p.N = N; p.K = K; p.out = y; p.ldo = ldy ? ldy : N; p.os = (unsigned char*)ys; p.los = ldys;
   p.bias = bias; p.bdtype = bdtype; p.res = r; p.ldr = ldr; p.act = act; p.dtype = dtype;
   hipStream_t st = (hipStream_t)stream;
   return hip_status(timed("linear_fp8", st, [&] { return launch_fp8_product(p, (float*)workspace, st); }), who);

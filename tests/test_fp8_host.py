@@ -199,3 +199,15 @@ def test_plan_and_workspace_agree():
                         assert a.value or M <= 1024
                         seen.add((a.value, dtype, into8, c.value))
     assert {s[0] for s in seen} == {0, 64, 128, 256} and {s[3] for s in seen} == {0, 1}
+
+
+def test_abi_stride_of_16_bit_outputs():
+    """y in 16 or 32 bits has a row stride as the other rows have: 0 (contiguous) or N and more."""
+    lib = _lib.load()
+
+    def linear(ldy, M=4, dt=0):
+        return lib.ccq_fp8_linear(P, 208, P, 4, P, 208, P, 4, None, 0, None, 0, P, ldy, None, 0, P, M, 32, 200, 0, dt, None)
+
+    for dt in (0, 1, 2):
+        assert linear(31, dt=dt) == SHAPE and linear(-32, dt=dt) == SHAPE and linear(1, dt=dt) == SHAPE
+        assert linear(0, M=0, dt=dt) == 0 and linear(32, M=0, dt=dt) == 0 and linear(40, M=0, dt=dt) == 0
