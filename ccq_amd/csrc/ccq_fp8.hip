@@ -987,8 +987,10 @@ hipError_t launch_tiles(const Fp8ProductArgs& args, hipStream_t st) {
   const long tiles = ((p.M + BM - 1) / BM) * ((p.N + NT - 1) / NT);
   p.later = BM == 256 ? half_tile(tiles, (p.K + kStep - 1) / kStep) : 0;
   const dim3 grid((unsigned)(BM == 256 ? std::min<long>(tiles, kCus) : tiles)), block(WM * WN * 64);
+  if (BM == 256 && OUT == kOut16 && p.dtype == kF32) return hipErrorInvalidConfiguration;  // (tiles of 256: 16 bits)
   if (p.act == kActSwiglu) {
-    if constexpr (OUT != kOut8 || BN == 256) hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActSwiglu, OUT>), grid, block, 0, st, p);
+    if constexpr (OUT == kOut8 && BN < 256) return hipErrorInvalidConfiguration;  // (a tile's outputs: half a block)
+    else hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActSwiglu, OUT>), grid, block, 0, st, p);
   } else if (p.act == kActNone) {
     hipLaunchKernelGGL((fp8_product_kernel<BM, BN, WM, WN, kActNone, OUT>), grid, block, 0, st, p);
   } else {
@@ -1098,7 +1100,7 @@ hipError_t launch_fp8_product(const Fp8ProductArgs& args, float* workspace, hipS
   if (plan.side == 0)
     e = out == kOut32 ? launch_thin<kOut32>(p, plan.parts, st) : p.os ? launch_thin<kOut8>(p, 1, st) : launch_thin<kOut16>(p, plan.parts, st);
   else if (out == kOut32) e = launch_tiles<64, kOut32>(p, st);
-  else if (plan.side == 64) e = launch_tiles<64, kOut16>(p, st);
+  else if (plan.side == 64) e = p.os ? hipErrorInvalidConfiguration : launch_tiles<64, kOut16>(p, st);
   else if (plan.side == 128) e = p.os ? launch_tiles<128, kOut8>(p, st) : launch_tiles<128, kOut16>(p, st);
   else e = p.os ? launch_tiles<256, kOut8>(p, st) : launch_tiles<256, kOut16>(p, st);
   if (e != hipSuccess || !plan.through) return e;

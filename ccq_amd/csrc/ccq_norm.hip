@@ -371,18 +371,21 @@ long norm_groups(const NormShape& s, long rows) {  // workgroups that give every
   return (rows + per - 1) / per;
 }
 
+// A shape for which no kernel is compiled is an error, not a call that leaves its outputs as they were.
 template <typename T, bool LAYER>
-void launch_typed(bool bwd, const NormArgs& a, const NormShape& s, unsigned blocks, hipStream_t st) {
+hipError_t launch_typed(bool bwd, const NormArgs& a, const NormShape& s, unsigned blocks, hipStream_t st) {
   const dim3 block(s.wpr == 16 ? 1024 : kThreads);
 #define CCQ_NORM(W, PP)                                                                                        \
   if (s.wpr == W && s.p == PP) {                                                                               \
     constexpr bool Q8 = !LAYER && (W != 16 || PP != 1); /* (4 waves hold those rows) */                        \
+    if (a.scales && (bwd || !Q8)) return hipErrorInvalidConfiguration;                                         \
     if (bwd)                                                                                                   \
       hipLaunchKernelGGL((norm_bwd_kernel<T, LAYER, W, PP>), dim3(blocks), block, 0, st, a, s.lanes);          \
-    else if (!Q8 || !a.scales)                                                                                 \
+    else if (!a.scales)                                                                                        \
       hipLaunchKernelGGL((norm_fwd_kernel<T, LAYER, W, PP, false>), dim3(blocks), block, 0, st, a, s.lanes);   \
     else                                                                                                       \
       hipLaunchKernelGGL((norm_fwd_kernel<T, LAYER, W, PP, Q8>), dim3(blocks), block, 0, st, a, s.lanes);      \
+    return hipGetLastError();                                                                                  \
   }
   CCQ_NORM(1, 1) CCQ_NORM(1, 2) CCQ_NORM(4, 1) CCQ_NORM(4, 2) CCQ_NORM(16, 1)
   if constexpr (sizeof(T) == 4) {  // (8192 of two bytes are one piece a thread)
@@ -390,20 +393,23 @@ void launch_typed(bool bwd, const NormArgs& a, const NormShape& s, unsigned bloc
   }
 #undef CCQ_NORM
   if constexpr (!LAYER)
-    if (s.p == 4) hipLaunchKernelGGL((norm_fwd_kernel<T, false, 4, 4, true>), dim3(blocks), block, 0, st, a, s.lanes);
+    if (s.wpr == 4 && s.p == 4 && a.scales && !bwd) {
+      hipLaunchKernelGGL((norm_fwd_kernel<T, false, 4, 4, true>), dim3(blocks), block, 0, st, a, s.lanes);
+      return hipGetLastError();
+    }
+  return hipErrorInvalidConfiguration;
 }
 
-void launch_norm(bool bwd, const NormArgs& a, unsigned blocks, hipStream_t st) {
+hipError_t launch_norm(bool bwd, const NormArgs& a, unsigned blocks, hipStream_t st) {
   const NormShape s = norm_shape(a.D, a.dtype, a.scales);
   if (a.layer) {
-    if (a.dtype == kBf16) launch_typed<bf16, true>(bwd, a, s, blocks, st);
-    else if (a.dtype == kF16) launch_typed<f16, true>(bwd, a, s, blocks, st);
-    else launch_typed<float, true>(bwd, a, s, blocks, st);
-  } else {
-    if (a.dtype == kBf16) launch_typed<bf16, false>(bwd, a, s, blocks, st);
-    else if (a.dtype == kF16) launch_typed<f16, false>(bwd, a, s, blocks, st);
-    else launch_typed<float, false>(bwd, a, s, blocks, st);
+    if (a.dtype == kBf16) return launch_typed<bf16, true>(bwd, a, s, blocks, st);
+    if (a.dtype == kF16) return launch_typed<f16, true>(bwd, a, s, blocks, st);
+    return launch_typed<float, true>(bwd, a, s, blocks, st);
   }
+  if (a.dtype == kBf16) return launch_typed<bf16, false>(bwd, a, s, blocks, st);
+  if (a.dtype == kF16) return launch_typed<f16, false>(bwd, a, s, blocks, st);
+  return launch_typed<float, false>(bwd, a, s, blocks, st);
 }
 
 }  // namespace
@@ -425,13 +431,13 @@ hipError_t launch_norm_fwd(const NormArgs& a, hipStream_t st) {
   // (16 waves: those that two workgroups to a CU hold, so that weights and the next row's pieces count: 8000 x 8192 into fp16
   // 47.3 -> 44.4 us, 2048 x 8192 17.9 -> 14.6)
   const long most = s.wpr == 16 ? 512 : s.p == 4 ? 1024 : kNormFwdBlocks;
-  launch_norm(false, a, (unsigned)std::min(most, norm_groups(s, a.rows)), st);
-  return hipGetLastError();
+  return launch_norm(false, a, (unsigned)std::min(most, norm_groups(s, a.rows)), st);
 }
 
 hipError_t launch_norm_bwd(const NormArgs& a, hipStream_t st) {
   const int nb = a.rows > 0 ? norm_bwd_blocks(a.rows, a.D, a.dtype) : 0;
-  if (nb) launch_norm(true, a, (unsigned)nb, st);
+  if (nb)
+    if (hipError_t e = launch_norm(true, a, (unsigned)nb, st)) return e;
   if (a.dw || a.db)  // (no rows: sums of nothing, zeros)
     hipLaunchKernelGGL(norm_sum_kernel, dim3((unsigned)((a.D + 63) / 64), a.dw && a.db ? 2 : 1), dim3(1024), 0, st, a, nb);
   return hipGetLastError();

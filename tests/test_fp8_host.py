@@ -211,3 +211,24 @@ def test_abi_stride_of_16_bit_outputs():
     for dt in (0, 1, 2):
         assert linear(31, dt=dt) == SHAPE and linear(-32, dt=dt) == SHAPE and linear(1, dt=dt) == SHAPE
         assert linear(0, M=0, dt=dt) == 0 and linear(32, M=0, dt=dt) == 0 and linear(40, M=0, dt=dt) == 0
+
+
+def test_plan_offers_what_is_compiled():
+    """Tiles of 256 write 16 and 8 bits, those of 64 16 and 32; a gated output in 8 bits needs 128 columns, so tiles of 256 or a
+    wave's sixteen."""
+    lib = _lib.load()
+    sizes = [int(1.7 ** i) + i % 3 for i in range(2, 24)]
+    for M in sizes:
+        for N in sizes:
+            for K in sizes[::3]:
+                for act in (0, 1, 5):
+                    for dtype, into8 in ((0, 0), (2, 0), (0, 1)):
+                        side, parts, through = (ctypes.c_int() for _ in range(3))
+                        assert lib.ccq_fp8_linear_plan(M, N, K, act, dtype, into8, *map(ctypes.byref, (side, parts, through))) == 0
+                        side, parts, through = side.value, parts.value, through.value
+                        if into8 and not through:
+                            assert side in ((0, 256) if act == 5 else (0, 128, 256)) and parts == 1
+                        elif into8:
+                            assert side in (0, 64, 128)
+                        elif dtype == 2:
+                            assert side in (0, 64)
