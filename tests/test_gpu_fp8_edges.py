@@ -1,5 +1,5 @@
 """``ccq_fp8_linear`` at the edges of each way that it runs: strides of outputs, scales far from one, numbers that are not
-finite.  Which way a size takes is asserted, as in
+finite; norms into 8 bits of more wide rows than workgroups.  Which way a size takes is asserted, as in
 ``test_gpu_fp8_paths.py``, whose whole numbers these are: outputs have to be equal bit for bit."""
 
 import ctypes
@@ -189,3 +189,11 @@ def test_exact_sums_of_mixed_scales(size, way):
     want, err = linear64(tuple(t[rows] for t in x), w, exact=True)
     y = fp8_linear(Fp8Rows(*to_device(x, dev)), Fp8Rows(*to_device(w, dev)), dtype=FL)
     close64(y[rows.to(dev)], want, err)
+
+
+@pytest.mark.parametrize("residual", [False, True], ids=["", "residual"])
+@pytest.mark.parametrize("dtype,rows,D", [(FL, 1100, 5003), (FL, 1100, 8192), (FL, 520, 4100), (BF, 2500, 8191)], ids=str)
+def test_more_wide_rows_than_workgroups(dtype, rows, D, residual):
+    """Norms into 8 bits of sixteen waves a row (fp32 above 4096 columns) and of four with four pieces a lane, each workgroup
+    over several rows."""
+    test_gpu_fp8.test_norm(rows, D, dtype, FL, residual)

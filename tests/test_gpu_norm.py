@@ -284,3 +284,11 @@ def test_norm_captured():
             assert torch.equal(a, b)
         step(sets[0])
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("layer", [False, True], ids=["rms", "layer"])
+@pytest.mark.parametrize("rows,D,dtype,residual", [(1100, 8191, FL, True), (600, 8192, FL, False), (1100, 4096, FL, True),
+                                                   (1100, 8191, BF, True), (600, 8192, HF, False)], ids=str)
+def test_more_wide_rows_than_workgroups(layer, rows, D, dtype, residual):
+    """Rows of sixteen waves each, several of them to a workgroup, both ways."""
+    check(layer, make(layer, rows, D, dtype, FL, rows + D, residual), D, dtype, FL)
