@@ -59,8 +59,10 @@ def fp8_linear(x: Fp8Rows, weight: Fp8Rows, bias: Optional[torch.Tensor] = None,
     once, to ``dtype`` (bf16, fp16 or fp32; ``residual`` has the same), or with ``quantize`` to 8 bits, as the next
     ``fp8_linear`` takes it (no residual then).  Sums into fp32 are exact but for fp32's additions; into 16 and 8 bits the
     matrix instruction cuts off, of each eight consecutive products, what lies below 2^-13 of the largest one's power of
-    two (1.4e-5 of a result on normal data; about one 8-bit output in a thousand rounds to its other neighbour).
-    Inference only, as ``rms_norm_fp8``."""
+    two: 1.5e-5 of a result on normal data (about one 8-bit output in a thousand rounds to its other neighbour), up to 9e-5
+    with channels 100 to 1000 times the others, and where such channels cancel in a result 3e-4 to 4e-3 of what is left.
+    Where that is too much, call it with ``dtype=torch.float32`` (and the residual in fp32) and round its result: ``.to`` of
+    a 16-bit type, or ``quantize_fp8``.  Inference only, as ``rms_norm_fp8``."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"fp8_linear: activation {activation!r} is unknown (expected one of "

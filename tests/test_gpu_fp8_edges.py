@@ -1,5 +1,5 @@
 """``ccq_fp8_linear`` at the edges of each way that it runs: strides of outputs, scales far from one, numbers that are not
-finite; norms into 8 bits of more wide rows than workgroups.  Which way a size takes is asserted, as in
+finite, channels far above the others; norms into 8 bits of more wide rows than workgroups.  Which way a size takes is asserted, as in
 ``test_gpu_fp8_paths.py``, whose whole numbers these are: outputs have to be equal bit for bit."""
 
 import ctypes
@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import test_gpu_fp8
-from _fp8 import laid_out, linear64, random_rows, to_device
+from _fp8 import check_rounded, laid_out, linear64, quantized, random_rows, to_device
 from test_gpu_fp8_paths import ACTS, BF, CASES, DTYPES, FL, HF, KINDS, _cuda, plan, whole
 
 pytestmark = pytest.mark.gpu
@@ -19,6 +19,12 @@ close64 = test_gpu_fp8._close
 
 def _bytes(t):
     return t.contiguous().view(torch.uint8)
+
+
+def rows8(x):
+    """Rows on the CPU in 8 bits, by the definition in 64 bits, laid out with NaN behind their ends."""
+    v, s = quantized(x)
+    return laid_out(v.float().to(torch.float8_e4m3fn), 16), laid_out(s.float().to(torch.float8_e8m0fnu), 4)
 
 
 #        M, N, K            act, dtype, way
@@ -189,6 +195,38 @@ def test_exact_sums_of_mixed_scales(size, way):
     want, err = linear64(tuple(t[rows] for t in x), w, exact=True)
     y = fp8_linear(Fp8Rows(*to_device(x, dev)), Fp8Rows(*to_device(w, dev)), dtype=FL)
     close64(y[rows.to(dev)], want, err)
+
+
+@pytest.mark.parametrize("M,N,K", [(70, 96, 520), (1300, 520, 520)], ids=str)
+@pytest.mark.parametrize("how", ["one channel", "two that cancel"])
+def test_outlying_channels(M, N, K, how):
+    """Channels a thousand times the others: 16-bit outputs within what the 8-bit instruction cuts off, and the sums in fp32,
+    from which a caller rounds to 16 or 8 bits by itself, within fp32's additions."""
+    from ccq_amd import Fp8Rows, fp8_linear, quantize_fp8
+    print("test_outlying_channels", M, N, K, how, flush=True)
+    dev = _cuda()
+    gen = torch.Generator().manual_seed(M + N + K)
+    x = torch.randn(M, K, generator=gen)
+    w = torch.randn(N, K, generator=gen) * K ** -0.5
+    x[:, 5] *= 1000
+    if how == "two that cancel":
+        x[:, 70], w[:, 70] = x[:, 5], -w[:, 5]
+    x, w = rows8(x), rows8(w)
+    xd, wd = Fp8Rows(*to_device(x, dev)), Fp8Rows(*to_device(w, dev))
+    res = torch.randn(M, N, generator=gen)
+    rows = torch.arange(0, M, max(1, M // 150))
+    some = tuple(t[rows] for t in x)
+    for dtype in (BF, HF):
+        r = res.to(dtype)
+        want, err = linear64(some, w, None, None, r[rows])
+        close64(fp8_linear(xd, wd, residual=r.to(dev), dtype=dtype)[rows.to(dev)], want, err)
+        want, err = linear64(some, w, None, None, r[rows], exact=True)
+        y = fp8_linear(xd, wd, residual=r.float().to(dev), dtype=FL)
+        close64(y[rows.to(dev)], want, err)
+        close64(y.to(dtype)[rows.to(dev)], want, err)
+    want, err = linear64(some, w, exact=True)
+    q = quantize_fp8(fp8_linear(xd, wd, dtype=FL))
+    check_rounded(q.values.cpu()[rows], q.scales.cpu()[rows], want, err)
 
 
 @pytest.mark.parametrize("residual", [False, True], ids=["", "residual"])
