@@ -26,7 +26,7 @@ namespace ccq {
 namespace {
 
 // ---------------------------------------------------------------------------
-// rows into 8 bits: 16 lanes a block, 8 elements a lane.  Bound by HBM: 16384 x 2048 bf16 18.5 us, 32000 x 1024 fp32 29.9 (both
+// rows into 8 bits: 16 lanes a block, 8 elements a lane.  Bound by HBM: 16384 x 2048 bf16 18.5 us, 32000 x 1024 fp32 30.0 (both
 // 5.5 TB/s); a wave takes one to four rows, so that narrow rows leave few lanes idle, and few rows many waves.
 // ---------------------------------------------------------------------------
 template <typename T>
@@ -165,10 +165,10 @@ enum : int { kOut16 = 0, kOut32 = 1, kOut8 = 2 };
 // middle: there stand the barriers, and behind each of them those halves of the step after next are loaded, between
 // products, a step and a half before they are read.
 //
-// Bound by the matrix cores: a step of a 256 tile takes 1.4 us, its instructions alone 1.1.  8192^3 365 - 400 us (2.75 - 3.0
+// Bound by the matrix cores: a step of a 256 tile takes 1.4 us, its instructions alone 1.1.  8192^3 387 - 414 us (2.65 - 2.84
 // PFLOP/s; fragments read a whole step at a time 727, halves loaded a step ahead 440); 32768 x 1024 over 2816 with residual
-// 92; 16384 x 2816 swiglu over 1024 into 8 bits 99 - 104, of which the outputs' arithmetic, with one wave a SIMD, is a third.
-// In fp32 (exactly) the conversions bound it, 64 a step and wave at half rate: 4096^3 184 us; fragments are held once and
+// 90 - 97; 16384 x 2816 swiglu over 1024 into 8 bits 99 - 108, of which the outputs' arithmetic, with one wave a SIMD, is a third.
+// In fp32 (exactly) the conversions bound it, 64 a step and wave at half rate: 4096^3 184 - 200 us; fragments are held once and
 // read between two barriers, so that three workgroups share a CU.
 template <int BM, int BN, int WM, int WN, int ACT, int OUT>
 __global__ __launch_bounds__(WM * WN * 64, OUT == kOut32 ? 3 : 1) void fp8_product_kernel(const Fp8ProductArgs p) {
@@ -598,7 +598,7 @@ __global__ __launch_bounds__(WM * WN * 64, OUT == kOut32 ? 3 : 1) void fp8_produ
   }
   counted = direct && cm + BM <= p->M;
   // Tiles that end within the columns: straight from the accumulators.  A lane holds, of each of its rows, W consecutive
-  // columns of each group->
+  // columns of each group.
   if constexpr (ACT != kActOther) {
     if (direct) {
       const long nw = cn + wn * COLS + g * W;
@@ -800,8 +800,8 @@ __global__ __launch_bounds__(WM * WN * 64, OUT == kOut32 ? 3 : 1) void fp8_produ
 // (Straight into registers a lane's neighbours would lie in other rows, and 16 bytes take a request each: 16 bytes a cycle
 // and CU, 64 so.)  The parts' sums meet in LDS, in their order.  An output in 8 bits needs its blocks' largest magnitudes:
 // its workgroup is eight groups of one wave, 128 columns.  Bound by latency, or by the weight's bytes: 16 x 1024 over 1024 4.3 us
-// (by tiles of 64 5.5), 16 x 2816 swiglu over 1024 into 8 bits, from HBM, 7.5, one row of 32000 over 1024 into fp32 7.9 (4.2
-// TB/s).
+// (by tiles of 64 5.5), 16 x 2816 swiglu over 1024 into 8 bits, from HBM, 7.5, one row of 32000 over 1024 into fp32 9.0
+// (3.7 TB/s; 7.9 where the last-level cache holds the weight).
 struct ThinArgs {
   Fp8ProductArgs p;
   int parts;  // waves to a group: 1, 2, 4 or 8
@@ -1006,8 +1006,8 @@ struct Fp8Plan {
   int parts;     // of the contraction (side 0)
   bool through;  // an output in 8 bits is written in fp32 first, and quantised by a second launch
 };
-// By what a call is expected to take, in us, out of measured times (`steps` of 128; an activation without a gate is code
-// that a tile's outputs pass through: `act`):
+// By what a call is expected to take, in us, out of times measured on one card (on another those of many rows were up to 7%
+// longer; `steps` of 128; an activation without a gate is code that a tile's outputs pass through: `act`):
 //   side 0: a workgroup a CU, 0.29 a step of a wave (swiglu 0.45, exactly 0.46), or the weight's bytes.  1024 over 1024, 64
 //     rows: 4.3 in eight parts, 5.9 in one, by 64 tiles 5.5; 4064 over 1728, 40 rows 10.9, 7.8 (two parts 6.0), 7.4; 2816
 //     over 1024, 600 rows 78, 20, 6.8
@@ -1017,8 +1017,9 @@ struct Fp8Plan {
 //     90, 111; 3520 over 3008, 25960 rows 316, 317, 344; 255, 302, 350; 2188 over 959, 4363 rows 22, 25, 29; 30, 35, 42;
 //     4096 over 4096, 2048 rows 35, 4096 rows 66; 47, 62), more where outputs end inside a tile (1100 over 700, 600 rows
 //     9.6, 1024 over 1024 7.8)
-//   256: a round of all CUs 1.4 a step (8192^3 365; fewer workgroups 1.0), and the outputs, more where they end inside a tile
-//     (swiglu 2816 over 1024, 9000 rows 74, 128 tiles 63; 16384 rows 104, 108; 1024 over 2816, 30000 rows 78, 91)
+//   256: a round of all CUs 1.4 a step (8192^3, four rounds with their outputs, 390; fewer workgroups 1.0), and the outputs,
+//     more where they end inside a tile (swiglu 2816 over 1024, 9000 rows 74, 128 tiles 63; 16384 rows 104, 108; 1024 over
+//     2816, 30000 rows 78, 91)
 //   through fp32: the second launch (its host time too), and 8 bytes an output to and fro
 Fp8Plan fp8_plan(long M, long N, long K, int act, int out) {
   const bool glu = act == kActSwiglu, other = !glu && act != kActNone;

@@ -433,8 +433,8 @@ hipError_t launch_norm_fwd(const NormArgs& a, hipStream_t st) {
   // one piece two.  2048 -> 512 workgroups, us: RMS norm 2048 x 8192 bf16 20.6 -> 16.6, fp32 30.0 -> 26.5, 8000 x 8192 bf16
   // 52.8 -> 50.3, 2048 x 4104 bf16 20.2 -> 15.0; layer norm 24.9 -> 20.9, 34.0 -> 28.2, 71.6 -> 70.4, 27.1 -> 20.0; into 8
   // bits 2048 x 8192 fp32 24.9 -> 20.2.  Up to 3 % more where HBM is busy with a residual's rows: 8000 x 8192 RMS norm bf16
-  // 94.6 -> 95.3, fp32 192.8 -> 195.1.  256 would give 16-bit rows little more (16.3, 50.3, 14.3) and take from fp32 rows of one piece
-  // (8000 x 2056 37.6, with 512 35.2, with 256 50.9).
+  // 94.6 -> 95.3, fp32 192.8 -> 195.1.  256 would give 16-bit rows little more (16.3, 50.3, 14.3) and take from fp32 rows of
+  // one piece (8000 x 2056 37.6, with 512 35.2, with 256 50.9).
   const long most = s.wpr == 16 ? 512 : s.p == 4 ? 1024 : kNormFwdBlocks;
   return launch_norm(false, a, (unsigned)std::min(most, norm_groups(s, a.rows)), st);
 }

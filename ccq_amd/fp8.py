@@ -43,9 +43,10 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Rows:
 
 def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-5,
                  residual: Optional[torch.Tensor] = None) -> Union[Fp8Rows, Tuple[Fp8Rows, torch.Tensor]]:
-    """``rms_norm`` with its result in 8 bits (``quantize_fp8`` of the result in fp32: one rounding).  With ``residual`` it
-    returns ``(y, s)``, the stream ``s = x + residual`` in x's type.  Inference only: tensors that need gradients are
-    refused while gradients are recorded."""
+    """``rms_norm`` with its result in 8 bits (``quantize_fp8`` of the result in fp32: one rounding), for rows of at most 8192 as
+    there; wider ones are normed by other means and given to ``quantize_fp8``.  With ``residual`` it returns ``(y, s)``, the
+    stream ``s = x + residual`` in x's type.  Inference only: tensors that need gradients are refused while gradients are
+    recorded."""
     values, scales, s = ops().rms_norm_fp8(x, weight, eps, residual)
     return Fp8Rows(values, scales) if residual is None else (Fp8Rows(values, scales), s)
 

@@ -577,8 +577,8 @@ int ccq_norm_fp8_fwd(const void* x, int64_t ldx, const void* r, int64_t ldr, con
  * rows, then up rows; values weight, ldw; scales ws, ldws), bias [N] (swiglu: [2 N]) of bdtype (nullable), r [M, N] of
  * dtype (row stride ldr, nullable), act CCQ_ACT_*.  Products, bias, activation and residual in fp32.  y [M, N] of dtype
  * (row stride ldy, 0: contiguous), rounded once; or, with ys not NULL, y [M, N] (ldy) and ys (ldys) in 8 bits (no r then;
- * dtype is not looked at).  workspace: ccq_fp8_linear_workspace_bytes bytes (into8 not 0: the output in 8 bits), for outputs in 8
- * bits of few rows.
+ * dtype is not looked at).  workspace: ccq_fp8_linear_workspace_bytes bytes (into8 not 0: the output in 8 bits; 0 for most
+ * calls), for outputs in 8 bits that are written in fp32 first, at any number of rows.
  */
 /* How such a product runs: sides of its square tiles (256, 128, 64; 0: 16 columns of 16 rows to a wave, in parts of the
  * contraction), and whether it goes through the workspace. */
